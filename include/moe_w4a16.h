@@ -236,6 +236,120 @@ int moe_fused_experts_v1(const uint16_t* x, int32_t T, const int32_t* topk_ids,
                          const uint16_t* shared_gate_w, void* workspace, int64_t workspace_bytes,
                          uint16_t* out, int32_t path, void* stream);
 
+/* ---------------------------------------------------------------- rows sorted by expert
+ * Rows of one dtype (0 bf16, 1 fp16, 2 fp32). No counterpart in the reference, whose expert sort
+ * exists inside its fused call only (moe_align_v1). At most 2^22 slots T * top_k, top_k <= 64,
+ * num_experts <= 512, hidden <= 65536. */
+
+/* Workspace bytes of moe_dispatch_v1 (0 for few slots: then workspace may be NULL). */
+int64_t moe_dispatch_workspace_bytes_v1(int32_t T, int32_t top_k, int32_t num_experts);
+
+/* Slot f = t * top_k + i. Rows are ordered by (expert, slot); a slot whose id is outside
+ * [0, num_experts) is dropped: it takes a row of zeros behind the last expert's rows.
+ *   rows     [T * top_k, hidden]  x[t] of each row's slot
+ *   offsets  int32 [num_experts + 1]  first row of each expert; the last is the rows' count
+ *   row_slot int32 [T * top_k]  the slot of each row
+ *   slot_row int32 [T, top_k]   the row of each slot; ~row (negative) for a dropped slot
+ * With T = 0 only offsets (zeros) is written. */
+int moe_dispatch_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype,
+                    const int32_t* topk_ids, int32_t top_k, int32_t num_experts, void* workspace,
+                    int64_t workspace_bytes, void* rows, int32_t* offsets, int32_t* row_slot,
+                    int32_t* slot_row, void* stream);
+
+/* out[t] = sum_i topk_weights[t, i] * rows[slot_row[t, i]] over the kept slots, in slot order in
+ * fp32, rounded once. topk_weights fp32 [T, top_k] or NULL (1: the gradient of moe_dispatch_v1's
+ * rows with respect to x). slot_row is moe_dispatch_v1's; a dropped slot's row is not looked at. */
+int moe_combine_v1(const void* rows, int32_t T, int32_t top_k, int32_t hidden, int32_t dtype,
+                   const int32_t* slot_row, const float* topk_weights, void* out, void* stream);
+
+/* Gradients of moe_combine_v1 with weights: drows[slot_row[t, i]] = topk_weights[t, i] * dout[t]
+ * (a dropped slot's row: zeros), dweights[t, i] = <dout[t], rows[slot_row[t, i]]> in fp32 (0 for a
+ * dropped slot). drows [T * top_k, hidden] or NULL; dweights fp32 [T, top_k] or NULL (then rows may
+ * be NULL). Sums in a fixed order. */
+int moe_combine_backward_v1(const void* dout, const void* rows, int32_t T, int32_t top_k,
+                            int32_t hidden, int32_t dtype, const int32_t* slot_row,
+                            const float* topk_weights, void* drows, float* dweights,
+                            void* stream);
+
+/* ---------------------------------------------------------------- int8 products
+ * Symmetric int8 with a scale per token and per output channel. dtype: that of the activations
+ * and the output (0 bf16, 1 fp16, 2 fp32). K % 16 == 0, K <= 65536 (exact 32-bit sums); T * K and
+ * N * K below 2 GiB; int8 bases on 16-byte boundaries. No counterpart in the reference. */
+
+/* scale[t] = a / 127, q[t, k] = round_half_even(127 * x[t, k] / a), a = max_k |x[t, k]|. A row of
+ * zeros: q = 0, scale 0. A row that holds an infinity or NaN: q = 0, scale a / 127 (inf or NaN).
+ * q int8 [T, K] (any K up to 65536), scale fp32 [T]. */
+int moe_quantize_tokens_v1(const void* x, int32_t T, int32_t K, int32_t dtype, int8_t* q,
+                           float* scale, void* stream);
+
+/* out[t, n] = round((float(sum_k q[t, k] * w[n, k]) * q_scale[t]) * w_scale[n] (+ bias[n])).
+ * w int8 [N, K], w_scale fp32 [N], bias NULL or [N] of dtype, out [T, N] of dtype. */
+int moe_int8_matmul_v1(const int8_t* q, const float* q_scale, int32_t T, int32_t K,
+                       const int8_t* w, const float* w_scale, int32_t N, const void* bias,
+                       int32_t dtype, void* out, void* stream);
+
+/* moe_quantize_tokens_v1 of x, then moe_int8_matmul_v1. */
+int64_t moe_int8_linear_workspace_bytes_v1(int32_t T, int32_t K);
+int moe_int8_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype, const int8_t* w,
+                       const float* w_scale, int32_t N, const void* bias, void* workspace,
+                       int64_t workspace_bytes, void* out, void* stream);
+
+/* int8 experts of one layer: gate and up [E, I, H], down [E, H, I], a scale per output channel
+ * (fp32 [E, I], [E, I], [E, H]). */
+typedef struct moe_int8_set_v1 {
+  const int8_t* gate;
+  const int8_t* up;
+  const int8_t* down;
+  const float* gate_scale;
+  const float* up_scale;
+  const float* down_scale;
+  int32_t num_experts;
+  int32_t hidden;
+  int32_t intermediate;
+} moe_int8_set_v1;
+
+/* Routed int8 experts with caller-given routing (topk_ids int32 and topk_weights fp32 [T, top_k];
+ * a slot whose id is outside [0, num_experts) is dropped). For every kept slot: the token is
+ * quantised, h = round(silu(g) * u) of its products with gate and up, h is quantised,
+ * y = round(product with down); out[t] = the weighted sum of the token's y, as moe_combine_v1.
+ * The int8 counterpart of moe_fused_experts_v1. hidden and intermediate multiples of 16; out may
+ * be x; neither may lie in the workspace. */
+int64_t moe_int8_experts_workspace_bytes_v1(int32_t T, int32_t top_k, const moe_int8_set_v1* experts,
+                                            int32_t dtype);
+int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* topk_ids,
+                        const float* topk_weights, int32_t top_k, const moe_int8_set_v1* experts,
+                        void* workspace, int64_t workspace_bytes, void* out, void* stream);
+
+/* ---------------------------------------------------------------- norms around a block */
+#define MOE_GATE_NONE 0
+#define MOE_GATE_TOKEN 1   /* [T] */
+#define MOE_GATE_CHANNEL 2 /* [hidden] */
+#define MOE_GATE_FULL 3    /* [T, hidden] */
+
+/* The norm behind a block, its gate, the scaled residual and the next block's norm in one pass:
+ *   p = y * rsqrt(mean(y^2) + eps) * (1 + post_w)                    (p = y with post_w NULL)
+ *   res_out = round(res_scale * res + branch_scale * gate * p)
+ *   x_out = round(res_out * rsqrt(mean(res_out^2) + eps) * (1 + pre_w))  (pre_w NULL: not written)
+ * with mtp_rms_norm's (1 + w) scaling (src/mtp_expert_prefetch/mtp/extra_tensors.py:40-48), which
+ * moe_rmsnorm_v1 applies to the plain residual sum. All tensors of one dtype (0 bf16, 1 fp16,
+ * 2 fp32); hidden in [1, 8192]; res_out may be res; otherwise outputs overlap nothing. */
+int moe_block_norm_v1(const void* y, const void* res, int32_t T, int32_t hidden, int32_t dtype,
+                      const void* post_w, const void* gate, int32_t gate_kind, float res_scale,
+                      float branch_scale, const void* pre_w, float eps, void* res_out, void* x_out,
+                      void* stream);
+
+/* Gradients of moe_block_norm_v1 from those of res_out (dres_out, NULL: zeros) and x_out (dx, NULL:
+ * x_out is not used; then pre_w does not matter): dy, dres [T, hidden], dpost_w, dpre_w [hidden],
+ * dgate as gate, each NULL where it is not wanted. Weights' and channel gates' gradients are fp32
+ * sums in a fixed order over the workspace (only they need it), rounded once. */
+int64_t moe_block_norm_workspace_bytes_v1(int32_t T, int32_t hidden);
+int moe_block_norm_backward_v1(const void* y, const void* res_out, int32_t T, int32_t hidden,
+                               int32_t dtype, const void* post_w, const void* gate,
+                               int32_t gate_kind, float res_scale, float branch_scale,
+                               const void* pre_w, float eps, const void* dres_out, const void* dx,
+                               void* workspace, int64_t workspace_bytes, void* dy, void* dres,
+                               void* dpost_w, void* dgate, void* dpre_w, void* stream);
+
 /* ---------------------------------------------------------------- AWQ checkpoints */
 #define MOE_AWQ_WNA16 1 /* vLLM int4 fused-MoE layout: uint8 [E, N, K/2], zeros uint8 [E, N/2, K/G] */
 #define MOE_AWQ_GEMM 2  /* AutoAWQ GEMM: int32 [E, K, N/8] and [E, K/G, N/8], order 0,2,4,6,1,3,5,7 */

@@ -48,6 +48,19 @@ EXPORTED = (
     "moe_layer_noalloc_v1",
     "moe_predictor_workspace_bytes_v1",
     "moe_predictor_v1",
+    "moe_dispatch_workspace_bytes_v1",
+    "moe_dispatch_v1",
+    "moe_combine_v1",
+    "moe_combine_backward_v1",
+    "moe_quantize_tokens_v1",
+    "moe_int8_matmul_v1",
+    "moe_int8_linear_workspace_bytes_v1",
+    "moe_int8_linear_v1",
+    "moe_int8_experts_workspace_bytes_v1",
+    "moe_int8_experts_v1",
+    "moe_block_norm_v1",
+    "moe_block_norm_workspace_bytes_v1",
+    "moe_block_norm_backward_v1",
     "moe_awq_to_gptq_v1",
     "moe_hr_predictor_workspace_bytes_v1",
     "moe_hr_predictor_v1",
@@ -127,6 +140,12 @@ class ExpertSet(ctypes.Structure):
     ]
 
 
+class Int8Set(ctypes.Structure):
+    _fields_ = [(name, c_void_p) for name in (
+        "gate", "up", "down", "gate_scale", "up_scale", "down_scale")] + [
+        (name, c_int32) for name in ("num_experts", "hidden", "intermediate")]
+
+
 class MoeLibraryError(RuntimeError):
     def __init__(self, code: int, message: str) -> None:
         super().__init__(f"[moe_w4a16 error {code}] {message}")
@@ -170,6 +189,22 @@ _SIGS = {
         c_int32),
     "moe_predictor_workspace_bytes_v1": ([_I, _I, _I, _I, _I], c_int64),
     "moe_predictor_v1": ([_P, _I, _I, _I, _P, _I, _P, _I, _I, _P, c_int64, _P, _P], c_int32),
+    "moe_dispatch_workspace_bytes_v1": ([_I, _I, _I], c_int64),
+    "moe_dispatch_v1": ([_P, _I, _I, _I, _P, _I, _I, _P, c_int64, _P, _P, _P, _P, _P], c_int32),
+    "moe_combine_v1": ([_P, _I, _I, _I, _I, _P, _P, _P, _P], c_int32),
+    "moe_combine_backward_v1": ([_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P], c_int32),
+    "moe_quantize_tokens_v1": ([_P, _I, _I, _I, _P, _P, _P], c_int32),
+    "moe_int8_matmul_v1": ([_P, _P, _I, _I, _P, _P, _I, _P, _I, _P, _P], c_int32),
+    "moe_int8_linear_workspace_bytes_v1": ([_I, _I], c_int64),
+    "moe_int8_linear_v1": ([_P, _I, _I, _I, _P, _P, _I, _P, _P, c_int64, _P, _P], c_int32),
+    "moe_int8_experts_workspace_bytes_v1": ([_I, _I, POINTER(Int8Set), _I], c_int64),
+    "moe_int8_experts_v1": ([_P, _I, _I, _P, _P, _I, POINTER(Int8Set), _P, c_int64, _P, _P],
+                            c_int32),
+    "moe_block_norm_v1": ([_P, _P, _I, _I, _I, _P, _P, _I, c_float, c_float, _P, c_float, _P, _P,
+                           _P], c_int32),
+    "moe_block_norm_workspace_bytes_v1": ([_I, _I], c_int64),
+    "moe_block_norm_backward_v1": ([_P, _P, _I, _I, _I, _P, _P, _I, c_float, c_float, _P, c_float,
+                                    _P, _P, _P, c_int64, _P, _P, _P, _P, _P, _P], c_int32),
     "moe_awq_to_gptq_v1": ([_I, _P, _P, _P, _I, _I, _I, _I, _I, POINTER(GptqProj), _P, _P], c_int32),
     "moe_hr_predictor_workspace_bytes_v1": ([_I, POINTER(HrPredictorParams)], c_int64),
     "moe_hr_predictor_v1": ([_P, _I, _P, POINTER(HrPredictorParams), _P, c_float, _P, _I, _P, c_int64,

@@ -1,0 +1,428 @@
+// The norms around a block, fused with its gate and the residual scale, and their gradients:
+//
+//   p = y * rsqrt(mean(y^2) + eps) * (1 + post_w)          (p = y without post_w)
+//   r = round(res_scale * res + branch_scale * gate * p)   the residual stream, in its type
+//   x = round(r * rsqrt(mean(r^2) + eps) * (1 + pre_w))    (only with pre_w) the next block's input
+//
+// The gate is one value per token, per channel or per element, or absent. p stays in fp32 between
+// the norm and the residual; x is computed from the rounded r, which is what the next layer and
+// the gradients read back. Backward, with s = rsqrt(mean(r^2) + eps), q = rsqrt(mean(y^2) + eps):
+//
+//   g   = d x (1 + pre_w);  du = s (g - r s mean(g r s)) + d r;   d pre_w = sum_t d x r s
+//   d res = res_scale du;   d gate = branch_scale du p, summed over what the gate broadcasts
+//   dp  = branch_scale gate du;                                     d post_w = sum_t dp y q
+//   d y = q (h - y q mean(h y q)),  h = dp (1 + post_w)             (d y = dp without post_w)
+//
+// HBM-bound in both directions: every tensor is read and written once, 8 columns a thread held in
+// registers across the reductions. A row takes a wave up to 512 columns, a workgroup of 256 threads
+// up to 2048, of 1024 up to 8192. Sums are fp32 in a fixed order: per thread over its columns, a
+// butterfly in each wave, the waves in order; the weights' gradients per workgroup over its rows in
+// order, then over the workgroups in order.
+#include <algorithm>
+#include <initializer_list>
+
+#include "common.h"
+#include "elem.h"
+#include "launch.h"
+
+namespace {
+
+constexpr int kMaxHidden = 8192;
+enum { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateFull = 3 };
+
+// Sums of N values over the NT threads of a row (all threads get them). NT = 64: no barrier.
+template <int NT, int N>
+MOE_DEV void row_sums(float (&v)[N], float (*s_part)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = bfly_sum(v[i]);
+  if constexpr (NT > 64) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();  // the previous sums have been read
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s_part[wave][i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) v[i] += s_part[w][i];
+    }
+  }
+}
+
+MOE_DEV float inv_rms(float sum, int H, float eps) {
+  return 1.0f / __builtin_sqrtf(sum / (float)H + eps);
+}
+
+struct NormArgs {
+  const void* y;
+  const void* res;  // forward: the residual; backward: r
+  const void* post;
+  const void* gate;
+  const void* pre;
+  int gate_kind;
+  int T, H;
+  float res_scale, branch_scale, eps;
+};
+
+template <int DT, int NT, bool VEC>
+MOE_DEV void load_gate(const NormArgs& a, int64_t t, int tid, float (&g)[8]) {
+  using T = typename Elem<DT>::T;
+  const T* p = static_cast<const T*>(a.gate);
+  if (a.gate_kind == kGateFull) {
+    Cols<DT, NT, VEC>::load(p + t * a.H, tid, a.H, g);
+  } else if (a.gate_kind == kGateChannel) {
+    Cols<DT, NT, VEC>::load(p, tid, a.H, g);
+  } else {
+    const float v = a.gate_kind == kGateToken ? Elem<DT>::get(p[t]) : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = v;
+  }
+}
+
+template <int NT>
+constexpr int block_threads() { return NT < 256 ? 256 : NT; }
+
+template <int DT, int NT, bool VEC>
+__global__ __launch_bounds__(block_threads<NT>()) void block_norm_kernel(NormArgs a, void* res_out,
+                                                                         void* x_out) {
+  using T = typename Elem<DT>::T;
+  using C = Cols<DT, NT, VEC>;
+  __shared__ float s_part[NT / 64][1];
+  const int tid = threadIdx.x % NT;
+  const int rows = block_threads<NT>() / NT;
+  const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
+  for (int64_t t = (int64_t)blockIdx.x * rows + sub; t < a.T; t += (int64_t)gridDim.x * rows) {
+    float p[8], r[8], g[8];
+    C::load(static_cast<const T*>(a.y) + t * a.H, tid, a.H, p);
+    C::load(static_cast<const T*>(a.res) + t * a.H, tid, a.H, r);
+    load_gate<DT, NT, VEC>(a, t, tid, g);
+    if (a.post) {
+      float w[8];
+      C::load(static_cast<const T*>(a.post), tid, a.H, w);
+      float ss[1] = {0.0f};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss[0] = __builtin_fmaf(p[e], p[e], ss[0]);
+      row_sums<NT>(ss, s_part);
+      const float q = inv_rms(ss[0], a.H, a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = (p[e] * q) * (1.0f + w[e]);
+    }
+    float ss[1] = {0.0f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      r[e] = rounded<DT>(a.res_scale * r[e] + (a.branch_scale * g[e]) * p[e]);
+      if (C::col(tid, e) < a.H) ss[0] = __builtin_fmaf(r[e], r[e], ss[0]);
+    }
+    C::store(static_cast<T*>(res_out) + t * a.H, tid, a.H, r);
+    if (a.pre) {
+      float w[8];
+      C::load(static_cast<const T*>(a.pre), tid, a.H, w);
+      row_sums<NT>(ss, s_part);
+      const float s = inv_rms(ss[0], a.H, a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = (r[e] * s) * (1.0f + w[e]);
+      C::store(static_cast<T*>(x_out) + t * a.H, tid, a.H, r);
+    }
+  }
+}
+
+struct NormGrads {
+  const void* dr;  // nullable
+  const void* dx;  // nullable (then pre is not looked at)
+  void* dy;        // the outputs are nullable
+  void* dres;
+  void* dgate;     // token and full gates
+  float* part;     // [3][partials][H]: d post_w, d gate per channel, d pre_w
+  int partials;
+  bool post, gate, pre;  // which of them are wanted
+};
+
+template <int DT, int NT, bool VEC>
+__global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kernel(NormArgs a,
+                                                                                  NormGrads d) {
+  using T = typename Elem<DT>::T;
+  using C = Cols<DT, NT, VEC>;
+  __shared__ float s3[NT / 64][3];
+  __shared__ float s2[NT / 64][2];
+  const int tid = threadIdx.x % NT;
+  const int rows = block_threads<NT>() / NT;
+  const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
+  float wpost[8], wpre[8], apost[8], agate[8], apre[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) wpost[e] = wpre[e] = apost[e] = agate[e] = apre[e] = 0.0f;
+  if (a.post) C::load(static_cast<const T*>(a.post), tid, a.H, wpost);
+  if (a.pre) C::load(static_cast<const T*>(a.pre), tid, a.H, wpre);
+  const float n = (float)a.H;
+  for (int64_t t = (int64_t)blockIdx.x * rows + sub; t < a.T; t += (int64_t)gridDim.x * rows) {
+    float y[8], r[8], g[8], du[8], dx[8];
+    C::load(static_cast<const T*>(a.y) + t * a.H, tid, a.H, y);
+    if (d.dx) {
+      C::load(static_cast<const T*>(a.res) + t * a.H, tid, a.H, r);
+      C::load(static_cast<const T*>(d.dx) + t * a.H, tid, a.H, dx);
+    }
+    if (d.dr) {
+      C::load(static_cast<const T*>(d.dr) + t * a.H, tid, a.H, du);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) du[e] = 0.0f;
+    }
+    load_gate<DT, NT, VEC>(a, t, tid, g);
+    float sum[3] = {0.0f, 0.0f, 0.0f};  // y^2, r^2, d x (1 + pre_w) r
+    if (a.post) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(y[e], y[e], sum[0]);
+    }
+    if (d.dx) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum[1] = __builtin_fmaf(r[e], r[e], sum[1]);
+        sum[2] = __builtin_fmaf(dx[e] * (1.0f + wpre[e]), r[e], sum[2]);
+      }
+    }
+    if (a.post || d.dx) row_sums<NT>(sum, s3);
+    if (d.dx) {
+      const float s = inv_rms(sum[1], a.H, a.eps);
+      const float m = sum[2] * s / n;  // mean(g r s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float rh = r[e] * s;
+        du[e] += s * (dx[e] * (1.0f + wpre[e]) - rh * m);
+        apre[e] = __builtin_fmaf(dx[e], rh, apre[e]);
+      }
+    }
+    if (d.dres) {
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = a.res_scale * du[e];
+      C::store(static_cast<T*>(d.dres) + t * a.H, tid, a.H, o);
+    }
+    const float q = a.post ? inv_rms(sum[0], a.H, a.eps) : 1.0f;
+    float dg[8], dp[8];
+    float tot[2] = {0.0f, 0.0f};  // h y, d gate
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float yh = y[e] * q;
+      const float db = a.branch_scale * du[e];
+      dg[e] = db * (yh * (1.0f + wpost[e]));
+      dp[e] = db * g[e];
+      apost[e] = __builtin_fmaf(dp[e], yh, apost[e]);
+      agate[e] += dg[e];
+      dp[e] *= 1.0f + wpost[e];
+      if (C::col(tid, e) < a.H) {  // 0 times a gate of infinity outside the row is no part of it
+        tot[0] = __builtin_fmaf(dp[e], y[e], tot[0]);
+        tot[1] += dg[e];
+      }
+    }
+    const bool token = a.gate_kind == kGateToken && d.dgate;
+    if (a.post || token) row_sums<NT>(tot, s2);
+    if (token && tid == 0) static_cast<T*>(d.dgate)[t] = Elem<DT>::put(tot[1]);
+    if (a.gate_kind == kGateFull && d.dgate)
+      C::store(static_cast<T*>(d.dgate) + t * a.H, tid, a.H, dg);
+    if (d.dy) {
+      if (a.post) {
+        const float m = tot[0] * q / n;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dp[e] = q * (dp[e] - (y[e] * q) * m);
+      }
+      C::store(static_cast<T*>(d.dy) + t * a.H, tid, a.H, dp);
+    }
+  }
+  const int64_t me = (int64_t)blockIdx.x * rows + sub, all = (int64_t)d.partials * a.H;
+  Cols<kFp32, NT, VEC> f;
+  if (d.post) f.store(d.part + me * a.H, tid, a.H, apost);
+  if (d.gate) f.store(d.part + all + me * a.H, tid, a.H, agate);
+  if (d.pre) f.store(d.part + 2 * all + me * a.H, tid, a.H, apre);
+}
+
+// The weights' gradients from the workgroups' sums: 32 columns a workgroup, 32 threads a column over
+// strided partials, then those 32 in order.
+constexpr int kSumCols = 32;
+struct SumOut {
+  void* out[3];
+};
+template <int DT>
+__global__ __launch_bounds__(1024) void block_norm_sum_kernel(const float* part, int partials,
+                                                              int H, SumOut o) {
+  __shared__ float s_sum[32][kSumCols + 1];
+  const int which = blockIdx.y;
+  if (!o.out[which]) return;
+  const int lane = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + lane;
+  const float* p = part + (int64_t)which * partials * H;
+  float s = 0.0f;
+  if (c < H) {
+#pragma unroll 8
+    for (int i = slot; i < partials; i += 32) s += p[(int64_t)i * H + c];
+  }
+  s_sum[slot][lane] = s;
+  __syncthreads();
+  if (slot == 0 && c < H) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v += s_sum[i][lane];
+    static_cast<typename Elem<DT>::T*>(o.out[which])[c] = Elem<DT>::put(v);
+  }
+}
+
+int threads_of(int H) { return H <= 512 ? 64 : H <= 2048 ? 256 : 1024; }
+int rows_of(int nt) { return nt < 256 ? 256 / nt : 1; }
+
+// Workgroups of the backward pass: each keeps the weights' gradients of its rows in registers and
+// writes them once.
+int backward_groups(int T, int H) {
+  const int nt = threads_of(H), rows = rows_of(nt);
+  const int most = nt == 1024 ? 512 : 1024;
+  return std::max(1, std::min((T + rows - 1) / rows, most));
+}
+
+#define MOE_NORM_NT(LAUNCH)                      \
+  if (nt == 64) {                                \
+    if (vec) LAUNCH(64, true); else LAUNCH(64, false);     \
+  } else if (nt == 256) {                        \
+    if (vec) LAUNCH(256, true); else LAUNCH(256, false);   \
+  } else {                                       \
+    if (vec) LAUNCH(1024, true); else LAUNCH(1024, false); \
+  }
+
+template <int DT>
+hipError_t launch_forward(const NormArgs& a, void* res_out, void* x_out, bool vec, hipStream_t s) {
+  const int nt = threads_of(a.H), rows = rows_of(nt);
+  const dim3 grid((unsigned)std::min<int64_t>((a.T + (int64_t)rows - 1) / rows, 1 << 20));
+#define MOE_NORM_FWD(NT, V)                                                                  \
+  hipLaunchKernelGGL((block_norm_kernel<DT, NT, V>), grid, dim3(block_threads<NT>()), 0, s, a, \
+                     res_out, x_out)
+  MOE_NORM_NT(MOE_NORM_FWD)
+#undef MOE_NORM_FWD
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_backward(const NormArgs& a, const NormGrads& d, void* dpost, void* dgate_channel,
+                           void* dpre, bool vec, hipStream_t s) {
+  const int nt = threads_of(a.H);
+  const dim3 grid((unsigned)backward_groups(a.T, a.H));
+#define MOE_NORM_BWD(NT, V)                                                                     \
+  hipLaunchKernelGGL((block_norm_backward_kernel<DT, NT, V>), grid, dim3(block_threads<NT>()), 0, \
+                     s, a, d)
+  MOE_NORM_NT(MOE_NORM_BWD)
+#undef MOE_NORM_BWD
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !(dpost || dgate_channel || dpre)) return e;
+  hipLaunchKernelGGL(block_norm_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 3),
+                     dim3(1024), 0, s, d.part, d.partials, a.H, SumOut{{dpost, dgate_channel, dpre}});
+  return hipGetLastError();
+}
+#undef MOE_NORM_NT
+
+int check_norm(const char* what, int32_t T, int32_t hidden, int32_t dtype, const void* gate,
+               int32_t gate_kind, float eps) {
+  if (dtype < kBf16 || dtype > kFp32)
+    return op_fail(MOE_ERR_UNSUPPORTED, "%s: dtype=%d (0 bf16, 1 fp16, 2 fp32)", what, dtype);
+  if (T < 0 || hidden < 1 || hidden > kMaxHidden)
+    return op_fail(MOE_ERR_SHAPE, "%s: T=%d hidden=%d (hidden in [1, 8192])", what, T, hidden);
+  if (gate_kind < kGateNone || gate_kind > kGateFull)
+    return op_fail(MOE_ERR_UNSUPPORTED, "%s: gate_kind=%d", what, gate_kind);
+  if ((gate != nullptr) != (gate_kind != kGateNone) && T > 0)
+    return op_fail(MOE_ERR_NULL, "%s: gate and gate_kind must be given together", what);
+  if (!(eps >= 0.0f)) return op_fail(MOE_ERR_SHAPE, "%s: eps must be >= 0", what);
+  return MOE_OK;
+}
+
+bool vec_ok(int H, std::initializer_list<const void*> ps) {
+  if (H % 8 != 0) return false;
+  for (const void* p : ps)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_block_norm_v1(const void* y, const void* res, int32_t T, int32_t hidden, int32_t dtype,
+                      const void* post_w, const void* gate, int32_t gate_kind, float res_scale,
+                      float branch_scale, const void* pre_w, float eps, void* res_out, void* x_out,
+                      void* stream) {
+  const int rc = check_norm("block norm", T, hidden, dtype, gate, gate_kind, eps);
+  if (rc) return rc;
+  if (T == 0) return MOE_OK;
+  if (!y || !res || !res_out || (pre_w && !x_out))
+    return op_fail(MOE_ERR_NULL, "block norm: NULL pointer");
+  const int64_t n = (int64_t)T * hidden * dtype_bytes(dtype);
+  const int64_t ng = gate_kind == kGateFull ? n : 0;
+  if (overlaps(res_out, n, y, n) || overlaps(res_out, n, gate, ng) ||
+      (res_out != res && overlaps(res_out, n, res, n)) ||
+      (pre_w && (overlaps(x_out, n, y, n) || overlaps(x_out, n, res, n) ||
+                 overlaps(x_out, n, res_out, n) || overlaps(x_out, n, gate, ng))))
+    return op_fail(MOE_ERR_SHAPE,
+                   "block norm: outputs must not overlap inputs or each other (res_out may be res)");
+  const NormArgs a{y, res, post_w, gate, pre_w, gate_kind, T, hidden, res_scale, branch_scale, eps};
+  const bool vec = vec_ok(hidden, {y, res, post_w, pre_w, res_out, x_out}) &&
+                   (gate_kind < kGateChannel || aligned16(gate));
+  const auto s = (hipStream_t)stream;
+  MOE_OP_HIP(dtype == kBf16   ? launch_forward<kBf16>(a, res_out, x_out, vec, s)
+             : dtype == kFp16 ? launch_forward<kFp16>(a, res_out, x_out, vec, s)
+                              : launch_forward<kFp32>(a, res_out, x_out, vec, s),
+             "block norm");
+  return MOE_OK;
+}
+
+int64_t moe_block_norm_workspace_bytes_v1(int32_t T, int32_t hidden) {
+  if (T < 0 || hidden < 1 || hidden > kMaxHidden) return -1;
+  return (int64_t)3 * backward_groups(T, hidden) * rows_of(threads_of(hidden)) * hidden * 4;
+}
+
+int moe_block_norm_backward_v1(const void* y, const void* res_out, int32_t T, int32_t hidden,
+                               int32_t dtype, const void* post_w, const void* gate,
+                               int32_t gate_kind, float res_scale, float branch_scale,
+                               const void* pre_w, float eps, const void* dres_out, const void* dx,
+                               void* workspace, int64_t workspace_bytes, void* dy, void* dres,
+                               void* dpost_w, void* dgate, void* dpre_w, void* stream) {
+  const int rc = check_norm("block norm backward", T, hidden, dtype, gate, gate_kind, eps);
+  if (rc) return rc;
+  if ((T > 0 && (!y || (dx && !res_out))) || (dx && !pre_w) || (dpost_w && !post_w) ||
+      (dgate && gate_kind == kGateNone) || (dpre_w && !dx))
+    return op_fail(MOE_ERR_NULL, "block norm backward: NULL pointer");
+  void* dchannel = gate_kind == kGateChannel ? dgate : nullptr;
+  if (dpost_w || dchannel || dpre_w) {
+    const int64_t need = moe_block_norm_workspace_bytes_v1(T, hidden);
+    if (!workspace || workspace_bytes < need)
+      return op_fail(MOE_ERR_WORKSPACE, "block norm backward: workspace of %lld bytes, needs %lld",
+                     (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (!workspace_aligned(workspace))
+      return op_fail(MOE_ERR_WORKSPACE, "block norm backward: workspace must be 256-byte aligned");
+  } else if (T == 0) {
+    return MOE_OK;
+  }
+  const int64_t n = (int64_t)T * hidden * dtype_bytes(dtype);
+  const int64_t ng = gate_kind == kGateFull ? n : 0;
+  const void* outs[] = {dy, dres, ng ? dgate : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    for (const void* in : {y, res_out, dres_out, dx, ng ? gate : nullptr})
+      if (overlaps(outs[i], n, in, n))
+        return op_fail(MOE_ERR_SHAPE, "block norm backward: gradients must not overlap inputs");
+    for (int j = 0; j < i; ++j)
+      if (overlaps(outs[i], n, outs[j], n))
+        return op_fail(MOE_ERR_SHAPE, "block norm backward: gradients must not overlap each other");
+  }
+  const NormArgs a{y, res_out, post_w, gate, pre_w, gate_kind, T, hidden,
+                   res_scale, branch_scale, eps};
+  const NormGrads d{dres_out, dx, dy, dres, gate_kind == kGateChannel ? nullptr : dgate,
+                    static_cast<float*>(workspace),
+                    backward_groups(T, hidden) * rows_of(threads_of(hidden)), dpost_w != nullptr,
+                    dchannel != nullptr, dpre_w != nullptr};
+  const bool vec = vec_ok(hidden, {y, res_out, post_w, pre_w, dres_out, dx, dy, dres, workspace}) &&
+                   (gate_kind < kGateChannel || aligned16(gate)) &&
+                   (gate_kind != kGateFull || aligned16(dgate));
+  const auto s = (hipStream_t)stream;
+  MOE_OP_HIP(dtype == kBf16   ? launch_backward<kBf16>(a, d, dpost_w, dchannel, dpre_w, vec, s)
+             : dtype == kFp16 ? launch_backward<kFp16>(a, d, dpost_w, dchannel, dpre_w, vec, s)
+                              : launch_backward<kFp32>(a, d, dpost_w, dchannel, dpre_w, vec, s),
+             "block norm backward");
+  return MOE_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,127 @@
+// Rows of bf16, fp16 or fp32 values as floats, 8 columns a thread: the I/O of the kernels that take
+// all three types, and the error reports of their entry points.
+#pragma once
+
+#include <cstdarg>
+#include <cstdio>
+
+#include "common.h"
+#include "launch.h"
+
+// dtype codes of the C ABI (the ones of moe_dequant_v1's out_dtype).
+enum { kBf16 = 0, kFp16 = 1, kFp32 = 2 };
+
+template <int DT>
+struct Elem {
+  using T = uint16_t;
+  MOE_DEV static float get(T v) { return DT == kBf16 ? bf16_to_f32(v) : f16_to_f32(v); }
+  // round to nearest even, as the hardware conversions do (v_cvt_pk_bf16_f32, v_cvt_f16_f32)
+  MOE_DEV static T put(float f) {
+    if constexpr (DT == kBf16) return __builtin_bit_cast(uint16_t, (__bf16)f);
+    return __builtin_bit_cast(uint16_t, (_Float16)f);
+  }
+};
+template <>
+struct Elem<kFp32> {
+  using T = float;
+  MOE_DEV static float get(float v) { return v; }
+  MOE_DEV static float put(float f) { return f; }
+};
+
+// The 8 columns c .. c + 7 of a row (16-byte aligned).
+template <int DT>
+MOE_DEV void ld8(const typename Elem<DT>::T* p, float (&v)[8]) {
+  if constexpr (DT == kFp32) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
+    }
+  } else {
+    const u32x4 d = ld128(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = Elem<DT>::get((uint16_t)(d[j] & 0xFFFFu));
+      v[2 * j + 1] = Elem<DT>::get((uint16_t)(d[j] >> 16));
+    }
+  }
+}
+template <int DT>
+MOE_DEV void st8(typename Elem<DT>::T* p, const float (&v)[8]) {
+  if constexpr (DT == kFp32) {
+    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    u32x4 d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      d[j] = (uint32_t)Elem<DT>::put(v[2 * j]) | ((uint32_t)Elem<DT>::put(v[2 * j + 1]) << 16);
+    *reinterpret_cast<u32x4*>(p) = d;
+  }
+}
+
+// The 8 columns of thread `tid` of NT in a row of H columns. VEC: columns 8 tid .. 8 tid + 7, all
+// inside or all outside the row (H % 8 == 0, rows 16-byte aligned); otherwise columns tid + NT e
+// (neighbouring threads on neighbouring elements), each checked. Columns outside read 0.
+template <int DT, int NT, bool VEC>
+struct Cols {
+  using T = typename Elem<DT>::T;
+  MOE_DEV static void load(const T* row, int tid, int H, float (&v)[8]) {
+    if constexpr (VEC) {
+      if (8 * tid < H) {
+        ld8<DT>(row + 8 * tid, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tid + NT * e < H ? Elem<DT>::get(row[tid + NT * e]) : 0.0f;
+    }
+  }
+  MOE_DEV static void store(T* row, int tid, int H, const float (&v)[8]) {
+    if constexpr (VEC) {
+      if (8 * tid < H) st8<DT>(row + 8 * tid, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (tid + NT * e < H) row[tid + NT * e] = Elem<DT>::put(v[e]);
+    }
+  }
+  MOE_DEV static int col(int tid, int e) { return VEC ? 8 * tid + e : tid + NT * e; }
+};
+
+// The value as it reads back after being stored in the type.
+template <int DT>
+MOE_DEV float rounded(float f) { return Elem<DT>::get(Elem<DT>::put(f)); }
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int64_t dtype_bytes(int dtype) { return dtype == kFp32 ? 4 : 2; }
+
+// An entry point's failure: the message for moe_w4a16_last_error, the code to return. A HIP error
+// is also cleared from the thread, so that it does not surface at the caller's next HIP call.
+inline int op_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(moe_error_buffer(), kErrorBufferBytes, fmt, ap);
+  va_end(ap);
+  return code;
+}
+inline int op_hip(hipError_t e, const char* where) {
+  if (e == hipSuccess) return MOE_OK;
+  (void)hipGetLastError();
+  return op_fail(MOE_ERR_HIP + ((int)e % 100), "%s: HIP error %d (%s)", where, (int)e,
+                 hipGetErrorString(e));
+}
+#define MOE_OP_HIP(expr, where)            \
+  do {                                     \
+    const int _rc = op_hip((expr), where); \
+    if (_rc) return _rc;                   \
+  } while (0)
+
+// Whether [a, a + na) and [b, b + nb) share a byte (NULL shares none).
+inline bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
+  return a && b && na > 0 && nb > 0 && p < q + (uintptr_t)nb && q < p + (uintptr_t)na;
+}

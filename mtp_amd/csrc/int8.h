@@ -1,0 +1,32 @@
+// The int8 products' kernels as the entry points see them.
+#pragma once
+
+#include "common.h"
+
+// a rows [rows][K] with a scale each; b [N][K] with a scale per channel, of one expert or of all
+// of them, N * K bytes apart. Output row r of a tile comes from a's row row_src[r] / src_div (r
+// without row_src).
+struct Int8Args {
+  const int8_t* a;
+  const float* a_scale;
+  const int32_t* row_src;
+  int src_div;
+  uint32_t a_bytes;
+  const int8_t* b0;       // SiLU products: gate
+  const int8_t* b1;       // SiLU products: up
+  const float* s0;
+  const float* s1;
+  const i32x4* tiles;     // {expert, first row, rows, 0}; NULL: consecutive rows of one matrix
+  int M, N, K;
+  void* out;              // [M][N]
+  const void* bias;       // [N] or NULL
+};
+
+// Quantise rows of the dtype to int8 with a scale each.
+hipError_t launch_quantize(const void* x, int T, int K, int dtype, int8_t* q, float* scale,
+                           hipStream_t s);
+// Rows per tile for M rows over E experts (the tile table's bm).
+int int8_block_m(int64_t M, int E);
+// m_tiles: entries of the tile table, or the row blocks of a single matrix.
+hipError_t launch_int8_product(const Int8Args& a, int bm, int m_tiles, bool silu, int dtype,
+                               hipStream_t s);

@@ -1,0 +1,196 @@
+// int8 x int8 products on MFMA with a scale per token and per channel, dense or over the tiles of
+// sorted expert rows, plain or as silu(gate) * up:
+//
+//   y[r, n] = round((float(sum_k a[r, k] b[n, k]) * a_scale[r]) * b_scale[n] (+ bias[n]))
+//   h[r, n] = round(silu(g) * u),  g and u as y in fp32 with the gate's and the up projection's b
+//
+// The sums are exact 32-bit integers (K <= 65536: |sum| <= 2^14 K < 2^31), so any split over K gives
+// the same bits.
+//
+// MFMA 16x16x64: the channels are the A operand's rows and the tokens the B operand's columns, so a
+// lane ends with 4 consecutive channels of one token: one 8-byte store for 16-bit outputs. Lane l
+// holds bytes [16 (l >> 4), 16 (l >> 4) + 16) of row l & 15 of both operands (the same k order on both
+// sides), and channels 4 (l >> 4) .. + 3 of token l & 15 of the result.
+#include <algorithm>
+
+#include "elem.h"
+#include "int8.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int64_t kMaxBlocks = int64_t(1) << 23;  // a launch holds under 2^32 threads
+
+struct Tile {
+  int expert, row0, rows;
+};
+
+// The workgroup's tile (uniform), rows 0 when there is nothing to do.
+MOE_DEV Tile tile_of(const Int8Args& a, int bm, int m) {
+  if (a.tiles) {
+    const i32x4 t = a.tiles[m];
+    return Tile{__builtin_amdgcn_readfirstlane(t[0]), __builtin_amdgcn_readfirstlane(t[1]),
+                __builtin_amdgcn_readfirstlane(t[2])};
+  }
+  return Tile{0, m * bm, min(bm, a.M - m * bm)};
+}
+
+MOE_DEV i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+// a's row of output row r.
+MOE_DEV int source_row(const Int8Args& a, int r) {
+  return a.row_src ? (int)((uint32_t)a.row_src[r] / (uint32_t)a.src_div) : r;
+}
+
+// Four channels n .. n + 3 of output row r, from the sums of one or (SiLU) two products.
+template <int DT, bool SILU>
+MOE_DEV void finish(const Int8Args& a, int expert, int64_t r, int n, float ra, i32x4 c0, i32x4 c1,
+                    bool vec) {
+  using T = typename Elem<DT>::T;
+  const int64_t sb = (int64_t)expert * a.N;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int ni = n + i < a.N ? n + i : a.N - 1;
+    v[i] = ((float)c0[i] * ra) * a.s0[sb + ni];
+    if constexpr (SILU)
+      v[i] = silu_f32(v[i]) * (((float)c1[i] * ra) * a.s1[sb + ni]);
+    else if (a.bias)
+      v[i] += Elem<DT>::get(static_cast<const T*>(a.bias)[ni]);
+  }
+  T* p = static_cast<T*>(a.out) + r * a.N + n;
+  if (vec && n + 3 < a.N) {
+    if constexpr (DT == kFp32) {
+      *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+      *reinterpret_cast<u32x2*>(p) =
+          u32x2{(uint32_t)Elem<DT>::put(v[0]) | (uint32_t)Elem<DT>::put(v[1]) << 16,
+                (uint32_t)Elem<DT>::put(v[2]) | (uint32_t)Elem<DT>::put(v[3]) << 16};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) p[i] = Elem<DT>::put(v[i]);
+  }
+}
+
+// ---------------------------------------------------------------- few rows a tile
+// Workgroup: 16 MT rows x 64 GEMM channels (SiLU: 32 gate channels and the same 32 of up, in
+// alternating groups of 16), the K steps of 64 dealt to the four waves in turn, whose sums meet in LDS.
+// Both operands go from memory to the registers the MFMA reads: a weight byte is used by one wave once.
+template <int MT, int DT, bool SILU>
+__global__ __launch_bounds__(kThreads) void int8_stream_kernel(Int8Args a, int vec) {
+  constexpr int NG = 4;  // groups of 16 channels
+  constexpr int KU = 4;  // K steps in flight
+  __shared__ i32x4 s_acc[kWaves][NG * MT][64];
+  const int blocks_n = (a.N + (SILU ? 31 : 63)) / (SILU ? 32 : 64);
+  const Tile tl = tile_of(a, 16 * MT, blockIdx.x / blocks_n);
+  if (tl.rows <= 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lr = lane & 15, lk = (lane >> 4) * 16;
+  const int n0 = (blockIdx.x % blocks_n) * (SILU ? 32 : 64);
+  const int64_t eb = (int64_t)tl.expert * a.N * a.K;
+  const uint32_t b_bytes = (uint32_t)((int64_t)a.N * a.K);
+  const __amdgpu_buffer_rsrc_t ra = buf_rsrc(a.a, a.a_bytes);
+  const __amdgpu_buffer_rsrc_t r0 = buf_rsrc(a.b0 + eb, b_bytes);
+  const __amdgpu_buffer_rsrc_t r1 = buf_rsrc(SILU ? a.b1 + eb : a.b0 + eb, b_bytes);
+  uint32_t aoff[MT], boff[NG];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = 16 * m + lr;
+    aoff[m] = r < tl.rows ? (uint32_t)source_row(a, tl.row0 + r) * (uint32_t)a.K + lk : kOutOfRange;
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const int n = n0 + 16 * (SILU ? g / 2 : g) + lr;
+    boff[g] = n < a.N ? (uint32_t)n * (uint32_t)a.K + lk : kOutOfRange;
+  }
+  i32x4 acc[NG][MT];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[g][m] = i32x4{0, 0, 0, 0};
+  for (int k0 = wave * 64; k0 < a.K; k0 += kWaves * 64 * KU) {
+    i32x4 fb[KU][NG], fa[KU][MT];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+      const int k = k0 + u * kWaves * 64;
+      const uint32_t out = k + lk < a.K ? 0u : kOutOfRange;  // K % 16 == 0: a lane's 16 bytes
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        fb[u][g] = __builtin_bit_cast(
+            i32x4, buf_ld128(SILU && (g & 1) ? r1 : r0, (boff[g] + (uint32_t)k) | out));
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        fa[u][m] = __builtin_bit_cast(i32x4, buf_ld128(ra, (aoff[m] + (uint32_t)k) | out));
+    }
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[g][m] = mfma_i8(fb[u][g], fa[u][m], acc[g][m]);
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) s_acc[wave][g * MT + m][lane] = acc[g][m];
+  __syncthreads();
+  auto total = [&](int f) {
+    i32x4 s = s_acc[0][f][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) s += s_acc[w][f][lane];
+    return s;
+  };
+  constexpr int kOut = SILU ? NG / 2 : NG;
+  for (int o = wave; o < kOut * MT; o += kWaves) {
+    const int g = o / MT, m = o % MT;
+    const int r = 16 * m + lr, n = n0 + 16 * g + (lane >> 4) * 4;
+    const i32x4 c0 = total((SILU ? 2 * g : g) * MT + m);
+    const i32x4 c1 = SILU ? total((2 * g + 1) * MT + m) : c0;
+    if (r < tl.rows && n < a.N)
+      finish<DT, SILU>(a, tl.expert, tl.row0 + r, n, a.a_scale[source_row(a, tl.row0 + r)], c0, c1,
+                       vec != 0);
+  }
+}
+
+template <int DT, bool SILU>
+hipError_t launch_stream(const Int8Args& a, int bm, int m_tiles, int vec, hipStream_t s) {
+  const int cols = SILU ? 32 : 64;
+  const int64_t blocks = (int64_t)((a.N + cols - 1) / cols) * m_tiles;
+  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks);
+#define MOE_INT8_STREAM(MT)                                                                   \
+  hipLaunchKernelGGL((int8_stream_kernel<MT, DT, SILU>), grid, dim3(kThreads), 0, s, a, vec)
+  if (bm == 16) MOE_INT8_STREAM(1);
+  else if (bm == 32) MOE_INT8_STREAM(2);
+  else MOE_INT8_STREAM(4);
+#undef MOE_INT8_STREAM
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_product(const Int8Args& a, int bm, int m_tiles, bool silu, hipStream_t s) {
+  const int es = DT == kFp32 ? 4 : 2;
+  const int vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (uintptr_t)(4 * es - 1)) == 0;
+  return silu ? launch_stream<DT, true>(a, bm, m_tiles, vec, s)
+              : launch_stream<DT, false>(a, bm, m_tiles, vec, s);
+}
+
+}  // namespace
+
+int int8_block_m(int64_t M, int E) {
+  const int64_t rows = (M + E - 1) / E;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+hipError_t launch_int8_product(const Int8Args& a, int bm, int m_tiles, bool silu, int dtype,
+                               hipStream_t s) {
+  if (m_tiles <= 0) return hipSuccess;
+  if (dtype == kBf16) return launch_product<kBf16>(a, bm, m_tiles, silu, s);
+  if (dtype == kFp16) return launch_product<kFp16>(a, bm, m_tiles, silu, s);
+  return launch_product<kFp32>(a, bm, m_tiles, silu, s);
+}

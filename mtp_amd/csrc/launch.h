@@ -201,3 +201,16 @@ hipError_t launch_hr_predictor(const uint16_t* x, int N, int H, const int32_t* l
                                const moe_hr_predictor_params_v1& p, const float* prior, float scale,
                                const float* scale_per_example, int top_k, void* workspace,
                                float* out, int32_t* ids, hipStream_t stream);
+
+// Token rows sorted by expert (dispatch.hip): rows (x NULL: the tables only), offsets [E + 1],
+// row_slot and slot_row [T * k]. ws: dispatch_scratch_bytes. tiles (nullable): the GEMM tiles of bm
+// rows, tile_cap entries {expert, first row, rows, 0}, those past the last expert's empty.
+typedef int32_t i32x4_tile __attribute__((ext_vector_type(4)));
+int64_t dispatch_scratch_bytes(int64_t slots, int E);
+hipError_t launch_dispatch(const int32_t* ids, int T, int k, int E, const void* x,
+                           int64_t row_bytes, void* rows, int32_t* offsets, int32_t* row_slot,
+                           int32_t* slot_row, void* ws, i32x4_tile* tiles, int bm, int tile_cap,
+                           hipStream_t s);
+// out[t] = sum of the token's kept rows, weighted (w NULL: by 1), in slot order (dispatch.hip).
+hipError_t launch_combine(const void* rows, int T, int k, int H, int dtype,
+                          const int32_t* slot_row, const float* w, void* out, hipStream_t s);

@@ -15,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from mtp_amd import ops
-from mtp_amd.weights import MoeExperts
+from mtp_amd.weights import Int8Experts, MoeExperts
 
 
 @dataclass(frozen=True)
@@ -26,12 +26,20 @@ class MoeRouterOutput:
 
 
 class MoeBlock(torch.nn.Module):
-    def __init__(self, experts: MoeExperts, router_weight: torch.Tensor, *,
+    """Router, routed experts and an optional sigmoid-gated shared expert. The experts are int4
+    (MoeExperts) or int8 (Int8Experts, without a shared expert: it can be one more expert of the
+    stacks, routed by the caller through ``ops.int8_experts``)."""
+
+    def __init__(self, experts: MoeExperts | Int8Experts, router_weight: torch.Tensor, *,
                  shared_expert: MoeExperts | None = None,
                  shared_expert_gate_weight: torch.Tensor | None = None, top_k: int = 8,
                  logit_bias: torch.Tensor | None = None) -> None:
         super().__init__()
-        experts.validate()
+        if isinstance(experts, Int8Experts):
+            if shared_expert is not None:
+                raise NotImplementedError("MoeBlock runs Int8Experts without a shared expert")
+        else:
+            experts.validate()
         if (shared_expert is None) != (shared_expert_gate_weight is None):
             raise ValueError("shared_expert and shared_expert_gate_weight must be given together")
         if shared_expert is not None:
@@ -79,14 +87,24 @@ class MoeBlock(torch.nn.Module):
         if bool(((ids < 0) | (ids >= self.num_experts)).any()):
             raise KeyError(f"expert ids must lie in [0, {self.num_experts})")
         w = expert_weights.reshape(T, k).to(device=flat.device, dtype=torch.float32).contiguous()
-        out = ops.fused_experts(flat, ids, w, self.experts, shared=self.shared_expert,
-                                shared_gate_w=self.shared_expert_gate_weight)
+        if isinstance(self.experts, Int8Experts):
+            out = ops.int8_experts(flat, ids, w, self.experts)
+        else:
+            out = ops.fused_experts(flat, ids, w, self.experts, shared=self.shared_expert,
+                                    shared_gate_w=self.shared_expert_gate_weight)
         return out.reshape(hidden_states.shape)
 
     def forward(self, hidden_states: torch.Tensor, *, path: str = "auto",
                 return_routing: bool = False):
-        """Router + routed experts (+ shared expert) in one stream-ordered call chain."""
+        """Router + routed experts (+ shared expert) in one stream-ordered call chain. ``path``
+        selects the int4 kernels (int8 experts choose theirs by the rows an expert gets)."""
         flat = self._flat(hidden_states)
+        if isinstance(self.experts, Int8Experts):
+            ops._path(path)
+            ids, w, _, _ = ops.router_topk(flat, self.router_weight, self.top_k,
+                                           logit_bias=self.logit_bias)
+            out = ops.int8_experts(flat, ids, w, self.experts).reshape(hidden_states.shape)
+            return (out, ids, w) if return_routing else out
         res = ops.moe_layer(flat, self.router_weight, self.experts, top_k=self.top_k,
                             logit_bias=self.logit_bias, shared=self.shared_expert,
                             shared_gate_w=self.shared_expert_gate_weight, path=path,

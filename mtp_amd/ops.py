@@ -8,11 +8,13 @@ torch.cuda.current_stream().
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from mtp_amd import _lib
-from mtp_amd.weights import MoeExperts
+from mtp_amd.weights import Int8Experts, MoeExperts
 
 PATHS = {"auto": _lib.PATH_AUTO, "decode": _lib.PATH_DECODE, "prefill": _lib.PATH_PREFILL}
 DECODE_BLOCK_M = 16
@@ -490,3 +492,333 @@ def predictor_topk(h: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, top_k: i
                                     top_k, workspace.data_ptr(), _nbytes(workspace),
                                     out.data_ptr(), _stream()))
     return out
+
+
+# ----------------------------------------------------------------------------- by expert and back
+def _call(entry: str, device: torch.device, *args) -> None:
+    """An entry point on ``device`` (which need not be the current one) and its current stream."""
+    fn = getattr(_lib.load(), entry)
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, _stream()))
+
+
+def _rows_2d(x: torch.Tensor, name: str) -> int:
+    """The dtype code of a [rows, columns] tensor of a supported type."""
+    if x.dtype not in OUT_DTYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
+    if x.ndim != 2:
+        raise ValueError(f"{name} must be 2D, got {tuple(x.shape)}")
+    return OUT_DTYPES[x.dtype]
+
+
+class Dispatch(NamedTuple):
+    """Token rows sorted by expert (``dispatch_tokens``)."""
+
+    rows: torch.Tensor      # [T * k, H]: expert by expert, slots in order; dropped slots' zeros last
+    offsets: torch.Tensor   # int32 [E + 1]: first row of each expert; offsets[E] rows are in use
+    row_slot: torch.Tensor  # int32 [T * k]: slot t * k + i of each row
+    slot_row: torch.Tensor  # int32 [T, k]: row of each slot; ~row (negative) where it is dropped
+
+
+def _dispatch(x, topk_ids, num_experts):
+    T, H = x.shape
+    k = topk_ids.shape[1]
+    dev = x.device
+    rows = torch.empty(T * k, H, dtype=x.dtype, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+    row_slot = torch.empty(T * k, dtype=torch.int32, device=dev)
+    slot_row = torch.empty(T, k, dtype=torch.int32, device=dev)
+    need = int(_lib.load().moe_dispatch_workspace_bytes_v1(T, k, num_experts))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _call("moe_dispatch_v1", dev, x.data_ptr(), T, H, OUT_DTYPES[x.dtype], topk_ids.data_ptr(), k,
+          num_experts, _ptr(ws), max(need, 0), rows.data_ptr(), offsets.data_ptr(),
+          row_slot.data_ptr(), slot_row.data_ptr())
+    return rows, offsets, row_slot, slot_row
+
+
+def _combine(rows, slot_row, topk_weights):
+    T, k = slot_row.shape
+    out = torch.empty(T, rows.shape[1], dtype=rows.dtype, device=rows.device)
+    _call("moe_combine_v1", rows.device, rows.data_ptr(), T, k, rows.shape[1],
+          OUT_DTYPES[rows.dtype], slot_row.data_ptr(), _ptr(topk_weights), out.data_ptr())
+    return out
+
+
+class _DispatchFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, topk_ids, num_experts):
+        rows, offsets, row_slot, slot_row = _dispatch(x, topk_ids, num_experts)
+        ctx.mark_non_differentiable(offsets, row_slot, slot_row)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(slot_row)
+        return rows, offsets, row_slot, slot_row
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_rows, *_):
+        if grad_rows is None:
+            return None, None, None
+        return _combine(grad_rows.contiguous(), ctx.saved_tensors[0], None), None, None
+
+
+class _CombineFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, slot_row, topk_weights):
+        ctx.save_for_backward(rows, slot_row, topk_weights)
+        return _combine(rows, slot_row, topk_weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        rows, slot_row, topk_weights = ctx.saved_tensors
+        want_rows, _, want_weights = ctx.needs_input_grad
+        grad_out = grad_out.contiguous()
+        T, k = slot_row.shape
+        drows = torch.empty_like(rows) if want_rows else None
+        dweights = torch.empty_like(topk_weights) if want_weights else None
+        _call("moe_combine_backward_v1", rows.device, grad_out.data_ptr(), rows.data_ptr(), T, k,
+              rows.shape[1], OUT_DTYPES[rows.dtype], slot_row.data_ptr(), topk_weights.data_ptr(),
+              _ptr(drows), _ptr(dweights))
+        return drows, None, dweights
+
+
+def dispatch_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -> Dispatch:
+    """Token rows sorted by expert, for products of the caller's own over each expert's rows.
+
+    x [T, H] (bf16, fp16 or fp32), topk_ids int32 [T, k]. Rows are ordered by (expert, slot), a
+    stable sort; a slot whose id is outside [0, num_experts) is dropped and takes a row of zeros
+    behind offsets[num_experts]. Differentiable in x: its gradient sums the rows' over each token's
+    kept slots in fp32. An expert may occur twice in a token's ids: each slot has its own row."""
+    _rows_2d(x, "x")
+    if topk_ids.dtype != torch.int32 or topk_ids.ndim != 2:
+        raise TypeError("topk_ids must be int32 [T, k]")
+    if topk_ids.shape[0] != x.shape[0]:
+        raise ValueError(f"topk_ids has {topk_ids.shape[0]} rows for {x.shape[0]} tokens")
+    _require_gpu(x, topk_ids)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return Dispatch(*_DispatchFn.apply(x, topk_ids, int(num_experts)))
+    return Dispatch(*_dispatch(x, topk_ids, int(num_experts)))
+
+
+def combine_tokens(rows: torch.Tensor, slot_row: torch.Tensor,
+                   topk_weights: torch.Tensor) -> torch.Tensor:
+    """The experts' rows back at their tokens: out[t] = sum_i topk_weights[t, i] *
+    rows[slot_row[t, i]] over the kept slots, in slot order in fp32, rounded once to rows' type.
+
+    rows [T * k, H] and slot_row int32 [T, k] as ``dispatch_tokens`` gives them (every row belongs
+    to one slot), topk_weights fp32 [T, k]. What a dropped slot's row and weight hold is not looked
+    at. Differentiable in rows (dropped slots' rows: zeros) and in topk_weights."""
+    _rows_2d(rows, "rows")
+    if slot_row.dtype != torch.int32 or topk_weights.dtype != torch.float32:
+        raise TypeError("slot_row must be int32 and topk_weights float32")
+    if slot_row.ndim != 2 or slot_row.shape != topk_weights.shape:
+        raise ValueError("slot_row and topk_weights must be [T, k]")
+    if rows.shape[0] != slot_row.numel():
+        raise ValueError(f"rows has {rows.shape[0]} rows for {slot_row.numel()} slots")
+    _require_gpu(rows, slot_row, topk_weights)
+    if torch.is_grad_enabled() and (rows.requires_grad or topk_weights.requires_grad):
+        return _CombineFn.apply(rows, slot_row, topk_weights)
+    return _combine(rows, slot_row, topk_weights)
+
+
+# ----------------------------------------------------------------------------- int8 products
+def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """int8 rows and their scales: scale = max|x[t]| / 127, q = x / scale rounded half to even.
+
+    x [T, K] bf16, fp16 or fp32 -> (int8 [T, K], fp32 [T]). A row that holds an infinity or NaN
+    gets q = 0 and a scale that is not finite, so its products are NaN."""
+    code = _rows_2d(x, "x")
+    _require_gpu(x)
+    T, K = x.shape
+    q = torch.empty(T, K, dtype=torch.int8, device=x.device)
+    scale = torch.empty(T, dtype=torch.float32, device=x.device)
+    _call("moe_quantize_tokens_v1", x.device, x.data_ptr(), T, K, code, q.data_ptr(),
+          scale.data_ptr())
+    return q, scale
+
+
+def _check_int8(weight, weight_scale, bias, K: int, dtype: torch.dtype) -> None:
+    if weight.dtype != torch.int8 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"weight must be int8 and weight_scale float32, got {weight.dtype} and "
+                        f"{weight_scale.dtype}")
+    if weight.ndim != 2 or weight.shape[1] != K or tuple(weight_scale.shape) != weight.shape[:1]:
+        raise ValueError(f"weight must be [N, {K}] and weight_scale [N], got "
+                         f"{tuple(weight.shape)} and {tuple(weight_scale.shape)}")
+    if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != weight.shape[:1]):
+        raise ValueError(f"bias must be {dtype} [N]")
+
+
+def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor,
+                weight_scale: torch.Tensor, *, bias: torch.Tensor | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Product of int8 rows and int8 weights with a scale for each token and each channel:
+    out[t, n] = (sum_k q[t, k] * weight[n, k]) * q_scale[t] * weight_scale[n] (+ bias[n]), the sum
+    exact in 32 bits, the rest fp32, rounded once to ``dtype``.
+
+    q int8 [T, K], q_scale fp32 [T], weight int8 [N, K], weight_scale fp32 [N], bias [N] of
+    ``dtype``. K is a multiple of 16, at most 65536."""
+    if dtype not in OUT_DTYPES:
+        raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    if q.dtype != torch.int8 or q_scale.dtype != torch.float32:
+        raise TypeError("q must be int8 and q_scale float32")
+    if q.ndim != 2 or tuple(q_scale.shape) != q.shape[:1]:
+        raise ValueError("q must be [T, K] and q_scale [T]")
+    T, K = q.shape
+    _check_int8(weight, weight_scale, bias, K, dtype)
+    _require_gpu(q, q_scale, weight, weight_scale, bias)
+    N = weight.shape[0]
+    out = torch.empty(T, N, dtype=dtype, device=q.device)
+    _call("moe_int8_matmul_v1", q.device, q.data_ptr(), q_scale.data_ptr(), T, K,
+          weight.data_ptr(), weight_scale.data_ptr(), N, _ptr(bias), OUT_DTYPES[dtype],
+          out.data_ptr())
+    return out
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
+                bias: torch.Tensor | None = None) -> torch.Tensor:
+    """A linear layer on int8 products: the values of ``quantize_tokens(x)`` followed by
+    ``int8_matmul``, in x's type. x [T, K], weight int8 [N, K], weight_scale fp32 [N]."""
+    code = _rows_2d(x, "x")
+    T, K = x.shape
+    _check_int8(weight, weight_scale, bias, K, x.dtype)
+    _require_gpu(x, weight, weight_scale, bias)
+    N = weight.shape[0]
+    dev = x.device
+    need = int(_lib.load().moe_int8_linear_workspace_bytes_v1(T, K))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    out = torch.empty(T, N, dtype=x.dtype, device=dev)
+    _call("moe_int8_linear_v1", dev, x.data_ptr(), T, K, code, weight.data_ptr(),
+          weight_scale.data_ptr(), N, _ptr(bias), ws.data_ptr(), need, out.data_ptr())
+    return out
+
+
+def int8_experts_workspace_bytes(T: int, top_k: int, experts: Int8Experts,
+                                 dtype: torch.dtype = torch.bfloat16) -> int:
+    ex = experts.struct()
+    n = int(_lib.load().moe_int8_experts_workspace_bytes_v1(T, top_k, ctypes.byref(ex),
+                                                            OUT_DTYPES[dtype]))
+    if n < 0:
+        raise ValueError(_lib.load().moe_w4a16_last_error().decode("utf-8", "replace"))
+    return n
+
+
+def int8_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
+                 experts: Int8Experts, *, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Routed int8 experts with caller-given routing: the int8 counterpart of ``fused_experts``.
+
+    Every kept slot's token is quantised and multiplied by the expert's gate and up projections,
+    h = silu(g) * u is rounded to x's type, quantised and multiplied by down; the slots' rows come
+    back as in ``combine_tokens``. x [T, H] bf16, fp16 or fp32; topk_ids int32 and topk_weights
+    fp32 [T, k]; a slot whose id is outside [0, E) contributes nothing. A shared expert goes in as
+    one more expert of the stacks, with its id and gate as one more slot of every token."""
+    code = _rows_2d(x, "x")
+    if x.shape[1] != experts.hidden_size:
+        raise ValueError(f"Expected x last dim {experts.hidden_size}, got {x.shape[1]}")
+    if topk_ids.dtype != torch.int32 or topk_weights.dtype != torch.float32:
+        raise TypeError("topk_ids must be int32 and topk_weights float32")
+    if topk_ids.shape != topk_weights.shape or topk_ids.ndim != 2 or topk_ids.shape[0] != x.shape[0]:
+        raise ValueError("topk_ids/topk_weights must be [T, k] matching the input rows")
+    _require_gpu(x, topk_ids, topk_weights)
+    if experts.device != x.device:
+        raise ValueError(f"expert weights on {experts.device}, activations on {x.device}")
+    T, k = topk_ids.shape
+    ex = experts.struct()
+    need = int(_lib.load().moe_int8_experts_workspace_bytes_v1(T, k, ctypes.byref(ex), code))
+    # a negative size (invalid sizes) leaves the error to the entry point's own checks
+    workspace = _workspace(workspace, need, x.device)
+    out = torch.empty_like(x)
+    _call("moe_int8_experts_v1", x.device, x.data_ptr(), T, code, topk_ids.data_ptr(),
+          topk_weights.data_ptr(), k, ctypes.byref(ex), workspace.data_ptr(), _nbytes(workspace),
+          out.data_ptr())
+    return out
+
+
+# ----------------------------------------------------------------------------- norms around a block
+GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = range(4)
+
+
+def _block_norm(y, res, post_w, gate, pre_w, kind, res_scale, branch_scale, eps):
+    T, H = y.shape
+    res_out = torch.empty_like(res)
+    x_out = torch.empty_like(res) if pre_w is not None else None
+    _call("moe_block_norm_v1", y.device, y.data_ptr(), res.data_ptr(), T, H, OUT_DTYPES[y.dtype],
+          _ptr(post_w), _ptr(gate), kind, res_scale, branch_scale, _ptr(pre_w), eps,
+          res_out.data_ptr(), _ptr(x_out))
+    return res_out, x_out
+
+
+class _BlockNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, res, post_w, gate, pre_w, kind, res_scale, branch_scale, eps):
+        res_out, x_out = _block_norm(y, res, post_w, gate, pre_w, kind, res_scale, branch_scale, eps)
+        ctx.save_for_backward(y, res_out, post_w, gate, pre_w)
+        ctx.consts = (kind, res_scale, branch_scale, eps)
+        ctx.set_materialize_grads(False)
+        return res_out if x_out is None else (res_out, x_out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dres_out, dx=None):
+        y, res_out, post_w, gate, pre_w = ctx.saved_tensors
+        kind, res_scale, branch_scale, eps = ctx.consts
+        if dres_out is None and dx is None:
+            return (None,) * 9
+        T, H = y.shape
+        make = torch.empty_like if T > 0 else torch.zeros_like
+        grads = [make(t) if want and t is not None else None
+                 for t, want in zip((y, res_out, post_w, gate, pre_w), ctx.needs_input_grad)]
+        if T == 0:
+            return (*grads, None, None, None, None)
+        dy, dres, dpost, dgate, dpre = grads
+        dres_out, dx = (None if g is None else g.contiguous() for g in (dres_out, dx))
+        if dx is None and dpre is not None:
+            dpre.zero_()
+        ws, need = None, 0
+        if dpost is not None or dpre is not None or kind == GATE_CHANNEL:
+            need = int(_lib.load().moe_block_norm_workspace_bytes_v1(T, H))
+            ws = torch.empty(need, dtype=torch.uint8, device=y.device)
+        _call("moe_block_norm_backward_v1", y.device, y.data_ptr(), res_out.data_ptr(), T, H,
+              OUT_DTYPES[y.dtype], _ptr(post_w), _ptr(gate), kind, res_scale, branch_scale,
+              _ptr(pre_w), eps, _ptr(dres_out), _ptr(dx), _ptr(ws), need, _ptr(dy), _ptr(dres),
+              _ptr(dpost), _ptr(dgate), _ptr(dpre if dx is not None else None))
+        return (*grads, None, None, None, None)
+
+
+def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | None = None,
+               gate: torch.Tensor | None = None, res_scale: float = 1.0,
+               branch_scale: float = 1.0, pre_w: torch.Tensor | None = None,
+               eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The norm behind a block, its gate, the scaled residual and the next block's norm at once:
+
+        p = y * rsqrt(mean(y^2) + eps) * (1 + post_w)        (p = y without post_w)
+        res_out = res_scale * res + branch_scale * gate * p
+        x = res_out * rsqrt(mean(res_out^2) + eps) * (1 + pre_w)   (None without pre_w)
+
+    with the (1 + w) scaling of ``rmsnorm``. y (the block's output) and res (the residual stream)
+    [T, H], post_w and pre_w [H], gate [H] (per channel), [T, 1] (per token) or [T, H], all of one
+    type (bf16, fp16 or fp32); H up to 8192. res_out is rounded to the type before x is computed
+    from it. Returns (res_out, x); differentiable in y, res, post_w, gate and pre_w."""
+    _rows_2d(y, "y")
+    T, H = y.shape
+    if res.shape != y.shape or res.dtype != y.dtype:
+        raise ValueError(f"res must be {y.dtype} {tuple(y.shape)}, got {res.dtype} "
+                         f"{tuple(res.shape)}")
+    for name, w in (("post_w", post_w), ("pre_w", pre_w)):
+        if w is not None and (w.dtype != y.dtype or tuple(w.shape) != (H,)):
+            raise ValueError(f"{name} must be {y.dtype} [{H}], got {w.dtype} {tuple(w.shape)}")
+    kind = GATE_NONE
+    if gate is not None:
+        kinds = {(T, 1): GATE_TOKEN, (H,): GATE_CHANNEL, (T, H): GATE_FULL}
+        kind = kinds.get(tuple(gate.shape), GATE_NONE)
+        if kind == GATE_NONE or gate.dtype != y.dtype:
+            raise ValueError(f"gate must be {y.dtype} [{H}], [{T}, 1] or [{T}, {H}], got "
+                             f"{gate.dtype} {tuple(gate.shape)}")
+    _require_gpu(y, res, post_w, gate, pre_w)
+    args = (y, res, post_w, gate, pre_w, kind, float(res_scale), float(branch_scale), float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+        out = _BlockNormFn.apply(*args)
+        return out if pre_w is not None else (out, None)
+    return _block_norm(*args)

@@ -155,3 +155,97 @@ class MoeExperts:
                 tensors[f"{prefix}{proj}.qweight"], tensors[f"{prefix}{proj}.qzeros"],
                 tensors[f"{prefix}{proj}.scales"], tensors.get(f"{prefix}{proj}.g_idx"))
         return cls(stacks["gate_proj"], stacks["up_proj"], stacks["down_proj"], group_size)
+
+
+@dataclass(frozen=True)
+class Int8Experts:
+    """Experts of one layer in int8 with a scale per output channel (``ops.int8_experts``):
+    gate and up int8 [E, I, H] with scales fp32 [E, I], down int8 [E, H, I] with scales fp32 [E, H];
+    W[e, n, k] = q[e, n, k] * scale[e, n]. H and I are multiples of 16."""
+
+    gate: torch.Tensor
+    gate_scale: torch.Tensor
+    up: torch.Tensor
+    up_scale: torch.Tensor
+    down: torch.Tensor
+    down_scale: torch.Tensor
+
+    def __post_init__(self) -> None:
+        if self.gate.ndim != 3:
+            raise ValueError(f"gate must be 3D [E, I, H], got {tuple(self.gate.shape)}")
+        e, i, h = self.gate.shape
+        for name, shape in (("gate", (e, i, h)), ("up", (e, i, h)), ("down", (e, h, i))):
+            q, scale = getattr(self, name), getattr(self, name + "_scale")
+            if q.dtype != torch.int8 or scale.dtype != torch.float32:
+                raise TypeError(f"{name} must be int8 and {name}_scale float32, got {q.dtype} and "
+                                f"{scale.dtype}")
+            if tuple(q.shape) != shape or tuple(scale.shape) != shape[:2]:
+                raise ValueError(f"{name} {tuple(q.shape)} and {name}_scale {tuple(scale.shape)} "
+                                 f"must be {shape} and {shape[:2]}")
+            for t in (q, scale):
+                if not t.is_contiguous() or t.device != self.gate.device:
+                    raise ValueError(f"{name} and {name}_scale must be contiguous and on the gate's "
+                                     "device")
+        if not 1 <= e <= 512 or h % 16 != 0 or i % 16 != 0 or h < 16 or i < 16:
+            raise ValueError(f"need 1 to 512 experts and H and I multiples of 16, got E={e} H={h} "
+                             f"I={i}")
+
+    @property
+    def num_experts(self) -> int:
+        return int(self.gate.shape[0])
+
+    @property
+    def hidden_size(self) -> int:
+        return int(self.gate.shape[2])
+
+    @property
+    def intermediate_size(self) -> int:
+        return int(self.gate.shape[1])
+
+    @property
+    def device(self) -> torch.device:
+        return self.gate.device
+
+    def struct(self) -> _lib.Int8Set:
+        return _lib.Int8Set(*(t.data_ptr() for t in (
+            self.gate, self.up, self.down, self.gate_scale, self.up_scale, self.down_scale)),
+            self.num_experts, self.hidden_size, self.intermediate_size)
+
+    def to(self, device) -> "Int8Experts":
+        return Int8Experts(*(t.to(device) for t in (
+            self.gate, self.gate_scale, self.up, self.up_scale, self.down, self.down_scale)))
+
+    @classmethod
+    def from_dense(cls, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor) -> "Int8Experts":
+        """Quantise dense stacks (bf16, fp16 or fp32 on the GPU): gate and up [E, I, H], down
+        [E, H, I], each output channel by its largest magnitude."""
+        from mtp_amd import ops
+
+        parts = []
+        for w in (gate, up, down):
+            if w.ndim != 3:
+                raise ValueError(f"expert stacks must be 3D, got {tuple(w.shape)}")
+            q, scale = ops.quantize_tokens(w.reshape(-1, w.shape[2]).contiguous())
+            parts += [q.view(w.shape), scale.view(w.shape[:2])]
+        return cls(*parts)
+
+    @classmethod
+    def from_gptq(cls, experts: MoeExperts) -> "Int8Experts":
+        """Requantise int4 GPTQ stacks (on the GPU, not a slot pool): dequantised in fp32, expert
+        by expert, then as ``from_dense``."""
+        from mtp_amd import ops
+
+        experts.validate()
+        if experts.expert_row is not None or experts.expert_stride_bytes:
+            raise ValueError("from_gptq needs the experts' own stacks, not a slot pool")
+        parts = []
+        for p in (experts.gate, experts.up, experts.down):
+            e, n, k = p.num_rows, p.out_features, p.in_features
+            q = torch.empty(e, n, k, dtype=torch.int8, device=experts.device)
+            scale = torch.empty(e, n, dtype=torch.float32, device=experts.device)
+            for i in range(e):
+                w = ops.dequantize(p.qweight[i], p.qzeros[i], p.scales[i],
+                                   group_size=experts.group_size, dtype=torch.float32)
+                q[i], scale[i] = ops.quantize_tokens(w)
+            parts += [q, scale]
+        return cls(*parts)
