@@ -99,8 +99,8 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 // lds wave-uniform). An out-of-range offset writes zeros. The load counts in vmcnt until the
 // bytes are in LDS. (A device function: the builtin inside a lambda of a kernel makes the host
 // pass drop the kernel's launch stub.)
-MOE_DEV void buf_ld128_lds(__amdgpu_buffer_rsrc_t r, uint16_t* lds, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 16, off, 0, 0, 0);
+MOE_DEV void buf_ld128_lds(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off, uint32_t soff = 0) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 16, off, soff, 0, 0);
 }
 
 MOE_DEV u32x4 ld128(const void* p) { return *reinterpret_cast<const u32x4*>(p); }

@@ -17,6 +17,8 @@ struct Int8Args {
   const float* s0;
   const float* s1;
   const i32x4* tiles;     // {expert, first row, rows, 0}; NULL: consecutive rows of one matrix
+  int m_tiles;            // entries of the tile table (behind them: how many are in use), or the
+                          // row blocks of one matrix
   int M, N, K;
   void* out;              // [M][N]
   const void* bias;       // [N] or NULL
@@ -27,6 +29,4 @@ hipError_t launch_quantize(const void* x, int T, int K, int dtype, int8_t* q, fl
                            hipStream_t s);
 // Rows per tile for M rows over E experts (the tile table's bm).
 int int8_block_m(int64_t M, int E);
-// m_tiles: entries of the tile table, or the row blocks of a single matrix.
-hipError_t launch_int8_product(const Int8Args& a, int bm, int m_tiles, bool silu, int dtype,
-                               hipStream_t s);
+hipError_t launch_int8_product(const Int8Args& a, int bm, bool silu, int dtype, hipStream_t s);

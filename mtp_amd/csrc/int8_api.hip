@@ -45,7 +45,8 @@ int matmul(const int8_t* q, const float* q_scale, int T, int K, const int8_t* w,
   a.out = out;
   a.bias = bias;
   const int bm = int8_block_m(T, 1);
-  MOE_OP_HIP(launch_int8_product(a, bm, (T + bm - 1) / bm, false, dtype, s), "int8 product");
+  a.m_tiles = (T + bm - 1) / bm;
+  MOE_OP_HIP(launch_int8_product(a, bm, false, dtype, s), "int8 product");
   return MOE_OK;
 }
 
@@ -70,7 +71,7 @@ ExpertsLayout experts_layout(int T, int k, const moe_int8_set_v1& ex, int dtype)
   L.offsets = take((int64_t)(ex.num_experts + 1) * 4);
   L.row_slot = take(S * 4);
   L.slot_row = take(S * 4);
-  L.tiles = take((int64_t)L.tile_cap * 16);
+  L.tiles = take((int64_t)(L.tile_cap + 1) * 16);
   L.scratch = take(dispatch_scratch_bytes(S, ex.num_experts));
   L.h = take(S * ex.intermediate * es);
   L.hq = take(S * ex.intermediate);
@@ -222,11 +223,12 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
   a.s0 = experts->gate_scale;
   a.s1 = experts->up_scale;
   a.tiles = tiles;
+  a.m_tiles = L.tile_cap;
   a.M = (int)S;
   a.N = I;
   a.K = H;
   a.out = h;
-  MOE_OP_HIP(launch_int8_product(a, L.bm, L.tile_cap, true, dtype, s), "gate and up");
+  MOE_OP_HIP(launch_int8_product(a, L.bm, true, dtype, s), "gate and up");
   // dropped slots' rows of h are never written; what they hold is quantised and not read again
   MOE_OP_HIP(launch_quantize(h, (int)S, I, dtype, hq, hs, s), "quantize h");
   Int8Args b{};
@@ -237,11 +239,12 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
   b.b0 = experts->down;
   b.s0 = experts->down_scale;
   b.tiles = tiles;
+  b.m_tiles = L.tile_cap;
   b.M = (int)S;
   b.N = H;
   b.K = I;
   b.out = y;
-  MOE_OP_HIP(launch_int8_product(b, L.bm, L.tile_cap, false, dtype, s), "down");
+  MOE_OP_HIP(launch_int8_product(b, L.bm, false, dtype, s), "down");
   MOE_OP_HIP(launch_combine(y, T, top_k, H, dtype, slot_row, topk_weights, out, s), "combine");
   return MOE_OK;
 }

@@ -157,10 +157,137 @@ __global__ __launch_bounds__(kThreads) void int8_stream_kernel(Int8Args a, int v
   }
 }
 
+// ---------------------------------------------------------------- many rows a tile
+// Workgroup: BM rows x BN GEMM channels on WM x WN waves, K steps of 128 bytes staged in LDS, two
+// stages: the loads of step s + 1 go straight to LDS (buffer_load ... lds) while step s is
+// multiplied; one wait and barrier a step order both the arrival and the reuse of a stage. LDS rows
+// are 128 bytes of K; the 16-byte chunk c of row r sits at position c ^ (r & 7), so that the 8 rows
+// that one phase of a 16-byte LDS read spans lie in different banks.
+// SiLU: the tile's groups of 16 channels alternate between gate and up, so that a wave holds both
+// sums of a channel in the same lane.
+template <int BM, int BN, int WM, int WN, int DT, bool SILU>
+__global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int vec) {
+  constexpr int NT = 64 * WM * WN;
+  constexpr int BK = 128;
+  constexpr int MT = BM / WM / 16, NG = BN / WN / 16;
+  constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT;  // 16-byte loads a thread and step
+  static_assert(LA * NT == BM * 8 && LB * NT == BN * 8 && NT % 256 == 0, "whole loads");
+  __shared__ __attribute__((aligned(16))) int8_t lds0[(BM + BN) * BK];
+  __shared__ __attribute__((aligned(16))) int8_t lds1[(BM + BN) * BK];
+  const int cols = SILU ? BN / 2 : BN;
+  const int blocks_n = (a.N + cols - 1) / cols;
+  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of consecutive tiles, channels
+  // fastest, so that its L2 sees the rows of few row blocks.
+  const int m_tiles = a.tiles ? __builtin_amdgcn_readfirstlane(a.tiles[a.m_tiles][0]) : a.m_tiles;
+  const int total = m_tiles * blocks_n, per = (total + 7) / 8;
+  const int idx = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + idx;
+  if (idx >= per || id >= total) return;
+  const Tile tl = tile_of(a, BM, id / blocks_n);
+  const int n0 = (id % blocks_n) * cols;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int lr = lane & 15;
+  const int64_t eb = (int64_t)tl.expert * a.N * a.K;
+  const uint32_t b_bytes = (uint32_t)((int64_t)a.N * a.K);
+  const __amdgpu_buffer_rsrc_t ra = buf_rsrc(a.a, a.a_bytes);
+  // a wave's 8 rows of a load lie in one group of 16 channels, the same parity in every load
+  const bool up = SILU && ((wave >> 1) & 1);
+  const __amdgpu_buffer_rsrc_t rb = buf_rsrc((up ? a.b1 : a.b0) + eb, b_bytes);
+  const uint32_t kc = (uint32_t)((tid & 7) ^ ((tid >> 3) & 7)) * 16;  // the chunk's byte of K
+  uint32_t aoff[LA], boff[LB];
+#pragma unroll
+  for (int j = 0; j < LA; ++j) {
+    const int r = (j * NT + tid) / 8;
+    aoff[j] = r < tl.rows ? (uint32_t)source_row(a, tl.row0 + r) * (uint32_t)a.K + kc : kOutOfRange;
+  }
+#pragma unroll
+  for (int j = 0; j < LB; ++j) {
+    const int i = (j * NT + tid) / 8;
+    const int n = n0 + (SILU ? (i >> 5) * 16 + (i & 15) : i);
+    boff[j] = n < a.N ? (uint32_t)n * (uint32_t)a.K + kc : kOutOfRange;
+  }
+  auto stage = [&](int8_t* lds, int k0) {
+    const uint32_t out = k0 + (int)kc < a.K ? 0u : kOutOfRange;  // zeros past K
+#pragma unroll
+    for (int j = 0; j < LA; ++j)
+      buf_ld128_lds(ra, lds + (j * NT + wave * 64) * 16, aoff[j] | out, (uint32_t)k0);
+#pragma unroll
+    for (int j = 0; j < LB; ++j)
+      buf_ld128_lds(rb, lds + BM * BK + (j * NT + wave * 64) * 16, boff[j] | out, (uint32_t)k0);
+  };
+  i32x4 acc[NG][MT];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[g][m] = i32x4{0, 0, 0, 0};
+  const int sw0 = (((lane >> 4) ^ (lr & 7)) * 16), sw1 = ((4 + (lane >> 4)) ^ (lr & 7)) * 16;
+  const int fa_at = (wm * MT * 16 + lr) * BK, fb_at = (BM + wn * NG * 16 + lr) * BK;
+  auto multiply = [&](const int8_t* lds) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int sw = kk ? sw1 : sw0;
+      i32x4 fa[MT], fb[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        fb[g] = *reinterpret_cast<const i32x4*>(lds + fb_at + g * 16 * BK + sw);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        fa[m] = *reinterpret_cast<const i32x4*>(lds + fa_at + m * 16 * BK + sw);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) acc[g][m] = mfma_i8(fb[g], fa[m], acc[g][m]);
+    }
+  };
+  auto step = [&](int8_t* here, int8_t* next, int k0) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    __syncthreads();  // every wave's loads of this stage landed; the other stage is free
+    if (k0 + BK < a.K) stage(next, k0 + BK);
+    multiply(here);
+  };
+  stage(lds0, 0);
+  for (int k0 = 0; k0 < a.K; k0 += 2 * BK) {
+    step(lds0, lds1, k0);
+    if (k0 + BK < a.K) step(lds1, lds0, k0 + BK);
+  }
+  float rs[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = (wm * MT + m) * 16 + lr;
+    rs[m] = r < tl.rows ? a.a_scale[source_row(a, tl.row0 + r)] : 0.0f;
+  }
+  constexpr int kOut = SILU ? NG / 2 : NG;
+#pragma unroll
+  for (int g = 0; g < kOut; ++g) {
+    const int n = n0 + (wn * kOut + g) * 16 + (lane >> 4) * 4;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = (wm * MT + m) * 16 + lr;
+      if (r < tl.rows && n < a.N)
+        finish<DT, SILU>(a, tl.expert, tl.row0 + r, n, rs[m], acc[SILU ? 2 * g : g][m],
+                         acc[SILU ? 2 * g + 1 : g][m], vec != 0);
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int DT, bool SILU>
+hipError_t launch_tile(const Int8Args& a, int vec, hipStream_t s) {
+  const int cols = SILU ? BN / 2 : BN;
+  const int64_t tiles = (int64_t)((a.N + cols - 1) / cols) * a.m_tiles;
+  const int64_t blocks = (tiles + 7) / 8 * 8;
+  if (blocks > kMaxBlocks / 2) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((int8_tile_kernel<BM, BN, WM, WN, DT, SILU>), dim3((unsigned)blocks),
+                     dim3(64 * WM * WN), 0, s, a, vec);
+  return hipGetLastError();
+}
+
 template <int DT, bool SILU>
-hipError_t launch_stream(const Int8Args& a, int bm, int m_tiles, int vec, hipStream_t s) {
+hipError_t launch_product(const Int8Args& a, int bm, int vec, hipStream_t s) {
+  if (bm == 256) return launch_tile<256, 256, 2, 4, DT, SILU>(a, vec, s);
+  if (bm == 128) return launch_tile<128, 256, 2, 4, DT, SILU>(a, vec, s);
   const int cols = SILU ? 32 : 64;
-  const int64_t blocks = (int64_t)((a.N + cols - 1) / cols) * m_tiles;
+  const int64_t blocks = (int64_t)((a.N + cols - 1) / cols) * a.m_tiles;
   if (blocks > kMaxBlocks) return hipErrorInvalidValue;
   const dim3 grid((unsigned)blocks);
 #define MOE_INT8_STREAM(MT)                                                                   \
@@ -173,24 +300,25 @@ hipError_t launch_stream(const Int8Args& a, int bm, int m_tiles, int vec, hipStr
 }
 
 template <int DT>
-hipError_t launch_product(const Int8Args& a, int bm, int m_tiles, bool silu, hipStream_t s) {
+hipError_t launch_product_t(const Int8Args& a, int bm, bool silu, hipStream_t s) {
   const int es = DT == kFp32 ? 4 : 2;
   const int vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (uintptr_t)(4 * es - 1)) == 0;
-  return silu ? launch_stream<DT, true>(a, bm, m_tiles, vec, s)
-              : launch_stream<DT, false>(a, bm, m_tiles, vec, s);
+  return silu ? launch_product<DT, true>(a, bm, vec, s) : launch_product<DT, false>(a, bm, vec, s);
 }
 
 }  // namespace
 
 int int8_block_m(int64_t M, int E) {
   const int64_t rows = (M + E - 1) / E;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  if (rows <= 16) return 16;
+  if (rows <= 32) return 32;
+  if (rows <= 64) return 64;
+  return rows <= 512 ? 128 : 256;
 }
 
-hipError_t launch_int8_product(const Int8Args& a, int bm, int m_tiles, bool silu, int dtype,
-                               hipStream_t s) {
-  if (m_tiles <= 0) return hipSuccess;
-  if (dtype == kBf16) return launch_product<kBf16>(a, bm, m_tiles, silu, s);
-  if (dtype == kFp16) return launch_product<kFp16>(a, bm, m_tiles, silu, s);
-  return launch_product<kFp32>(a, bm, m_tiles, silu, s);
+hipError_t launch_int8_product(const Int8Args& a, int bm, bool silu, int dtype, hipStream_t s) {
+  if (a.m_tiles <= 0) return hipSuccess;
+  if (dtype == kBf16) return launch_product_t<kBf16>(a, bm, silu, s);
+  if (dtype == kFp16) return launch_product_t<kFp16>(a, bm, silu, s);
+  return launch_product_t<kFp32>(a, bm, silu, s);
 }

@@ -496,13 +496,18 @@ def predictor_topk(h: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, top_k: i
 
 # ----------------------------------------------------------------------------- by expert and back
 def _call(entry: str, device: torch.device, *args) -> None:
-    """An entry point on ``device`` (which need not be the current one) and its current stream."""
+    """An entry point on ``device`` (which need not be the current one) and its current stream.
+    The raw stream query takes 0.1 us; torch.cuda.current_stream builds an object in 3 us, a
+    quarter of a small call's time on the host."""
     fn = getattr(_lib.load(), entry)
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, _stream()))
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream()))
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _lib.check(code)
 
 
 def _rows_2d(x: torch.Tensor, name: str) -> int:
