@@ -159,12 +159,15 @@ __global__ __launch_bounds__(kThreads) void int8_stream_kernel(Int8Args a, int v
 
 // ---------------------------------------------------------------- many rows a tile
 // Workgroup: BM rows x BN GEMM channels on WM x WN waves, K steps of 128 bytes staged in LDS, two
-// stages: the loads of step s + 1 go straight to LDS (buffer_load ... lds) while step s is
-// multiplied; one wait and barrier a step order both the arrival and the reuse of a stage. LDS rows
+// stages filled by loads that go straight to LDS (buffer_load ... lds). One wait and barrier in the
+// middle of a step orders the arrival of the next stage and the reuse of this one, whose second half
+// is in registers by then: the loads of step s + 2 have a whole step to arrive. LDS rows
 // are 128 bytes of K; the 16-byte chunk c of row r sits at position c ^ (r & 7), so that the 8 rows
 // that one phase of a 16-byte LDS read spans lie in different banks.
 // SiLU: the tile's groups of 16 channels alternate between gate and up, so that a wave holds both
 // sums of a channel in the same lane.
+constexpr int kGroupM = 4;
+
 template <int BM, int BN, int WM, int WN, int DT, bool SILU>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int vec) {
   constexpr int NT = 64 * WM * WN;
@@ -176,14 +179,22 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   __shared__ __attribute__((aligned(16))) int8_t lds1[(BM + BN) * BK];
   const int cols = SILU ? BN / 2 : BN;
   const int blocks_n = (a.N + cols - 1) / cols;
-  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of consecutive tiles, channels
-  // fastest, so that its L2 sees the rows of few row blocks.
+  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of consecutive tiles. Of one matrix they
+  // run down kGroupM row blocks before the next channels, so that the 32 tiles an XCD works on at a
+  // time are about 4 x 8 and share their operands in its L2; of experts they run along the channels.
   const int m_tiles = a.tiles ? __builtin_amdgcn_readfirstlane(a.tiles[a.m_tiles][0]) : a.m_tiles;
   const int total = m_tiles * blocks_n, per = (total + 7) / 8;
   const int idx = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + idx;
   if (idx >= per || id >= total) return;
-  const Tile tl = tile_of(a, BM, id / blocks_n);
-  const int n0 = (id % blocks_n) * cols;
+  int tile_m = id / blocks_n, tile_n = id % blocks_n;
+  if (!a.tiles) {
+    const int group = id / (kGroupM * blocks_n), in = id - group * kGroupM * blocks_n;
+    const int rows = min(kGroupM, m_tiles - group * kGroupM);
+    tile_m = group * kGroupM + in % rows;
+    tile_n = in / rows;
+  }
+  const Tile tl = tile_of(a, BM, tile_m);
+  const int n0 = tile_n * cols;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -223,30 +234,48 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
     for (int m = 0; m < MT; ++m) acc[g][m] = i32x4{0, 0, 0, 0};
   const int sw0 = (((lane >> 4) ^ (lr & 7)) * 16), sw1 = ((4 + (lane >> 4)) ^ (lr & 7)) * 16;
   const int fa_at = (wm * MT * 16 + lr) * BK, fb_at = (BM + wn * NG * 16 + lr) * BK;
-  auto multiply = [&](const int8_t* lds) {
+  // A step's two halves of 64 bytes of K, pipelined through two register sets: while one half is
+  // multiplied the next one's operands are read from LDS.
+  i32x4 fa[2][MT], fb[2][NG];
+  auto fetch = [&](const int8_t* lds, int half) {
+    const int sw = half ? sw1 : sw0;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int sw = kk ? sw1 : sw0;
-      i32x4 fa[MT], fb[NG];
+    for (int g = 0; g < NG; ++g)
+      fb[half][g] = *reinterpret_cast<const i32x4*>(lds + fb_at + g * 16 * BK + sw);
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        fb[g] = *reinterpret_cast<const i32x4*>(lds + fb_at + g * 16 * BK + sw);
+    for (int m = 0; m < MT; ++m)
+      fa[half][m] = *reinterpret_cast<const i32x4*>(lds + fa_at + m * 16 * BK + sw);
+  };
+  auto multiply = [&](int half) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        fa[m] = *reinterpret_cast<const i32x4*>(lds + fa_at + m * 16 * BK + sw);
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int g = 0; g < NG; ++g) acc[g][m] = mfma_i8(fb[half][g], fa[half][m], acc[g][m]);
+    // one LDS read of the next half among every few multiplications of this one
 #pragma unroll
-        for (int g = 0; g < NG; ++g) acc[g][m] = mfma_i8(fb[g], fa[m], acc[g][m]);
+    for (int i = 0; i < MT + NG; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, MT * NG / (MT + NG), 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, MT * NG, 0);
+    __builtin_amdgcn_sched_barrier(0);
   };
   auto step = [&](int8_t* here, int8_t* next, int k0) {
+    fetch(here, 1);
+    multiply(0);
+    // The other half of this stage is in registers, so the stage is free; the next one has landed.
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    __syncthreads();  // every wave's loads of this stage landed; the other stage is free
-    if (k0 + BK < a.K) stage(next, k0 + BK);
-    multiply(here);
+    __syncthreads();
+    if (k0 + 2 * BK < a.K) stage(here, k0 + 2 * BK);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(next, 0);  // behind the last step: LDS bytes that nothing multiplies
+    multiply(1);
   };
   stage(lds0, 0);
+  if (BK < a.K) stage(lds1, BK);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+  __syncthreads();
+  fetch(lds0, 0);
   for (int k0 = 0; k0 < a.K; k0 += 2 * BK) {
     step(lds0, lds1, k0);
     if (k0 + BK < a.K) step(lds1, lds0, k0 + BK);
