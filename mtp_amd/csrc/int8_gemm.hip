@@ -12,6 +12,7 @@
 // holds bytes [16 (l >> 4), 16 (l >> 4) + 16) of row l & 15 of both operands (the same k order on both
 // sides), and channels 4 (l >> 4) .. + 3 of token l & 15 of the result.
 #include <algorithm>
+#include <type_traits>
 
 #include "elem.h"
 #include "int8.h"
@@ -233,53 +234,67 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[g][m] = i32x4{0, 0, 0, 0};
   const int sw0 = (((lane >> 4) ^ (lr & 7)) * 16), sw1 = ((4 + (lane >> 4)) ^ (lr & 7)) * 16;
-  const int fa_at = (wm * MT * 16 + lr) * BK, fb_at = (BM + wn * NG * 16 + lr) * BK;
-  // A step's two halves of 64 bytes of K, pipelined through two register sets: while one half is
-  // multiplied the next one's operands are read from LDS.
-  i32x4 fa[2][MT], fb[2][NG];
-  auto fetch = [&](const int8_t* lds, int half) {
-    const int sw = half ? sw1 : sw0;
+  const int fa_at = (wm * 16 + lr) * BK, fb_at = (BM + wn * NG * 16 + lr) * BK;
+  // The product over K of the first L row groups of each wave (group m of wave wm holds the tile's
+  // rows 16 (m WM + wm) .. + 15, so that a tile's rows spread over its waves).
+  auto product = [&](auto live_c) {
+    constexpr int L = decltype(live_c)::value;
+    // A step's two halves of 64 bytes of K, pipelined through two register sets: while one half is
+    // multiplied the next one's operands are read from LDS.
+    i32x4 fa[2][L], fb[2][NG];
+    auto fetch = [&](const int8_t* lds, int half) {
+      const int sw = half ? sw1 : sw0;
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
-      fb[half][g] = *reinterpret_cast<const i32x4*>(lds + fb_at + g * 16 * BK + sw);
+      for (int g = 0; g < NG; ++g)
+        fb[half][g] = *reinterpret_cast<const i32x4*>(lds + fb_at + g * 16 * BK + sw);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      fa[half][m] = *reinterpret_cast<const i32x4*>(lds + fa_at + m * 16 * BK + sw);
-  };
-  auto multiply = [&](int half) {
+      for (int m = 0; m < L; ++m)
+        fa[half][m] = *reinterpret_cast<const i32x4*>(lds + fa_at + m * WM * 16 * BK + sw);
+    };
+    auto multiply = [&](int half) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < L; ++m)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) acc[g][m] = mfma_i8(fb[half][g], fa[half][m], acc[g][m]);
-    // one LDS read of the next half among every few multiplications of this one
+        for (int g = 0; g < NG; ++g) acc[g][m] = mfma_i8(fb[half][g], fa[half][m], acc[g][m]);
+      // one LDS read of the next half among every few multiplications of this one
+      constexpr int kReads = L + NG, kEach = L * NG / kReads > 0 ? L * NG / kReads : 1;
 #pragma unroll
-    for (int i = 0; i < MT + NG; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, MT * NG / (MT + NG), 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, MT * NG, 0);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  auto step = [&](int8_t* here, int8_t* next, int k0) {
-    fetch(here, 1);
-    multiply(0);
-    // The other half of this stage is in registers, so the stage is free; the next one has landed.
+      for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, L * NG, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](int8_t* here, int8_t* next, int k0) {
+      fetch(here, 1);
+      multiply(0);
+      // The other half of this stage is in registers, so the stage is free; the next has landed.
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      __syncthreads();
+      if (k0 + 2 * BK < a.K) stage(here, k0 + 2 * BK);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(next, 0);  // behind the last step: LDS bytes that nothing multiplies
+      multiply(1);
+    };
+    stage(lds0, 0);
+    if (BK < a.K) stage(lds1, BK);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     __syncthreads();
-    if (k0 + 2 * BK < a.K) stage(here, k0 + 2 * BK);
-    __builtin_amdgcn_sched_barrier(0);
-    fetch(next, 0);  // behind the last step: LDS bytes that nothing multiplies
-    multiply(1);
+    fetch(lds0, 0);
+    for (int k0 = 0; k0 < a.K; k0 += 2 * BK) {
+      step(lds0, lds1, k0);
+      if (k0 + BK < a.K) step(lds1, lds0, k0 + BK);
+    }
   };
-  stage(lds0, 0);
-  if (BK < a.K) stage(lds1, BK);
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-  __syncthreads();
-  fetch(lds0, 0);
-  for (int k0 = 0; k0 < a.K; k0 += 2 * BK) {
-    step(lds0, lds1, k0);
-    if (k0 + BK < a.K) step(lds1, lds0, k0 + BK);
-  }
+  // Tiles of few rows (an expert's last, or all it has) multiply only the groups that hold some.
+  const int live = (tl.rows + 16 * WM - 1) / (16 * WM);
+  if (live <= MT / 4)
+    product(std::integral_constant<int, MT / 4>{});
+  else if (live <= MT / 2)
+    product(std::integral_constant<int, MT / 2>{});
+  else
+    product(std::integral_constant<int, MT>{});
   // Epilogue: 16 rows at a time through the wave's share of LDS, from which a lane stores 16
   // consecutive bytes (whole lines for 64 channels of 16 bits). Stored from the accumulators, with the
   // scales loaded again between the stores, it took 30 us a tile of 256 x 256 instead of 6.
@@ -302,14 +317,14 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   float rs[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int r = (wm * MT + m) * 16 + lr;
+    const int r = (m * WM + wm) * 16 + lr;
     rs[m] = r < tl.rows ? a.a_scale[source_row(a, tl.row0 + r)] : 0.0f;
   }
   __syncthreads();  // the stages have been read
   int8_t* mine = lds0 + wave * 16 * PITCH;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int r0w = (wm * MT + m) * 16;
+    const int r0w = (m * WM + wm) * 16;
     if (r0w >= tl.rows) continue;
 #pragma unroll
     for (int g = 0; g < kOut; ++g) {
