@@ -27,6 +27,12 @@ struct Int8Args {
 // Quantise rows of the dtype to int8 with a scale each.
 hipError_t launch_quantize(const void* x, int T, int K, int dtype, int8_t* q, float* scale,
                            hipStream_t s);
-// Rows per tile for M rows over E experts (the tile table's bm).
-int int8_block_m(int64_t M, int E);
-hipError_t launch_int8_product(const Int8Args& a, int bm, bool silu, int dtype, hipStream_t s);
+// The kernel of a product and its rows per tile (the bm of an expert table).
+enum { kInt8Stream = 0, kInt8Ring = 1, kInt8Tile = 2 };
+struct Int8Plan {
+  int kind, bm;
+};
+Int8Plan int8_experts_plan(int64_t slots, int E);
+Int8Plan int8_matrix_plan(int64_t M, int64_t N);
+hipError_t launch_int8_product(const Int8Args& a, Int8Plan plan, bool silu, int dtype,
+                               hipStream_t s);

@@ -44,22 +44,23 @@ int matmul(const int8_t* q, const float* q_scale, int T, int K, const int8_t* w,
   a.K = K;
   a.out = out;
   a.bias = bias;
-  const int bm = int8_block_m(T, 1);
-  a.m_tiles = (T + bm - 1) / bm;
-  MOE_OP_HIP(launch_int8_product(a, bm, false, dtype, s), "int8 product");
+  const Int8Plan plan = int8_matrix_plan(T, N);
+  a.m_tiles = (T + plan.bm - 1) / plan.bm;
+  MOE_OP_HIP(launch_int8_product(a, plan, false, dtype, s), "int8 product");
   return MOE_OK;
 }
 
 struct ExpertsLayout {
   int64_t q, qs, offsets, row_slot, slot_row, tiles, scratch, h, hq, hs, y, total;
-  int bm, tile_cap;
+  Int8Plan plan;
+  int tile_cap;
 };
 
 ExpertsLayout experts_layout(int T, int k, const moe_int8_set_v1& ex, int dtype) {
   ExpertsLayout L{};
   const int64_t S = (int64_t)T * k, es = dtype_bytes(dtype);
-  L.bm = int8_block_m(S, ex.num_experts);
-  L.tile_cap = (int)(S / L.bm + std::min<int64_t>(S, ex.num_experts));
+  L.plan = int8_experts_plan(S, ex.num_experts);
+  L.tile_cap = (int)(S / L.plan.bm + std::min<int64_t>(S, ex.num_experts));
   int64_t o = 0;
   auto take = [&o](int64_t bytes) {
     const int64_t at = o;
@@ -210,7 +211,7 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
   MOE_OP_HIP(launch_quantize(x, T, H, dtype, q, qs, s), "quantize");
   MOE_OP_HIP(launch_dispatch(topk_ids, T, top_k, E, nullptr, 16, nullptr,
                              at<int32_t>(workspace, L.offsets), row_slot, slot_row,
-                             at<void>(workspace, L.scratch), tiles, L.bm, L.tile_cap, s),
+                             at<void>(workspace, L.scratch), tiles, L.plan.bm, L.tile_cap, s),
              "sort");
   Int8Args a{};
   a.a = q;
@@ -228,7 +229,7 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
   a.N = I;
   a.K = H;
   a.out = h;
-  MOE_OP_HIP(launch_int8_product(a, L.bm, true, dtype, s), "gate and up");
+  MOE_OP_HIP(launch_int8_product(a, L.plan, true, dtype, s), "gate and up");
   // dropped slots' rows of h are never written; what they hold is quantised and not read again
   MOE_OP_HIP(launch_quantize(h, (int)S, I, dtype, hq, hs, s), "quantize h");
   Int8Args b{};
@@ -244,7 +245,7 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
   b.N = H;
   b.K = I;
   b.out = y;
-  MOE_OP_HIP(launch_int8_product(b, L.bm, false, dtype, s), "down");
+  MOE_OP_HIP(launch_int8_product(b, L.plan, false, dtype, s), "down");
   MOE_OP_HIP(launch_combine(y, T, top_k, H, dtype, slot_row, topk_weights, out, s), "combine");
   return MOE_OK;
 }

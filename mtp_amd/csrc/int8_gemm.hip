@@ -168,9 +168,12 @@ __global__ __launch_bounds__(kThreads) void int8_stream_kernel(Int8Args a, int v
 // SiLU: the tile's groups of 16 channels alternate between gate and up, so that a wave holds both
 // sums of a channel in the same lane.
 constexpr int kGroupM = 4;
+// s_waitcnt immediate waiting for lgkmcnt <= 0 only.
+constexpr int kWaitLgkm0 = 15 | (3 << 14) | (0x7 << 4);
 
 template <int BM, int BN, int WM, int WN, int DT, bool SILU>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int vec) {
+  using T = typename Elem<DT>::T;
   constexpr int NT = 64 * WM * WN;
   constexpr int BK = 128;
   constexpr int MT = BM / WM / 16, NG = BN / WN / 16;
@@ -178,23 +181,29 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   static_assert(LA * NT == BM * 8 && LB * NT == BN * 8 && NT % 256 == 0, "whole loads");
   __shared__ __attribute__((aligned(16))) int8_t lds0[(BM + BN) * BK];
   __shared__ __attribute__((aligned(16))) int8_t lds1[(BM + BN) * BK];
+  __shared__ __attribute__((aligned(16))) float s_row[BM], s_col[BN], s_bias[SILU ? 4 : BN];
   const int cols = SILU ? BN / 2 : BN;
   const int blocks_n = (a.N + cols - 1) / cols;
-  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of consecutive tiles. Of one matrix they
-  // run down kGroupM row blocks before the next channels, so that the 32 tiles an XCD works on at a
-  // time are about 4 x 8 and share their operands in its L2; of experts they run along the channels.
-  const int m_tiles = a.tiles ? __builtin_amdgcn_readfirstlane(a.tiles[a.m_tiles][0]) : a.m_tiles;
-  const int total = m_tiles * blocks_n, per = (total + 7) / 8;
-  const int idx = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + idx;
-  if (idx >= per || id >= total) return;
-  int tile_m = id / blocks_n, tile_n = id % blocks_n;
-  if (!a.tiles) {
+  // Workgroups go to the 8 XCDs in turn. Of one matrix each XCD takes a run of consecutive tiles,
+  // down kGroupM row blocks before the next channels, so that the 32 tiles it works on at a time are
+  // about 4 x 8 and share their operands in its L2. Of experts each XCD takes every eighth row block,
+  // all its channels in a row.
+  const int idx = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+  int tile_m, tile_n;
+  if (a.tiles) {
+    tile_m = idx / blocks_n * 8 + xcd;
+    tile_n = idx % blocks_n;
+    if (tile_m >= a.m_tiles) return;
+  } else {
+    const int total = a.m_tiles * blocks_n, per = (total + 7) / 8, id = xcd * per + idx;
+    if (idx >= per || id >= total) return;
     const int group = id / (kGroupM * blocks_n), in = id - group * kGroupM * blocks_n;
-    const int rows = min(kGroupM, m_tiles - group * kGroupM);
+    const int rows = min(kGroupM, a.m_tiles - group * kGroupM);
     tile_m = group * kGroupM + in % rows;
     tile_n = in / rows;
   }
   const Tile tl = tile_of(a, BM, tile_m);
+  if (tl.rows <= 0) return;
   const int n0 = tile_n * cols;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -228,6 +237,17 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
     for (int j = 0; j < LB; ++j)
       buf_ld128_lds(rb, lds + BM * BK + (j * NT + wave * 64) * 16, boff[j] | out, (uint32_t)k0);
   };
+  // the epilogue's scales, loaded now: a dependent chain of loads there would be waited for
+  const int64_t sb = (int64_t)tl.expert * a.N;
+#pragma unroll
+  for (int r = tid; r < BM; r += NT)
+    s_row[r] = r < tl.rows ? a.a_scale[source_row(a, tl.row0 + r)] : 0.0f;
+#pragma unroll
+  for (int i = tid; i < BN; i += NT) {
+    const int n = min(n0 + (SILU ? (i >> 5) * 16 + (i & 15) : i), a.N - 1);
+    s_col[i] = (SILU && (i & 16) ? a.s1 : a.s0)[sb + n];
+    if (!SILU && a.bias) s_bias[i] = Elem<DT>::get(static_cast<const T*>(a.bias)[n]);
+  }
   i32x4 acc[NG][MT];
 #pragma unroll
   for (int g = 0; g < NG; ++g)
@@ -289,36 +309,25 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   };
   // Tiles of few rows (an expert's last, or all it has) multiply only the groups that hold some.
   const int live = (tl.rows + 16 * WM - 1) / (16 * WM);
-  if (live <= MT / 4)
-    product(std::integral_constant<int, MT / 4>{});
-  else if (live <= MT / 2)
-    product(std::integral_constant<int, MT / 2>{});
+  if (MT >= 4 && live <= MT / 4)
+    product(std::integral_constant<int, (MT >= 4 ? MT / 4 : 1)>{});
+  else if (MT >= 2 && live <= MT / 2)
+    product(std::integral_constant<int, (MT >= 2 ? MT / 2 : 1)>{});
   else
     product(std::integral_constant<int, MT>{});
   // Epilogue: 16 rows at a time through the wave's share of LDS, from which a lane stores 16
   // consecutive bytes (whole lines for 64 channels of 16 bits). Stored from the accumulators, with the
   // scales loaded again between the stores, it took 30 us a tile of 256 x 256 instead of 6.
-  using T = typename Elem<DT>::T;
   constexpr int kOut = SILU ? NG / 2 : NG;
   constexpr int CH = kOut * 16, PITCH = CH * (int)sizeof(T) + 16;  // channels a wave, bytes a row
   static_assert(NT / 64 * 16 * PITCH <= (BM + BN) * BK, "the rows fit a stage");
   const int n_wave = n0 + wn * CH, lk4 = (lane >> 4) * 4;
-  const int64_t sb = (int64_t)tl.expert * a.N;
-  float sc[kOut][4], sc1[kOut][4], bias[kOut][4];
+  f32x4 sc[NG], bias[NG];
 #pragma unroll
-  for (int g = 0; g < kOut; ++g)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = min(n_wave + g * 16 + lk4 + i, a.N - 1);
-      sc[g][i] = a.s0[sb + n];
-      if constexpr (SILU) sc1[g][i] = a.s1[sb + n];
-      bias[g][i] = !SILU && a.bias ? Elem<DT>::get(static_cast<const T*>(a.bias)[n]) : 0.0f;
-    }
-  float rs[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int r = (m * WM + wm) * 16 + lr;
-    rs[m] = r < tl.rows ? a.a_scale[source_row(a, tl.row0 + r)] : 0.0f;
+  for (int g = 0; g < NG; ++g) {
+    const int i = wn * NG * 16 + g * 16 + lk4;
+    sc[g] = *reinterpret_cast<const f32x4*>(s_col + i);
+    if (!SILU && a.bias) bias[g] = *reinterpret_cast<const f32x4*>(s_bias + i);
   }
   __syncthreads();  // the stages have been read
   int8_t* mine = lds0 + wave * 16 * PITCH;
@@ -326,14 +335,15 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   for (int m = 0; m < MT; ++m) {
     const int r0w = (m * WM + wm) * 16;
     if (r0w >= tl.rows) continue;
+    const float rs = s_row[r0w + lr];
 #pragma unroll
     for (int g = 0; g < kOut; ++g) {
       T v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float f = ((float)acc[SILU ? 2 * g : g][m][i] * rs[m]) * sc[g][i];
+        float f = ((float)acc[SILU ? 2 * g : g][m][i] * rs) * sc[SILU ? 2 * g : g][i];
         if constexpr (SILU)
-          f = silu_f32(f) * (((float)acc[2 * g + 1][m][i] * rs[m]) * sc1[g][i]);
+          f = silu_f32(f) * (((float)acc[2 * g + 1][m][i] * rs) * sc[2 * g + 1][i]);
         else if (a.bias)
           f += bias[g][i];
         v[i] = Elem<DT>::put(f);
@@ -347,12 +357,12 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
     if (vec) {
       constexpr int kVec = 16 / (int)sizeof(T), kPerRow = CH / kVec;  // lanes a row
 #pragma unroll
-      for (int q = 0; q < 16 * kPerRow / 64; ++q) {
+      for (int q = 0; q < (16 * kPerRow + 63) / 64; ++q) {
         const int row = (q * 64 + lane) / kPerRow, c = (lane % kPerRow) * kVec;
-        const u32x4 d = *reinterpret_cast<const u32x4*>(mine + row * PITCH + c * sizeof(T));
-        if (r0w + row < tl.rows && n_wave + c < a.N)
+        if (row < 16 && r0w + row < tl.rows && n_wave + c < a.N)
           *reinterpret_cast<u32x4*>(static_cast<T*>(a.out) + (int64_t)(tl.row0 + r0w + row) * a.N +
-                                    n_wave + c) = d;
+                                    n_wave + c) =
+              *reinterpret_cast<const u32x4*>(mine + row * PITCH + c * sizeof(T));
       }
     } else {
       for (int row = 0; row < 16 && r0w + row < tl.rows; ++row)
@@ -371,52 +381,248 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
 template <int BM, int BN, int WM, int WN, int DT, bool SILU>
 hipError_t launch_tile(const Int8Args& a, int vec, hipStream_t s) {
   const int cols = SILU ? BN / 2 : BN;
-  const int64_t tiles = (int64_t)((a.N + cols - 1) / cols) * a.m_tiles;
-  const int64_t blocks = (tiles + 7) / 8 * 8;
+  const int64_t blocks_n = (a.N + cols - 1) / cols;
+  const int64_t blocks =
+      a.tiles ? (a.m_tiles + 7) / 8 * 8 * blocks_n : (a.m_tiles * blocks_n + 7) / 8 * 8;
   if (blocks > kMaxBlocks / 2) return hipErrorInvalidValue;
   hipLaunchKernelGGL((int8_tile_kernel<BM, BN, WM, WN, DT, SILU>), dim3((unsigned)blocks),
                      dim3(64 * WM * WN), 0, s, a, vec);
   return hipGetLastError();
 }
 
-template <int DT, bool SILU>
-hipError_t launch_product(const Int8Args& a, int bm, int vec, hipStream_t s) {
-  const int wide = a.N % (DT == kFp32 ? 4 : 8) == 0 && aligned16(a.out);
-  if (bm == 256) return launch_tile<256, 256, 2, 4, DT, SILU>(a, wide, s);
-  if (bm == 128) return launch_tile<128, 256, 2, 4, DT, SILU>(a, wide, s);
-  const int cols = SILU ? 32 : 64;
-  const int64_t blocks = (int64_t)((a.N + cols - 1) / cols) * a.m_tiles;
+// ---------------------------------------------------------------- few tiles
+// One matrix whose tiles do not fill the chip: a workgroup has its CU to itself and streams its
+// weights at what it keeps in flight. BM rows x BN channels on WM x WN waves, both operands through LDS
+// as in the tile kernel, in a ring of four stages of 128 bytes of K, three of them in flight. The
+// steps are made a multiple of four (steps past K load zeros without a memory access), so that the
+// ring's places are fixed arrays and the loads in flight always as many. Weights are not loaded
+// straight into the registers the MFMA reads: 16 lanes then touch 16 lines, which passes 36 GB/s a
+// CU (measured, L2-resident); rows of 128 bytes pass 100 GB/s.
+constexpr int kRing = 4;
+
+template <int BM, int BN, int WM, int WN, int DT>
+__global__ __launch_bounds__(kThreads) void int8_ring_kernel(Int8Args a, int vec) {
+  static_assert(WM * WN == kWaves, "four waves");
+  using T = typename Elem<DT>::T;
+  constexpr int BK = 128;
+  constexpr int MT = BM / WM / 16, NG = BN / WN / 16;
+  constexpr int LA = BM * 8 / kThreads, LB = BN * 8 / kThreads;  // 16-byte loads a thread and step
+  constexpr int PITCH = BN * (int)sizeof(T) + 16, kRows = 16 * WM;
+  constexpr int kStage = (BM + BN) * BK;
+  // separate arrays: the compiler then knows which stage a load to LDS writes
+  __shared__ __attribute__((aligned(16))) int8_t lds0[kStage];
+  __shared__ __attribute__((aligned(16))) int8_t lds1[kStage];
+  __shared__ __attribute__((aligned(16))) int8_t lds2[kStage];
+  __shared__ __attribute__((aligned(16))) int8_t lds3[kStage];
+  __shared__ __attribute__((aligned(16))) int8_t lds_out[kRows * PITCH];
+  __shared__ float s_scale[BM];  // the rows' scales
+  const int blocks_n = (a.N + BN - 1) / BN;
+  const Tile tl{0, (int)blockIdx.x / blocks_n * BM, min(BM, a.M - (int)blockIdx.x / blocks_n * BM)};
+  const int n0 = (int)blockIdx.x % blocks_n * BN;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int lr = lane & 15, lk4 = (lane >> 4) * 4;
+  const __amdgpu_buffer_rsrc_t ra = buf_rsrc(a.a, a.a_bytes);
+  const __amdgpu_buffer_rsrc_t rb = buf_rsrc(a.b0, (uint32_t)((int64_t)a.N * a.K));
+  const uint32_t kc = (uint32_t)((tid & 7) ^ ((tid >> 3) & 7)) * 16;  // the chunk's byte of K
+  uint32_t aoff[LA], boff[LB];
+#pragma unroll
+  for (int j = 0; j < LA; ++j) {
+    const int r = (j * kThreads + tid) / 8;
+    aoff[j] = r < tl.rows ? (uint32_t)(tl.row0 + r) * (uint32_t)a.K + kc : kOutOfRange;
+  }
+#pragma unroll
+  for (int j = 0; j < LB; ++j) {
+    const int i = (j * kThreads + tid) / 8;
+    boff[j] = n0 + i < a.N ? (uint32_t)(n0 + i) * (uint32_t)a.K + kc : kOutOfRange;
+  }
+  auto stage = [&](int8_t* lds, int k0) {
+    const uint32_t out = k0 + (int)kc < a.K ? 0u : kOutOfRange;  // zeros past K
+#pragma unroll
+    for (int j = 0; j < LB; ++j)
+      buf_ld128_lds(rb, lds + BM * BK + (j * kThreads + wave * 64) * 16, boff[j] | out, (uint32_t)k0);
+#pragma unroll
+    for (int j = 0; j < LA; ++j)
+      buf_ld128_lds(ra, lds + (j * kThreads + wave * 64) * 16, aoff[j] | out, (uint32_t)k0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (tid < BM)
+    s_scale[tid] = tid < tl.rows ? a.a_scale[tl.row0 + tid] : 0.0f;
+  const int sw0 = (((lane >> 4) ^ (lr & 7)) * 16), sw1 = ((4 + (lane >> 4)) ^ (lr & 7)) * 16;
+  const int fa_at = (wm * 16 + lr) * BK, fb_at = (BM + wn * NG * 16 + lr) * BK;
+  // The barrier without __syncthreads' release fence, which would wait for every load to LDS: this
+  // wave's LDS accesses ahead of it are waited for, and the compiler keeps accesses on their sides.
+  auto barrier = [] {
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  i32x4 acc[NG][MT], fa[2][MT], fb[2][NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[g][m] = i32x4{0, 0, 0, 0};
+  auto fetch = [&](const int8_t* lds, int half) {
+    const int sw = half ? sw1 : sw0;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      fb[half][g] = *reinterpret_cast<const i32x4*>(lds + fb_at + g * 16 * BK + sw);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      fa[half][m] = *reinterpret_cast<const i32x4*>(lds + fa_at + m * WM * 16 * BK + sw);
+  };
+  auto multiply = [&](int half) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) acc[g][m] = mfma_i8(fb[half][g], fa[half][m], acc[g][m]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](int8_t* here, int8_t* next, int k0) {
+    fetch(here, 1);
+    multiply(0);
+    // This wave's loads of the next stage have landed (the two stages after it stay in flight);
+    // behind the barrier everybody's have, and this stage, all of it in registers, is free.
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm((kRing - 2) * (LA + LB)));
+    barrier();
+    stage(here, k0 + kRing * BK);
+    fetch(next, 0);  // behind the last step: zeros that nothing multiplies
+    multiply(1);
+  };
+  stage(lds0, 0);
+  stage(lds1, BK);
+  stage(lds2, 2 * BK);
+  stage(lds3, 3 * BK);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm((kRing - 1) * (LA + LB)));
+  barrier();
+  fetch(lds0, 0);
+#pragma unroll 1
+  for (int k0 = 0; k0 < a.K; k0 += kRing * BK) {
+    step(lds0, lds1, k0);
+    step(lds1, lds2, k0 + BK);
+    step(lds2, lds3, k0 + 2 * BK);
+    step(lds3, lds0, k0 + 3 * BK);
+  }
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no load to LDS may outlive the workgroup
+  // Results 16 WM rows at a time through LDS, from which a thread stores 16 consecutive bytes.
+  const int n_wave = wn * NG * 16 + lk4;  // in the tile
+  float sc[NG][4], bias[NG][4];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = min(n0 + n_wave + g * 16 + i, a.N - 1);
+      sc[g][i] = a.s0[n];
+      bias[g][i] = a.bias ? Elem<DT>::get(static_cast<const T*>(a.bias)[n]) : 0.0f;
+    }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m * kRows >= tl.rows) break;  // the same for the whole workgroup
+    if (m > 0) __syncthreads();       // the rows before these have been read
+    const float rs = s_scale[(m * WM + wm) * 16 + lr];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      T v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f = ((float)acc[g][m][i] * rs) * sc[g][i];
+        if (a.bias) f += bias[g][i];
+        v[i] = Elem<DT>::put(f);
+      }
+      __builtin_memcpy(__builtin_assume_aligned(
+                           lds_out + (wm * 16 + lr) * PITCH + (n_wave + g * 16) * sizeof(T), 8),
+                       v, sizeof(v));
+    }
+    __syncthreads();
+    const int64_t first = (int64_t)tl.row0 + m * kRows;
+    const int rows = min(kRows, tl.rows - m * kRows);
+    if (vec) {
+      constexpr int kVec = 16 / (int)sizeof(T), kPerRow = BN / kVec;  // threads a row
+#pragma unroll
+      for (int q = 0; q < (kRows * kPerRow + kThreads - 1) / kThreads; ++q) {
+        const int i = q * kThreads + tid, row = i / kPerRow, c = i % kPerRow * kVec;
+        if (row < rows && n0 + c < a.N)
+          *reinterpret_cast<u32x4*>(static_cast<T*>(a.out) + (first + row) * a.N + n0 + c) =
+              *reinterpret_cast<const u32x4*>(lds_out + row * PITCH + c * sizeof(T));
+      }
+    } else {
+#pragma unroll 1
+      for (int i = tid; i < rows * BN; i += kThreads) {
+        const int row = i / BN, c = i % BN;
+        if (n0 + c < a.N)
+          static_cast<T*>(a.out)[(first + row) * a.N + n0 + c] =
+              *reinterpret_cast<const T*>(lds_out + row * PITCH + c * sizeof(T));
+      }
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int DT>
+hipError_t launch_ring(const Int8Args& a, int vec, hipStream_t s) {
+  const int64_t blocks = (int64_t)((a.N + BN - 1) / BN) * a.m_tiles;
   if (blocks > kMaxBlocks) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks);
-#define MOE_INT8_STREAM(MT)                                                                   \
-  hipLaunchKernelGGL((int8_stream_kernel<MT, DT, SILU>), grid, dim3(kThreads), 0, s, a, vec)
-  if (bm == 16) MOE_INT8_STREAM(1);
-  else if (bm == 32) MOE_INT8_STREAM(2);
-  else MOE_INT8_STREAM(4);
-#undef MOE_INT8_STREAM
+  hipLaunchKernelGGL((int8_ring_kernel<BM, BN, WM, WN, DT>), dim3((unsigned)blocks),
+                     dim3(kThreads), 0, s, a, vec);
   return hipGetLastError();
 }
 
+template <int DT, bool SILU>
+hipError_t launch_product(const Int8Args& a, Int8Plan plan, int vec, hipStream_t s) {
+  const int wide = a.N % (DT == kFp32 ? 4 : 8) == 0 && aligned16(a.out);
+  if (plan.kind == kInt8Tile) {
+    if (plan.bm == 256) return launch_tile<256, 256, 2, 4, DT, SILU>(a, wide, s);
+    if (plan.bm == 128) return launch_tile<128, 128, 2, 2, DT, SILU>(a, wide, s);
+    return launch_tile<64, 128, 2, 2, DT, SILU>(a, wide, s);
+  }
+  if constexpr (!SILU) {
+    if (plan.kind == kInt8Ring)
+      return plan.bm == 32 ? launch_ring<32, 64, 2, 2, DT>(a, wide, s)
+                           : launch_ring<64, 64, 2, 2, DT>(a, wide, s);
+    const int64_t blocks = (int64_t)((a.N + 63) / 64) * a.m_tiles;
+    if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((int8_stream_kernel<1, DT, SILU>), dim3((unsigned)blocks), dim3(kThreads), 0,
+                       s, a, vec);
+    return hipGetLastError();
+  }
+  return hipErrorInvalidValue;
+}
+
 template <int DT>
-hipError_t launch_product_t(const Int8Args& a, int bm, bool silu, hipStream_t s) {
+hipError_t launch_product_t(const Int8Args& a, Int8Plan plan, bool silu, hipStream_t s) {
   const int es = DT == kFp32 ? 4 : 2;
   const int vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (uintptr_t)(4 * es - 1)) == 0;
-  return silu ? launch_product<DT, true>(a, bm, vec, s) : launch_product<DT, false>(a, bm, vec, s);
+  return silu ? launch_product<DT, true>(a, plan, vec, s)
+              : launch_product<DT, false>(a, plan, vec, s);
 }
 
 }  // namespace
 
-int int8_block_m(int64_t M, int E) {
-  const int64_t rows = (M + E - 1) / E;
-  if (rows <= 16) return 16;
-  if (rows <= 32) return 32;
-  if (rows <= 64) return 64;
-  return rows <= 512 ? 128 : 256;
+// Rows a tile by the rows an expert has on average, whatever the shapes (hidden 2048, intermediate
+// 512, 256 experts, top-8, us a layer with tiles of 64 / 128 / 256 rows): 512 tokens 184 / 191 / 207,
+// 2048 tokens 248 / 244 / 261, 4096 tokens 349 / 320 / 328, 8192 tokens 564 / 489 / 458.
+Int8Plan int8_experts_plan(int64_t slots, int E) {
+  const int64_t rows = (slots + E - 1) / E;
+  return Int8Plan{kInt8Tile, rows <= 48 ? 64 : rows < 192 ? 128 : 256};
 }
 
-hipError_t launch_int8_product(const Int8Args& a, int bm, bool silu, int dtype, hipStream_t s) {
+// One matrix: the larger the tile the fewer bytes a product moves, the smaller the more workgroups
+// there are. By the number of 64 x 128 tiles (us, 4096 x 8192 channels, ring / 64 / 128 / 256 rows):
+// 256 tiles 17 / 22 / 25 / 43, 512 30 / 25 / 28 / 45, 1024 55 / 48 / 38 / 48, 2048 107 / 81 / 70 / 57.
+Int8Plan int8_matrix_plan(int64_t M, int64_t N) {
+  if (M <= 16) return Int8Plan{kInt8Stream, 16};
+  const int64_t tiles = (M + 63) / 64 * ((N + 127) / 128);
+  if (tiles <= 256) return Int8Plan{kInt8Ring, M <= 64 ? 32 : 64};
+  return Int8Plan{kInt8Tile, tiles <= 768 ? 64 : tiles <= 1408 ? 128 : 256};
+}
+
+hipError_t launch_int8_product(const Int8Args& a, Int8Plan plan, bool silu, int dtype,
+                               hipStream_t s) {
   if (a.m_tiles <= 0) return hipSuccess;
-  if (dtype == kBf16) return launch_product_t<kBf16>(a, bm, silu, s);
-  if (dtype == kFp16) return launch_product_t<kFp16>(a, bm, silu, s);
-  return launch_product_t<kFp32>(a, bm, silu, s);
+  if (dtype == kBf16) return launch_product_t<kBf16>(a, plan, silu, s);
+  if (dtype == kFp16) return launch_product_t<kFp16>(a, plan, silu, s);
+  return launch_product_t<kFp32>(a, plan, silu, s);
 }
