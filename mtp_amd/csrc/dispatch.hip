@@ -26,6 +26,9 @@ constexpr int kMaxE = 512;
 
 MOE_DEV int key_of(int id, int E) { return (unsigned)id < (unsigned)E ? id : E; }
 
+// Orders as (key, slot) does: keys up to 512, slots below 2^22.
+MOE_DEV uint32_t pair_of(int key, int slot) { return ((uint32_t)key << 22) | (uint32_t)slot; }
+
 struct SortOut {
   int32_t* offsets;   // [E + 1]
   int32_t* row_slot;  // [T * k]
@@ -91,8 +94,8 @@ MOE_DEV void write_tables(const int* cnt, int E, int32_t* offsets, i32x4* tiles,
 }
 
 // ---------------------------------------------------------------- few slots: one launch
-// Workgroup (t, y): every thread compares its share of all keys with the token's k keys; the
-// ballots' population counts are the rows. S keys per workgroup from L2 instead of two further
+// Workgroup (t, y): every thread compares its share of all (key, slot) pairs with the token's k; the
+// ballots' population counts are the rows. S ids per workgroup from L2 instead of two further
 // launches. Workgroup (T, 0) counts the experts' slots for the tables.
 template <typename U>
 __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
@@ -114,18 +117,20 @@ __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
   }
   const int t = blockIdx.x;
   for (int i0 = 0; i0 < k; i0 += 8) {
-    int key[8], cnt[8];
+    uint32_t mine[8];
+    int cnt[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      key[j] = i0 + j < k ? key_of(ids[t * k + i0 + j], E) : -1;
+      const int f = t * k + i0 + j;
+      mine[j] = i0 + j < k ? pair_of(key_of(ids[f], E), f) : 0u;
       cnt[j] = 0;
     }
+#pragma unroll 2
     for (int s0 = wave * 64; s0 < S; s0 += kThreads) {
       const int s = s0 + lane;
-      const int kk = s < S ? key_of(ids[s], E) : E + 1;
+      const uint32_t pair = s < S ? pair_of(key_of(ids[s], E), s) : ~0u;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        cnt[j] += __popcll(__ballot(kk < key[j] || (kk == key[j] && s < t * k + i0 + j)));
+      for (int j = 0; j < 8; ++j) cnt[j] += __popcll(__ballot(pair < mine[j]));
     }
     if (lane == 0) {
 #pragma unroll
@@ -279,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void dispatch_copy_kernel(
 }
 
 // Slots up to which every workgroup ranks its token's slots itself.
-constexpr int kSmallSlots = 2048;
+constexpr int kSmallSlots = 4096;
 
 template <typename U>
 hipError_t launch_dispatch_units(const int32_t* ids, int T, int k, int E, const void* x,
@@ -311,46 +316,43 @@ hipError_t launch_dispatch_units(const int32_t* ids, int T, int k, int E, const 
 }
 
 // ---------------------------------------------------------------- combine
-// Thread = 8 columns (VEC) or one column of a token. Slots are taken 8 at a time, all their loads
-// in flight together; dropped slots (and slot_row entries outside the rows) read row 0 and count
-// as +0 by a bit mask, so that nothing a dropped row holds reaches the sum.
-template <int DT, bool VEC, bool WEIGHTED>
+// NT threads a token (a wave, or the workgroup) and 8 NT of its columns. Slots are taken 8 at a time,
+// all their loads in flight together; a dropped slot (and a slot_row entry outside the rows) reads
+// row 0 and does not count, so that nothing a dropped row holds reaches the sum.
+template <int DT, int NT, bool VEC, bool WEIGHTED>
 __global__ __launch_bounds__(kThreads) void combine_kernel(
-    const typename Elem<DT>::T* __restrict__ rows, int S, int T, int k, int H,
+    const typename Elem<DT>::T* __restrict__ rows, int T, int k, int H,
     const int32_t* __restrict__ slot_row, const float* __restrict__ w,
     typename Elem<DT>::T* __restrict__ out) {
-  constexpr int N = VEC ? 8 : 1;
-  const int per = VEC ? H / 8 : H;
-  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t t = idx / per;
+  using C = Cols<DT, NT, VEC>;
+  const int tid = threadIdx.x % NT, c = blockIdx.y * 8 * NT;
+  const int64_t t = (int64_t)blockIdx.x * (kThreads / NT) +
+                    __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
   if (t >= T) return;
-  const int c = (int)(idx - t * per) * N;
-  float s[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) s[j] = 0.0f;
+  const int S = T * k;
+  float s[8] = {};
   for (int i0 = 0; i0 < k; i0 += 8) {
-    float wt[8], v[8][N];
+    float wt[8], v[8][8];
     bool ok[8];
+    int row[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const bool in = i0 + i < k;
       const int64_t f = t * k + (in ? i0 + i : 0);
       const int r = slot_row[f];
       ok[i] = in && (unsigned)r < (unsigned)S;
+      row[i] = ok[i] ? r : 0;
       wt[i] = WEIGHTED ? w[f] : 1.0f;
-      const typename Elem<DT>::T* p = rows + (int64_t)(ok[i] ? r : 0) * H + c;
-      if constexpr (VEC) ld8<DT>(p, v[i]);
-      else v[i][0] = Elem<DT>::get(*p);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) C::load(rows + (int64_t)row[i] * H + c, tid, H - c, v[i]);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < N; ++j)
+      for (int j = 0; j < 8; ++j)
         s[j] = ok[i] ? __builtin_fmaf(wt[i], v[i][j], s[j]) : s[j];
   }
-  typename Elem<DT>::T* p = out + t * H + c;
-  if constexpr (VEC) st8<DT>(p, s);
-  else *p = Elem<DT>::put(s[0]);
+  C::store(out + t * H + c, tid, H - c, s);
 }
 
 // NT threads a token (a wave, or the workgroup). d rows from the token's d out, and the slots' dot
@@ -435,26 +437,25 @@ hipError_t launch_combine_t(const void* rows, int T, int k, int H, const int32_t
   const E* r = static_cast<const E*>(rows);
   E* o = static_cast<E*>(out);
   const bool vec = H % 8 == 0 && aligned16(rows) && aligned16(out);
-  const int per = vec ? H / 8 : H;
-  // one launch holds under 2^31 threads
-  const int step = (int)std::min<int64_t>(T, (int64_t(1) << 30) / per);
-  for (int t0 = 0; t0 < T; t0 += step) {
-    const int n = std::min(step, T - t0);
-    const dim3 grid((unsigned)(((int64_t)n * per + kThreads - 1) / kThreads));
-    const int32_t* sr = slot_row + (int64_t)t0 * k;
-    const float* wt = w ? w + (int64_t)t0 * k : nullptr;
-#define MOE_COMBINE(V, W)                                                                         \
-  hipLaunchKernelGGL((combine_kernel<DT, V, W>), grid, dim3(kThreads), 0, s, r, T * k, n, k, H, sr, \
-                     wt, o + (int64_t)t0 * H)
-    if (vec) {
-      if (w) MOE_COMBINE(true, true);
-      else MOE_COMBINE(true, false);
-    } else {
-      if (w) MOE_COMBINE(false, true);
-      else MOE_COMBINE(false, false);
-    }
-#undef MOE_COMBINE
+#define MOE_COMBINE(NT, V, W)                                                                   \
+  hipLaunchKernelGGL((combine_kernel<DT, NT, V, W>),                                            \
+                     dim3((unsigned)((T + kThreads / NT - 1) / (kThreads / NT)),                \
+                          (unsigned)((H + 8 * NT - 1) / (8 * NT))),                             \
+                     dim3(kThreads), 0, s, r, T, k, H, slot_row, w, o)
+#define MOE_COMBINE_W(NT, V)        \
+  do {                              \
+    if (w) MOE_COMBINE(NT, V, true); \
+    else MOE_COMBINE(NT, V, false); \
+  } while (0)
+  if (H <= 1024) {
+    if (vec) MOE_COMBINE_W(64, true);
+    else MOE_COMBINE_W(64, false);
+  } else {
+    if (vec) MOE_COMBINE_W(256, true);
+    else MOE_COMBINE_W(256, false);
   }
+#undef MOE_COMBINE_W
+#undef MOE_COMBINE
   return hipGetLastError();
 }
 

@@ -67,17 +67,18 @@ MOE_DEV void st8(typename Elem<DT>::T* p, const float (&v)[8]) {
 template <int DT, int NT, bool VEC>
 struct Cols {
   using T = typename Elem<DT>::T;
+  // Without branches: a thread outside the row reads columns inside it and drops them (in branches
+  // every load was waited for before the next was issued).
   MOE_DEV static void load(const T* row, int tid, int H, float (&v)[8]) {
     if constexpr (VEC) {
-      if (8 * tid < H) {
-        ld8<DT>(row + 8 * tid, v);
-      } else {
+      ld8<DT>(row + min(8 * tid, H - 8), v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      }
+      for (int e = 0; e < 8; ++e) v[e] = 8 * tid < H ? v[e] : 0.0f;
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = tid + NT * e < H ? Elem<DT>::get(row[tid + NT * e]) : 0.0f;
+      for (int e = 0; e < 8; ++e) v[e] = Elem<DT>::get(row[min(tid + NT * e, H - 1)]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tid + NT * e < H ? v[e] : 0.0f;
     }
   }
   MOE_DEV static void store(T* row, int tid, int H, const float (&v)[8]) {
@@ -90,6 +91,42 @@ struct Cols {
     }
   }
   MOE_DEV static int col(int tid, int e) { return VEC ? 8 * tid + e : tid + NT * e; }
+};
+
+// The same columns as the registers they are loaded into, unpacked where they are used: half the
+// registers of floats, for rows whose loads run ahead of their use.
+template <int DT, int NT, bool VEC>
+struct RawCols {
+  using T = typename Elem<DT>::T;
+  using C = Cols<DT, NT, VEC>;
+  static constexpr int kWords = VEC ? 2 * (int)sizeof(T) : 8;
+  uint32_t w[kWords];
+  MOE_DEV void load(const T* row, int tid, int H) {
+    if constexpr (VEC) {
+      const T* p = row + min(8 * tid, H - 8);
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const u32x4 d = ld128(reinterpret_cast<const u32x4*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * i + j] = d[j];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const T v = row[min(tid + NT * e, H - 1)];
+        if constexpr (DT == kFp32) w[e] = __float_as_uint(v);
+        else w[e] = v;
+      }
+    }
+  }
+  // column e of the thread; 0 outside the row
+  MOE_DEV float get(int e, int tid, int H) const {
+    float v;
+    if constexpr (DT == kFp32) v = __uint_as_float(w[e]);
+    else if constexpr (VEC) v = Elem<DT>::get((T)(w[e / 2] >> (16 * (e & 1))));
+    else v = Elem<DT>::get((T)w[e]);
+    return C::col(tid, e) < H ? v : 0.0f;
+  }
 };
 
 // The value as it reads back after being stored in the type.

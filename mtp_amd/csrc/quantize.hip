@@ -101,6 +101,7 @@ hipError_t launch_quantize_t(const void* x, int T, int K, int8_t* q, float* scal
   } while (0)
   if (K <= 512) MOE_QUANT(64, 1);
   else if (K <= 2048) MOE_QUANT(256, 1);
+  else if (K <= 4096) MOE_QUANT(256, 2);
   else if (K <= 8192) MOE_QUANT(256, 4);
   else MOE_QUANT(1024, 8);
 #undef MOE_QUANT
