@@ -24,6 +24,42 @@ struct Int8Args {
   const void* bias;       // [N] or NULL
 };
 
+// Symmetric quantisation of a row of values whose largest magnitude has the bits `top` (NaN above
+// infinity): q = rint(127 x / a). 127 x is exact for bf16 and fp16 values (8 and 11 bits by 7) and an
+// IEEE division then rounds only once: a quotient that is a tie is represented, and one that is not
+// lies further from the tie than the division's half step, so q equals that of exact arithmetic
+// (ties to even). Rows are scaled by a power of two first, where 127 x could overflow or the
+// quotient's operands be subnormal. A row of zeros, and one that holds an infinity or NaN, gives 0.
+struct Quantizer {
+  float f, d;
+  MOE_DEV explicit Quantizer(uint32_t top) {
+    const float a = __uint_as_float(top);
+    const bool usable = top != 0 && top < 0x7F800000u;
+    const float m = a >= 0x1p64f ? 0x1p-64f : a < 0x1p-64f ? 0x1p64f : 1.0f;
+    f = usable ? m : 0.0f;
+    d = usable ? a * m : 1.0f;
+  }
+  MOE_DEV int operator()(float x) const {
+    const float n = f == 0.0f ? 0.0f : x * f * 127.0f;
+    return (int)__builtin_rintf(n / d);
+  }
+  // a / 127: inf or NaN for rows that hold one, so that their products are NaN
+  MOE_DEV static float scale(uint32_t top) { return __uint_as_float(top) / 127.0f; }
+};
+MOE_DEV uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+MOE_DEV uint32_t pack_i8x4(int b0, int b1, int b2, int b3) {
+  return (uint32_t)(b0 & 255) | (uint32_t)(b1 & 255) << 8 | (uint32_t)(b2 & 255) << 16 |
+         (uint32_t)(b3 & 255) << 24;
+}
+MOE_DEV uint32_t bfly_umax(uint32_t v) {
+  v = max(v, __float_as_uint(xor_partner<32>(__uint_as_float(v))));
+  v = max(v, __float_as_uint(xor_partner<16>(__uint_as_float(v))));
+  v = max(v, __float_as_uint(xor_partner<8>(__uint_as_float(v))));
+  v = max(v, __float_as_uint(xor_partner<4>(__uint_as_float(v))));
+  v = max(v, __float_as_uint(xor_partner<2>(__uint_as_float(v))));
+  return max(v, __float_as_uint(xor_partner<1>(__uint_as_float(v))));
+}
+
 // Quantise rows of the dtype to int8 with a scale each.
 hipError_t launch_quantize(const void* x, int T, int K, int dtype, int8_t* q, float* scale,
                            hipStream_t s);
@@ -36,3 +72,7 @@ Int8Plan int8_experts_plan(int64_t slots, int E);
 Int8Plan int8_matrix_plan(int64_t M, int64_t N);
 hipError_t launch_int8_product(const Int8Args& a, Int8Plan plan, bool silu, int dtype,
                                hipStream_t s);
+// The product of few rows of the dtype, quantised by the product's own workgroups (a's int8 rows and
+// scales are not looked at): one launch, no workspace.
+bool int8_fused_fits(int M, int K);
+hipError_t launch_int8_fused(const Int8Args& a, const void* x, int dtype, hipStream_t s);

@@ -140,6 +140,7 @@ int moe_int8_matmul_v1(const int8_t* q, const float* q_scale, int32_t T, int32_t
 
 int64_t moe_int8_linear_workspace_bytes_v1(int32_t T, int32_t K) {
   if (T < 0 || K < 1) return -1;
+  if (T == 0 || int8_fused_fits(T, K)) return 0;
   return align256((int64_t)T * K) + align256((int64_t)T * 4);
 }
 
@@ -154,16 +155,30 @@ int moe_int8_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype, const
   if (!aligned16(w))
     return op_fail(MOE_ERR_SHAPE, "int8 linear: w must start on a 16-byte boundary");
   const int64_t need = moe_int8_linear_workspace_bytes_v1(T, K);
-  if (!workspace || workspace_bytes < need)
-    return op_fail(MOE_ERR_WORKSPACE, "int8 linear: workspace of %lld bytes, needs %lld",
-                   (long long)(workspace ? workspace_bytes : 0), (long long)need);
-  if (!workspace_aligned(workspace))
-    return op_fail(MOE_ERR_WORKSPACE, "int8 linear: workspace must be 256-byte aligned");
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return op_fail(MOE_ERR_WORKSPACE, "int8 linear: workspace of %lld bytes, needs %lld",
+                     (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (!workspace_aligned(workspace))
+      return op_fail(MOE_ERR_WORKSPACE, "int8 linear: workspace must be 256-byte aligned");
+  }
   const int64_t es = dtype_bytes(dtype), nx = (int64_t)T * K * es, no = (int64_t)T * N * es;
   if (overlaps(out, no, workspace, need) || overlaps(out, no, w, (int64_t)N * K) ||
       overlaps(x, nx, workspace, need) || overlaps(out, no, x, nx))
     return op_fail(MOE_ERR_SHAPE, "int8 linear: x, out, w and the workspace must not overlap");
   const auto s = (hipStream_t)stream;
+  if (need == 0) {
+    Int8Args a{};
+    a.b0 = w;
+    a.s0 = w_scale;
+    a.M = T;
+    a.N = N;
+    a.K = K;
+    a.out = out;
+    a.bias = bias;
+    MOE_OP_HIP(launch_int8_fused(a, x, dtype, s), "int8 linear");
+    return MOE_OK;
+  }
   int8_t* q = static_cast<int8_t*>(workspace);
   float* qs = at<float>(workspace, align256((int64_t)T * K));
   MOE_OP_HIP(launch_quantize(x, T, K, dtype, q, qs, s), "quantize");

@@ -46,21 +46,16 @@ MOE_DEV int source_row(const Int8Args& a, int r) {
   return a.row_src ? (int)((uint32_t)a.row_src[r] / (uint32_t)a.src_div) : r;
 }
 
-// Four channels n .. n + 3 of output row r, from the sums of one or (SiLU) two products.
-template <int DT, bool SILU>
-MOE_DEV void finish(const Int8Args& a, int expert, int64_t r, int n, float ra, i32x4 c0, i32x4 c1,
-                    bool vec) {
+// Four channels n .. n + 3 of output row r.
+template <int DT>
+MOE_DEV void finish(const Int8Args& a, int64_t r, int n, float rs, i32x4 sum, bool vec) {
   using T = typename Elem<DT>::T;
-  const int64_t sb = (int64_t)expert * a.N;
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int ni = n + i < a.N ? n + i : a.N - 1;
-    v[i] = ((float)c0[i] * ra) * a.s0[sb + ni];
-    if constexpr (SILU)
-      v[i] = silu_f32(v[i]) * (((float)c1[i] * ra) * a.s1[sb + ni]);
-    else if (a.bias)
-      v[i] += Elem<DT>::get(static_cast<const T*>(a.bias)[ni]);
+    v[i] = ((float)sum[i] * rs) * a.s0[ni];
+    if (a.bias) v[i] += Elem<DT>::get(static_cast<const T*>(a.bias)[ni]);
   }
   T* p = static_cast<T*>(a.out) + r * a.N + n;
   if (vec && n + 3 < a.N) {
@@ -78,84 +73,156 @@ MOE_DEV void finish(const Int8Args& a, int expert, int64_t r, int n, float ra, i
   }
 }
 
-// ---------------------------------------------------------------- few rows a tile
-// Workgroup: 16 MT rows x 64 GEMM channels (SiLU: 32 gate channels and the same 32 of up, in
-// alternating groups of 16), the K steps of 64 dealt to the four waves in turn, whose sums meet in LDS.
-// Both operands go from memory to the registers the MFMA reads: a weight byte is used by one wave once.
-template <int MT, int DT, bool SILU>
-__global__ __launch_bounds__(kThreads) void int8_stream_kernel(Int8Args a, int vec) {
-  constexpr int NG = 4;  // groups of 16 channels
-  constexpr int KU = 4;  // K steps in flight
-  __shared__ i32x4 s_acc[kWaves][NG * MT][64];
-  const int blocks_n = (a.N + (SILU ? 31 : 63)) / (SILU ? 32 : 64);
-  const Tile tl = tile_of(a, 16 * MT, blockIdx.x / blocks_n);
-  if (tl.rows <= 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int lr = lane & 15, lk = (lane >> 4) * 16;
-  const int n0 = (blockIdx.x % blocks_n) * (SILU ? 32 : 64);
-  const int64_t eb = (int64_t)tl.expert * a.N * a.K;
-  const uint32_t b_bytes = (uint32_t)((int64_t)a.N * a.K);
+// ---------------------------------------------------------------- up to 16 rows
+// Workgroup: all rows x 16 channels, the K steps of 64 dealt to the four waves in turn, whose sums
+// meet in LDS. Weights go from memory to the registers the MFMA reads, kKU steps ahead; a byte is used
+// by one wave once. 16 channels a workgroup keep 256 CUs streaming from 4096 channels on (one row of
+// 2048 x 4096: 3.9 us, with 32 channels 5.0).
+// FUSED: the rows come as values of the dtype and every workgroup quantises them itself, into LDS,
+// while its first weights arrive: one launch instead of two, but every workgroup reads and divides
+// all of x. 2048 x 4096: 5.0 us for one row (two launches 3.9 + 2.1), 11.6 for eight (4.2 + 2.3).
+constexpr int kKU = 8;  // steps a load
+constexpr int kFusedRows = 4, kFusedBytes = 48 << 10;
+
+template <int DT, bool FUSED>
+__global__ __launch_bounds__(kThreads) void int8_stream_kernel(
+    Int8Args a, const typename Elem<DT>::T* __restrict__ x, int vec, int x_vec) {
+  extern __shared__ __attribute__((aligned(16))) int8_t s_q[];  // FUSED: [M][K + 16]
+  __shared__ i32x4 s_acc[kWaves][64];
+  __shared__ uint32_t s_top[kWaves][kFusedRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lk = (lane >> 4) * 16, lk4 = (lane >> 4) * 4;
+  const int n0 = blockIdx.x * 16, pitch = a.K + 16;
   const __amdgpu_buffer_rsrc_t ra = buf_rsrc(a.a, a.a_bytes);
-  const __amdgpu_buffer_rsrc_t r0 = buf_rsrc(a.b0 + eb, b_bytes);
-  const __amdgpu_buffer_rsrc_t r1 = buf_rsrc(SILU ? a.b1 + eb : a.b0 + eb, b_bytes);
-  uint32_t aoff[MT], boff[NG];
+  const __amdgpu_buffer_rsrc_t rb = buf_rsrc(a.b0, (uint32_t)((int64_t)a.N * a.K));
+  const uint32_t aoff = lr < a.M ? (uint32_t)lr * (uint32_t)a.K + lk : kOutOfRange;
+  const uint32_t boff = n0 + lr < a.N ? (uint32_t)(n0 + lr) * (uint32_t)a.K + lk : kOutOfRange;
+  // the wave's steps s0 .. s0 + kKU - 1 (64 bytes of K, kWaves apart); zeros past K
+  auto load = [&](i32x4 (&fb)[kKU], int s0) {
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int r = 16 * m + lr;
-    aoff[m] = r < tl.rows ? (uint32_t)source_row(a, tl.row0 + r) * (uint32_t)a.K + lk : kOutOfRange;
-  }
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int n = n0 + 16 * (SILU ? g / 2 : g) + lr;
-    boff[g] = n < a.N ? (uint32_t)n * (uint32_t)a.K + lk : kOutOfRange;
-  }
-  i32x4 acc[NG][MT];
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[g][m] = i32x4{0, 0, 0, 0};
-  for (int k0 = wave * 64; k0 < a.K; k0 += kWaves * 64 * KU) {
-    i32x4 fb[KU][NG], fa[KU][MT];
-#pragma unroll
-    for (int u = 0; u < KU; ++u) {
-      const int k = k0 + u * kWaves * 64;
+    for (int u = 0; u < kKU; ++u) {
+      const int k = ((s0 + u) * kWaves + wave) * 64;
       const uint32_t out = k + lk < a.K ? 0u : kOutOfRange;  // K % 16 == 0: a lane's 16 bytes
+      fb[u] = __builtin_bit_cast(i32x4, buf_ld128(rb, (boff + (uint32_t)k) | out));
+    }
+  };
+  i32x4 acc{0, 0, 0, 0};
+  auto multiply = [&](const i32x4 (&fb)[kKU], int s0) {
+    i32x4 fa[kKU];
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        fb[u][g] = __builtin_bit_cast(
-            i32x4, buf_ld128(SILU && (g & 1) ? r1 : r0, (boff[g] + (uint32_t)k) | out));
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        fa[u][m] = __builtin_bit_cast(i32x4, buf_ld128(ra, (aoff[m] + (uint32_t)k) | out));
+    for (int u = 0; u < kKU; ++u) {
+      const int k = ((s0 + u) * kWaves + wave) * 64;
+      const bool in = k + lk < a.K;
+      if constexpr (FUSED) {
+        // a token past the rows or a step past K reads another place; its product is not used, or
+        // meets weights of zero
+        fa[u] = *reinterpret_cast<const i32x4*>(s_q + min(lr, a.M - 1) * pitch + (in ? k + lk : 0));
+      } else {
+        fa[u] = __builtin_bit_cast(i32x4,
+                                   buf_ld128(ra, (aoff + (uint32_t)k) | (in ? 0u : kOutOfRange)));
+      }
     }
 #pragma unroll
-    for (int u = 0; u < KU; ++u)
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[g][m] = mfma_i8(fb[u][g], fa[u][m], acc[g][m]);
-  }
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) s_acc[wave][g * MT + m][lane] = acc[g][m];
-  __syncthreads();
-  auto total = [&](int f) {
-    i32x4 s = s_acc[0][f][lane];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) s += s_acc[w][f][lane];
-    return s;
+    for (int u = 0; u < kKU; ++u) acc = mfma_i8(fb[u], fa[u], acc);
   };
-  constexpr int kOut = SILU ? NG / 2 : NG;
-  for (int o = wave; o < kOut * MT; o += kWaves) {
-    const int g = o / MT, m = o % MT;
-    const int r = 16 * m + lr, n = n0 + 16 * g + (lane >> 4) * 4;
-    const i32x4 c0 = total((SILU ? 2 * g : g) * MT + m);
-    const i32x4 c1 = SILU ? total((2 * g + 1) * MT + m) : c0;
-    if (r < tl.rows && n < a.N)
-      finish<DT, SILU>(a, tl.expert, tl.row0 + r, n, a.a_scale[source_row(a, tl.row0 + r)], c0, c1,
-                       vec != 0);
+  const int steps = (a.K + kWaves * 64 - 1) / (kWaves * 64);
+  i32x4 f0[kKU], f1[kKU];
+  load(f0, 0);
+  uint32_t top[kFusedRows];
+  if constexpr (FUSED) {
+    __builtin_amdgcn_sched_barrier(0);
+    auto load_x = [&](int r, int c, float (&v)[8]) {
+      const typename Elem<DT>::T* p = x + (int64_t)r * a.K + c;
+      if (x_vec) {
+        ld8<DT>(p, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = Elem<DT>::get(p[e]);
+      }
+    };
+#pragma unroll
+    for (int r = 0; r < kFusedRows; ++r) {
+      top[r] = 0;
+      if (r < a.M) {
+#pragma unroll 2
+        for (int c = 8 * tid; c < a.K; c += 8 * kThreads) {
+          float v[8];
+          load_x(r, c, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top[r] = max(top[r], magnitude(v[e]));
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kFusedRows; ++r) {
+      if (r < a.M) {
+        const uint32_t t = bfly_umax(top[r]);
+        if (lane == 0) s_top[wave][r] = t;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kFusedRows; ++r) {
+      if (r >= a.M) break;
+      top[r] = s_top[0][r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top[r] = max(top[r], s_top[w][r]);
+      const Quantizer quant(top[r]);
+#pragma unroll 2
+      for (int c = 8 * tid; c < a.K; c += 8 * kThreads) {
+        float v[8];
+        load_x(r, c, v);
+        int b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = quant(v[e]);
+        *reinterpret_cast<u32x2*>(s_q + r * pitch + c) =
+            u32x2{pack_i8x4(b[0], b[1], b[2], b[3]), pack_i8x4(b[4], b[5], b[6], b[7])};
+      }
+    }
+    __syncthreads();
   }
+  for (int s0 = 0;; s0 += 2 * kKU) {
+    load(f1, s0 + kKU);
+    multiply(f0, s0);
+    if (s0 + kKU >= steps) break;
+    load(f0, s0 + 2 * kKU);
+    multiply(f1, s0 + kKU);
+    if (s0 + 2 * kKU >= steps) break;
+  }
+  s_acc[wave][lane] = acc;
+  __syncthreads();
+  if (wave == 0) {
+    const int n = n0 + lk4;
+    i32x4 sum = s_acc[0][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum += s_acc[w][lane];
+    if (lr < a.M && n < a.N) {
+      float rs;
+      if constexpr (FUSED) {
+        uint32_t t = s_top[0][lr];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) t = max(t, s_top[w][lr]);
+        rs = Quantizer::scale(t);
+      } else {
+        rs = a.a_scale[lr];
+      }
+      finish<DT>(a, lr, n, rs, sum, vec != 0);
+    }
+  }
+}
+
+template <int DT, bool FUSED>
+hipError_t launch_few_rows(const Int8Args& a, const void* x, hipStream_t s) {
+  constexpr int es = DT == kFp32 ? 4 : 2;
+  const int vec =
+      a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (uintptr_t)(4 * es - 1)) == 0;
+  const int64_t blocks = (a.N + 15) / 16;
+  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((int8_stream_kernel<DT, FUSED>), dim3((unsigned)blocks), dim3(kThreads),
+                     FUSED ? a.M * (a.K + 16) : 0, s, a,
+                     static_cast<const typename Elem<DT>::T*>(x), vec, aligned16(x) ? 1 : 0);
+  return hipGetLastError();
 }
 
 // ---------------------------------------------------------------- many rows a tile
@@ -571,7 +638,7 @@ hipError_t launch_ring(const Int8Args& a, int vec, hipStream_t s) {
 }
 
 template <int DT, bool SILU>
-hipError_t launch_product(const Int8Args& a, Int8Plan plan, int vec, hipStream_t s) {
+hipError_t launch_product(const Int8Args& a, Int8Plan plan, hipStream_t s) {
   const int wide = a.N % (DT == kFp32 ? 4 : 8) == 0 && aligned16(a.out);
   if (plan.kind == kInt8Tile) {
     if (plan.bm == 256) return launch_tile<256, 256, 2, 4, DT, SILU>(a, wide, s);
@@ -582,21 +649,14 @@ hipError_t launch_product(const Int8Args& a, Int8Plan plan, int vec, hipStream_t
     if (plan.kind == kInt8Ring)
       return plan.bm == 32 ? launch_ring<32, 64, 2, 2, DT>(a, wide, s)
                            : launch_ring<64, 64, 2, 2, DT>(a, wide, s);
-    const int64_t blocks = (int64_t)((a.N + 63) / 64) * a.m_tiles;
-    if (blocks > kMaxBlocks) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((int8_stream_kernel<1, DT, SILU>), dim3((unsigned)blocks), dim3(kThreads), 0,
-                       s, a, vec);
-    return hipGetLastError();
+    return launch_few_rows<DT, false>(a, nullptr, s);
   }
   return hipErrorInvalidValue;
 }
 
 template <int DT>
 hipError_t launch_product_t(const Int8Args& a, Int8Plan plan, bool silu, hipStream_t s) {
-  const int es = DT == kFp32 ? 4 : 2;
-  const int vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (uintptr_t)(4 * es - 1)) == 0;
-  return silu ? launch_product<DT, true>(a, plan, vec, s)
-              : launch_product<DT, false>(a, plan, vec, s);
+  return silu ? launch_product<DT, true>(a, plan, s) : launch_product<DT, false>(a, plan, s);
 }
 
 }  // namespace
@@ -625,4 +685,14 @@ hipError_t launch_int8_product(const Int8Args& a, Int8Plan plan, bool silu, int 
   if (dtype == kBf16) return launch_product_t<kBf16>(a, plan, silu, s);
   if (dtype == kFp16) return launch_product_t<kFp16>(a, plan, silu, s);
   return launch_product_t<kFp32>(a, plan, silu, s);
+}
+
+bool int8_fused_fits(int M, int K) {
+  return M >= 1 && M <= kFusedRows && (int64_t)M * (K + 16) <= kFusedBytes;
+}
+
+hipError_t launch_int8_fused(const Int8Args& a, const void* x, int dtype, hipStream_t s) {
+  if (dtype == kBf16) return launch_few_rows<kBf16, true>(a, x, s);
+  if (dtype == kFp16) return launch_few_rows<kFp16, true>(a, x, s);
+  return launch_few_rows<kFp32, true>(a, x, s);
 }

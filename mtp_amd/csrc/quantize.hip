@@ -1,29 +1,11 @@
 // Symmetric int8 quantisation of token rows: q = rint(127 x / a), scale = a / 127, a = max |x|.
 //
-// The quotient is taken in this order because 127 x is exact for bf16 and fp16 values (8 and 11 bits
-// by 7 bits) and an IEEE division then rounds only once: a quotient that is a tie is represented, and
-// one that is not lies further from the tie than the division's half step, so q equals the one of
-// exact arithmetic (ties to even). Rows are scaled by a power of two before, where 127 x could
-// overflow or the quotient's operands be subnormal. A row of zeros gives q = 0, scale = 0; a row with
-// an infinity or NaN gives q = 0 and scale = a / 127 (inf or NaN), so that its products are NaN.
-//
 // HBM-bound: one read of x, half (a quarter for fp32) of it written. The row stays in registers
-// between the maximum and the quotients; the maximum is taken over magnitude bits (NaN above
-// infinity).
+// between the maximum, taken over magnitude bits, and the quotients.
 #include "elem.h"
 #include "int8.h"
 
 namespace {
-
-MOE_DEV uint32_t bfly_umax(uint32_t v) {
-  auto step = [](uint32_t a, float b) { return max(a, __float_as_uint(b)); };
-  v = step(v, xor_partner<32>(__uint_as_float(v)));
-  v = step(v, xor_partner<16>(__uint_as_float(v)));
-  v = step(v, xor_partner<8>(__uint_as_float(v)));
-  v = step(v, xor_partner<4>(__uint_as_float(v)));
-  v = step(v, xor_partner<2>(__uint_as_float(v)));
-  return step(v, xor_partner<1>(__uint_as_float(v)));
-}
 
 // NT threads a row, NC chunks of 8 NT columns.
 template <int DT, int NT, int NC, bool VEC>
@@ -44,7 +26,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void quantize_kernel(
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[c][e]) & 0x7FFFFFFFu);
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[c][e]));
   top = bfly_umax(top);
   if constexpr (NT > 64) {
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
@@ -52,28 +34,18 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void quantize_kernel(
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) top = max(top, s_max[w]);
   }
-  const float a = __uint_as_float(top);
-  if (tid == 0) scale[t] = a / 127.0f;
-  const bool usable = top != 0 && top < 0x7F800000u;
-  const float m = a >= 0x1p64f ? 0x1p-64f : a < 0x1p-64f ? 0x1p64f : 1.0f;
-  const float d = usable ? a * m : 1.0f, f = usable ? m : 0.0f;
+  if (tid == 0) scale[t] = Quantizer::scale(top);
+  const Quantizer quant(top);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     int b[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float n = usable ? v[c][e] * f * 127.0f : 0.0f;
-      b[e] = (int)__builtin_rintf(n / d);
-    }
+    for (int e = 0; e < 8; ++e) b[e] = quant(v[c][e]);
     int8_t* p = q + t * K + c * 8 * NT;
     const int left = K - c * 8 * NT;
     if constexpr (VEC) {
       if (8 * tid < left) {
-        u32x2 o;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          o[h] = (uint32_t)(b[4 * h] & 255) | (uint32_t)(b[4 * h + 1] & 255) << 8 |
-                 (uint32_t)(b[4 * h + 2] & 255) << 16 | (uint32_t)(b[4 * h + 3] & 255) << 24;
+        const u32x2 o{pack_i8x4(b[0], b[1], b[2], b[3]), pack_i8x4(b[4], b[5], b[6], b[7])};
         *reinterpret_cast<u32x2*>(p + 8 * tid) = o;
       }
     } else {

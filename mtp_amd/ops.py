@@ -536,10 +536,10 @@ def _dispatch(x, topk_ids, num_experts):
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     row_slot = torch.empty(T * k, dtype=torch.int32, device=dev)
     slot_row = torch.empty(T, k, dtype=torch.int32, device=dev)
-    need = int(_lib.load().moe_dispatch_workspace_bytes_v1(T, k, num_experts))
+    need = _lib.load().moe_dispatch_workspace_bytes_v1(T, k, num_experts)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _call("moe_dispatch_v1", dev, x.data_ptr(), T, H, OUT_DTYPES[x.dtype], topk_ids.data_ptr(), k,
-          num_experts, _ptr(ws), max(need, 0), rows.data_ptr(), offsets.data_ptr(),
+          num_experts, _ptr(ws), need, rows.data_ptr(), offsets.data_ptr(),
           row_slot.data_ptr(), slot_row.data_ptr())
     return rows, offsets, row_slot, slot_row
 
@@ -692,11 +692,11 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     _require_gpu(x, weight, weight_scale, bias)
     N = weight.shape[0]
     dev = x.device
-    need = int(_lib.load().moe_int8_linear_workspace_bytes_v1(T, K))
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    need = _lib.load().moe_int8_linear_workspace_bytes_v1(T, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     out = torch.empty(T, N, dtype=x.dtype, device=dev)
     _call("moe_int8_linear_v1", dev, x.data_ptr(), T, K, code, weight.data_ptr(),
-          weight_scale.data_ptr(), N, _ptr(bias), ws.data_ptr(), need, out.data_ptr())
+          weight_scale.data_ptr(), N, _ptr(bias), _ptr(ws), need, out.data_ptr())
     return out
 
 
@@ -822,8 +822,9 @@ def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | Non
             raise ValueError(f"gate must be {y.dtype} [{H}], [{T}, 1] or [{T}, {H}], got "
                              f"{gate.dtype} {tuple(gate.shape)}")
     _require_gpu(y, res, post_w, gate, pre_w)
-    args = (y, res, post_w, gate, pre_w, kind, float(res_scale), float(branch_scale), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
-        out = _BlockNormFn.apply(*args)
+    scales = (kind, float(res_scale), float(branch_scale), float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (y, res, post_w, gate, pre_w)):
+        out = _BlockNormFn.apply(y, res, post_w, gate, pre_w, *scales)
         return out if pre_w is not None else (out, None)
-    return _block_norm(*args)
+    return _block_norm(y, res, post_w, gate, pre_w, *scales)

@@ -96,6 +96,9 @@ def host_product(q, qs, w, ws):
 
 SHAPES = [  # T, K, N, dtype, bias
     (1, 16, 1, torch.bfloat16, False), (1, 2048, 4096, torch.bfloat16, False),
+    (8, 4096, 8200, torch.float16, True), (5, 8192, 96, torch.float32, False),
+    (7, 4224, 24, torch.bfloat16, True), (8, 6160, 40, torch.bfloat16, False),
+    (9, 320, 8193, torch.float32, False), (3, 272, 19, torch.float32, False),
     (2, 48, 33, torch.float16, True), (15, 1040, 100, torch.bfloat16, True),
     (16, 64, 64, torch.float32, False), (17, 80, 65, torch.float16, False),
     (31, 2048, 96, torch.float32, True), (33, 144, 200, torch.bfloat16, False),
@@ -125,6 +128,17 @@ def test_matmul_and_linear(T, K, N, dtype, bias):
         slack = 2 * U * (want.double().abs() + b.double().abs())
         tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134
         assert bool((err <= half(dtype) * (full.abs() + slack) + slack + tiny).all())
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_linear_of_unaligned_rows(T):
+    x = torch.randn(T, 96).to(torch.bfloat16).cuda()
+    buf = torch.empty(T * 96 + 1, dtype=torch.bfloat16, device="cuda")
+    xo = buf[1:].view(T, 96)
+    xo.copy_(x)
+    w, ws = make_weight(50, 96, 4)
+    assert torch.equal(ops.int8_linear(xo, w.cuda(), ws.cuda()),
+                       ops.int8_linear(x, w.cuda(), ws.cuda()))
 
 
 def test_extreme_sums():

@@ -110,8 +110,9 @@ A, B, C, D, G, W = (0x1000000 * i for i in range(1, 7))  # never dereferenced
     (SHAPE, "moe_int8_matmul_v1", (A, B, 4, 64, C, D, 8, None, 0, A)),
     (NULL, "moe_int8_matmul_v1", (A, None, 4, 64, C, D, 8, None, 0, G)),
     (UNSUP, "moe_int8_matmul_v1", (A, B, 4, 64, C, D, 8, None, 7, G)),
-    (WS, "moe_int8_linear_v1", (A, 4, 64, 0, B, C, 8, None, D, 16, G)),
-    (WS, "moe_int8_linear_v1", (A, 4, 64, 0, B, C, 8, None, D + 16, 1 << 20, G)),
+    (WS, "moe_int8_linear_v1", (A, 40, 64, 0, B, C, 8, None, D, 16, G)),
+    (WS, "moe_int8_linear_v1", (A, 40, 64, 0, B, C, 8, None, None, 1 << 20, G)),
+    (WS, "moe_int8_linear_v1", (A, 40, 64, 0, B, C, 8, None, D + 16, 1 << 20, G)),
     (SHAPE, "moe_int8_linear_v1", (A, 4, 64, 0, B, C, 8, None, D, 1 << 20, A)),
     (SHAPE, "moe_block_norm_v1", (A, B, 4, 8193, 0, None, None, 0, 1.0, 1.0, None, 1e-6, C, None)),
     (SHAPE, "moe_block_norm_v1", (A, B, 4, 64, 0, None, None, 0, 1.0, 1.0, None, -1.0, C, None)),
@@ -158,4 +159,6 @@ def test_workspace_queries_refuse_sizes():
     assert lib.moe_dispatch_workspace_bytes_v1(-1, 8, 16) == -1
     assert lib.moe_dispatch_workspace_bytes_v1(8, 8, 16) == 0
     assert lib.moe_int8_linear_workspace_bytes_v1(-1, 64) == -1
+    assert lib.moe_int8_linear_workspace_bytes_v1(4, 64) == 0
+    assert lib.moe_int8_linear_workspace_bytes_v1(40, 64) > 0
     assert lib.moe_block_norm_workspace_bytes_v1(4, 8193) == -1
