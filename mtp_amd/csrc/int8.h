@@ -25,32 +25,41 @@ struct Int8Args {
 };
 
 // Symmetric quantisation of a row of values whose largest magnitude has the bits `top` (NaN above
-// infinity): q = rint(127 x / a). 127 x is exact for bf16 and fp16 values (8 and 11 bits by 7) and an
-// IEEE division then rounds only once: a quotient that is a tie is represented, and one that is not
-// lies further from the tie than the division's half step, so q equals that of exact arithmetic
-// (ties to even). Rows are scaled by a power of two first, where 127 x could overflow or the
-// quotient's operands be subnormal. A row of zeros, and one that holds an infinity or NaN, gives 0.
+// infinity): q = rint(127 x / a). 127 x is exact for bf16 and fp16 values (8 and 11 bits by 7) and a
+// correctly rounded division then rounds only once: a quotient that is a tie is represented, and
+// one that is not lies further from the tie than the division's half step, so q equals that of exact
+// arithmetic (ties to even). Rows are scaled by a power of two first, where 127 x could overflow or
+// the quotient's operands be subnormal. A row of zeros, and one that holds an infinity or NaN, gives 0.
+// The quotient is that of an IEEE division: with y = 1 / d correctly rounded (once a row) and
+// c = n y, c + (n - c d) y in fused operations is (Markstein). The compiler's division per value took
+// two thirds of the kernel's time (8192 x 4096: 24 -> 16 us).
 struct Quantizer {
-  float f, d;
+  float f, d, y;
+  uint32_t keep;
   MOE_DEV explicit Quantizer(uint32_t top) {
     const float a = __uint_as_float(top);
     const bool usable = top != 0 && top < 0x7F800000u;
     const float m = a >= 0x1p64f ? 0x1p-64f : a < 0x1p-64f ? 0x1p64f : 1.0f;
-    f = usable ? m : 0.0f;
+    f = usable ? 127.0f * m : 0.0f;
     d = usable ? a * m : 1.0f;
+    y = 1.0f / d;
+    keep = usable ? ~0u : 0u;
   }
-  MOE_DEV int operator()(float x) const {
-    const float n = f == 0.0f ? 0.0f : x * f * 127.0f;
-    return (int)__builtin_rintf(n / d);
+  // q in the low byte: adding 1.5 * 2^23 rounds to an integer, half to even, in the low bits
+  MOE_DEV uint32_t bits(float x) const {
+    const float n = x * f, c = n * y;
+    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-c, d, n), y, c) + 12582912.0f);
   }
+  MOE_DEV uint32_t four(float x0, float x1, float x2, float x3) const {
+    const uint32_t lo = __builtin_amdgcn_perm(bits(x1), bits(x0), 0x0C0C0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(bits(x3), bits(x2), 0x04000C0Cu);
+    return (lo | hi) & keep;
+  }
+  MOE_DEV int8_t one(float x) const { return (int8_t)(bits(x) & keep); }
   // a / 127: inf or NaN for rows that hold one, so that their products are NaN
   MOE_DEV static float scale(uint32_t top) { return __uint_as_float(top) / 127.0f; }
 };
 MOE_DEV uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
-MOE_DEV uint32_t pack_i8x4(int b0, int b1, int b2, int b3) {
-  return (uint32_t)(b0 & 255) | (uint32_t)(b1 & 255) << 8 | (uint32_t)(b2 & 255) << 16 |
-         (uint32_t)(b3 & 255) << 24;
-}
 MOE_DEV uint32_t bfly_umax(uint32_t v) {
   v = max(v, __float_as_uint(xor_partner<32>(__uint_as_float(v))));
   v = max(v, __float_as_uint(xor_partner<16>(__uint_as_float(v))));

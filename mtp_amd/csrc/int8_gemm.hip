@@ -173,11 +173,8 @@ __global__ __launch_bounds__(kThreads) void int8_stream_kernel(
       for (int c = 8 * tid; c < a.K; c += 8 * kThreads) {
         float v[8];
         load_x(r, c, v);
-        int b[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = quant(v[e]);
         *reinterpret_cast<u32x2*>(s_q + r * pitch + c) =
-            u32x2{pack_i8x4(b[0], b[1], b[2], b[3]), pack_i8x4(b[4], b[5], b[6], b[7])};
+            u32x2{quant.four(v[0], v[1], v[2], v[3]), quant.four(v[4], v[5], v[6], v[7])};
       }
     }
     __syncthreads();

@@ -38,20 +38,17 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void quantize_kernel(
   const Quantizer quant(top);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    int b[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = quant(v[c][e]);
     int8_t* p = q + t * K + c * 8 * NT;
     const int left = K - c * 8 * NT;
     if constexpr (VEC) {
-      if (8 * tid < left) {
-        const u32x2 o{pack_i8x4(b[0], b[1], b[2], b[3]), pack_i8x4(b[4], b[5], b[6], b[7])};
-        *reinterpret_cast<u32x2*>(p + 8 * tid) = o;
-      }
+      const float (&x8)[8] = v[c];
+      if (8 * tid < left)
+        *reinterpret_cast<u32x2*>(p + 8 * tid) =
+            u32x2{quant.four(x8[0], x8[1], x8[2], x8[3]), quant.four(x8[4], x8[5], x8[6], x8[7])};
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (tid + NT * e < left) p[tid + NT * e] = (int8_t)b[e];
+        if (tid + NT * e < left) p[tid + NT * e] = quant.one(v[c][e]);
     }
   }
 }
@@ -71,8 +68,10 @@ hipError_t launch_quantize_t(const void* x, int T, int K, int8_t* q, float* scal
       hipLaunchKernelGGL((quantize_kernel<DT, NT, NC, false>), grid, block, 0, s, xt, T, K, q,  \
                          scale);                                                                \
   } while (0)
+  // a wave a row while it holds the row: no barrier between the loads and the quotients
   if (K <= 512) MOE_QUANT(64, 1);
-  else if (K <= 2048) MOE_QUANT(256, 1);
+  else if (K <= 1024) MOE_QUANT(64, 2);
+  else if (K <= 2048) MOE_QUANT(64, 4);
   else if (K <= 4096) MOE_QUANT(256, 2);
   else if (K <= 8192) MOE_QUANT(256, 4);
   else MOE_QUANT(1024, 8);

@@ -535,7 +535,7 @@ def _dispatch(x, topk_ids, num_experts):
     rows = torch.empty(T * k, H, dtype=x.dtype, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     row_slot = torch.empty(T * k, dtype=torch.int32, device=dev)
-    slot_row = torch.empty(T, k, dtype=torch.int32, device=dev)
+    slot_row = torch.empty_like(topk_ids)
     need = _lib.load().moe_dispatch_workspace_bytes_v1(T, k, num_experts)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _call("moe_dispatch_v1", dev, x.data_ptr(), T, H, OUT_DTYPES[x.dtype], topk_ids.data_ptr(), k,
