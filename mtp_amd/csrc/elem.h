@@ -68,7 +68,9 @@ template <int DT, int NT, bool VEC>
 struct Cols {
   using T = typename Elem<DT>::T;
   // Without branches: a thread outside the row reads columns inside it and drops them (in branches
-  // every load was waited for before the next was issued).
+  // every load was waited for before the next was issued). `row` may be a chunk of a row behind its
+  // end (H <= 0): the row's last columns are read then, so the row itself holds at least 8 columns
+  // (VEC) or one.
   MOE_DEV static void load(const T* row, int tid, int H, float (&v)[8]) {
     if constexpr (VEC) {
       ld8<DT>(row + min(8 * tid, H - 8), v);
@@ -99,7 +101,7 @@ template <int DT, int NT, bool VEC>
 struct RawCols {
   using T = typename Elem<DT>::T;
   using C = Cols<DT, NT, VEC>;
-  static constexpr int kWords = VEC ? 2 * (int)sizeof(T) : 8;
+  static constexpr int kWords = 2 * (int)sizeof(T);
   uint32_t w[kWords];
   MOE_DEV void load(const T* row, int tid, int H) {
     if constexpr (VEC) {
@@ -110,21 +112,21 @@ struct RawCols {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[4 * i + j] = d[j];
       }
+    } else if constexpr (DT == kFp32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(row[min(tid + NT * e, H - 1)]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const T v = row[min(tid + NT * e, H - 1)];
-        if constexpr (DT == kFp32) w[e] = __float_as_uint(v);
-        else w[e] = v;
-      }
+      for (int e = 0; e < 8; e += 2)
+        w[e / 2] = (uint32_t)row[min(tid + NT * e, H - 1)] |
+                   (uint32_t)row[min(tid + NT * (e + 1), H - 1)] << 16;
     }
   }
   // column e of the thread; 0 outside the row
   MOE_DEV float get(int e, int tid, int H) const {
     float v;
     if constexpr (DT == kFp32) v = __uint_as_float(w[e]);
-    else if constexpr (VEC) v = Elem<DT>::get((T)(w[e / 2] >> (16 * (e & 1))));
-    else v = Elem<DT>::get((T)w[e]);
+    else v = Elem<DT>::get((T)(w[e / 2] >> (16 * (e & 1))));
     return C::col(tid, e) < H ? v : 0.0f;
   }
 };

@@ -77,7 +77,7 @@ enum { kInt8Stream = 0, kInt8Ring = 1, kInt8Tile = 2 };
 struct Int8Plan {
   int kind, bm;
 };
-Int8Plan int8_experts_plan(int64_t slots, int E);
+Int8Plan int8_experts_plan(int64_t slots, int E, int I);
 Int8Plan int8_matrix_plan(int64_t M, int64_t N);
 hipError_t launch_int8_product(const Int8Args& a, Int8Plan plan, bool silu, int dtype,
                                hipStream_t s);

@@ -59,7 +59,7 @@ struct ExpertsLayout {
 ExpertsLayout experts_layout(int T, int k, const moe_int8_set_v1& ex, int dtype) {
   ExpertsLayout L{};
   const int64_t S = (int64_t)T * k, es = dtype_bytes(dtype);
-  L.plan = int8_experts_plan(S, ex.num_experts);
+  L.plan = int8_experts_plan(S, ex.num_experts, ex.intermediate);
   L.tile_cap = (int)(S / L.plan.bm + std::min<int64_t>(S, ex.num_experts));
   int64_t o = 0;
   auto take = [&o](int64_t bytes) {

@@ -658,12 +658,16 @@ hipError_t launch_product_t(const Int8Args& a, Int8Plan plan, bool silu, hipStre
 
 }  // namespace
 
-// Rows a tile by the rows an expert has on average, whatever the shapes (hidden 2048, intermediate
-// 512, 256 experts, top-8, us a layer with tiles of 64 / 128 / 256 rows): 512 tokens 184 / 191 / 207,
-// 2048 tokens 248 / 244 / 261, 4096 tokens 349 / 320 / 328, 8192 tokens 564 / 489 / 458.
-Int8Plan int8_experts_plan(int64_t slots, int E) {
+// Rows a tile by the rows an expert has on average (hidden 2048, intermediate 512, 256 experts, top-8,
+// us a layer with tiles of 64 / 128 / 256 rows): 512 tokens 184 / 191 / 207, 2048 tokens 248 / 244 /
+// 261, 4096 tokens 349 / 320 / 328, 8192 tokens 564 / 489 / 458. Where few experts share the rows
+// the larger tiles also have to be enough for the chip (4096 rows of 8 experts of 2048 x 1024: 105 /
+// 101 / 90, 4000 rows of 8 experts of 512 x 128: 34 / 36 / 44).
+Int8Plan int8_experts_plan(int64_t slots, int E, int I) {
   const int64_t rows = (slots + E - 1) / E;
-  return Int8Plan{kInt8Tile, rows <= 48 ? 64 : rows < 192 ? 128 : 256};
+  if (rows >= 192 && slots / 256 * ((I + 127) / 128) >= 96) return Int8Plan{kInt8Tile, 256};
+  if (rows > 48 && slots / 128 * ((I + 63) / 64) >= 256) return Int8Plan{kInt8Tile, 128};
+  return Int8Plan{kInt8Tile, 64};
 }
 
 // One matrix: the larger the tile the fewer bytes a product moves, the smaller the more workgroups
