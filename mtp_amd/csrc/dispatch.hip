@@ -38,7 +38,7 @@ struct SortOut {
 // ---------------------------------------------------------------- tables of the experts
 // offsets and the GEMM tiles from the keys' counts in LDS (cnt [E], E <= kMaxE), by one workgroup
 // of NT threads. tiles (nullable): {expert, first row, rows, 0} of each block of bm rows, behind
-// them entries of no rows up to tile_cap, and then one entry with the blocks' number.
+// them entries of no rows up to tile_cap.
 template <int NT>
 MOE_DEV void write_tables(const int* cnt, int E, int32_t* offsets, i32x4* tiles, int bm,
                           int tile_cap) {
@@ -87,10 +87,8 @@ MOE_DEV void write_tables(const int* cnt, int E, int32_t* offsets, i32x4* tiles,
     row += c[j];
   }
   if (tid * kPer + kPer == E && E == NT * kPer) offsets[E] = row;  // E fills the last thread
-  if (tiles) {
+  if (tiles)
     for (int i = all + tid; i < tile_cap; i += NT) tiles[i] = i32x4{0, 0, 0, 0};
-    if (tid == 0) tiles[tile_cap] = i32x4{all, 0, 0, 0};
-  }
 }
 
 // ---------------------------------------------------------------- few slots: one launch

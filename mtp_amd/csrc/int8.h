@@ -17,8 +17,7 @@ struct Int8Args {
   const float* s0;
   const float* s1;
   const i32x4* tiles;     // {expert, first row, rows, 0}; NULL: consecutive rows of one matrix
-  int m_tiles;            // entries of the tile table (behind them: how many are in use), or the
-                          // row blocks of one matrix
+  int m_tiles;            // entries of the tile table, or the row blocks of one matrix
   int M, N, K;
   void* out;              // [M][N]
   const void* bias;       // [N] or NULL

@@ -72,7 +72,7 @@ ExpertsLayout experts_layout(int T, int k, const moe_int8_set_v1& ex, int dtype)
   L.offsets = take((int64_t)(ex.num_experts + 1) * 4);
   L.row_slot = take(S * 4);
   L.slot_row = take(S * 4);
-  L.tiles = take((int64_t)(L.tile_cap + 1) * 16);
+  L.tiles = take((int64_t)L.tile_cap * 16);
   L.scratch = take(dispatch_scratch_bytes(S, ex.num_experts));
   L.h = take(S * ex.intermediate * es);
   L.hq = take(S * ex.intermediate);

@@ -204,8 +204,7 @@ hipError_t launch_hr_predictor(const uint16_t* x, int N, int H, const int32_t* l
 
 // Token rows sorted by expert (dispatch.hip): rows (x NULL: the tables only), offsets [E + 1],
 // row_slot and slot_row [T * k]. ws: dispatch_scratch_bytes. tiles (nullable): the GEMM tiles of bm
-// rows, tile_cap entries {expert, first row, rows, 0}, those past the last expert's empty, and one
-// more with the number in use.
+// rows, tile_cap entries {expert, first row, rows, 0}, those past the last expert's empty.
 typedef int32_t i32x4_tile __attribute__((ext_vector_type(4)));
 int64_t dispatch_scratch_bytes(int64_t slots, int E);
 hipError_t launch_dispatch(const int32_t* ids, int T, int k, int E, const void* x,
