@@ -15,9 +15,9 @@
 //
 // HBM-bound in both directions: every tensor is read and written once, 8 columns a thread held in
 // registers across the reductions. A row takes a wave up to 512 columns, a workgroup of 256 threads
-// up to 2048, of 512 up to 4096, of 1024 up to 8192. Sums are fp32 in a fixed order: per thread over its columns, a
-// butterfly in each wave, the waves in order; the weights' gradients per workgroup over its rows in
-// order, then over the workgroups in order.
+// up to 2048, of 512 up to 4096, of 1024 up to 8192. Sums are taken in a fixed order: in fp32 per
+// thread over its columns, in fp64 in a butterfly in each wave and over the waves; the weights'
+// gradients in fp32 per workgroup over its rows, then over the workgroups.
 #include <algorithm>
 #include <initializer_list>
 
@@ -30,11 +30,30 @@ namespace {
 constexpr int kMaxHidden = 8192;
 enum { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateFull = 3 };
 
-// Sums of N values over the NT threads of a row (all threads get them). NT = 64: no barrier.
+// Lane i's partner value for a butterfly over doubles.
+template <int M>
+MOE_DEV double xor_partner64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)b)));
+  const uint32_t hi = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)(b >> 32))));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Sums of N values over the NT threads of a row (all threads get them), in 64 bits: the norms'
+// factors come out within half an fp32 step of exact ones, at a cost that HBM's time hides. NT = 64:
+// no barrier.
 template <int NT, int N>
-MOE_DEV void row_sums(float (&v)[N], float (*s_part)[N]) {
+MOE_DEV void row_sums(const float (&part)[N], double (&v)[N], double (*s_part)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = bfly_sum(v[i]);
+  for (int i = 0; i < N; ++i) {
+    v[i] = part[i];
+    v[i] += xor_partner64<32>(v[i]);
+    v[i] += xor_partner64<16>(v[i]);
+    v[i] += xor_partner64<8>(v[i]);
+    v[i] += xor_partner64<4>(v[i]);
+    v[i] += xor_partner64<2>(v[i]);
+    v[i] += xor_partner64<1>(v[i]);
+  }
   if constexpr (NT > 64) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();  // the previous sums have been read
@@ -45,15 +64,20 @@ MOE_DEV void row_sums(float (&v)[N], float (*s_part)[N]) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = 0.0f;
+      v[i] = 0.0;
 #pragma unroll
       for (int w = 0; w < NT / 64; ++w) v[i] += s_part[w][i];
     }
   }
 }
 
-MOE_DEV float inv_rms(float sum, int H, float eps) {
-  return 1.0f / __builtin_sqrtf(sum / (float)H + eps);
+// 1 / sqrt(sum / H + eps): the hardware's approximation and a Newton step in 64 bits.
+MOE_DEV float inv_rms(double sum, double inv_h, float eps) {
+  const double m = sum * inv_h + (double)eps;
+  const float v = (float)m;
+  if (!(v >= 0x1p-100f && v < __builtin_inff())) return 1.0f / __builtin_sqrtf(v);
+  const double r = (double)__builtin_amdgcn_rsqf(v);
+  return (float)(r + 0.5 * r * (1.0 - m * r * r));
 }
 
 struct NormArgs {
@@ -90,7 +114,8 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_kernel(NormArg
                                                                          void* x_out) {
   using T = typename Elem<DT>::T;
   using C = Cols<DT, NT, VEC>;
-  __shared__ float s_part[NT / 64][1];
+  __shared__ double s_part[NT / 64][1];
+  const double inv_h = 1.0 / (double)a.H;
   const int tid = threadIdx.x % NT;
   const int rows = block_threads<NT>() / NT;
   const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
@@ -105,8 +130,9 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_kernel(NormArg
       float ss[1] = {0.0f};
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss[0] = __builtin_fmaf(p[e], p[e], ss[0]);
-      row_sums<NT>(ss, s_part);
-      const float q = inv_rms(ss[0], a.H, a.eps);
+      double sum[1];
+      row_sums<NT>(ss, sum, s_part);
+      const float q = inv_rms(sum[0], inv_h, a.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = (p[e] * q) * (1.0f + w[e]);
     }
@@ -120,8 +146,9 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_kernel(NormArg
     if (a.pre) {
       float w[8];
       C::load(static_cast<const T*>(a.pre), tid, a.H, w);
-      row_sums<NT>(ss, s_part);
-      const float s = inv_rms(ss[0], a.H, a.eps);
+      double sum[1];
+      row_sums<NT>(ss, sum, s_part);
+      const float s = inv_rms(sum[0], inv_h, a.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) r[e] = (r[e] * s) * (1.0f + w[e]);
       C::store(static_cast<T*>(x_out) + t * a.H, tid, a.H, r);
@@ -141,15 +168,16 @@ struct NormGrads {
 };
 
 // The next row's loads are in flight while a row is worked on (two reductions with their barriers):
-// 16384 x 2048 bf16 with both norms and a channel gate 140 -> 83 us, 4.9 TB/s.
+// 16384 x 2048 bf16 with both norms and a channel gate 140 -> 88 us, 4.6 TB/s.
 template <int DT, int NT, bool VEC>
 __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kernel(NormArgs a,
                                                                                   NormGrads d) {
   using T = typename Elem<DT>::T;
   using C = Cols<DT, NT, VEC>;
   using Raw = RawCols<DT, NT, VEC>;
-  __shared__ float s3[NT / 64][3];
-  __shared__ float s2[NT / 64][2];
+  __shared__ double s3[NT / 64][3];
+  __shared__ double s2[NT / 64][2];
+  const double inv_h = 1.0 / (double)a.H;
   const int tid = threadIdx.x % NT, H = a.H;
   const int rows = block_threads<NT>() / NT;
   const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
@@ -208,27 +236,28 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
     Row row = next;
     if (kAhead) load(t + stride);
     if (a.gate_kind == kGateChannel) row.gate = gate;
-    float sum[3] = {0.0f, 0.0f, 0.0f};  // y^2, r^2, d x (1 + pre_w) r
+    float part[3] = {0.0f, 0.0f, 0.0f};  // y^2, r^2, d x (1 + pre_w) r
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float y = row.y.get(e, tid, H);
-      sum[0] = __builtin_fmaf(y, y, sum[0]);
+      part[0] = __builtin_fmaf(y, y, part[0]);
     }
     if (pre) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float r = row.r.get(e, tid, H);
-        sum[1] = __builtin_fmaf(r, r, sum[1]);
-        sum[2] = __builtin_fmaf(row.dx.get(e, tid, H) * (1.0f + wpre.get(e, tid, H)), r, sum[2]);
+        part[1] = __builtin_fmaf(r, r, part[1]);
+        part[2] = __builtin_fmaf(row.dx.get(e, tid, H) * (1.0f + wpre.get(e, tid, H)), r, part[2]);
       }
     }
-    if (post || pre) row_sums<NT>(sum, s3);
+    double sum[3] = {0.0, 0.0, 0.0};
+    if (post || pre) row_sums<NT>(part, sum, s3);
     float du[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) du[e] = dr ? row.dr.get(e, tid, H) : 0.0f;
     if (pre) {
-      const float s = inv_rms(sum[1], H, a.eps);
-      const float m = sum[2] * s / (float)H;  // mean(g r s)
+      const float s = inv_rms(sum[1], inv_h, a.eps);
+      const float m = (float)(sum[2] * inv_h) * s;  // mean(g r s)
       if constexpr (!kAhead) at(2, apre, false);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -244,12 +273,12 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
       for (int e = 0; e < 8; ++e) o[e] = a.res_scale * du[e];
       C::store(static_cast<T*>(d.dres) + t * H, tid, H, o);
     }
-    const float q = post ? inv_rms(sum[0], H, a.eps) : 1.0f;
+    const float q = post ? inv_rms(sum[0], inv_h, a.eps) : 1.0f;
     const float one = a.gate_kind == kGateToken ? row.token : 1.0f;
     const bool wide = a.gate_kind >= kGateChannel;
     const bool full = a.gate_kind == kGateFull && d.dgate;
     float dg[8], dp[8];
-    float tot[2] = {0.0f, 0.0f};  // h y, d gate
+    float some[2] = {0.0f, 0.0f};  // h y, d gate
     if constexpr (!kAhead) {
       at(0, apost, false);
       at(1, agate, false);
@@ -265,8 +294,8 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
       agate[e] += dg[e];
       dp[e] *= w1;
       if (C::col(tid, e) < H) {  // 0 times a gate of infinity outside the row is no part of it
-        tot[0] = __builtin_fmaf(dp[e], y, tot[0]);
-        tot[1] += dg[e];
+        some[0] = __builtin_fmaf(dp[e], y, some[0]);
+        some[1] += dg[e];
       }
     }
     if constexpr (!kAhead) {
@@ -274,12 +303,13 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
       at(1, agate, true);
     }
     const bool token = a.gate_kind == kGateToken && d.dgate;
-    if (post || token) row_sums<NT>(tot, s2);
-    if (token && tid == 0) static_cast<T*>(d.dgate)[t] = Elem<DT>::put(tot[1]);
+    double tot[2] = {0.0, 0.0};
+    if (post || token) row_sums<NT>(some, tot, s2);
+    if (token && tid == 0) static_cast<T*>(d.dgate)[t] = Elem<DT>::put((float)tot[1]);
     if (full) C::store(static_cast<T*>(d.dgate) + t * H, tid, H, dg);
     if (d.dy) {
       if (post) {
-        const float m = tot[0] * q / (float)H;
+        const float m = (float)(tot[0] * inv_h) * q;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           dp[e] = q * (dp[e] - (row.y.get(e, tid, H) * q) * m);

@@ -131,9 +131,13 @@ struct RawCols {
   }
 };
 
-// The value as it reads back after being stored in the type.
+// The value as it reads back after being stored in the type: an fp32 result rounded to it (and not
+// the last operation's exact result, as a fused multiply-add with an fp16 result would give).
 template <int DT>
-MOE_DEV float rounded(float f) { return Elem<DT>::get(Elem<DT>::put(f)); }
+MOE_DEV float rounded(float f) {
+  if constexpr (DT == kFp16) asm("" : "+v"(f));
+  return Elem<DT>::get(Elem<DT>::put(f));
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int64_t dtype_bytes(int dtype) { return dtype == kFp32 ? 4 : 2; }
