@@ -278,7 +278,7 @@ int moe_combine_backward_v1(const void* dout, const void* rows, int32_t T, int32
 
 /* scale[t] = a / 127, q[t, k] = round_half_even(127 * x[t, k] / a), a = max_k |x[t, k]|. A row of
  * zeros: q = 0, scale 0. A row that holds an infinity or NaN: q = 0, scale a / 127 (inf or NaN).
- * q int8 [T, K] (any K up to 65536), scale fp32 [T]. */
+ * q int8 [T, K] (any K up to 65536, T < 2^22), scale fp32 [T]. */
 int moe_quantize_tokens_v1(const void* x, int32_t T, int32_t K, int32_t dtype, int8_t* q,
                            float* scale, void* stream);
 

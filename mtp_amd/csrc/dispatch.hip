@@ -16,6 +16,7 @@
 
 #include "common.h"
 #include "elem.h"
+#include "int8.h"
 #include "launch.h"
 
 namespace {
@@ -96,16 +97,16 @@ MOE_DEV void write_tables(const int* cnt, int E, int32_t* offsets, i32x4* tiles,
 // ballots' population counts are the rows. S ids per workgroup from L2 instead of two further
 // launches. Workgroup (T, 0) counts the experts' slots for the tables.
 template <typename U>
-__global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
-    const int32_t* __restrict__ ids, int T, int k, int E, const U* __restrict__ x, int64_t units,
-    U* __restrict__ rows, SortOut o, i32x4* tiles, int bm, int tile_cap) {
+MOE_DEV void dispatch_small(int bx, int by, const int32_t* __restrict__ ids, int T, int k, int E,
+                            const U* __restrict__ x, int64_t units, U* __restrict__ rows, SortOut o,
+                            i32x4* tiles, int bm, int tile_cap) {
   __shared__ int s_cnt[kThreads / 64][kMaxK];
   __shared__ int s_row[kMaxK];
   __shared__ int s_hist[kMaxE + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = T * k;
-  if ((int)blockIdx.x == T) {
-    if (blockIdx.y != 0) return;
+  if (bx == T) {
+    if (by != 0) return;
     for (int e = tid; e <= E; e += kThreads) s_hist[e] = 0;
     __syncthreads();
     for (int s = tid; s < S; s += kThreads) atomicAdd(&s_hist[key_of(ids[s], E)], 1);
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
     write_tables<kThreads>(s_hist, E, o.offsets, tiles, bm, tile_cap);
     return;
   }
-  const int t = blockIdx.x;
+  const int t = bx;
   for (int i0 = 0; i0 < k; i0 += 8) {
     uint32_t mine[8];
     int cnt[8];
@@ -144,14 +145,14 @@ __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
     for (int w = 0; w < kThreads / 64; ++w) r += s_cnt[w][tid];
     const int v = key_of(ids[f], E) < E ? r : ~r;
     s_row[tid] = v;
-    if (blockIdx.y == 0) {
+    if (by == 0) {
       o.slot_row[f] = v;
       o.row_slot[r] = f;
     }
   }
   if (!x) return;
   __syncthreads();
-  const int64_t c = (int64_t)blockIdx.y * kThreads + tid;
+  const int64_t c = (int64_t)by * kThreads + tid;
   if (c >= units) return;
   const U v = x[(int64_t)t * units + c];
   for (int i = 0; i < k; ++i) {
@@ -160,22 +161,27 @@ __global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
   }
 }
 
+template <typename U>
+__global__ __launch_bounds__(kThreads) void dispatch_small_kernel(
+    const int32_t* __restrict__ ids, int T, int k, int E, const U* __restrict__ x, int64_t units,
+    U* __restrict__ rows, SortOut o, i32x4* tiles, int bm, int tile_cap) {
+  dispatch_small<U>(blockIdx.x, blockIdx.y, ids, T, k, E, x, units, rows, o, tiles, bm, tile_cap);
+}
+
 // ---------------------------------------------------------------- many slots: count, scan, copy
-constexpr int kCountThreads = 512;
-constexpr int kCountWaves = kCountThreads / 64;
+constexpr int kCountWaves = kThreads / 64;
 constexpr int kPerLane = 4;
-constexpr int kChunk = kCountThreads * kPerLane;  // slots a workgroup
+constexpr int kChunk = kThreads * kPerLane;  // slots a workgroup
 
 // rank[s] = how many slots of the chunk ahead of s have its key; hist[chunk][e] = the keys' counts.
 // A wave ranks 64 slots at a time: lanes of equal keys find each other by ballots over the key's
 // bits, the first of them moves the wave's running count.
-__global__ __launch_bounds__(kCountThreads) void dispatch_count_kernel(
-    const int32_t* __restrict__ ids, int S, int E, uint16_t* __restrict__ rank,
-    int32_t* __restrict__ hist) {
+MOE_DEV void dispatch_count(int block, const int32_t* __restrict__ ids, int S, int E,
+                            uint16_t* __restrict__ rank, int32_t* __restrict__ hist) {
   __shared__ int s_cnt[kCountWaves][kMaxE + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int i = tid; i < kCountWaves * (kMaxE + 1); i += kCountThreads) (&s_cnt[0][0])[i] = 0;
-  const int first = blockIdx.x * kChunk + wave * 64 * kPerLane;
+  for (int i = tid; i < kCountWaves * (kMaxE + 1); i += kThreads) (&s_cnt[0][0])[i] = 0;
+  const int first = block * kChunk + wave * 64 * kPerLane;
   int key[kPerLane], local[kPerLane];
 #pragma unroll
   for (int j = 0; j < kPerLane; ++j) {
@@ -201,7 +207,7 @@ __global__ __launch_bounds__(kCountThreads) void dispatch_count_kernel(
     local[j] = before + ahead;
   }
   __syncthreads();
-  for (int e = tid; e <= E; e += kCountThreads) {
+  for (int e = tid; e <= E; e += kThreads) {
     int run = 0;
 #pragma unroll
     for (int w = 0; w < kCountWaves; ++w) {
@@ -209,13 +215,19 @@ __global__ __launch_bounds__(kCountThreads) void dispatch_count_kernel(
       s_cnt[w][e] = run;
       run += n;
     }
-    hist[(int64_t)blockIdx.x * (E + 1) + e] = run;
+    hist[(int64_t)block * (E + 1) + e] = run;
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kPerLane; ++j)
     if (key[j] >= 0)
       rank[first + 64 * j + lane] = (uint16_t)(s_cnt[wave][key[j]] + local[j]);
+}
+
+__global__ __launch_bounds__(kThreads) void dispatch_count_kernel(
+    const int32_t* __restrict__ ids, int S, int E, uint16_t* __restrict__ rank,
+    int32_t* __restrict__ hist) {
+  dispatch_count(blockIdx.x, ids, S, E, rank, hist);
 }
 
 constexpr int kScanThreads = 1024;
@@ -281,6 +293,33 @@ __global__ __launch_bounds__(kThreads) void dispatch_copy_kernel(
   }
 }
 
+// The workspace of many slots: the chunks' counts and the slots' ranks in their chunks.
+struct LargeSort {
+  int chunks;
+  int32_t* hist;
+  uint16_t* rank;
+  LargeSort(int S, int E, void* ws)
+      : chunks((S + kChunk - 1) / kChunk),
+        hist(static_cast<int32_t*>(ws)),
+        rank(reinterpret_cast<uint16_t*>(hist + (int64_t)chunks * (E + 1))) {}
+};
+
+// The scan and the copy behind the chunks' counts.
+template <typename U>
+hipError_t launch_ranked(const LargeSort& w, const int32_t* ids, int T, int k, int E, const U* x,
+                         int64_t units, U* rows, const SortOut& o, i32x4* tiles, int bm,
+                         int tile_cap, hipStream_t s) {
+  hipLaunchKernelGGL(dispatch_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, w.hist, w.chunks, E,
+                     o.offsets, tiles, bm, tile_cap);
+  int tpt_log = 5;
+  while (tpt_log < 8 && (int64_t(1) << tpt_log) < units) ++tpt_log;
+  const int per = kThreads >> tpt_log;
+  const unsigned gy = x ? (unsigned)((units + (1 << tpt_log) - 1) >> tpt_log) : 1u;
+  hipLaunchKernelGGL(dispatch_copy_kernel<U>, dim3((T + per - 1) / per, gy), dim3(kThreads), 0, s,
+                     ids, T, k, E, x, units, rows, o, w.rank, w.hist, tpt_log);
+  return hipGetLastError();
+}
+
 // Slots up to which every workgroup ranks its token's slots itself.
 constexpr int kSmallSlots = 4096;
 
@@ -297,20 +336,53 @@ hipError_t launch_dispatch_units(const int32_t* ids, int T, int k, int E, const 
                        E, xu, units, ru, o, tiles, bm, tile_cap);
     return hipGetLastError();
   }
-  const int chunks = (S + kChunk - 1) / kChunk;
-  int32_t* hist = static_cast<int32_t*>(ws);
-  uint16_t* rank = reinterpret_cast<uint16_t*>(hist + (int64_t)chunks * (E + 1));
-  hipLaunchKernelGGL(dispatch_count_kernel, dim3(chunks), dim3(kCountThreads), 0, s, ids, S, E,
-                     rank, hist);
-  hipLaunchKernelGGL(dispatch_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, hist, chunks, E,
-                     o.offsets, tiles, bm, tile_cap);
-  int tpt_log = 5;
-  while (tpt_log < 8 && (int64_t(1) << tpt_log) < units) ++tpt_log;
-  const int per = kThreads >> tpt_log;
-  const unsigned gy = x ? (unsigned)((units + (1 << tpt_log) - 1) >> tpt_log) : 1u;
-  hipLaunchKernelGGL(dispatch_copy_kernel<U>, dim3((T + per - 1) / per, gy), dim3(kThreads), 0, s,
-                     ids, T, k, E, xu, units, ru, o, rank, hist, tpt_log);
-  return hipGetLastError();
+  const LargeSort w(S, E, ws);
+  hipLaunchKernelGGL(dispatch_count_kernel, dim3(w.chunks), dim3(kThreads), 0, s, ids, S, E, w.rank,
+                     w.hist);
+  return launch_ranked<U>(w, ids, T, k, E, xu, units, ru, o, tiles, bm, tile_cap, s);
+}
+
+// ---------------------------------------------------------------- the experts' first launch
+// Workgroups [0, qblocks) quantise four rows each, the others sort (SMALL: the whole sort, else the
+// chunks' counts): neither waits for the other, and one launch less. 16 tokens of 2048 over 128
+// experts 60.9 -> 55.9 us a call, 4096 tokens 312 -> 309 us. Only where a wave holds a row: a
+// workgroup of 1024 threads a row has no use for the sort's 256.
+template <int DT, int NC, bool VEC, bool SMALL>
+__global__ __launch_bounds__(kThreads) void quantize_and_sort_kernel(
+    const typename Elem<DT>::T* __restrict__ x, int T, int K, int8_t* __restrict__ q,
+    float* __restrict__ scale, int qblocks, const int32_t* __restrict__ ids, int k, int E, SortOut o,
+    uint16_t* __restrict__ rank, int32_t* __restrict__ hist, i32x4* tiles, int bm, int tile_cap) {
+  if ((int)blockIdx.x < qblocks)
+    quantize_rows<DT, 64, NC, VEC>(blockIdx.x, x, T, K, q, scale);
+  else if constexpr (SMALL)
+    dispatch_small<u32x4>(blockIdx.x - qblocks, 0, ids, T, k, E, nullptr, 0, nullptr, o, tiles, bm,
+                          tile_cap);
+  else
+    dispatch_count(blockIdx.x - qblocks, ids, T * k, E, rank, hist);
+}
+
+template <int DT, int NC>
+hipError_t launch_quantize_and_sort_t(const void* x, int T, int K, int8_t* q, float* scale,
+                                      const int32_t* ids, int k, int E, const SortOut& o, void* ws,
+                                      i32x4* tiles, int bm, int tile_cap, hipStream_t s) {
+  const int S = T * k, qblocks = (T + 3) / 4;
+  const bool vec = K % 8 == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  const auto* xt = static_cast<const typename Elem<DT>::T*>(x);
+  const bool small = S <= kSmallSlots;
+  const LargeSort w(S, E, ws);
+  const dim3 grid((unsigned)(qblocks + (small ? T + 1 : w.chunks)));
+#define MOE_QUANT_SORT(V, SM)                                                                    \
+  hipLaunchKernelGGL((quantize_and_sort_kernel<DT, NC, V, SM>), grid, dim3(kThreads), 0, s, xt, T, \
+                     K, q, scale, qblocks, ids, k, E, o, w.rank, w.hist, tiles, bm, tile_cap)
+  if (small) {
+    if (vec) MOE_QUANT_SORT(true, true);
+    else MOE_QUANT_SORT(false, true);
+    return hipGetLastError();
+  }
+  if (vec) MOE_QUANT_SORT(true, false);
+  else MOE_QUANT_SORT(false, false);
+#undef MOE_QUANT_SORT
+  return launch_ranked<u32x4>(w, ids, T, k, E, nullptr, 1, nullptr, o, tiles, bm, tile_cap, s);
 }
 
 // ---------------------------------------------------------------- combine
@@ -517,6 +589,30 @@ hipError_t launch_dispatch(const int32_t* ids, int T, int k, int E, const void* 
                                            tile_cap, s);
   return launch_dispatch_units<uint16_t>(ids, T, k, E, x, row_bytes / 2, rows, o, ws, tiles, bm,
                                          tile_cap, s);
+}
+
+hipError_t launch_quantize_and_sort(const void* x, int T, int K, int dtype, int8_t* q, float* scale,
+                                    const int32_t* ids, int k, int E, int32_t* offsets,
+                                    int32_t* row_slot, int32_t* slot_row, void* ws, i32x4* tiles,
+                                    int bm, int tile_cap, hipStream_t s) {
+  const SortOut o{offsets, row_slot, slot_row};
+  if (K > 2048) {
+    const hipError_t e = launch_quantize(x, T, K, dtype, q, scale, s);
+    if (e != hipSuccess) return e;
+    return launch_dispatch(ids, T, k, E, nullptr, 16, nullptr, offsets, row_slot, slot_row, ws, tiles,
+                           bm, tile_cap, s);
+  }
+#define MOE_QUANT_SORT_DT(DT)                                                                     \
+  (K <= 512    ? launch_quantize_and_sort_t<DT, 1>(x, T, K, q, scale, ids, k, E, o, ws, tiles, bm, \
+                                                   tile_cap, s)                                   \
+   : K <= 1024 ? launch_quantize_and_sort_t<DT, 2>(x, T, K, q, scale, ids, k, E, o, ws, tiles, bm, \
+                                                   tile_cap, s)                                   \
+               : launch_quantize_and_sort_t<DT, 4>(x, T, K, q, scale, ids, k, E, o, ws, tiles, bm, \
+                                                   tile_cap, s))
+  if (dtype == kBf16) return MOE_QUANT_SORT_DT(kBf16);
+  if (dtype == kFp16) return MOE_QUANT_SORT_DT(kFp16);
+  return MOE_QUANT_SORT_DT(kFp32);
+#undef MOE_QUANT_SORT_DT
 }
 
 hipError_t launch_combine(const void* rows, int T, int k, int H, int dtype,

@@ -1,7 +1,7 @@
 // The int8 products' kernels as the entry points see them.
 #pragma once
 
-#include "common.h"
+#include "elem.h"
 
 // a rows [rows][K] with a scale each; b [N][K] with a scale per channel, of one expert or of all
 // of them, N * K bytes apart. Output row r of a tile comes from a's row row_src[r] / src_div (r
@@ -68,9 +68,60 @@ MOE_DEV uint32_t bfly_umax(uint32_t v) {
   return max(v, __float_as_uint(xor_partner<1>(__uint_as_float(v))));
 }
 
+// The rows of one workgroup: NT threads a row, NC chunks of 8 NT columns.
+template <int DT, int NT, int NC, bool VEC>
+MOE_DEV void quantize_rows(int block, const typename Elem<DT>::T* __restrict__ x, int T, int K,
+                           int8_t* __restrict__ q, float* __restrict__ scale) {
+  using C = Cols<DT, NT, VEC>;
+  __shared__ uint32_t s_max[NT / 64];
+  const int tid = threadIdx.x % NT;
+  constexpr int kRows = NT < 256 ? 256 / NT : 1;
+  const int64_t t = (int64_t)block * kRows +
+                    __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
+  if (t >= T) return;  // a whole wave (NT = 64, no barrier below), or never
+  float v[NC][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) C::load(x + t * K + c * 8 * NT, tid, K - c * 8 * NT, v[c]);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[c][e]));
+  top = bfly_umax(top);
+  if constexpr (NT > 64) {
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) top = max(top, s_max[w]);
+  }
+  if (tid == 0) scale[t] = Quantizer::scale(top);
+  const Quantizer quant(top);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    int8_t* p = q + t * K + c * 8 * NT;
+    const int left = K - c * 8 * NT;
+    if constexpr (VEC) {
+      const float (&x8)[8] = v[c];
+      if (8 * tid < left)
+        *reinterpret_cast<u32x2*>(p + 8 * tid) =
+            u32x2{quant.four(x8[0], x8[1], x8[2], x8[3]), quant.four(x8[4], x8[5], x8[6], x8[7])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (tid + NT * e < left) p[tid + NT * e] = quant.one(v[c][e]);
+    }
+  }
+}
+
 // Quantise rows of the dtype to int8 with a scale each.
 hipError_t launch_quantize(const void* x, int T, int K, int dtype, int8_t* q, float* scale,
                            hipStream_t s);
+// launch_quantize of x [T][K] and launch_dispatch's tables (no rows), which do not depend on each
+// other, in one launch where a wave holds a row (K <= 2048), two or three otherwise.
+hipError_t launch_quantize_and_sort(const void* x, int T, int K, int dtype, int8_t* q, float* scale,
+                                    const int32_t* ids, int k, int E, int32_t* offsets,
+                                    int32_t* row_slot, int32_t* slot_row, void* ws, i32x4* tiles,
+                                    int bm, int tile_cap, hipStream_t s);
 // The kernel of a product and its rows per tile (the bm of an expert table).
 enum { kInt8Stream = 0, kInt8Ring = 1, kInt8Tile = 2 };
 struct Int8Plan {

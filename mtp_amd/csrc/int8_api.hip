@@ -110,13 +110,14 @@ int moe_quantize_tokens_v1(const void* x, int32_t T, int32_t K, int32_t dtype, i
                            float* scale, void* stream) {
   const int rc = check_dtype("quantize", dtype);
   if (rc) return rc;
-  if (T < 0 || T > (1 << 22) || K < 1 || K > kMaxK)
-    return op_fail(MOE_ERR_SHAPE, "quantize: T=%d K=%d (T <= 2^22, K in [1, 65536])", T, K);
+  if (T < 0 || T >= (1 << 22) || K < 1 || K > kMaxK)  // a launch has fewer than 2^32 threads
+    return op_fail(MOE_ERR_SHAPE, "quantize: T=%d K=%d (T < 2^22, K in [1, 65536])", T, K);
   if (T == 0) return MOE_OK;
   if (!x || !q || !scale) return op_fail(MOE_ERR_NULL, "quantize: NULL pointer");
   if (overlaps(q, (int64_t)T * K, x, (int64_t)T * K * dtype_bytes(dtype)) ||
-      overlaps(scale, (int64_t)T * 4, x, (int64_t)T * K * dtype_bytes(dtype)))
-    return op_fail(MOE_ERR_SHAPE, "quantize: outputs must not overlap x");
+      overlaps(scale, (int64_t)T * 4, x, (int64_t)T * K * dtype_bytes(dtype)) ||
+      overlaps(scale, (int64_t)T * 4, q, (int64_t)T * K))
+    return op_fail(MOE_ERR_SHAPE, "quantize: x and the outputs must not overlap");
   MOE_OP_HIP(launch_quantize(x, T, K, dtype, q, scale, (hipStream_t)stream), "quantize");
   return MOE_OK;
 }
@@ -223,11 +224,11 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
   int8_t* hq = at<int8_t>(workspace, L.hq);
   float* hs = at<float>(workspace, L.hs);
   void* y = at<void>(workspace, L.y);
-  MOE_OP_HIP(launch_quantize(x, T, H, dtype, q, qs, s), "quantize");
-  MOE_OP_HIP(launch_dispatch(topk_ids, T, top_k, E, nullptr, 16, nullptr,
-                             at<int32_t>(workspace, L.offsets), row_slot, slot_row,
-                             at<void>(workspace, L.scratch), tiles, L.plan.bm, L.tile_cap, s),
-             "sort");
+  MOE_OP_HIP(launch_quantize_and_sort(x, T, H, dtype, q, qs, topk_ids, top_k, E,
+                                      at<int32_t>(workspace, L.offsets), row_slot, slot_row,
+                                      at<void>(workspace, L.scratch), tiles, L.plan.bm, L.tile_cap,
+                                      s),
+             "quantize and sort");
   Int8Args a{};
   a.a = q;
   a.a_scale = qs;
