@@ -106,7 +106,9 @@ SHAPES = [  # T, K, N, dtype, bias
     (130, 512, 511, torch.bfloat16, True), (203, 1040, 2001, torch.float16, True),
     (257, 128, 256, torch.bfloat16, False), (300, 2064, 640, torch.float32, False),
     (513, 1552, 1000, torch.bfloat16, True), (1030, 256, 514, torch.float16, False),
-    (2048, 2048, 2048, torch.bfloat16, False), (1100, 1168, 2500, torch.bfloat16, False)]
+    (2048, 2048, 2048, torch.bfloat16, False), (1100, 1168, 2500, torch.bfloat16, False),
+    (3000, 272, 3001, torch.float32, True), (2990, 80, 3000, torch.bfloat16, False),
+    (4099, 272, 3001, torch.float16, True), (5001, 144, 2500, torch.bfloat16, False)]
 
 
 @pytest.mark.parametrize("T,K,N,dtype,bias", SHAPES)
@@ -242,18 +244,23 @@ def test_experts(T, k, E, H, I, dtype):
     assert float(got[dropped].abs().sum()) == 0.0
 
 
-def test_experts_equal_their_parts():
+@pytest.mark.parametrize("T,k,E,H,I", [
+    (90, 4, 6, 64, 32), (11, 8, 70, 2064, 48), (600, 8, 5, 2064, 48), (1024, 4, 64, 144, 512),
+    (1500, 3, 5, 272, 1008), (2048, 4, 4, 144, 512), (1300, 8, 40, 96, 1552)])
+def test_experts_equal_their_parts(T, k, E, H, I):
     """Rows whose h is the same give what dispatch, int8_matmul over each expert's rows, and combine
     give: with gates so large that silu(g) = g exactly and up sums that make h exact in the type."""
-    T, k, E, H, I = 90, 4, 6, 64, 32
+    gen = torch.Generator().manual_seed(T)
     ex = make_experts(E, H, I, 9).to("cuda")
-    ids = torch.randint(0, E, (T, k), dtype=torch.int32).cuda()
-    w = torch.rand(T, k).cuda()
+    ids = torch.randint(-1, E, (T, k), generator=gen, dtype=torch.int32).cuda()
+    w = torch.rand(T, k, generator=gen).cuda()
     x = torch.zeros(T, H, dtype=torch.float32, device="cuda")
     x[:, 0] = 127.0  # q = (127, 0, ...): g = gate[e, :, 0] * 127 * scale
+    x[:, H - 1] = torch.randint(-127, 128, (T,), generator=gen).float().cuda()
     gate, up = torch.zeros_like(ex.gate), torch.zeros_like(ex.up)
     gate[:, :, 0] = 64
-    up[:, :, 0] = torch.randint(-127, 128, (E, I), dtype=torch.int8).cuda()
+    up[:, :, 0] = torch.randint(-127, 128, (E, I), generator=gen, dtype=torch.int8).cuda()
+    up[:, :, H - 1] = torch.randint(-127, 128, (E, I), generator=gen, dtype=torch.int8).cuda()
     one = torch.ones(E, I, device="cuda")
     ex = Int8Experts(gate, one, up, one / 127, ex.down, ex.down_scale)
     got = ops.int8_experts(x, ids, w, ex)

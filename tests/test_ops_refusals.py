@@ -101,6 +101,8 @@ A, B, C, D, G, W = (0x1000000 * i for i in range(1, 7))  # never dereferenced
     (SHAPE, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, D, B, None)),
     (SHAPE, "moe_quantize_tokens_v1", (A, 4, 65537, 0, B, C)),
     (SHAPE, "moe_quantize_tokens_v1", (A, 4, 64, 0, A + 8, C)),
+    (SHAPE, "moe_quantize_tokens_v1", (A, 4, 64, 0, B, B + 128)),
+    (SHAPE, "moe_quantize_tokens_v1", (A, 1 << 22, 16384, 0, B, C)),
     (NULL, "moe_quantize_tokens_v1", (A, 4, 64, 0, None, C)),
     (SHAPE, "moe_int8_matmul_v1", (A, B, 4, 40, C, D, 8, None, 0, G)),
     (SHAPE, "moe_int8_matmul_v1", (A, B, 4, 65552, C, D, 8, None, 0, G)),
