@@ -503,12 +503,15 @@ __global__ __launch_bounds__(kThreads) void int8_ring_kernel(Int8Args a, int vec
   }
   auto stage = [&](int8_t* lds, int k0) {
     const uint32_t out = k0 + (int)kc < a.K ? 0u : kOutOfRange;  // zeros past K
+    // The bounds check takes the scalar offset off the buffer's size, so it stays inside it: a step
+    // past K of a small matrix could lie behind its end.
+    const uint32_t soff = k0 < a.K ? (uint32_t)k0 : 0u;
 #pragma unroll
     for (int j = 0; j < LB; ++j)
-      buf_ld128_lds(rb, lds + BM * BK + (j * kThreads + wave * 64) * 16, boff[j] | out, (uint32_t)k0);
+      buf_ld128_lds(rb, lds + BM * BK + (j * kThreads + wave * 64) * 16, boff[j] | out, soff);
 #pragma unroll
     for (int j = 0; j < LA; ++j)
-      buf_ld128_lds(ra, lds + (j * kThreads + wave * 64) * 16, aoff[j] | out, (uint32_t)k0);
+      buf_ld128_lds(ra, lds + (j * kThreads + wave * 64) * 16, aoff[j] | out, soff);
     __builtin_amdgcn_sched_barrier(0);
   };
   if (tid < BM)

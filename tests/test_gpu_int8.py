@@ -100,7 +100,8 @@ SHAPES = [  # T, K, N, dtype, bias
     (7, 4224, 24, torch.bfloat16, True), (8, 6160, 40, torch.bfloat16, False),
     (9, 320, 8193, torch.float32, False), (3, 272, 19, torch.float32, False),
     (2, 48, 33, torch.float16, True), (15, 1040, 100, torch.bfloat16, True),
-    (16, 64, 64, torch.float32, False), (17, 80, 65, torch.float16, False),
+    (16, 64, 64, torch.float32, False), (17, 16, 1, torch.bfloat16, False),
+    (20, 32, 7, torch.float16, True), (80, 16, 3, torch.float32, False), (17, 80, 65, torch.float16, False),
     (31, 2048, 96, torch.float32, True), (33, 144, 200, torch.bfloat16, False),
     (64, 4096, 130, torch.bfloat16, False), (65, 272, 257, torch.float16, True),
     (130, 512, 511, torch.bfloat16, True), (203, 1040, 2001, torch.float16, True),
