@@ -514,8 +514,8 @@ def _rows_2d(x: torch.Tensor, name: str) -> int:
     """The dtype code of a [rows, columns] tensor of a supported type."""
     if x.dtype not in OUT_DTYPES:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.ndim != 2:
-        raise ValueError(f"{name} must be 2D, got {tuple(x.shape)}")
+    if x.ndim != 2 or max(x.shape) >= 1 << 31:  # sizes are int32 in the library
+        raise ValueError(f"{name} must be 2D with sizes below 2^31, got {tuple(x.shape)}")
     return OUT_DTYPES[x.dtype]
 
 
@@ -600,8 +600,11 @@ def dispatch_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -
     _rows_2d(x, "x")
     if topk_ids.dtype != torch.int32 or topk_ids.ndim != 2:
         raise TypeError("topk_ids must be int32 [T, k]")
-    if topk_ids.shape[0] != x.shape[0]:
-        raise ValueError(f"topk_ids has {topk_ids.shape[0]} rows for {x.shape[0]} tokens")
+    if topk_ids.shape[0] != x.shape[0] or topk_ids.shape[1] > 64:
+        raise ValueError(f"topk_ids must be [{x.shape[0]}, k] with k <= 64, got "
+                         f"{tuple(topk_ids.shape)}")
+    if not 1 <= num_experts <= 512:
+        raise ValueError(f"num_experts must lie in [1, 512], got {num_experts}")
     _require_gpu(x, topk_ids)
     if torch.is_grad_enabled() and x.requires_grad:
         return Dispatch(*_DispatchFn.apply(x, topk_ids, int(num_experts)))
@@ -614,8 +617,9 @@ def combine_tokens(rows: torch.Tensor, slot_row: torch.Tensor,
     rows[slot_row[t, i]] over the kept slots, in slot order in fp32, rounded once to rows' type.
 
     rows [T * k, H] and slot_row int32 [T, k] as ``dispatch_tokens`` gives them (every row belongs
-    to one slot), topk_weights fp32 [T, k]. What a dropped slot's row and weight hold is not looked
-    at. Differentiable in rows (dropped slots' rows: zeros) and in topk_weights."""
+    to one slot; a slot is dropped by giving ``dispatch_tokens`` an id outside the experts, not by
+    changing slot_row), topk_weights fp32 [T, k]. What a dropped slot's row and weight hold is not
+    looked at. Differentiable in rows (dropped slots' rows: zeros) and in topk_weights."""
     _rows_2d(rows, "rows")
     if slot_row.dtype != torch.int32 or topk_weights.dtype != torch.float32:
         raise TypeError("slot_row must be int32 and topk_weights float32")
@@ -652,6 +656,8 @@ def _check_int8(weight, weight_scale, bias, K: int, dtype: torch.dtype) -> None:
     if weight.ndim != 2 or weight.shape[1] != K or tuple(weight_scale.shape) != weight.shape[:1]:
         raise ValueError(f"weight must be [N, {K}] and weight_scale [N], got "
                          f"{tuple(weight.shape)} and {tuple(weight_scale.shape)}")
+    if max(weight.shape) >= 1 << 31:
+        raise ValueError(f"weight's sizes must be below 2^31, got {tuple(weight.shape)}")
     if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != weight.shape[:1]):
         raise ValueError(f"bias must be {dtype} [N]")
 
@@ -669,8 +675,8 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor,
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     if q.dtype != torch.int8 or q_scale.dtype != torch.float32:
         raise TypeError("q must be int8 and q_scale float32")
-    if q.ndim != 2 or tuple(q_scale.shape) != q.shape[:1]:
-        raise ValueError("q must be [T, K] and q_scale [T]")
+    if q.ndim != 2 or tuple(q_scale.shape) != q.shape[:1] or q.shape[0] >= 1 << 31:
+        raise ValueError("q must be [T, K] with T below 2^31 and q_scale [T]")
     T, K = q.shape
     _check_int8(weight, weight_scale, bias, K, dtype)
     _require_gpu(q, q_scale, weight, weight_scale, bias)

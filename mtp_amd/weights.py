@@ -225,8 +225,11 @@ class Int8Experts:
         for w in (gate, up, down):
             if w.ndim != 3:
                 raise ValueError(f"expert stacks must be 3D, got {tuple(w.shape)}")
-            q, scale = ops.quantize_tokens(w.reshape(-1, w.shape[2]).contiguous())
-            parts += [q.view(w.shape), scale.view(w.shape[:2])]
+            q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
+            scale = torch.empty(w.shape[:2], dtype=torch.float32, device=w.device)
+            for i in range(w.shape[0]):
+                q[i], scale[i] = ops.quantize_tokens(w[i].contiguous())
+            parts += [q, scale]
         return cls(*parts)
 
     @classmethod

@@ -272,3 +272,22 @@ def test_layer_step_of_the_operators():
     want = torch.autograd.grad(plain(*ref), ref, v.double())
     for a, b in zip(got, want):
         assert float((a.cpu().double() - b).abs().max()) <= 2.0 ** -12 * float(b.abs().max())
+
+
+def test_tensors_beyond_4_gib():
+    """Rows do not depend on each other: the last rows of tensors of more than 2^32 bytes (4.3 GB of
+    bf16), and their gradients, are those of a call on these rows alone."""
+    T, H, last = (1 << 21) + 5, 1032, 700
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    y = torch.randn(T, H, generator=gen, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    assert y.numel() * 2 > 1 << 32
+    w = (torch.randn(H, generator=gen, device="cuda") / 8).to(torch.bfloat16)
+
+    def run(t):
+        res, gate = t.detach() * 0.5, t.detach()[:, :1].contiguous()
+        r, x = ops.block_norm(t, res, post_w=w, pre_w=w, gate=gate)
+        return (r.detach(), x.detach(), *torch.autograd.grad((r, x), t, (res, res)))
+
+    full = [t[-last:].clone() for t in run(y)]
+    part = run(y.detach()[-last:].clone().requires_grad_())
+    assert all(torch.equal(a, b) for a, b in zip(full, part))

@@ -255,3 +255,36 @@ def test_two_streams_and_graph_replays():
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b.detach()) for a, b in zip(held, want))
+
+
+def test_rows_beyond_4_gib():
+    """The copies and sums of a routing whose rows take more than 2^32 bytes (4.4 GB of bf16), against
+    the same values gathered and summed for some of the tokens."""
+    T, k, E, H = 1 << 17, 8, 64, 2096
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.randint(-1, E, (T, k), generator=gen, dtype=torch.int32, device="cuda")
+    x = torch.randn(T, H, generator=gen, dtype=torch.bfloat16, device="cuda")
+    w = torch.rand(T, k, generator=gen, device="cuda")
+    d = ops.dispatch_tokens(x, ids, E)
+    assert d.rows.numel() * 2 > 1 << 32
+    want = plain_tables(ids.cpu(), E)
+    for a, b in zip((d.offsets, d.row_slot, d.slot_row), want):
+        assert torch.equal(a.cpu().long(), b)
+    kept = int(d.offsets[-1])
+    for a in range(0, T * k, 1 << 17):
+        slots = d.row_slot[a:a + (1 << 17)].long()
+        rows = x[slots // k]
+        rows[max(kept - a, 0):] = 0
+        assert torch.equal(d.rows[a:a + (1 << 17)], rows)
+    out = ops.combine_tokens(d.rows, d.slot_row, w)
+    some = torch.cat([torch.arange(512), torch.arange(T - 512, T)]).cuda()
+    part = ops.dispatch_tokens(x[some], ids[some], E)
+    assert torch.equal(out[some], ops.combine_tokens(part.rows, part.slot_row, w[some]))
+    rows, wl = d.rows.requires_grad_(), w.clone().requires_grad_()
+    drows, dw = torch.autograd.grad(ops.combine_tokens(rows, d.slot_row, wl), (rows, wl), x)
+    prows, pw = part.rows.requires_grad_(), w[some].requires_grad_()
+    pdrows, pdw = torch.autograd.grad(ops.combine_tokens(prows, part.slot_row, pw), (prows, pw),
+                                      x[some])
+    assert torch.equal(dw[some], pdw)
+    at, pat = d.slot_row[some].long().view(-1), part.slot_row.long().view(-1)
+    assert torch.equal(drows[torch.where(at < 0, ~at, at)], pdrows[torch.where(pat < 0, ~pat, pat)])

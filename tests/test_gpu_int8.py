@@ -347,3 +347,31 @@ def test_from_gptq_and_moe_block():
     assert torch.equal(y8.view(40, 512), flat)
     assert torch.equal(b8.moe_tokens(x, ids8.view(2, 20, 4), w8.view(2, 20, 4)), y8)
     assert float((y8.float() - y4.float()).abs().max() / y4.float().abs().max()) < 0.05
+
+
+def test_weights_and_outputs_beyond_4_gib():
+    """The last experts of stacks of more than 2^32 bytes give what they give as a set of their own,
+    and the last rows of an output of more than 2^32 bytes what they give alone."""
+    E, H, I, T, k = 300, 4096, 3584, 40, 3
+    gen = torch.Generator(device="cuda").manual_seed(1)
+
+    def weights(*shape):
+        return torch.randint(-127, 128, shape, generator=gen, dtype=torch.int8, device="cuda")
+
+    parts = []
+    for n, K in ((I, H), (I, H), (H, I)):
+        parts += [weights(E, n, K), torch.rand(E, n, generator=gen, device="cuda") / 8192]
+    assert parts[0].numel() > 1 << 32
+    last = Int8Experts(*(t[-4:].clone() for t in parts))
+    x = torch.randn(T, H, generator=gen, dtype=torch.bfloat16, device="cuda")
+    ids = torch.randint(0, 4, (T, k), generator=gen, dtype=torch.int32, device="cuda")
+    w = torch.rand(T, k, generator=gen, device="cuda")
+    assert torch.equal(ops.int8_experts(x, ids + (E - 4), w, Int8Experts(*parts)),
+                       ops.int8_experts(x, ids, w, last))
+    del parts
+    T, K, N = 66000, 64, 32776
+    x = torch.randn(T, K, generator=gen, dtype=torch.bfloat16, device="cuda")
+    wq, ws = weights(N, K), torch.rand(N, generator=gen, device="cuda")
+    out = ops.int8_linear(x, wq, ws)
+    assert out.numel() * 2 > 1 << 32
+    assert torch.equal(out[-300:], ops.int8_linear(x[-300:].clone(), wq, ws))

@@ -24,6 +24,12 @@ def z(*shape, dtype=F):
     (lambda: ops.dispatch_tokens(z(4, 8), z(4, 2, dtype=torch.int64), 8), TypeError),
     (lambda: ops.dispatch_tokens(z(4, 8), z(3, 2, dtype=I), 8), ValueError),
     (lambda: ops.dispatch_tokens(z(4, 8), z(4, 2, dtype=I), 8), ValueError),  # host tensors
+    (lambda: ops.dispatch_tokens(z(4, 8), z(4, 65, dtype=I), 8), ValueError),
+    (lambda: ops.dispatch_tokens(z(4, 8), z(4, 2, dtype=I), 0), ValueError),
+    (lambda: ops.dispatch_tokens(z(4, 8), z(4, 2, dtype=I), 2 ** 32 + 8), ValueError),
+    (lambda: ops.quantize_tokens(z(1, 1).expand(2 ** 32 + 1, 1)), ValueError),
+    (lambda: ops.int8_linear(z(4, 16), torch.zeros(1, 16, dtype=torch.int8).expand(2 ** 31, 16),
+                             torch.zeros(1).expand(2 ** 31)), ValueError),
     (lambda: ops.combine_tokens(z(8, 8), z(4, 2, dtype=I), z(4, 2)), TypeError),
     (lambda: ops.combine_tokens(z(8, 8), z(4, 2, dtype=I), torch.zeros(4, 3)), ValueError),
     (lambda: ops.combine_tokens(z(7, 8), z(4, 2, dtype=I), torch.zeros(4, 2)), ValueError),
@@ -94,11 +100,19 @@ A, B, C, D, G, W = (0x1000000 * i for i in range(1, 7))  # never dereferenced
     (NULL, "moe_combine_v1", (A, 4, 8, 64, 0, None, B, C)),
     (SHAPE, "moe_combine_v1", (A, 4, 8, 64, 0, D, B, A + 128)),
     (SHAPE, "moe_combine_v1", (A, 4, 8, 65537, 0, D, B, C)),
+    (SHAPE, "moe_combine_v1", (A, 4, 8, 64, 0, C + 64, B, C)),
+    (SHAPE, "moe_combine_v1", (A, 4, 8, 64, 0, D, C + 64, C)),
+    (SHAPE, "moe_dispatch_v1", (A, 4, 64, 0, B, 8, 16, None, 0, C, D, G, B)),
+    (SHAPE, "moe_dispatch_v1", (A, 4, 64, 0, B, 8, 16, None, 0, C, B + 64, G, W)),
+    (SHAPE, "moe_dispatch_v1", (A, 600, 64, 0, B, 8, 16, A + 1024, 1 << 30, C, D, G, W)),
     (UNSUP, "moe_combine_v1", (A, 4, 8, 64, -1, D, B, C)),
     (NULL, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, D, None, None)),
     (NULL, "moe_combine_backward_v1", (A, None, 4, 8, 64, 0, C, D, None, G)),
     (NULL, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, None, G, None)),
     (SHAPE, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, D, B, None)),
+    (SHAPE, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, D, G, D)),
+    (SHAPE, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, D, G, C)),
+    (SHAPE, "moe_combine_backward_v1", (A, B, 4, 8, 64, 0, C, D, G, G + 256)),
     (SHAPE, "moe_quantize_tokens_v1", (A, 4, 65537, 0, B, C)),
     (SHAPE, "moe_quantize_tokens_v1", (A, 4, 64, 0, A + 8, C)),
     (SHAPE, "moe_quantize_tokens_v1", (A, 4, 64, 0, B, B + 128)),
