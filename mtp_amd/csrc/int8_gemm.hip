@@ -662,10 +662,11 @@ hipError_t launch_product_t(const Int8Args& a, Int8Plan plan, bool silu, hipStre
 }  // namespace
 
 // Rows a tile by the rows an expert has on average (hidden 2048, intermediate 512, 256 experts, top-8,
-// us a layer with tiles of 64 / 128 / 256 rows): 512 tokens 184 / 191 / 207, 2048 tokens 248 / 244 /
-// 261, 4096 tokens 349 / 320 / 328, 8192 tokens 564 / 489 / 458. Where few experts share the rows
-// the larger tiles also have to be enough for the chip (4096 rows of 8 experts of 2048 x 1024: 105 /
-// 101 / 90, 4000 rows of 8 experts of 512 x 128: 34 / 36 / 44).
+// us a layer with tiles of 64 / 128 / 256 rows): 512 tokens 173 / 180 / 196, 2048 tokens 238 / 234 /
+// 251, 4096 tokens 339 / 310 / 319, 8192 tokens 552 / 484 / 453. Where few experts share the rows the
+// larger tiles also have to be enough for the chip: 8192 rows over 8 experts of 2048 x 1024 106 / 101 /
+// 82 (256 tiles of 256 rows), 4096 rows over 16 of them 93 / 80 / 67 (128 tiles), over 8 of 2048 x 512
+// 57 / 47 / 59 (64 tiles), 4000 rows over 8 of 512 x 128 24 / 27 / 35.
 Int8Plan int8_experts_plan(int64_t slots, int E, int I) {
   const int64_t rows = (slots + E - 1) / E;
   if (rows >= 192 && slots / 256 * ((I + 127) / 128) >= 96) return Int8Plan{kInt8Tile, 256};

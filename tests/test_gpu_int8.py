@@ -311,6 +311,39 @@ def test_experts_graph_streams_and_workspace(T):
         assert torch.equal(ops.int8_experts(xs[i], ids[i], w, ex), want[i])
 
 
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_linear_in_a_graph(T):
+    """A captured linear layer replayed on new inputs between eager calls gives the eager results: the
+    fused kernel, and the ones that keep quantised rows in a workspace."""
+    w, ws = make_weight(130, 272, T)
+    w, ws = w.cuda(), ws.cuda()
+    xs = [torch.randn(T, 272).to(torch.bfloat16).cuda() for _ in range(2)]
+    want = [ops.int8_linear(x, w, ws) for x in xs]
+    x0 = xs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.int8_linear(x0, w, ws)
+    for i in (1, 0, 1):
+        x0.copy_(xs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+        assert torch.equal(ops.int8_linear(xs[i], w, ws), want[i])
+
+
+@pytest.mark.parametrize("T", [5, 700])
+def test_experts_of_unaligned_rows(T):
+    ex = make_experts(9, 96, 48, 3).to("cuda")
+    x = torch.randn(T, 96).to(torch.float16).cuda()
+    buf = torch.empty(T * 96 + 1, dtype=torch.float16, device="cuda")
+    xo = buf[1:].view(T, 96)
+    xo.copy_(x)
+    ids = torch.randint(0, 9, (T, 8), dtype=torch.int32).cuda()
+    w = torch.rand(T, 8).cuda()
+    assert torch.equal(ops.int8_experts(xo, ids, w, ex), ops.int8_experts(x, ids, w, ex))
+
+
 def test_no_tokens():
     ex = make_experts(4, 64, 32, 1).to("cuda")
     x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
