@@ -16,8 +16,8 @@
 // HBM-bound in both directions: every tensor is read and written once, 8 columns a thread held in
 // registers across the reductions. A row takes a wave up to 512 columns, a workgroup of 256 threads
 // up to 2048, of 512 up to 4096, of 1024 up to 8192. Sums are taken in a fixed order: in fp32 per
-// thread over its columns, in fp64 in a butterfly in each wave and over the waves; the weights'
-// gradients in fp32 per workgroup over its rows, then over the workgroups.
+// thread over its columns, then in a butterfly in each wave and over the waves, where squares are summed
+// in fp64; the weights' gradients in fp32 per workgroup over its rows, then over the workgroups.
 #include <algorithm>
 #include <initializer_list>
 
@@ -30,29 +30,32 @@ namespace {
 constexpr int kMaxHidden = 8192;
 enum { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateFull = 3 };
 
-// Lane i's partner value for a butterfly over doubles.
+// The value of lane i ^ M.
 template <int M>
-MOE_DEV double xor_partner64(double v) {
+MOE_DEV double partner(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
   const uint32_t lo = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)b)));
   const uint32_t hi = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)(b >> 32))));
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Sums of N values over the NT threads of a row (all threads get them), in 64 bits: the norms'
-// factors come out within half an fp32 step of exact ones, at a cost that HBM's time hides. NT = 64:
-// no barrier.
-template <int NT, int N>
-MOE_DEV void row_sums(const float (&part)[N], double (&v)[N], double (*s_part)[N]) {
+template <int M>
+MOE_DEV float partner(float v) { return xor_partner<M>(v); }
+
+// Sums of N values over the NT threads of a row (all threads get them). A is double for the sums of
+// squares, so that the norms' factors come out within half an fp32 step of exact ones, at a cost that
+// HBM's time mostly hides; float for the means that the gradients subtract. NT = 64: no barrier.
+template <int NT, int N, class A>
+MOE_DEV void row_sums(const float (&part)[N], A (&v)[N], A (*s_part)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     v[i] = part[i];
-    v[i] += xor_partner64<32>(v[i]);
-    v[i] += xor_partner64<16>(v[i]);
-    v[i] += xor_partner64<8>(v[i]);
-    v[i] += xor_partner64<4>(v[i]);
-    v[i] += xor_partner64<2>(v[i]);
-    v[i] += xor_partner64<1>(v[i]);
+    v[i] += partner<32>(v[i]);
+    v[i] += partner<16>(v[i]);
+    v[i] += partner<8>(v[i]);
+    v[i] += partner<4>(v[i]);
+    v[i] += partner<2>(v[i]);
+    v[i] += partner<1>(v[i]);
   }
   if constexpr (NT > 64) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -64,7 +67,7 @@ MOE_DEV void row_sums(const float (&part)[N], double (&v)[N], double (*s_part)[N
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = 0.0;
+      v[i] = A(0);
 #pragma unroll
       for (int w = 0; w < NT / 64; ++w) v[i] += s_part[w][i];
     }
@@ -168,7 +171,7 @@ struct NormGrads {
 };
 
 // The next row's loads are in flight while a row is worked on (two reductions with their barriers):
-// 16384 x 2048 bf16 with both norms and a channel gate 140 -> 88 us, 4.6 TB/s.
+// 16384 x 2048 bf16 with both norms and a channel gate 140 -> 87 us, 4.6 TB/s.
 template <int DT, int NT, bool VEC>
 __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kernel(NormArgs a,
                                                                                   NormGrads d) {
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
   using C = Cols<DT, NT, VEC>;
   using Raw = RawCols<DT, NT, VEC>;
   __shared__ double s3[NT / 64][3];
-  __shared__ double s2[NT / 64][2];
+  __shared__ float s2[NT / 64][2];
   const double inv_h = 1.0 / (double)a.H;
   const int tid = threadIdx.x % NT, H = a.H;
   const int rows = block_threads<NT>() / NT;
@@ -303,13 +306,13 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
       at(1, agate, true);
     }
     const bool token = a.gate_kind == kGateToken && d.dgate;
-    double tot[2] = {0.0, 0.0};
+    float tot[2] = {0.0f, 0.0f};
     if (post || token) row_sums<NT>(some, tot, s2);
-    if (token && tid == 0) static_cast<T*>(d.dgate)[t] = Elem<DT>::put((float)tot[1]);
+    if (token && tid == 0) static_cast<T*>(d.dgate)[t] = Elem<DT>::put(tot[1]);
     if (full) C::store(static_cast<T*>(d.dgate) + t * H, tid, H, dg);
     if (d.dy) {
       if (post) {
-        const float m = (float)(tot[0] * inv_h) * q;
+        const float m = (tot[0] * (float)inv_h) * q;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           dp[e] = q * (dp[e] - (row.y.get(e, tid, H) * q) * m);
