@@ -497,11 +497,11 @@ def predictor_topk(h: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, top_k: i
 # ----------------------------------------------------------------------------- by expert and back
 def _call(entry: str, device: torch.device, *args) -> None:
     """An entry point on ``device`` (which need not be the current one) and its current stream.
-    The raw stream query takes 0.1 us; torch.cuda.current_stream builds an object in 3 us, a
-    quarter of a small call's time on the host."""
+    The raw queries take 0.1 us; torch.cuda.current_stream builds an object in 3 us, a quarter of a
+    small call's time on the host, and torch.cuda.current_device takes 3 us on autograd's thread."""
     fn = getattr(_lib.load(), entry)
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
@@ -512,11 +512,13 @@ def _call(entry: str, device: torch.device, *args) -> None:
 
 def _rows_2d(x: torch.Tensor, name: str) -> int:
     """The dtype code of a [rows, columns] tensor of a supported type."""
-    if x.dtype not in OUT_DTYPES:
+    code = OUT_DTYPES.get(x.dtype)
+    if code is None:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.ndim != 2 or max(x.shape) >= 1 << 31:  # sizes are int32 in the library
-        raise ValueError(f"{name} must be 2D with sizes below 2^31, got {tuple(x.shape)}")
-    return OUT_DTYPES[x.dtype]
+    shape = x.shape
+    if len(shape) != 2 or shape[0] >> 31 or shape[1] >> 31:  # sizes are int32 in the library
+        raise ValueError(f"{name} must be 2D with sizes below 2^31, got {tuple(shape)}")
+    return code
 
 
 class Dispatch(NamedTuple):
@@ -779,23 +781,28 @@ class _BlockNormFn(torch.autograd.Function):
             return (None,) * 9
         T, H = y.shape
         make = torch.empty_like if T > 0 else torch.zeros_like
-        grads = [make(t) if want and t is not None else None
-                 for t, want in zip((y, res_out, post_w, gate, pre_w), ctx.needs_input_grad)]
-        if T == 0:
-            return (*grads, None, None, None, None)
-        dy, dres, dpost, dgate, dpre = grads
-        dres_out, dx = (None if g is None else g.contiguous() for g in (dres_out, dx))
-        if dx is None and dpre is not None:
-            dpre.zero_()
-        ws, need = None, 0
-        if dpost is not None or dpre is not None or kind == GATE_CHANNEL:
-            need = int(_lib.load().moe_block_norm_workspace_bytes_v1(T, H))
-            ws = torch.empty(need, dtype=torch.uint8, device=y.device)
-        _call("moe_block_norm_backward_v1", y.device, y.data_ptr(), res_out.data_ptr(), T, H,
-              OUT_DTYPES[y.dtype], _ptr(post_w), _ptr(gate), kind, res_scale, branch_scale,
-              _ptr(pre_w), eps, _ptr(dres_out), _ptr(dx), _ptr(ws), need, _ptr(dy), _ptr(dres),
-              _ptr(dpost), _ptr(dgate), _ptr(dpre if dx is not None else None))
-        return (*grads, None, None, None, None)
+        want_y, want_res, want_post, want_gate, want_pre = ctx.needs_input_grad[:5]
+        dy = make(y) if want_y else None
+        dres = make(res_out) if want_res else None
+        dpost = make(post_w) if want_post else None
+        dgate = make(gate) if want_gate else None
+        dpre = make(pre_w) if want_pre else None
+        if T > 0:
+            if dres_out is not None:
+                dres_out = dres_out.contiguous()
+            if dx is not None:
+                dx = dx.contiguous()
+            elif want_pre:
+                dpre.zero_()
+            ws, need = None, 0
+            if want_post or want_pre or kind == GATE_CHANNEL:
+                need = _lib.load().moe_block_norm_workspace_bytes_v1(T, H)
+                ws = torch.empty(need, dtype=torch.uint8, device=y.device)
+            _call("moe_block_norm_backward_v1", y.device, y.data_ptr(), res_out.data_ptr(), T, H,
+                  OUT_DTYPES[y.dtype], _ptr(post_w), _ptr(gate), kind, res_scale, branch_scale,
+                  _ptr(pre_w), eps, _ptr(dres_out), _ptr(dx), _ptr(ws), need, _ptr(dy), _ptr(dres),
+                  _ptr(dpost), _ptr(dgate), _ptr(dpre) if dx is not None else None)
+        return dy, dres, dpost, dgate, dpre, None, None, None, None
 
 
 def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | None = None,
@@ -829,8 +836,10 @@ def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | Non
                              f"{gate.dtype} {tuple(gate.shape)}")
     _require_gpu(y, res, post_w, gate, pre_w)
     scales = (kind, float(res_scale), float(branch_scale), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (y, res, post_w, gate, pre_w)):
+    if torch.is_grad_enabled() and (
+            y.requires_grad or res.requires_grad or (post_w is not None and post_w.requires_grad)
+            or (gate is not None and gate.requires_grad)
+            or (pre_w is not None and pre_w.requires_grad)):
         out = _BlockNormFn.apply(y, res, post_w, gate, pre_w, *scales)
         return out if pre_w is not None else (out, None)
     return _block_norm(y, res, post_w, gate, pre_w, *scales)
