@@ -126,6 +126,7 @@ hipError_t launch_quantize_and_sort(const void* x, int T, int K, int dtype, int8
 enum { kInt8Stream = 0, kInt8Ring = 1, kInt8Tile = 2 };
 struct Int8Plan {
   int kind, bm;
+  int bn = 0;  // channels a tile of the ring
 };
 Int8Plan int8_experts_plan(int64_t slots, int E, int I);
 Int8Plan int8_matrix_plan(int64_t M, int64_t N);

@@ -647,8 +647,9 @@ hipError_t launch_product(const Int8Args& a, Int8Plan plan, hipStream_t s) {
   }
   if constexpr (!SILU) {
     if (plan.kind == kInt8Ring)
-      return plan.bm == 32 ? launch_ring<32, 64, 2, 2, DT>(a, wide, s)
-                           : launch_ring<64, 64, 2, 2, DT>(a, wide, s);
+      return plan.bn == 32   ? launch_ring<32, 32, 2, 2, DT>(a, wide, s)
+             : plan.bm == 32 ? launch_ring<32, 64, 2, 2, DT>(a, wide, s)
+                             : launch_ring<64, 64, 2, 2, DT>(a, wide, s);
     return launch_few_rows<DT, false>(a, nullptr, s);
   }
   return hipErrorInvalidValue;
@@ -677,10 +678,13 @@ Int8Plan int8_experts_plan(int64_t slots, int E, int I) {
 // One matrix: the larger the tile the fewer bytes a product moves, the smaller the more workgroups
 // there are. By the number of 64 x 128 tiles (us, 4096 x 8192 channels, ring / 64 / 128 / 256 rows):
 // 256 tiles 17 / 22 / 25 / 43, 512 30 / 25 / 28 / 45, 1024 55 / 48 / 38 / 48, 2048 107 / 81 / 70 / 57.
+// In the ring by the number of 64 x 64 tiles (us with tiles of 32 x 32 / 32 x 64 / 64 x 64): 64 of 4096 x
+// 1024 6.2 / 7.7 / 9.9, 128 of 1040 x 2001 4.9 / 5.5 / 7.1, 128 of 2048 x 4096 5.2 / 5.6 / 6.8, 256 of 2048
+// x 4096 8.2 / 6.7 / 7.1, 448 of it 12.7 / 11.5 / 8.9.
 Int8Plan int8_matrix_plan(int64_t M, int64_t N) {
   if (M <= 16) return Int8Plan{kInt8Stream, 16};
-  const int64_t tiles = (M + 63) / 64 * ((N + 127) / 128);
-  if (tiles <= 256) return Int8Plan{kInt8Ring, M <= 64 ? 32 : 64};
+  const int64_t tiles = (M + 63) / 64 * ((N + 127) / 128), small = (M + 63) / 64 * ((N + 63) / 64);
+  if (tiles <= 256) return Int8Plan{kInt8Ring, small <= 256 ? 32 : 64, small <= 128 ? 32 : 64};
   return Int8Plan{kInt8Tile, tiles <= 768 ? 64 : tiles <= 1408 ? 128 : 256};
 }
 

@@ -108,6 +108,8 @@ SHAPES = [  # T, K, N, dtype, bias
     (257, 128, 256, torch.bfloat16, False), (300, 2064, 640, torch.float32, False),
     (513, 1552, 1000, torch.bfloat16, True), (1030, 256, 514, torch.float16, False),
     (2048, 2048, 2048, torch.bfloat16, False), (1100, 1168, 2500, torch.bfloat16, False),
+    (400, 272, 3001, torch.float32, True), (513, 144, 2504, torch.bfloat16, False),
+    (300, 96, 1200, torch.float32, False), (450, 400, 900, torch.float16, True),
     (3000, 272, 3001, torch.float32, True), (2990, 80, 3000, torch.bfloat16, False),
     (4099, 272, 3001, torch.float16, True), (5001, 144, 2500, torch.bfloat16, False)]
 
