@@ -560,6 +560,21 @@ __global__ __launch_bounds__(kThreads) void int8_ring_kernel(Int8Args a, int vec
     fetch(next, 0);  // behind the last step: zeros that nothing multiplies
     multiply(1);
   };
+  // the channels' scales and biases, asked for now: in the epilogue each would be waited for
+  const int n_wave = wn * NG * 16 + lk4;  // in the tile
+  float sc[NG][4];
+  T bias[NG][4] = {};
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[g][i] = a.s0[min(n0 + n_wave + g * 16 + i, a.N - 1)];
+  if (a.bias) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        bias[g][i] = static_cast<const T*>(a.bias)[min(n0 + n_wave + g * 16 + i, a.N - 1)];
+  }
   stage(lds0, 0);
   stage(lds1, BK);
   stage(lds2, 2 * BK);
@@ -576,16 +591,6 @@ __global__ __launch_bounds__(kThreads) void int8_ring_kernel(Int8Args a, int vec
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no load to LDS may outlive the workgroup
   // Results 16 WM rows at a time through LDS, from which a thread stores 16 consecutive bytes.
-  const int n_wave = wn * NG * 16 + lk4;  // in the tile
-  float sc[NG][4], bias[NG][4];
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = min(n0 + n_wave + g * 16 + i, a.N - 1);
-      sc[g][i] = a.s0[n];
-      bias[g][i] = a.bias ? Elem<DT>::get(static_cast<const T*>(a.bias)[n]) : 0.0f;
-    }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if (m * kRows >= tl.rows) break;  // the same for the whole workgroup
@@ -597,7 +602,7 @@ __global__ __launch_bounds__(kThreads) void int8_ring_kernel(Int8Args a, int vec
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float f = ((float)acc[g][m][i] * rs) * sc[g][i];
-        if (a.bias) f += bias[g][i];
+        if (a.bias) f += Elem<DT>::get(bias[g][i]);
         v[i] = Elem<DT>::put(f);
       }
       __builtin_memcpy(__builtin_assume_aligned(
