@@ -648,6 +648,7 @@ hipError_t launch_product(const Int8Args& a, Int8Plan plan, hipStream_t s) {
   if (plan.kind == kInt8Tile) {
     if (plan.bm == 256) return launch_tile<256, 256, 2, 4, DT, SILU>(a, wide, s);
     if (plan.bm == 128) return launch_tile<128, 128, 2, 2, DT, SILU>(a, wide, s);
+    if (plan.bm == 32) return launch_tile<32, 64, 2, 2, DT, SILU>(a, wide, s);
     return launch_tile<64, 128, 2, 2, DT, SILU>(a, wide, s);
   }
   if constexpr (!SILU) {
@@ -672,9 +673,14 @@ hipError_t launch_product_t(const Int8Args& a, Int8Plan plan, bool silu, hipStre
 // 251, 4096 tokens 339 / 310 / 319, 8192 tokens 552 / 484 / 453. Where few experts share the rows the
 // larger tiles also have to be enough for the chip: 8192 rows over 8 experts of 2048 x 1024 106 / 101 /
 // 82 (256 tiles of 256 rows), 4096 rows over 16 of them 93 / 80 / 67 (128 tiles), over 8 of 2048 x 512
-// 57 / 47 / 59 (64 tiles), 4000 rows over 8 of 512 x 128 24 / 27 / 35.
+// 57 / 47 / 59 (64 tiles), 4000 rows over 8 of 512 x 128 24 / 27 / 35. Where experts have a few rows each
+// tiles of 32 x 64 keep twice the workgroups of 64 x 128 on a CU, all of them streaming weights (us on
+// the GPU, 32 x 64 / 64 x 128): 1 token 20.5 / 22.6, 16 tokens 45.0 / 47.6, 256 tokens 149 / 153, 512 tokens
+// (16 rows an expert) 182 / 174. So do they where tiles are few at up to 32 rows (64 tokens, top-2 of 8
+// experts of 1024 x 512 18.4 / 20.8; 50 tokens, top-4 of 16 of 512 x 256 15.9 / 17.1).
 Int8Plan int8_experts_plan(int64_t slots, int E, int I) {
   const int64_t rows = (slots + E - 1) / E;
+  if (rows <= 8 || (rows <= 32 && (int64_t)E * ((I + 63) / 64) < 256)) return Int8Plan{kInt8Tile, 32};
   if (rows >= 192 && slots / 256 * ((I + 127) / 128) >= 96) return Int8Plan{kInt8Tile, 256};
   if (rows > 48 && slots / 128 * ((I + 63) / 64) >= 256) return Int8Plan{kInt8Tile, 128};
   return Int8Plan{kInt8Tile, 64};

@@ -279,6 +279,22 @@ def test_experts_equal_their_parts(T, k, E, H, I):
     assert torch.equal(got, ops.combine_tokens(y, d.slot_row, w))
 
 
+@pytest.mark.parametrize("T,k,E,dtype", [(130, 2, 300, torch.bfloat16), (90, 1, 64, torch.float32),
+                                         (500, 3, 40, torch.float16)])
+def test_experts_of_uneven_routing(T, k, E, dtype):
+    """Most tokens at two experts of many (several tiles of an expert while the average is a few rows):
+    a token's values are those of a call of its own."""
+    ex = make_experts(E, 96, 144, 8).to("cuda")
+    gen = torch.Generator().manual_seed(T)
+    ids = torch.where(torch.rand(T, k, generator=gen) < 0.8, torch.randint(3, 5, (T, k), generator=gen),
+                      torch.randint(0, E, (T, k), generator=gen)).to(torch.int32).cuda()
+    w = torch.rand(T, k, generator=gen).cuda()
+    x = torch.randn(T, 96, generator=gen).to(dtype).cuda()
+    got = ops.int8_experts(x, ids, w, ex)
+    for t in range(0, T, 7):
+        assert torch.equal(got[t:t + 1], ops.int8_experts(x[t:t + 1], ids[t:t + 1], w[t:t + 1], ex)), t
+
+
 @pytest.mark.parametrize("T", [3, 700])
 def test_experts_graph_streams_and_workspace(T):
     """A captured call replayed on new inputs between eager calls, two calls on two streams, and a
