@@ -422,7 +422,8 @@ int check_norm(const char* what, int32_t T, int32_t hidden, int32_t dtype, const
     return op_fail(MOE_ERR_SHAPE, "%s: T=%d hidden=%d (hidden in [1, 8192])", what, T, hidden);
   if (gate_kind < kGateNone || gate_kind > kGateFull)
     return op_fail(MOE_ERR_UNSUPPORTED, "%s: gate_kind=%d", what, gate_kind);
-  if ((gate != nullptr) != (gate_kind != kGateNone) && T > 0)
+  // A channel gate is read ahead of the rows; the other kinds hold nothing where there are no tokens.
+  if ((gate != nullptr) != (gate_kind != kGateNone) && (T > 0 || gate_kind == kGateChannel))
     return op_fail(MOE_ERR_NULL, "%s: gate and gate_kind must be given together", what);
   if (!(eps >= 0.0f)) return op_fail(MOE_ERR_SHAPE, "%s: eps must be >= 0", what);
   return MOE_OK;
