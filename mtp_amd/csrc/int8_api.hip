@@ -30,6 +30,13 @@ int check_sizes(const char* what, int32_t T, int32_t K, int32_t N) {
   return MOE_OK;
 }
 
+// Whether [p, p + n) holds a byte of a product's weights, scales or bias.
+bool weights_overlap(const void* p, int64_t n, const int8_t* w, const float* w_scale,
+                     const void* bias, int N, int K, int dtype) {
+  return overlaps(p, n, w, (int64_t)N * K) || overlaps(p, n, w_scale, (int64_t)N * 4) ||
+         overlaps(p, n, bias, (int64_t)N * dtype_bytes(dtype));
+}
+
 int matmul(const int8_t* q, const float* q_scale, int T, int K, const int8_t* w,
            const float* w_scale, int N, const void* bias, int dtype, void* out, hipStream_t s) {
   Int8Args a{};
@@ -134,8 +141,9 @@ int moe_int8_matmul_v1(const int8_t* q, const float* q_scale, int32_t T, int32_t
   if (!aligned16(q) || !aligned16(w))
     return op_fail(MOE_ERR_SHAPE, "int8 matmul: q and w must start on 16-byte boundaries");
   const int64_t no = (int64_t)T * N * dtype_bytes(dtype);
-  if (overlaps(out, no, q, (int64_t)T * K) || overlaps(out, no, w, (int64_t)N * K))
-    return op_fail(MOE_ERR_SHAPE, "int8 matmul: out must not overlap q or w");
+  if (overlaps(out, no, q, (int64_t)T * K) || overlaps(out, no, q_scale, (int64_t)T * 4) ||
+      weights_overlap(out, no, w, w_scale, bias, N, K, dtype))
+    return op_fail(MOE_ERR_SHAPE, "int8 matmul: out must not overlap the inputs");
   return matmul(q, q_scale, T, K, w, w_scale, N, bias, dtype, out, (hipStream_t)stream);
 }
 
@@ -164,9 +172,11 @@ int moe_int8_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype, const
       return op_fail(MOE_ERR_WORKSPACE, "int8 linear: workspace must be 256-byte aligned");
   }
   const int64_t es = dtype_bytes(dtype), nx = (int64_t)T * K * es, no = (int64_t)T * N * es;
-  if (overlaps(out, no, workspace, need) || overlaps(out, no, w, (int64_t)N * K) ||
-      overlaps(x, nx, workspace, need) || overlaps(out, no, x, nx))
-    return op_fail(MOE_ERR_SHAPE, "int8 linear: x, out, w and the workspace must not overlap");
+  if (overlaps(out, no, workspace, need) || overlaps(x, nx, workspace, need) ||
+      overlaps(out, no, x, nx) || weights_overlap(out, no, w, w_scale, bias, N, K, dtype) ||
+      weights_overlap(workspace, need, w, w_scale, bias, N, K, dtype))
+    return op_fail(MOE_ERR_SHAPE,
+                   "int8 linear: out and the workspace must not overlap the inputs or each other");
   const auto s = (hipStream_t)stream;
   if (need == 0) {
     Int8Args a{};

@@ -27,3 +27,30 @@ def test_block_norm_backward_refuses_a_missing_channel_gate_without_tokens(grads
     """The weights' gradients are written (zeros) also where there are no tokens, and the kernel that
     does it reads a channel gate, [hidden], ahead of its first row."""
     assert norm_backward(0, 64, kind=2, gate=None, **grads) == NULL
+
+
+@pytest.mark.parametrize("shared", ["q_scale", "w_scale", "bias"])
+def test_int8_matmul_refuses_out_over_scales_and_bias(shared):
+    """Every workgroup loads the scales and the bias for itself: one could read another's results."""
+    at = {"q_scale": B, "w_scale": D, "bias": P, "out": G}
+    at[shared] = G + 16
+    assert code_of("moe_int8_matmul_v1", A, at["q_scale"], 40, 64, C, at["w_scale"], 32, at["bias"], 0,
+                   G) == SHAPE
+
+
+@pytest.mark.parametrize("T", [2, 40])  # with and without a workspace
+@pytest.mark.parametrize("shared", ["w_scale", "bias"])
+def test_int8_linear_refuses_out_over_scales_and_bias(T, shared):
+    at = {"w_scale": D, "bias": P}
+    at[shared] = G + 16
+    assert code_of("moe_int8_linear_v1", A, T, 64, 0, C, at["w_scale"], 32, at["bias"], W, 1 << 20,
+                   G) == SHAPE
+
+
+@pytest.mark.parametrize("shared", ["w", "w_scale", "bias"])
+def test_int8_linear_refuses_a_workspace_over_the_weights(shared):
+    """The quantised rows would be written over what the product reads."""
+    at = {"w": C, "w_scale": D, "bias": P}
+    at[shared] = W + 256
+    assert code_of("moe_int8_linear_v1", A, 40, 64, 0, at["w"], at["w_scale"], 32, at["bias"], W, 1 << 20,
+                   G) == SHAPE
