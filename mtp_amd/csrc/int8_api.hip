@@ -224,6 +224,16 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
     return op_fail(MOE_ERR_SHAPE,
                    "int8 experts: x, out and the routing must not overlap the workspace, nor out "
                    "the weights");
+  const int64_t nw = (int64_t)E * H * I;
+  const struct {
+    const void* p;
+    int64_t bytes;
+  } weights[] = {{experts->gate, nw}, {experts->gate_scale, (int64_t)E * I * 4},
+                 {experts->up, nw}, {experts->up_scale, (int64_t)E * I * 4},
+                 {experts->down, nw}, {experts->down_scale, (int64_t)E * H * 4}};
+  for (const auto& w : weights)
+    if (overlaps(w.p, w.bytes, workspace, L.total))
+      return op_fail(MOE_ERR_SHAPE, "int8 experts: the workspace must not overlap the weights");
   const auto s = (hipStream_t)stream;
   int8_t* q = at<int8_t>(workspace, L.q);
   float* qs = at<float>(workspace, L.qs);

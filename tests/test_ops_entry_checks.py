@@ -4,6 +4,8 @@ a launch. Nothing here launches anything (no GPU needed)."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
 from mtp_amd import _lib
@@ -54,3 +56,14 @@ def test_int8_linear_refuses_a_workspace_over_the_weights(shared):
     at[shared] = W + 256
     assert code_of("moe_int8_linear_v1", A, 40, 64, 0, at["w"], at["w_scale"], 32, at["bias"], W, 1 << 20,
                    G) == SHAPE
+
+
+@pytest.mark.parametrize("shared", ["gate", "up", "down", "gate_scale", "up_scale", "down_scale"])
+def test_int8_experts_refuse_a_workspace_over_the_weights(shared):
+    """The workspace's rows would be written over what the products read."""
+    big = 0x10000000
+    ptrs = {n: big + 0x1000000 * i for i, n in enumerate(
+        ("gate", "up", "down", "gate_scale", "up_scale", "down_scale"))}
+    ptrs[shared] = W + 256
+    ex = _lib.Int8Set(**ptrs, num_experts=8, hidden=64, intermediate=32)
+    assert code_of("moe_int8_experts_v1", A, 4, 0, B, C, 2, ctypes.byref(ex), W, 1 << 20, D) == SHAPE
