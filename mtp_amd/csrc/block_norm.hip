@@ -429,6 +429,17 @@ int check_norm(const char* what, int32_t T, int32_t hidden, int32_t dtype, const
   return MOE_OK;
 }
 
+// A tensor's memory.
+struct Span {
+  const void* p;
+  int64_t bytes;
+};
+int64_t row_bytes(int H, int dtype) { return H * dtype_bytes(dtype); }
+int64_t gate_bytes(int kind, int T, int H, int dtype) {
+  return (kind == kGateNone ? 0 : kind == kGateToken ? T : kind == kGateChannel ? H : (int64_t)T * H) *
+         dtype_bytes(dtype);
+}
+
 bool vec_ok(int H, std::initializer_list<const void*> ps) {
   if (H % 8 != 0) return false;
   for (const void* p : ps)
@@ -450,11 +461,14 @@ int moe_block_norm_v1(const void* y, const void* res, int32_t T, int32_t hidden,
   if (!y || !res || !res_out || (pre_w && !x_out))
     return op_fail(MOE_ERR_NULL, "block norm: NULL pointer");
   const int64_t n = (int64_t)T * hidden * dtype_bytes(dtype);
-  const int64_t ng = gate_kind == kGateFull ? n : 0;
-  if (overlaps(res_out, n, y, n) || overlaps(res_out, n, gate, ng) ||
-      (res_out != res && overlaps(res_out, n, res, n)) ||
-      (pre_w && (overlaps(x_out, n, y, n) || overlaps(x_out, n, res, n) ||
-                 overlaps(x_out, n, res_out, n) || overlaps(x_out, n, gate, ng))))
+  const Span outs[] = {{res_out, n}, {pre_w ? x_out : nullptr, n}};
+  const Span ins[] = {{y, n}, {post_w, row_bytes(hidden, dtype)}, {pre_w, row_bytes(hidden, dtype)},
+                      {gate, gate_bytes(gate_kind, T, hidden, dtype)}};
+  bool shared = overlaps(outs[0].p, n, outs[1].p, n) || overlaps(outs[1].p, n, res, n) ||
+                (res_out != res && overlaps(res_out, n, res, n));
+  for (const Span& o : outs)
+    for (const Span& i : ins) shared |= overlaps(o.p, o.bytes, i.p, i.bytes);
+  if (shared)
     return op_fail(MOE_ERR_SHAPE,
                    "block norm: outputs must not overlap inputs or each other (res_out may be res)");
   const NormArgs a{y, res, post_w, gate, pre_w, gate_kind, T, hidden, res_scale, branch_scale, eps};

@@ -67,3 +67,18 @@ def test_int8_experts_refuse_a_workspace_over_the_weights(shared):
     ptrs[shared] = W + 256
     ex = _lib.Int8Set(**ptrs, num_experts=8, hidden=64, intermediate=32)
     assert code_of("moe_int8_experts_v1", A, 4, 0, B, C, 2, ctypes.byref(ex), W, 1 << 20, D) == SHAPE
+
+
+def norm(T, H, *, post=None, gate=None, kind=0, pre=None, r=C, x=None):
+    return code_of("moe_block_norm_v1", A, B, T, H, 0, post, gate, kind, 1.0, 1.0, pre, 1e-6, r, x)
+
+
+@pytest.mark.parametrize("over", [C, D])  # the residual stream, the next block's input
+def test_block_norm_refuses_outputs_over_weights_and_gates(over):
+    """Weights and gates are read again for each row, while other rows are written."""
+    at = over + 8 * 64 * 2 - 2  # the outputs' last element
+    assert norm(8, 64, post=at, pre=P, x=D) == SHAPE
+    assert norm(8, 64, post=P, pre=at, x=D) == SHAPE
+    assert norm(8, 64, pre=P, x=D, gate=at, kind=1) == SHAPE
+    assert norm(8, 64, pre=P, x=D, gate=at, kind=2) == SHAPE
+    assert norm(8, 64, pre=P, x=D, gate=at, kind=3) == SHAPE
