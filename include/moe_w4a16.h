@@ -342,7 +342,8 @@ int moe_block_norm_v1(const void* y, const void* res, int32_t T, int32_t hidden,
 /* Gradients of moe_block_norm_v1 from those of res_out (dres_out, NULL: zeros) and x_out (dx, NULL:
  * x_out is not used; then pre_w does not matter): dy, dres [T, hidden], dpost_w, dpre_w [hidden],
  * dgate as gate, each NULL where it is not wanted. Weights' and channel gates' gradients are fp32
- * sums in a fixed order over the workspace (only they need it), rounded once. */
+ * sums in a fixed order over the workspace (only they need it), rounded once (zeros with T = 0).
+ * Gradients and the workspace overlap nothing. */
 int64_t moe_block_norm_workspace_bytes_v1(int32_t T, int32_t hidden);
 int moe_block_norm_backward_v1(const void* y, const void* res_out, int32_t T, int32_t hidden,
                                int32_t dtype, const void* post_w, const void* gate,

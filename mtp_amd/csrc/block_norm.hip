@@ -499,8 +499,9 @@ int moe_block_norm_backward_v1(const void* y, const void* res_out, int32_t T, in
       (dgate && gate_kind == kGateNone) || (dpre_w && !dx))
     return op_fail(MOE_ERR_NULL, "block norm backward: NULL pointer");
   void* dchannel = gate_kind == kGateChannel ? dgate : nullptr;
+  int64_t need = 0;
   if (dpost_w || dchannel || dpre_w) {
-    const int64_t need = moe_block_norm_workspace_bytes_v1(T, hidden);
+    need = moe_block_norm_workspace_bytes_v1(T, hidden);
     if (!workspace || workspace_bytes < need)
       return op_fail(MOE_ERR_WORKSPACE, "block norm backward: workspace of %lld bytes, needs %lld",
                      (long long)(workspace ? workspace_bytes : 0), (long long)need);
@@ -509,16 +510,19 @@ int moe_block_norm_backward_v1(const void* y, const void* res_out, int32_t T, in
   } else if (T == 0) {
     return MOE_OK;
   }
-  const int64_t n = (int64_t)T * hidden * dtype_bytes(dtype);
-  const int64_t ng = gate_kind == kGateFull ? n : 0;
-  const void* outs[] = {dy, dres, ng ? dgate : nullptr};
-  for (int i = 0; i < 3; ++i) {
-    for (const void* in : {y, res_out, dres_out, dx, ng ? gate : nullptr})
-      if (overlaps(outs[i], n, in, n))
-        return op_fail(MOE_ERR_SHAPE, "block norm backward: gradients must not overlap inputs");
-    for (int j = 0; j < i; ++j)
-      if (overlaps(outs[i], n, outs[j], n))
-        return op_fail(MOE_ERR_SHAPE, "block norm backward: gradients must not overlap each other");
+  const int64_t n = (int64_t)T * hidden * dtype_bytes(dtype), nw = row_bytes(hidden, dtype);
+  const int64_t ng = gate_bytes(gate_kind, T, hidden, dtype);
+  const Span outs[] = {{dy, n}, {dres, n}, {dpost_w, nw}, {dgate, ng}, {dpre_w, nw}, {workspace, need}};
+  const Span ins[] = {{y, n}, {res_out, n}, {post_w, nw}, {gate, ng}, {pre_w, nw}, {dres_out, n}, {dx, n}};
+  for (const Span& o : outs) {
+    for (const Span& i : ins)
+      if (overlaps(o.p, o.bytes, i.p, i.bytes))
+        return op_fail(MOE_ERR_SHAPE,
+                       "block norm backward: gradients and workspace must not overlap inputs");
+    for (const Span* i = outs; i != &o; ++i)
+      if (overlaps(o.p, o.bytes, i->p, i->bytes))
+        return op_fail(MOE_ERR_SHAPE,
+                       "block norm backward: gradients and workspace must not overlap each other");
   }
   const NormArgs a{y, res_out, post_w, gate, pre_w, gate_kind, T, hidden,
                    res_scale, branch_scale, eps};

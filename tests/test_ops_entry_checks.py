@@ -82,3 +82,29 @@ def test_block_norm_refuses_outputs_over_weights_and_gates(over):
     assert norm(8, 64, pre=P, x=D, gate=at, kind=1) == SHAPE
     assert norm(8, 64, pre=P, x=D, gate=at, kind=2) == SHAPE
     assert norm(8, 64, pre=P, x=D, gate=at, kind=3) == SHAPE
+
+
+BACKWARD = {  # a valid call of 8 x 64 bf16 with every input and output
+    "y": A, "r": B, "post": C, "gate": D, "pre": G, "dr": P, "dx": W, "ws": 0x20000000,
+    "dy": 0x11000000, "dres": 0x12000000, "dpost": 0x13000000, "dgate": 0x14000000, "dpre": 0x15000000}
+
+
+@pytest.mark.parametrize("kind", [1, 2, 3])
+@pytest.mark.parametrize("out", ["dy", "dres", "dpost", "dgate", "dpre", "ws"])
+def test_block_norm_backward_refuses_shared_memory(out, kind):
+    """A gradient, or the workspace's partial sums, over an input or over each other: rows, weights and
+    partial sums are read while others are written."""
+    for other in BACKWARD:
+        if other != out:
+            # the output's first byte is the other's; the workspace begins on 256 bytes
+            call = {**BACKWARD, **({other: BACKWARD[out]} if out == "ws" else {out: BACKWARD[other]})}
+            assert norm_backward(8, 64, kind=kind, **call) == SHAPE, other
+
+
+def test_block_norm_backward_refuses_partly_shared_memory():
+    last = 8 * 64 * 2 - 2  # a gradient's last element
+    for out, other in (("dy", "pre"), ("dres", "gate"), ("dgate", "post"), ("dy", "dpost")):
+        call = {**BACKWARD, other: BACKWARD[out] + last}
+        assert norm_backward(8, 64, kind=3, **call) == SHAPE, (out, other)
+    need = _lib.load().moe_block_norm_workspace_bytes_v1(8, 64)
+    assert norm_backward(8, 64, kind=2, **{**BACKWARD, "dr": BACKWARD["ws"] + need - 4}) == SHAPE
