@@ -655,9 +655,13 @@ int moe_dispatch_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype,
     int64_t bytes;
   } outs[] = {{rows, nr}, {offsets, (num_experts + 1) * (int64_t)4}, {row_slot, S * 4},
               {slot_row, S * 4}, {workspace, need}};
-  for (const auto& o : outs)
+  for (const auto& o : outs) {
     if (overlaps(o.p, o.bytes, x, T * row_bytes) || overlaps(o.p, o.bytes, topk_ids, S * 4))
       return op_fail(MOE_ERR_SHAPE, "dispatch: outputs and workspace must not overlap x or the ids");
+    for (const auto* i = outs; i != &o; ++i)
+      if (overlaps(o.p, o.bytes, i->p, i->bytes))
+        return op_fail(MOE_ERR_SHAPE, "dispatch: outputs and workspace must not overlap each other");
+  }
   MOE_OP_HIP(launch_dispatch(topk_ids, T, top_k, num_experts, T ? x : nullptr, row_bytes, rows,
                              offsets, row_slot, slot_row, workspace, nullptr, 1, 0,
                              (hipStream_t)stream),

@@ -108,3 +108,17 @@ def test_block_norm_backward_refuses_partly_shared_memory():
         assert norm_backward(8, 64, kind=3, **call) == SHAPE, (out, other)
     need = _lib.load().moe_block_norm_workspace_bytes_v1(8, 64)
     assert norm_backward(8, 64, kind=2, **{**BACKWARD, "dr": BACKWARD["ws"] + need - 4}) == SHAPE
+
+
+@pytest.mark.parametrize("T", [4, 4096])  # without and with a workspace
+def test_dispatch_refuses_outputs_over_each_other(T):
+    """Workgroups write rows while others still read the tables and the workspace's counts."""
+    outs = {"rows": 0x40000000, "offsets": 0x51000000, "row_slot": 0x52000000, "slot_row": 0x53000000}
+    if T > 512:
+        outs["ws"] = 0x54000000
+    for out in outs:
+        for other in outs:
+            if other != out:
+                o = {**outs, out: outs[other] + (0 if out == "ws" else 4)}
+                assert code_of("moe_dispatch_v1", A, T, 64, 0, B, 8, 16, o.get("ws"), 1 << 20, o["rows"],
+                               o["offsets"], o["row_slot"], o["slot_row"]) == SHAPE, (out, other)
