@@ -370,7 +370,7 @@ int rows_of(int nt) { return nt < 256 ? 256 / nt : 1; }
 int backward_groups(int T, int H) {
   const int nt = threads_of(H), rows = rows_of(nt);
   const int most = nt > 256 ? 512 : 768;
-  return std::max(1, std::min((T + rows - 1) / rows, most));
+  return std::max(1, std::min((T - 1) / rows + 1, most));  // T + rows may pass 32 bits
 }
 
 #define MOE_NORM_NT(LAUNCH)                      \

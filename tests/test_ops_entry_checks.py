@@ -122,3 +122,10 @@ def test_dispatch_refuses_outputs_over_each_other(T):
                 o = {**outs, out: outs[other] + (0 if out == "ws" else 4)}
                 assert code_of("moe_dispatch_v1", A, T, 64, 0, B, 8, 16, o.get("ws"), 1 << 20, o["rows"],
                                o["offsets"], o["row_slot"], o["slot_row"]) == SHAPE, (out, other)
+
+
+@pytest.mark.parametrize("hidden", [8, 512, 513, 4097])
+def test_block_norm_workspace_of_the_most_tokens(hidden):
+    """Many tokens share a fixed number of workgroups: from there on the size stays."""
+    query = _lib.load().moe_block_norm_workspace_bytes_v1
+    assert query(2 ** 31 - 1, hidden) == query(1 << 20, hidden) > query(1, hidden)
