@@ -289,7 +289,7 @@ int moe_int8_matmul_v1(const int8_t* q, const float* q_scale, int32_t T, int32_t
                        int32_t dtype, void* out, void* stream);
 
 /* The values of moe_quantize_tokens_v1 of x, then moe_int8_matmul_v1. The workspace query gives 0
- * for few rows, which the product quantises itself: then workspace may be NULL. */
+ * for few rows, which the product quantises itself: then workspace may be NULL. T < 2^26. */
 int64_t moe_int8_linear_workspace_bytes_v1(int32_t T, int32_t K);
 int moe_int8_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype, const int8_t* w,
                        const float* w_scale, int32_t N, const void* bias, void* workspace,

@@ -159,6 +159,8 @@ int moe_int8_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype, const
   int rc = check_dtype("int8 linear", dtype);
   if (!rc) rc = check_sizes("int8 linear", T, K, N);
   if (rc) return rc;
+  if (T >= (1 << 26))  // a wave a row to quantise, and a launch has fewer than 2^32 threads
+    return op_fail(MOE_ERR_SHAPE, "int8 linear: T=%d (T < 2^26)", T);
   if (T == 0) return MOE_OK;
   if (!x || !w || !w_scale || !out) return op_fail(MOE_ERR_NULL, "int8 linear: NULL pointer");
   if (!aligned16(w))

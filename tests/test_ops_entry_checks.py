@@ -129,3 +129,11 @@ def test_block_norm_workspace_of_the_most_tokens(hidden):
     """Many tokens share a fixed number of workgroups: from there on the size stays."""
     query = _lib.load().moe_block_norm_workspace_bytes_v1
     assert query(2 ** 31 - 1, hidden) == query(1 << 20, hidden) > query(1, hidden)
+
+
+def test_int8_linear_refuses_more_rows_than_a_launch():
+    """Quantising takes 64 threads a row, of which a launch has fewer than 2^32: rows of 16 columns
+    pass that below the operands' 2 GiB."""
+    big = 1 << 40
+    assert code_of("moe_int8_linear_v1", A, 1 << 26, 16, 0, big, big + 4096, 16, None, 2 * big, 1 << 40,
+                   3 * big) == SHAPE
