@@ -14,6 +14,7 @@
 // launches and the latency of ids -> rank -> copy.
 #include <algorithm>
 
+#include "access.h"
 #include "common.h"
 #include "elem.h"
 #include "int8.h"
@@ -580,11 +581,11 @@ hipError_t launch_dispatch(const int32_t* ids, int T, int k, int E, const void* 
                            int32_t* slot_row, void* ws, i32x4* tiles, int bm, int tile_cap,
                            hipStream_t s) {
   const SortOut o{offsets, row_slot, slot_row};
-  const bool a16 = aligned16(x) && aligned16(rows);
-  if (row_bytes % 16 == 0 && a16)
+  const int width = copy_access_bytes(row_bytes, x, rows);
+  if (width == 16)
     return launch_dispatch_units<u32x4>(ids, T, k, E, x, row_bytes / 16, rows, o, ws, tiles, bm,
                                         tile_cap, s);
-  if (row_bytes % 4 == 0)
+  if (width == 4)
     return launch_dispatch_units<uint32_t>(ids, T, k, E, x, row_bytes / 4, rows, o, ws, tiles, bm,
                                            tile_cap, s);
   return launch_dispatch_units<uint16_t>(ids, T, k, E, x, row_bytes / 2, rows, o, ws, tiles, bm,
