@@ -11,6 +11,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from mtp_amd import _lib
@@ -521,6 +522,28 @@ def _rows_2d(x: torch.Tensor, name: str) -> int:
     return code
 
 
+def _recorded(*tensors: torch.Tensor | None) -> bool:
+    """Whether the call goes through its autograd function: a gradient may be asked for, or a forward-
+    mode derivative carried (the function then refuses a dual tensor; without it the tangent would
+    be lost)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _refuse_dual(*grads: torch.Tensor | None) -> None:
+    """A backward pass carries no forward-mode derivative of its incoming gradients either."""
+    if forward_ad._current_level >= 0:
+        for g in grads:
+            if g is not None and forward_ad.unpack_dual(g).tangent is not None:
+                raise NotImplementedError("the backward pass has no jvp: dual gradients are refused")
+
+
 class Dispatch(NamedTuple):
     """Token rows sorted by expert (``dispatch_tokens``)."""
 
@@ -568,6 +591,7 @@ class _DispatchFn(torch.autograd.Function):
     def backward(ctx, grad_rows, *_):
         if grad_rows is None:
             return None, None, None
+        _refuse_dual(grad_rows)
         return _combine(grad_rows.contiguous(), ctx.saved_tensors[0], None), None, None
 
 
@@ -581,6 +605,7 @@ class _CombineFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         rows, slot_row, topk_weights = ctx.saved_tensors
+        _refuse_dual(grad_out)
         want_rows, _, want_weights = ctx.needs_input_grad
         grad_out = grad_out.contiguous()
         T, k = slot_row.shape
@@ -608,7 +633,7 @@ def dispatch_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -
     if not 1 <= num_experts <= 512:
         raise ValueError(f"num_experts must lie in [1, 512], got {num_experts}")
     _require_gpu(x, topk_ids)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _recorded(x):
         return Dispatch(*_DispatchFn.apply(x, topk_ids, int(num_experts)))
     return Dispatch(*_dispatch(x, topk_ids, int(num_experts)))
 
@@ -630,7 +655,7 @@ def combine_tokens(rows: torch.Tensor, slot_row: torch.Tensor,
     if rows.shape[0] != slot_row.numel():
         raise ValueError(f"rows has {rows.shape[0]} rows for {slot_row.numel()} slots")
     _require_gpu(rows, slot_row, topk_weights)
-    if torch.is_grad_enabled() and (rows.requires_grad or topk_weights.requires_grad):
+    if _recorded(rows, topk_weights):
         return _CombineFn.apply(rows, slot_row, topk_weights)
     return _combine(rows, slot_row, topk_weights)
 
@@ -779,6 +804,7 @@ class _BlockNormFn(torch.autograd.Function):
         kind, res_scale, branch_scale, eps = ctx.consts
         if dres_out is None and dx is None:
             return (None,) * 9
+        _refuse_dual(dres_out, dx)
         T, H = y.shape
         make = torch.empty_like if T > 0 else torch.zeros_like
         want_y, want_res, want_post, want_gate, want_pre = ctx.needs_input_grad[:5]
@@ -836,10 +862,7 @@ def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | Non
                              f"{gate.dtype} {tuple(gate.shape)}")
     _require_gpu(y, res, post_w, gate, pre_w)
     scales = (kind, float(res_scale), float(branch_scale), float(eps))
-    if torch.is_grad_enabled() and (
-            y.requires_grad or res.requires_grad or (post_w is not None and post_w.requires_grad)
-            or (gate is not None and gate.requires_grad)
-            or (pre_w is not None and pre_w.requires_grad)):
+    if _recorded(y, res, post_w, gate, pre_w):
         out = _BlockNormFn.apply(y, res, post_w, gate, pre_w, *scales)
         return out if pre_w is not None else (out, None)
     return _block_norm(y, res, post_w, gate, pre_w, *scales)
