@@ -661,11 +661,32 @@ def combine_tokens(rows: torch.Tensor, slot_row: torch.Tensor,
 
 
 # ----------------------------------------------------------------------------- int8 products
+class _NoGradientFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, out, name, *inputs):
+        ctx.name = name
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError(f"{ctx.name} has no gradient: detach its inputs where it is to end "
+                                  "there")
+
+
+def _no_gradient(out: torch.Tensor, name: str, *inputs: torch.Tensor | None) -> torch.Tensor:
+    """The result of a call without a derivative. Where one of the inputs is part of a graph, a backward
+    pass that reaches the call raises; a result detached from them would lose their gradients in
+    silence."""
+    return _NoGradientFn.apply(out, name, *inputs) if _recorded(*inputs) else out
+
+
 def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """int8 rows and their scales: scale = max|x[t]| / 127, q = x / scale rounded half to even.
 
     x [T, K] bf16, fp16 or fp32 -> (int8 [T, K], fp32 [T]). A row that holds an infinity or NaN
-    gets q = 0 and a scale that is not finite, so its products are NaN."""
+    gets q = 0 and a scale that is not finite, so its products are NaN. No gradient: a backward pass
+    through the scale raises (q is an integer, of which there is none)."""
     code = _rows_2d(x, "x")
     _require_gpu(x)
     T, K = x.shape
@@ -673,7 +694,7 @@ def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale = torch.empty(T, dtype=torch.float32, device=x.device)
     _call("moe_quantize_tokens_v1", x.device, x.data_ptr(), T, K, code, q.data_ptr(),
           scale.data_ptr())
-    return q, scale
+    return q, _no_gradient(scale, "quantize_tokens", x)
 
 
 def _check_int8(weight, weight_scale, bias, K: int, dtype: torch.dtype) -> None:
@@ -697,7 +718,8 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor,
     exact in 32 bits, the rest fp32, rounded once to ``dtype``.
 
     q int8 [T, K], q_scale fp32 [T], weight int8 [N, K], weight_scale fp32 [N], bias [N] of
-    ``dtype``. K is a multiple of 16, at most 65536."""
+    ``dtype``. K is a multiple of 16, at most 65536. No gradient: a backward pass that reaches the
+    call raises."""
     if dtype not in OUT_DTYPES:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     if q.dtype != torch.int8 or q_scale.dtype != torch.float32:
@@ -712,13 +734,14 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor,
     _call("moe_int8_matmul_v1", q.device, q.data_ptr(), q_scale.data_ptr(), T, K,
           weight.data_ptr(), weight_scale.data_ptr(), N, _ptr(bias), OUT_DTYPES[dtype],
           out.data_ptr())
-    return out
+    return _no_gradient(out, "int8_matmul", q_scale, weight_scale, bias)
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
                 bias: torch.Tensor | None = None) -> torch.Tensor:
     """A linear layer on int8 products: the values of ``quantize_tokens(x)`` followed by
-    ``int8_matmul``, in x's type. x [T, K], weight int8 [N, K], weight_scale fp32 [N]."""
+    ``int8_matmul``, in x's type. x [T, K], weight int8 [N, K], weight_scale fp32 [N]. No gradient: a
+    backward pass that reaches the call raises."""
     code = _rows_2d(x, "x")
     T, K = x.shape
     _check_int8(weight, weight_scale, bias, K, x.dtype)
@@ -730,7 +753,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     out = torch.empty(T, N, dtype=x.dtype, device=dev)
     _call("moe_int8_linear_v1", dev, x.data_ptr(), T, K, code, weight.data_ptr(),
           weight_scale.data_ptr(), N, _ptr(bias), _ptr(ws), need, out.data_ptr())
-    return out
+    return _no_gradient(out, "int8_linear", x, weight_scale, bias)
 
 
 def int8_experts_workspace_bytes(T: int, top_k: int, experts: Int8Experts,
@@ -751,7 +774,8 @@ def int8_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Te
     h = silu(g) * u is rounded to x's type, quantised and multiplied by down; the slots' rows come
     back as in ``combine_tokens``. x [T, H] bf16, fp16 or fp32; topk_ids int32 and topk_weights
     fp32 [T, k]; a slot whose id is outside [0, E) contributes nothing. A shared expert goes in as
-    one more expert of the stacks, with its id and gate as one more slot of every token."""
+    one more expert of the stacks, with its id and gate as one more slot of every token. No gradient:
+    a backward pass that reaches the call raises."""
     code = _rows_2d(x, "x")
     if x.shape[1] != experts.hidden_size:
         raise ValueError(f"Expected x last dim {experts.hidden_size}, got {x.shape[1]}")
@@ -771,7 +795,8 @@ def int8_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Te
     _call("moe_int8_experts_v1", x.device, x.data_ptr(), T, code, topk_ids.data_ptr(),
           topk_weights.data_ptr(), k, ctypes.byref(ex), workspace.data_ptr(), _nbytes(workspace),
           out.data_ptr())
-    return out
+    return _no_gradient(out, "int8_experts", x, topk_weights, experts.gate_scale, experts.up_scale,
+                        experts.down_scale)
 
 
 # ----------------------------------------------------------------------------- norms around a block

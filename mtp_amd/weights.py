@@ -228,7 +228,7 @@ class Int8Experts:
             q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
             scale = torch.empty(w.shape[:2], dtype=torch.float32, device=w.device)
             for i in range(w.shape[0]):
-                q[i], scale[i] = ops.quantize_tokens(w[i].contiguous())
+                q[i], scale[i] = ops.quantize_tokens(w[i].detach().contiguous())
             parts += [q, scale]
         return cls(*parts)
 

@@ -8,12 +8,14 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 from mtp_amd import ops
+from mtp_amd.weights import Int8Experts
 
 
 @pytest.fixture(autouse=True)
 def no_launch(monkeypatch):
     monkeypatch.setattr(ops, "_require_gpu", lambda *tensors: None)
     monkeypatch.setattr(ops, "_call", lambda entry, device, *args: None)
+    monkeypatch.setattr(ops, "_workspace", lambda workspace, need, device: torch.empty(1))
 
 
 T, H, E, K = 4, 32, 8, 2
@@ -84,3 +86,62 @@ def test_only_wanted_gradients_are_recorded(name):
     assert not first(call(torch.ones)).requires_grad
     with torch.no_grad():
         assert not first(call(leaf)).requires_grad
+
+
+def int8(*shape):
+    return torch.ones(*shape, dtype=torch.int8)
+
+
+def experts(t, name):
+    at = {"x": (T, H), "topk_weights": (T, K), "gate_scale": (E, 16), "up_scale": (E, 16),
+          "down_scale": (E, H)}
+    at = {n: t(*s) if n == name else torch.ones(s) for n, s in at.items()}
+    ex = Int8Experts(int8(E, 16, H), at["gate_scale"], int8(E, 16, H), at["up_scale"], int8(E, H, 16),
+                     at["down_scale"])
+    return ops.int8_experts(at["x"], IDS, at["topk_weights"], ex, workspace=None)
+
+
+NOT_DIFFERENTIABLE = {
+    "quantize x": lambda t: ops.quantize_tokens(t(T, H))[1],
+    "matmul q_scale": lambda t: ops.int8_matmul(int8(T, H), t(T), int8(16, H), torch.ones(16)),
+    "matmul weight_scale": lambda t: ops.int8_matmul(int8(T, H), torch.ones(T), int8(16, H), t(16)),
+    "matmul bias": lambda t: ops.int8_matmul(int8(T, H), torch.ones(T), int8(16, H), torch.ones(16),
+                                             bias=t(16), dtype=torch.float32),
+    "linear x": lambda t: ops.int8_linear(t(T, H), int8(16, H), torch.ones(16)),
+    "linear weight_scale": lambda t: ops.int8_linear(torch.ones(T, H), int8(16, H), t(16)),
+    "linear bias": lambda t: ops.int8_linear(torch.ones(T, H), int8(16, H), torch.ones(16), bias=t(16)),
+    **{f"experts {n}": (lambda t, n=n: experts(t, n))
+       for n in ("x", "topk_weights", "gate_scale", "up_scale", "down_scale")}}
+
+
+@pytest.mark.parametrize("name", NOT_DIFFERENTIABLE)
+def test_a_gradient_that_does_not_exist_is_an_error(name):
+    """The int8 products have no gradient. The call itself runs, as inference without no_grad does; a
+    backward pass that reaches it raises instead of going on without what lies ahead of it."""
+    call = NOT_DIFFERENTIABLE[name]
+    leaf = lambda *shape: torch.ones(*shape, requires_grad=True)  # noqa: E731
+    out = call(leaf)
+    assert out.requires_grad and not out._is_view()
+    with pytest.raises(NotImplementedError, match=name.split()[0]):
+        out.float().sum().backward()
+    assert not call(torch.ones).requires_grad
+    with torch.no_grad():
+        assert not call(leaf).requires_grad
+    assert not call(lambda *shape: leaf(*shape).detach()).requires_grad
+
+
+@pytest.mark.parametrize("name", NOT_DIFFERENTIABLE)
+def test_forward_mode_of_the_int8_products_is_refused(name):
+    call = NOT_DIFFERENTIABLE[name]
+    with fwd.dual_level():
+        dual = lambda *shape: fwd.make_dual(torch.ones(*shape), torch.ones(*shape))  # noqa: E731
+        with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+            call(dual)
+        assert not call(torch.ones).requires_grad
+
+
+def test_quantising_stacks_records_no_gradient():
+    """Weights are often parameters; quantising them is no part of a graph."""
+    w = torch.ones(E, 16, H, requires_grad=True)
+    ex = Int8Experts.from_dense(w, w, torch.ones(E, H, 16, requires_grad=True))
+    assert not ex.gate_scale.requires_grad and not ex.down_scale.requires_grad
