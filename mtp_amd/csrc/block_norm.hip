@@ -43,8 +43,10 @@ template <int M>
 MOE_DEV float partner(float v) { return xor_partner<M>(v); }
 
 // Sums of N values over the NT threads of a row (all threads get them). A is double for the sums of
-// squares, so that the norms' factors come out within half an fp32 step of exact ones, at a cost that
-// HBM's time mostly hides; float for the means that the gradients subtract. NT = 64: no barrier.
+// squares, at a cost that HBM's time mostly hides: what is left of their error are the 8 fp32 roundings of
+// a thread's own columns, and a norm's factor is off by at most 5 half steps of fp32 (the root halves
+// them, and it is rounded itself) whatever the row's width. A is float for the means that the gradients
+// subtract. NT = 64: no barrier.
 template <int NT, int N, class A>
 MOE_DEV void row_sums(const float (&part)[N], A (&v)[N], A (*s_part)[N]) {
 #pragma unroll
