@@ -522,18 +522,9 @@ def _rows_2d(x: torch.Tensor, name: str) -> int:
     return code
 
 
-def _recorded(*tensors: torch.Tensor | None) -> bool:
-    """Whether the call goes through its autograd function: a gradient may be asked for, or a forward-
-    mode derivative carried (the function then refuses a dual tensor; without it the tangent would
-    be lost)."""
-    if forward_ad._current_level >= 0:
-        return True
-    if not torch.is_grad_enabled():
-        return False
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
+# The calls below go through their autograd function where a gradient may be asked for, and inside a dual
+# level, where the function refuses a dual tensor (past it the tangent would be lost). Each looks at
+# its own inputs: with a helper for all of them an int8_linear of one row took 9.1 us instead of 8.8.
 
 
 def _refuse_dual(*grads: torch.Tensor | None) -> None:
@@ -633,7 +624,7 @@ def dispatch_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -
     if not 1 <= num_experts <= 512:
         raise ValueError(f"num_experts must lie in [1, 512], got {num_experts}")
     _require_gpu(x, topk_ids)
-    if _recorded(x):
+    if (x.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
         return Dispatch(*_DispatchFn.apply(x, topk_ids, int(num_experts)))
     return Dispatch(*_dispatch(x, topk_ids, int(num_experts)))
 
@@ -655,13 +646,17 @@ def combine_tokens(rows: torch.Tensor, slot_row: torch.Tensor,
     if rows.shape[0] != slot_row.numel():
         raise ValueError(f"rows has {rows.shape[0]} rows for {slot_row.numel()} slots")
     _require_gpu(rows, slot_row, topk_weights)
-    if _recorded(rows, topk_weights):
+    if (((rows.requires_grad or topk_weights.requires_grad) and torch.is_grad_enabled())
+            or forward_ad._current_level >= 0):
         return _CombineFn.apply(rows, slot_row, topk_weights)
     return _combine(rows, slot_row, topk_weights)
 
 
 # ----------------------------------------------------------------------------- int8 products
 class _NoGradientFn(torch.autograd.Function):
+    """The result of a call without a derivative, one of whose inputs is part of a graph: a backward pass
+    that reaches the call raises. Detached from them it would lose their gradients in silence."""
+
     @staticmethod
     def forward(ctx, out, name, *inputs):
         ctx.name = name
@@ -672,13 +667,6 @@ class _NoGradientFn(torch.autograd.Function):
     def backward(ctx, *_):
         raise NotImplementedError(f"{ctx.name} has no gradient: detach its inputs where it is to end "
                                   "there")
-
-
-def _no_gradient(out: torch.Tensor, name: str, *inputs: torch.Tensor | None) -> torch.Tensor:
-    """The result of a call without a derivative. Where one of the inputs is part of a graph, a backward
-    pass that reaches the call raises; a result detached from them would lose their gradients in
-    silence."""
-    return _NoGradientFn.apply(out, name, *inputs) if _recorded(*inputs) else out
 
 
 def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -694,7 +682,9 @@ def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale = torch.empty(T, dtype=torch.float32, device=x.device)
     _call("moe_quantize_tokens_v1", x.device, x.data_ptr(), T, K, code, q.data_ptr(),
           scale.data_ptr())
-    return q, _no_gradient(scale, "quantize_tokens", x)
+    if (x.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        scale = _NoGradientFn.apply(scale, "quantize_tokens", x)
+    return q, scale
 
 
 def _check_int8(weight, weight_scale, bias, K: int, dtype: torch.dtype) -> None:
@@ -734,7 +724,10 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor,
     _call("moe_int8_matmul_v1", q.device, q.data_ptr(), q_scale.data_ptr(), T, K,
           weight.data_ptr(), weight_scale.data_ptr(), N, _ptr(bias), OUT_DTYPES[dtype],
           out.data_ptr())
-    return _no_gradient(out, "int8_matmul", q_scale, weight_scale, bias)
+    if ((q_scale.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad))
+            and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        out = _NoGradientFn.apply(out, "int8_matmul", q_scale, weight_scale, bias)
+    return out
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
@@ -753,7 +746,10 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     out = torch.empty(T, N, dtype=x.dtype, device=dev)
     _call("moe_int8_linear_v1", dev, x.data_ptr(), T, K, code, weight.data_ptr(),
           weight_scale.data_ptr(), N, _ptr(bias), _ptr(ws), need, out.data_ptr())
-    return _no_gradient(out, "int8_linear", x, weight_scale, bias)
+    if ((x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad))
+            and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        out = _NoGradientFn.apply(out, "int8_linear", x, weight_scale, bias)
+    return out
 
 
 def int8_experts_workspace_bytes(T: int, top_k: int, experts: Int8Experts,
@@ -795,8 +791,11 @@ def int8_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Te
     _call("moe_int8_experts_v1", x.device, x.data_ptr(), T, code, topk_ids.data_ptr(),
           topk_weights.data_ptr(), k, ctypes.byref(ex), workspace.data_ptr(), _nbytes(workspace),
           out.data_ptr())
-    return _no_gradient(out, "int8_experts", x, topk_weights, experts.gate_scale, experts.up_scale,
-                        experts.down_scale)
+    scales = experts.gate_scale, experts.up_scale, experts.down_scale
+    if ((x.requires_grad or topk_weights.requires_grad or any(s.requires_grad for s in scales))
+            and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        out = _NoGradientFn.apply(out, "int8_experts", x, topk_weights, *scales)
+    return out
 
 
 # ----------------------------------------------------------------------------- norms around a block
@@ -887,7 +886,9 @@ def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | Non
                              f"{gate.dtype} {tuple(gate.shape)}")
     _require_gpu(y, res, post_w, gate, pre_w)
     scales = (kind, float(res_scale), float(branch_scale), float(eps))
-    if _recorded(y, res, post_w, gate, pre_w):
+    if ((y.requires_grad or res.requires_grad or (post_w is not None and post_w.requires_grad)
+         or (gate is not None and gate.requires_grad) or (pre_w is not None and pre_w.requires_grad))
+            and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
         out = _BlockNormFn.apply(y, res, post_w, gate, pre_w, *scales)
         return out if pre_w is not None else (out, None)
     return _block_norm(y, res, post_w, gate, pre_w, *scales)
