@@ -754,6 +754,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
 def int8_experts_workspace_bytes(T: int, top_k: int, experts: Int8Experts,
                                  dtype: torch.dtype = torch.bfloat16) -> int:
+    if T >> 31 or top_k >> 31:  # sizes are int32 in the library
+        raise ValueError(f"T and top_k must lie in [0, 2^31), got {T} and {top_k}")
     ex = experts.struct()
     n = int(_lib.load().moe_int8_experts_workspace_bytes_v1(T, top_k, ctypes.byref(ex),
                                                             OUT_DTYPES[dtype]))

@@ -7,8 +7,10 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
-from mtp_amd import _lib
+from mtp_amd import _lib, ops
+from mtp_amd.weights import Int8Experts
 
 NULL, SHAPE = _lib.MOE_ERR_NULL, _lib.MOE_ERR_SHAPE
 A, B, C, D, G, P, W = (0x1000000 * i for i in range(1, 8))  # never dereferenced
@@ -137,3 +139,13 @@ def test_int8_linear_refuses_more_rows_than_a_launch():
     big = 1 << 40
     assert code_of("moe_int8_linear_v1", A, 1 << 26, 16, 0, big, big + 4096, 16, None, 2 * big, 1 << 40,
                    3 * big) == SHAPE
+
+
+@pytest.mark.parametrize("T,k", [(2 ** 32 + 8, 2), (8, 2 ** 32 + 2), (2 ** 31, 1), (-1, 2), (8, 0)])
+def test_int8_experts_workspace_query_refuses_sizes(T, k):
+    """Sizes are int32 in the library, and passing a larger one cuts it off."""
+    ex = Int8Experts(*(t for n, K in ((32, 64), (32, 64), (64, 32)) for t in (
+        torch.zeros(4, n, K, dtype=torch.int8), torch.ones(4, n))))
+    assert ops.int8_experts_workspace_bytes(8, 2, ex) > 0
+    with pytest.raises(ValueError):
+        ops.int8_experts_workspace_bytes(T, k, ex)
