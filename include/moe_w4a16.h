@@ -322,6 +322,72 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
                         const float* topk_weights, int32_t top_k, const moe_int8_set_v1* experts,
                         void* workspace, int64_t workspace_bytes, void* out, void* stream);
 
+/* ---------------------------------------------------------------- int4 linear layer */
+
+/* out[t, n] = round(sum_g s[g, n] * (sum_{k in g} x[t, k] * (q[k, n] - z[g, n])) (+ bias[n])): one
+ * projection in the experts' GPTQ layout (qweight [K/8, N], qzeros [K/G, N/8], scales fp16 [K/G, N],
+ * group g = k / G), products and sums in fp32 on unrounded weights. The dense counterpart of
+ * moe_w2_down_v1; no counterpart in the reference, which multiplies by moe_dequant_v1's weights.
+ * x [T, K], bias NULL or [N], out [T, N] of one dtype (0 bf16, 1 fp16). N a multiple of 8; group_size a
+ * multiple of 32 that divides K; K <= 65536; x, qweight and scales below 2 GiB each, T * N < 2^33. An
+ * infinity in x may come out as a NaN. The workspace query gives 0 where none is needed (then workspace
+ * may be NULL). */
+int64_t moe_int4_linear_workspace_bytes_v1(int32_t T, int32_t K, int32_t N, int32_t group_size);
+int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,
+                       const moe_gptq_proj_v1* weight, int32_t N, int32_t group_size,
+                       const void* bias, void* workspace, int64_t workspace_bytes, void* out,
+                       void* stream);
+
+/* ---------------------------------------------------------------- routing with its losses
+ * Logits [T, num_experts] of one dtype (0 bf16, 1 fp16, 2 fp32) to routed ids and weights, with what
+ * training needs beside moe_router_topk_v1's selection. num_experts <= 512, top_k <= 64 and at most the
+ * experts, at most 2^22 slots. No counterpart in the reference. */
+
+/* p = softmax(logits) of a token; topk_ids [T, top_k] its largest logits, equal ones by the lower id;
+ * topk_weights their p, divided by its sum over them with renormalize. A logit of -inf is not chosen:
+ * a place without an expert has id -1 and weight 0, behind the others. A token does not count if its
+ * mask (uint8 [T], NULL: ones) is 0 or no logit is above -inf: ids -1, weights 0. A NaN or +inf makes
+ * the weights and losses of a counted token NaN. Over the n tokens that count:
+ *   counts[e]  int32, slots of expert e
+ *   balance    num_experts * sum_e (counts[e] / (n * top_k)) * mean_t p[t, e]
+ *   z          mean_t (log sum exp logits[t])^2                          (both 0 for n = 0)
+ *   lse        NULL, or fp32 [T + 1] for the backward pass: log sum exp of each token (+inf: does not
+ *              count), then n
+ * Sums in a fixed order. The workspace query gives 0 for few tokens. */
+int64_t moe_route_workspace_bytes_v1(int32_t T, int32_t num_experts);
+int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dtype, int32_t top_k,
+                 const uint8_t* mask, int32_t renormalize, void* workspace,
+                 int64_t workspace_bytes, int32_t* topk_ids, float* topk_weights, int32_t* counts,
+                 float* balance, float* z, float* lse, void* stream);
+
+/* dlogits [T, num_experts] from the gradients of topk_weights (fp32 [T, top_k]), balance and z (fp32
+ * [1]; each NULL: zeros) and moe_route_v1's results; counts are constants. Tokens that do not count get
+ * zeros; what dweights holds at places without an expert is not looked at. */
+int moe_route_backward_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dtype,
+                          int32_t top_k, int32_t renormalize, const int32_t* topk_ids,
+                          const float* topk_weights, const int32_t* counts, const float* lse,
+                          const float* dweights, const float* dbalance, const float* dz,
+                          void* dlogits, void* stream);
+
+/* ---------------------------------------------------------------- layer norm */
+
+/* y = round((x - mean) / sqrt(var + eps) * weight + bias) with the biased variance of each row; weight
+ * (NULL: ones) and bias (NULL: zeros) [hidden], x and y [T, hidden] of one dtype (0 bf16, 1 fp16,
+ * 2 fp32); hidden in [1, 8192]. stats: NULL, or fp32 [T, 4] on a 16-byte boundary for the backward pass
+ * (the mean in two parts, 1 / sqrt(var + eps), 0). Outputs overlap nothing. The reference's LayerNorm
+ * stands inside its predictor only (src/mtp_expert_prefetch/training/hidden_residual.py:44-106). */
+int moe_layer_norm_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype, const void* weight,
+                      const void* bias, float eps, void* y, float* stats, void* stream);
+
+/* Gradients of moe_layer_norm_v1: dx [T, hidden], dweight and dbias [hidden], each NULL where it is not
+ * wanted. dweight and dbias are fp32 sums in a fixed order over the workspace (only they need it),
+ * rounded once (zeros with T = 0). Gradients and the workspace overlap nothing. */
+int64_t moe_layer_norm_workspace_bytes_v1(int32_t T, int32_t hidden);
+int moe_layer_norm_backward_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype,
+                               const void* weight, const float* stats, const void* dy,
+                               void* workspace, int64_t workspace_bytes, void* dx, void* dweight,
+                               void* dbias, void* stream);
+
 /* ---------------------------------------------------------------- norms around a block */
 #define MOE_GATE_NONE 0
 #define MOE_GATE_TOKEN 1   /* [T] */

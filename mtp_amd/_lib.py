@@ -58,6 +58,14 @@ EXPORTED = (
     "moe_int8_linear_v1",
     "moe_int8_experts_workspace_bytes_v1",
     "moe_int8_experts_v1",
+    "moe_int4_linear_workspace_bytes_v1",
+    "moe_int4_linear_v1",
+    "moe_route_workspace_bytes_v1",
+    "moe_route_v1",
+    "moe_route_backward_v1",
+    "moe_layer_norm_v1",
+    "moe_layer_norm_workspace_bytes_v1",
+    "moe_layer_norm_backward_v1",
     "moe_block_norm_v1",
     "moe_block_norm_workspace_bytes_v1",
     "moe_block_norm_backward_v1",
@@ -200,6 +208,16 @@ _SIGS = {
     "moe_int8_experts_workspace_bytes_v1": ([_I, _I, POINTER(Int8Set), _I], c_int64),
     "moe_int8_experts_v1": ([_P, _I, _I, _P, _P, _I, POINTER(Int8Set), _P, c_int64, _P, _P],
                             c_int32),
+    "moe_int4_linear_workspace_bytes_v1": ([_I, _I, _I, _I], c_int64),
+    "moe_int4_linear_v1": ([_P, _I, _I, _I, POINTER(GptqProj), _I, _I, _P, _P, c_int64, _P, _P],
+                           c_int32),
+    "moe_route_workspace_bytes_v1": ([_I, _I], c_int64),
+    "moe_route_v1": ([_P, _I, _I, _I, _I, _P, _I, _P, c_int64, _P, _P, _P, _P, _P, _P, _P], c_int32),
+    "moe_route_backward_v1": ([_P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P], c_int32),
+    "moe_layer_norm_v1": ([_P, _I, _I, _I, _P, _P, c_float, _P, _P, _P], c_int32),
+    "moe_layer_norm_workspace_bytes_v1": ([_I, _I], c_int64),
+    "moe_layer_norm_backward_v1": ([_P, _I, _I, _I, _P, _P, _P, _P, c_int64, _P, _P, _P, _P],
+                                   c_int32),
     "moe_block_norm_v1": ([_P, _P, _I, _I, _I, _P, _P, _I, c_float, c_float, _P, c_float, _P, _P,
                            _P], c_int32),
     "moe_block_norm_workspace_bytes_v1": ([_I, _I], c_int64),

@@ -19,70 +19,22 @@
 // thread over its columns, then in a butterfly in each wave and over the waves, where squares are summed
 // in fp64; the weights' gradients in fp32 per workgroup over its rows, then over the workgroups.
 #include <algorithm>
-#include <initializer_list>
 
 #include "common.h"
 #include "elem.h"
 #include "launch.h"
+#include "row_sums.h"
 
 namespace {
 
-constexpr int kMaxHidden = 8192;
 enum { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateFull = 3 };
 
-// The value of lane i ^ M.
-template <int M>
-MOE_DEV double partner(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)b)));
-  const uint32_t hi = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)(b >> 32))));
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-
-template <int M>
-MOE_DEV float partner(float v) { return xor_partner<M>(v); }
-
-// Sums of N values over the NT threads of a row (all threads get them). A is double for the sums of
-// squares, at a cost that HBM's time mostly hides: what is left of their error are the 8 fp32 roundings of
-// a thread's own columns, and a norm's factor is off by at most 5 half steps of fp32 (the root halves
-// them, and it is rounded itself) whatever the row's width. A is float for the means that the gradients
-// subtract. NT = 64: no barrier.
-template <int NT, int N, class A>
-MOE_DEV void row_sums(const float (&part)[N], A (&v)[N], A (*s_part)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = part[i];
-    v[i] += partner<32>(v[i]);
-    v[i] += partner<16>(v[i]);
-    v[i] += partner<8>(v[i]);
-    v[i] += partner<4>(v[i]);
-    v[i] += partner<2>(v[i]);
-    v[i] += partner<1>(v[i]);
-  }
-  if constexpr (NT > 64) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();  // the previous sums have been read
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) s_part[wave][i] = v[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = A(0);
-#pragma unroll
-      for (int w = 0; w < NT / 64; ++w) v[i] += s_part[w][i];
-    }
-  }
-}
-
-// 1 / sqrt(sum / H + eps): the hardware's approximation and a Newton step in 64 bits.
+// 1 / sqrt(sum / H + eps). The sums of squares are doubles, at a cost that HBM's time mostly hides: what is
+// left of their error are the 8 fp32 roundings of a thread's own columns, and a norm's factor is off by at
+// most 5 half steps of fp32 (the root halves them, and it is rounded itself) whatever the row's width. The
+// means that the gradients subtract are floats.
 MOE_DEV float inv_rms(double sum, double inv_h, float eps) {
-  const double m = sum * inv_h + (double)eps;
-  const float v = (float)m;
-  if (!(v >= 0x1p-100f && v < __builtin_inff())) return 1.0f / __builtin_sqrtf(v);
-  const double r = (double)__builtin_amdgcn_rsqf(v);
-  return (float)(r + 0.5 * r * (1.0 - m * r * r));
+  return inv_sqrt(sum * inv_h + (double)eps);
 }
 
 struct NormArgs {
@@ -110,9 +62,6 @@ MOE_DEV void load_gate(const NormArgs& a, int64_t t, int tid, float (&g)[8]) {
     for (int e = 0; e < 8; ++e) g[e] = v;
   }
 }
-
-template <int NT>
-constexpr int block_threads() { return NT < 256 ? 256 : NT; }
 
 template <int DT, int NT, bool VEC>
 __global__ __launch_bounds__(block_threads<NT>()) void block_norm_kernel(NormArgs a, void* res_out,
@@ -334,39 +283,6 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
   if (d.pre) f.store(d.part + 2 * all + me * H, tid, H, apre);
 }
 
-// The weights' gradients from the workgroups' sums: 32 columns a workgroup, 32 threads a column over
-// strided partials, then those 32 in order.
-constexpr int kSumCols = 32;
-struct SumOut {
-  void* out[3];
-};
-template <int DT>
-__global__ __launch_bounds__(1024) void block_norm_sum_kernel(const float* part, int partials,
-                                                              int H, SumOut o) {
-  __shared__ float s_sum[32][kSumCols + 1];
-  const int which = blockIdx.y;
-  if (!o.out[which]) return;
-  const int lane = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols;
-  const int c = blockIdx.x * kSumCols + lane;
-  const float* p = part + (int64_t)which * partials * H;
-  float s = 0.0f;
-  if (c < H) {
-#pragma unroll 8
-    for (int i = slot; i < partials; i += 32) s += p[(int64_t)i * H + c];
-  }
-  s_sum[slot][lane] = s;
-  __syncthreads();
-  if (slot == 0 && c < H) {
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v += s_sum[i][lane];
-    static_cast<typename Elem<DT>::T*>(o.out[which])[c] = Elem<DT>::put(v);
-  }
-}
-
-int threads_of(int H) { return H <= 512 ? 64 : H <= 2048 ? 256 : H <= 4096 ? 512 : 1024; }
-int rows_of(int nt) { return nt < 256 ? 256 / nt : 1; }
-
 // Workgroups of the backward pass: each keeps the weights' gradients of its rows in registers and
 // writes them once.
 int backward_groups(int T, int H) {
@@ -375,17 +291,6 @@ int backward_groups(int T, int H) {
   return std::max(1, std::min((T - 1) / rows + 1, most));  // T + rows may pass 32 bits
 }
 
-#define MOE_NORM_NT(LAUNCH)                      \
-  if (nt == 64) {                                \
-    if (vec) LAUNCH(64, true); else LAUNCH(64, false);     \
-  } else if (nt == 256) {                        \
-    if (vec) LAUNCH(256, true); else LAUNCH(256, false);   \
-  } else if (nt == 512) {                        \
-    if (vec) LAUNCH(512, true); else LAUNCH(512, false);   \
-  } else {                                       \
-    if (vec) LAUNCH(1024, true); else LAUNCH(1024, false); \
-  }
-
 template <int DT>
 hipError_t launch_forward(const NormArgs& a, void* res_out, void* x_out, bool vec, hipStream_t s) {
   const int nt = threads_of(a.H), rows = rows_of(nt);
@@ -393,7 +298,7 @@ hipError_t launch_forward(const NormArgs& a, void* res_out, void* x_out, bool ve
 #define MOE_NORM_FWD(NT, V)                                                                  \
   hipLaunchKernelGGL((block_norm_kernel<DT, NT, V>), grid, dim3(block_threads<NT>()), 0, s, a, \
                      res_out, x_out)
-  MOE_NORM_NT(MOE_NORM_FWD)
+  MOE_ROW_NT(MOE_NORM_FWD)
 #undef MOE_NORM_FWD
   return hipGetLastError();
 }
@@ -406,15 +311,14 @@ hipError_t launch_backward(const NormArgs& a, const NormGrads& d, void* dpost, v
 #define MOE_NORM_BWD(NT, V)                                                                     \
   hipLaunchKernelGGL((block_norm_backward_kernel<DT, NT, V>), grid, dim3(block_threads<NT>()), 0, \
                      s, a, d)
-  MOE_NORM_NT(MOE_NORM_BWD)
+  MOE_ROW_NT(MOE_NORM_BWD)
 #undef MOE_NORM_BWD
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(dpost || dgate_channel || dpre)) return e;
-  hipLaunchKernelGGL(block_norm_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 3),
+  hipLaunchKernelGGL(column_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 3),
                      dim3(1024), 0, s, d.part, d.partials, a.H, SumOut{{dpost, dgate_channel, dpre}});
   return hipGetLastError();
 }
-#undef MOE_NORM_NT
 
 int check_norm(const char* what, int32_t T, int32_t hidden, int32_t dtype, const void* gate,
                int32_t gate_kind, float eps) {
@@ -431,22 +335,10 @@ int check_norm(const char* what, int32_t T, int32_t hidden, int32_t dtype, const
   return MOE_OK;
 }
 
-// A tensor's memory.
-struct Span {
-  const void* p;
-  int64_t bytes;
-};
 int64_t row_bytes(int H, int dtype) { return H * dtype_bytes(dtype); }
 int64_t gate_bytes(int kind, int T, int H, int dtype) {
   return (kind == kGateNone ? 0 : kind == kGateToken ? T : kind == kGateChannel ? H : (int64_t)T * H) *
          dtype_bytes(dtype);
-}
-
-bool vec_ok(int H, std::initializer_list<const void*> ps) {
-  if (H % 8 != 0) return false;
-  for (const void* p : ps)
-    if (!aligned16(p)) return false;
-  return true;
 }
 
 }  // namespace

@@ -1,0 +1,125 @@
+// Sums over a row held 8 columns a thread, and over rows: what the norms share.
+#pragma once
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "common.h"
+#include "elem.h"
+
+constexpr int kMaxHidden = 8192;
+
+// The value of lane i ^ M.
+template <int M>
+MOE_DEV double partner(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)b)));
+  const uint32_t hi = __float_as_uint(xor_partner<M>(__uint_as_float((uint32_t)(b >> 32))));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+template <int M>
+MOE_DEV float partner(float v) { return xor_partner<M>(v); }
+
+// Sums of N values over the NT threads of a row (all threads get them), in a fixed order. A is the type
+// they are taken in, P that of a thread's own part. NT = 64: no barrier.
+template <int NT, int N, class P, class A>
+MOE_DEV void row_sums(const P (&part)[N], A (&v)[N], A (*s_part)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = part[i];
+    v[i] += partner<32>(v[i]);
+    v[i] += partner<16>(v[i]);
+    v[i] += partner<8>(v[i]);
+    v[i] += partner<4>(v[i]);
+    v[i] += partner<2>(v[i]);
+    v[i] += partner<1>(v[i]);
+  }
+  if constexpr (NT > 64) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();  // the previous sums have been read
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s_part[wave][i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = A(0);
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) v[i] += s_part[w][i];
+    }
+  }
+}
+
+// 1 / sqrt(m), rounded to fp32 at the end: the hardware's approximation and a Newton step in 64 bits.
+MOE_DEV float inv_sqrt(double m) {
+  const float v = (float)m;
+  if (!(v >= 0x1p-100f && v < __builtin_inff())) return 1.0f / __builtin_sqrtf(v);
+  const double r = (double)__builtin_amdgcn_rsqf(v);
+  return (float)(r + 0.5 * r * (1.0 - m * r * r));
+}
+
+// Threads a row takes, and the workgroup of (at least 256) threads they lie in.
+inline int threads_of(int H) { return H <= 512 ? 64 : H <= 2048 ? 256 : H <= 4096 ? 512 : 1024; }
+inline int rows_of(int nt) { return nt < 256 ? 256 / nt : 1; }
+template <int NT>
+constexpr int block_threads() { return NT < 256 ? 256 : NT; }
+
+#define MOE_ROW_NT(LAUNCH)                       \
+  if (nt == 64) {                                \
+    if (vec) LAUNCH(64, true); else LAUNCH(64, false);     \
+  } else if (nt == 256) {                        \
+    if (vec) LAUNCH(256, true); else LAUNCH(256, false);   \
+  } else if (nt == 512) {                        \
+    if (vec) LAUNCH(512, true); else LAUNCH(512, false);   \
+  } else {                                       \
+    if (vec) LAUNCH(1024, true); else LAUNCH(1024, false); \
+  }
+
+// Column sums of the workgroups' parts [outputs][partials][H]: 32 columns a workgroup, 32 threads a
+// column over strided partials, then those 32 in order.
+// (Unnamed: each source has its own kernel.)
+namespace {
+constexpr int kSumCols = 32;
+struct SumOut {
+  void* out[3];
+};
+template <int DT>
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, int partials, int H,
+                                                          SumOut o) {
+  __shared__ float s_sum[32][kSumCols + 1];
+  const int which = blockIdx.y;
+  if (!o.out[which]) return;
+  const int lane = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + lane;
+  const float* p = part + (int64_t)which * partials * H;
+  float s = 0.0f;
+  if (c < H) {
+#pragma unroll 8
+    for (int i = slot; i < partials; i += 32) s += p[(int64_t)i * H + c];
+  }
+  s_sum[slot][lane] = s;
+  __syncthreads();
+  if (slot == 0 && c < H) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v += s_sum[i][lane];
+    static_cast<typename Elem<DT>::T*>(o.out[which])[c] = Elem<DT>::put(v);
+  }
+}
+}  // namespace
+
+// A tensor's memory.
+struct Span {
+  const void* p;
+  int64_t bytes;
+};
+
+// Whether rows of H columns can be taken 8 at a time (Cols<..., VEC = true>) in all of the tensors.
+inline bool vec_ok(int H, std::initializer_list<const void*> ps) {
+  if (H % 8 != 0) return false;
+  for (const void* p : ps)
+    if (!aligned16(p)) return false;
+  return true;
+}

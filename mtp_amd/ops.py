@@ -800,6 +800,192 @@ def int8_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Te
     return out
 
 
+# ----------------------------------------------------------------------------- int4 linear layer
+def int4_linear(x: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch.Tensor, *,
+                group_size: int = 128, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """A linear layer on one GPTQ projection, as the experts' are stored:
+    out[t, n] = sum_g scales[g, n] * (sum_{k in g} x[t, k] * (q[k, n] - z[g, n])) (+ bias[n]) with
+    g = k // group_size, sums in fp32 on unrounded weights, rounded once to x's type.
+
+    x [T, K] bf16 or fp16, qweight int32 [K/8, N], qzeros int32 [K/G, N/8], scales fp16 [K/G, N], bias
+    [N] of x's type. N is a multiple of 8, group_size a multiple of 32. An infinity in x may come out as a
+    NaN. No gradient: a backward pass that reaches the call raises."""
+    code = _rows_2d(x, "x")
+    if code == OUT_DTYPES[torch.float32]:
+        raise TypeError("x must be bfloat16 or float16, got torch.float32")
+    if qweight.dtype != torch.int32 or qzeros.dtype != torch.int32 or scales.dtype != torch.float16:
+        raise TypeError(f"qweight and qzeros must be int32 and scales float16, got {qweight.dtype}, "
+                        f"{qzeros.dtype} and {scales.dtype}")
+    T, K = x.shape
+    if qweight.ndim != 2 or qweight.shape[0] * 8 != K or qweight.shape[1] >> 31:
+        raise ValueError(f"qweight must be [{K} / 8, N], got {tuple(qweight.shape)}")
+    N = qweight.shape[1]
+    if not 0 < group_size < 1 << 31 or K % group_size:
+        raise ValueError(f"group_size {group_size} does not divide in_features {K}")
+    ng = K // group_size
+    if tuple(scales.shape) != (ng, N) or tuple(qzeros.shape) != (ng, N // 8):
+        raise ValueError(f"scales {tuple(scales.shape)} / qzeros {tuple(qzeros.shape)} do not match "
+                         f"qweight {tuple(qweight.shape)} with group_size {group_size}")
+    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (N,)):
+        raise ValueError(f"bias must be {x.dtype} [{N}]")
+    _require_gpu(x, qweight, qzeros, scales, bias)
+    dev = x.device
+    need = _lib.load().moe_int4_linear_workspace_bytes_v1(T, K, N, group_size)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    out = torch.empty(T, N, dtype=x.dtype, device=dev)
+    proj = _lib.GptqProj(qweight.data_ptr(), qzeros.data_ptr(), scales.data_ptr())
+    _call("moe_int4_linear_v1", dev, x.data_ptr(), T, K, code, proj, N, group_size, _ptr(bias), _ptr(ws),
+          need, out.data_ptr())
+    if ((x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad))
+            and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        out = _NoGradientFn.apply(out, "int4_linear", x, scales, bias)
+    return out
+
+
+# ----------------------------------------------------------------------------- routing with its losses
+class Routing(NamedTuple):
+    """What ``route_tokens`` makes of router logits."""
+
+    topk_ids: torch.Tensor      # int32 [T, k]; -1 where there is no expert
+    topk_weights: torch.Tensor  # fp32 [T, k]
+    counts: torch.Tensor        # int32 [E]: slots of each expert
+    balance_loss: torch.Tensor  # fp32 scalar
+    z_loss: torch.Tensor        # fp32 scalar
+
+
+def _route(logits, top_k, mask, renormalize, want_lse):
+    T, E = logits.shape
+    dev = logits.device
+    ids = torch.empty(T, top_k, dtype=torch.int32, device=dev)
+    weights = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    balance = torch.empty((), dtype=torch.float32, device=dev)
+    z = torch.empty((), dtype=torch.float32, device=dev)
+    lse = torch.empty(T + 1, dtype=torch.float32, device=dev) if want_lse else None
+    need = _lib.load().moe_route_workspace_bytes_v1(T, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _call("moe_route_v1", dev, logits.data_ptr(), T, E, OUT_DTYPES[logits.dtype], top_k, _ptr(mask),
+          renormalize, _ptr(ws), need, ids.data_ptr(), weights.data_ptr(), counts.data_ptr(),
+          balance.data_ptr(), z.data_ptr(), _ptr(lse))
+    return ids, weights, counts, balance, z, lse
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, mask, renormalize):
+        ids, weights, counts, balance, z, lse = _route(logits, top_k, mask, renormalize, True)
+        ctx.mark_non_differentiable(ids, counts)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, ids, weights, counts, lse)
+        ctx.renormalize = renormalize
+        return ids, weights, counts, balance, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _ids, dweights, _counts, dbalance, dz):
+        if dweights is None and dbalance is None and dz is None:
+            return None, None, None, None
+        _refuse_dual(dweights, dbalance, dz)
+        logits, ids, weights, counts, lse = ctx.saved_tensors
+        if dweights is not None:
+            dweights = dweights.contiguous()
+        T, E = logits.shape
+        dlogits = torch.empty_like(logits)
+        _call("moe_route_backward_v1", logits.device, logits.data_ptr(), T, E,
+              OUT_DTYPES[logits.dtype], ids.shape[1], ctx.renormalize, ids.data_ptr(),
+              weights.data_ptr(), counts.data_ptr(), lse.data_ptr(), _ptr(dweights), _ptr(dbalance),
+              _ptr(dz), dlogits.data_ptr())
+        return dlogits, None, None, None
+
+
+def route_tokens(logits: torch.Tensor, top_k: int = 8, *, mask: torch.Tensor | None = None,
+                 renormalize: bool = True) -> Routing:
+    """Router logits to routed ids and weights, with the losses that keep a router in training balanced:
+
+        p = softmax(logits);  topk_ids = the top_k largest, equal ones by the lower id
+        topk_weights = p[topk_ids] (/ their sum with renormalize)
+        balance_loss = E * sum_e (counts[e] / (n * top_k)) * mean_t p[t, e]     (1 for even routing)
+        z_loss = mean_t logsumexp(logits[t])^2
+
+    over the n tokens that count: those of ``mask`` (bool [T], None: all) with a logit above -inf. Other
+    tokens get ids -1, which ``dispatch_tokens`` drops, weights 0 and no gradient; so does a place for
+    which no logit above -inf is left. Both losses are 0 for n = 0. A NaN or +inf among the logits of a
+    counted token makes its weights and both losses NaN. logits [T, E] bf16, fp16 or fp32; E <= 512,
+    top_k <= 64. Differentiable in logits through topk_weights and both losses (counts are constants);
+    the gradient is rounded once to logits' type."""
+    _rows_2d(logits, "logits")
+    T, E = logits.shape
+    if not 1 <= E <= 512:
+        raise ValueError(f"logits must be [T, E] with E in [1, 512], got {tuple(logits.shape)}")
+    if not 1 <= top_k <= min(E, 64):
+        raise ValueError(f"top_k must lie in [1, {min(E, 64)}], got {top_k}")
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (T,)):
+        raise ValueError(f"mask must be bool [{T}], got {mask.dtype} {tuple(mask.shape)}")
+    _require_gpu(logits, mask)
+    if (logits.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        return Routing(*_RouteFn.apply(logits, int(top_k), mask, bool(renormalize)))
+    return Routing(*_route(logits, int(top_k), mask, bool(renormalize), False)[:5])
+
+
+# ----------------------------------------------------------------------------- layer norm
+def _layer_norm(x, weight, bias, eps, want_stats):
+    T, H = x.shape
+    y = torch.empty_like(x)
+    stats = torch.empty(T, 4, dtype=torch.float32, device=x.device) if want_stats else None
+    _call("moe_layer_norm_v1", x.device, x.data_ptr(), T, H, OUT_DTYPES[x.dtype], _ptr(weight),
+          _ptr(bias), eps, y.data_ptr(), _ptr(stats))
+    return y, stats
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _layer_norm(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        _refuse_dual(dy)
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
+        T, H = x.shape
+        dy = dy.contiguous()
+        dx = torch.empty_like(x) if want_x else None
+        dw = torch.empty_like(weight) if want_w else None
+        db = torch.empty(H, dtype=x.dtype, device=x.device) if want_b else None
+        ws, need = None, 0
+        if want_w or want_b:
+            need = _lib.load().moe_layer_norm_workspace_bytes_v1(T, H)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _call("moe_layer_norm_backward_v1", x.device, x.data_ptr(), T, H, OUT_DTYPES[x.dtype],
+              _ptr(weight), stats.data_ptr(), dy.data_ptr(), _ptr(ws), need, _ptr(dx), _ptr(dw),
+              _ptr(db))
+        return dx, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, *, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over each row with the biased variance: the norm of
+    the predictor's encoder (src/mtp_expert_prefetch/training/hidden_residual.py:44-106) as an operator.
+
+    x [T, H], weight (None: ones) and bias (None: zeros) [H], all of one type (bf16, fp16 or fp32); H up
+    to 8192. Moments are taken in 64 bits, the result is rounded once. Differentiable in x, weight and
+    bias."""
+    _rows_2d(x, "x")
+    H = x.shape[1]
+    for name, w in (("weight", weight), ("bias", bias)):
+        if w is not None and (w.dtype != x.dtype or tuple(w.shape) != (H,)):
+            raise ValueError(f"{name} must be {x.dtype} [{H}], got {w.dtype} {tuple(w.shape)}")
+    _require_gpu(x, weight, bias)
+    if ((x.requires_grad or (weight is not None and weight.requires_grad)
+         or (bias is not None and bias.requires_grad))
+            and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
+        return _LayerNormFn.apply(x, weight, bias, float(eps))
+    return _layer_norm(x, weight, bias, float(eps), False)[0]
+
+
 # ----------------------------------------------------------------------------- norms around a block
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_FULL = range(4)
 
