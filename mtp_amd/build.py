@@ -37,8 +37,10 @@ COMMON_FLAGS = [
 
 
 # Per-source flags. The decode GEMMs fold each group's MFMA partial sums with VALU arithmetic:
-# MFMA results in VGPRs (instead of AGPRs) spare one v_accvgpr_read per partial sum.
+# MFMA results in VGPRs (instead of AGPRs) spare one v_accvgpr_read per partial sum. The int4 linear
+# layer's tiles rescale theirs at every group's end.
 SOURCE_FLAGS = {
+    "int4_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "gemm_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 

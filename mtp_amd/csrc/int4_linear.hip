@@ -6,6 +6,7 @@
 // The weights are not rounded: a group's products are summed in fp32 on the integers q - z and scaled
 // after that.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "elem.h"
@@ -23,14 +24,599 @@ struct Int4Args {
   const uint16_t* scales;   // fp16 [K / G][N]
   const void* bias;         // nullable
   void* out;
-  int T, K, N, G;
+  int T, K, N, G, groups;
+  void* workspace;
 };
 
+// ---------------------------------------------------------------- operands
+// A packed word holds 8 consecutive k of one channel, which is what one lane contributes to a 16x16x32
+// MFMA. The word becomes the operand in the types' own bits, in the order of k: a nibble lands in the
+// mantissa of a constant OFF whose last place it then counts in, so a value is OFF + q, exact (bf16
+// 16 + q: 0x4180 | q << 3; fp16 64 + q: 0x5400 | q << 4): two nibbles a register by a byte permute, a
+// mask and an or, 10 VALU operations a word and 9. The offset and the zero point leave by the sum of x:
+//   sum x (q - z) = sum x (OFF + q) - (OFF + z) sum x
+// with OFF small, so that little is cancelled (a magnitude of up to 31 or 79 for q - z of up to 15).
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// Byte i of each word into a half of register i, masked, in the constant: one v_perm_b32 and one
+// v_and_or_b32, which takes one scalar and no literal (left to itself the compiler used two literals in
+// two operations).
+MOE_DEV uint32_t constant_s(uint32_t c) {
+  asm("" : "+s"(c));
+  return c;
+}
+MOE_DEV uint32_t constant_v(uint32_t c) {
+  asm("" : "+v"(c));
+  return c;
+}
+MOE_DEV u32x4 spread(uint32_t even, uint32_t odd, uint32_t mask, uint32_t base) {
+  u32x4 v;
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i)
+    v[i] = (__builtin_amdgcn_perm(odd, even, 0x0C040C00u + 0x00010001u * i) & mask) | base;
+  return v;
+}
+
+template <int DT>
+struct Op;
+template <>
+struct Op<kBf16> {
+  static constexpr float kOff = 16.0f;
+  static constexpr uint32_t kOnes = 0x3F803F80u;
+  // OFF + the nibble at bit `at`, as a float
+  MOE_DEV static float zero_point(uint32_t z, int at) {
+    return __uint_as_float(((at <= 19 ? z << (19 - at) : z >> (at - 19)) & 0x00780000u) | 0x41800000u);
+  }
+  MOE_DEV static u32x4 weights(uint32_t w) {
+    return spread(w << 3, w >> 1, constant_s(0x00780078u), constant_v(0x41804180u));
+  }
+  MOE_DEV static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Op<kFp16> {
+  static constexpr float kOff = 64.0f;
+  static constexpr uint32_t kOnes = 0x3C003C00u;
+  MOE_DEV static float zero_point(uint32_t z, int at) {
+    return __uint_as_float(((at <= 17 ? z << (17 - at) : z >> (at - 17)) & 0x001E0000u) | 0x42800000u);
+  }
+  MOE_DEV static u32x4 weights(uint32_t w) {
+    return spread(w << 4, w, constant_s(0x00F000F0u), constant_v(0x54005400u));
+  }
+  MOE_DEV static f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+};
+
+// ---------------------------------------------------------------- few rows
+// Workgroup: 16 MT tokens x 16 CT channels, K dealt to its KS waves in chunks of 32 SPG (a quantisation
+// group or a part of one) in turn; the waves' sums meet in LDS. Weights and x go from memory to the
+// registers that the MFMA reads, the next chunk's while this one is multiplied. The channels are the A
+// operand's rows (lane l: channels CT (l & 15) .. + CT - 1, one load) and the tokens the B operand's
+// columns, so a lane ends with channels 4 CT (l >> 4) .. + 4 CT - 1 of token l & 15. The sum of x comes
+// from an MFMA with ones.
+template <int MT, int CT, int SPG>
+struct Chunk {
+  u32x4 x[MT][SPG];
+  uint32_t w[SPG][CT];
+  uint32_t s[2 * CT];          // fp16 pairs of the lane's 4 CT results
+  uint32_t z[(CT + 1) / 2];
+};
+
+template <int DT, int MT, int CT, int SPG, int KS>
+__global__ __launch_bounds__(64 * KS) void int4_stream_kernel(Int4Args a, uint32_t row_tiles, uint32_t row_magic, uint32_t group_magic) {
+  using T = typename Elem<DT>::T;
+  using O = Op<DT>;
+  __shared__ f32x4 red[KS][MT * CT][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // A channel tile's row tiles run behind each other on one XCD, which then holds its weights in L2.
+  const uint32_t idx = blockIdx.x >> 3;
+  const uint32_t ct = row_magic ? __umulhi(idx, row_magic) : idx;
+  const int c0 = (int)(ct * 8 + (blockIdx.x & 7)) * 16 * CT, t0 = (int)(idx - ct * row_tiles) * 16 * MT;
+  if (c0 >= a.N) return;
+  const int lr = lane & 15, lq = lane >> 4;
+  const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.K * 2u);
+  const __amdgpu_buffer_rsrc_t rw = buf_rsrc(a.qweight, (uint32_t)(a.K / 8) * (uint32_t)a.N * 4u);
+  const __amdgpu_buffer_rsrc_t rs = buf_rsrc(a.scales, (uint32_t)a.groups * (uint32_t)a.N * 2u);
+  const __amdgpu_buffer_rsrc_t rz = buf_rsrc(a.qzeros, (uint32_t)a.groups * (uint32_t)(a.N / 8) * 4u);
+  uint32_t xoff[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int t = t0 + 16 * m + lr;
+    xoff[m] = t < a.T ? (uint32_t)t * (uint32_t)a.K * 2u + 16u * lq : kOutOfRange;
+  }
+  const int cw = c0 + CT * lr, cd = c0 + 4 * CT * lq;  // first channel loaded, first one of the result
+  const uint32_t woff = cw < a.N ? ((uint32_t)lq * (uint32_t)a.N + (uint32_t)cw) * 4u : kOutOfRange;
+  const uint32_t soff = cd < a.N ? (uint32_t)cd * 2u : kOutOfRange;
+  const uint32_t zoff = cd < a.N ? (uint32_t)(cd / 8) * 4u : kOutOfRange;
+  const int chunks = a.K / (32 * SPG);
+  // a chunk past the last reads zeros without a memory access
+  auto load = [&](Chunk<MT, CT, SPG>& c, int at) {
+    const bool in = at < chunks;
+    const uint32_t out = in ? 0u : kOutOfRange;
+    const uint32_t k = in ? (uint32_t)at * 32u * SPG : 0u, g = in ? (group_magic ? __umulhi((uint32_t)at, group_magic) : (uint32_t)at) : 0u;
+#pragma unroll
+    for (int s = 0; s < SPG; ++s) {
+      const uint32_t row = (k / 8 + 4 * s) * (uint32_t)a.N * 4u;
+      if constexpr (CT == 1) {
+        c.w[s][0] = buf_ld32(rw, woff | out, row);
+      } else if constexpr (CT == 2) {
+        const u32x2 v = buf_ld64(rw, woff | out, row);
+        c.w[s][0] = v[0];
+        c.w[s][1] = v[1];
+      } else {
+        const u32x4 v = buf_ld128(rw, woff | out, row);
+#pragma unroll
+        for (int j = 0; j < CT; ++j) c.w[s][j] = v[j];
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int s = 0; s < SPG; ++s) c.x[m][s] = buf_ld128(rx, (xoff[m] + 64u * s) | out, k * 2u);
+    const uint32_t srow = g * (uint32_t)a.N * 2u, zrow = g * (uint32_t)(a.N / 8) * 4u;
+    if constexpr (CT == 1) {
+      const u32x2 v = buf_ld64(rs, soff | out, srow);
+      c.s[0] = v[0];
+      c.s[1] = v[1];
+    } else {
+#pragma unroll
+      for (int h = 0; h < CT / 2; ++h) {
+        const u32x4 v = buf_ld128(rs, (soff + 16u * h) | out, srow);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c.s[4 * h + i] = v[i];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < (CT + 1) / 2; ++h) c.z[h] = buf_ld32(rz, (zoff + 4u * h) | out, zrow);
+  };
+  f32x4 acc[MT][CT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < CT; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
+  const u32x4 ones{O::kOnes, O::kOnes, O::kOnes, O::kOnes};
+  auto multiply = [&](const Chunk<MT, CT, SPG>& c) {
+    f32x4 part[MT][CT], sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      sum[m] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < CT; ++j) part[m][j] = f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int s = 0; s < SPG; ++s) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) sum[m] = O::mfma(ones, c.x[m][s], sum[m]);
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const u32x4 w = O::weights(c.w[s][j]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) part[m][j] = O::mfma(w, c.x[m][s], part[m][j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const int v = CT * i + j;  // the lane's channel
+        const float s = f16_to_f32(v & 1 ? c.s[v / 2] >> 16 : c.s[v / 2] & 0xFFFFu);
+        const uint32_t z = CT == 1 ? c.z[0] >> (16 * (lq & 1)) : c.z[v / 8];
+        const float zb = O::zero_point(z, 4 * (v & 7));
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          acc[m][j][i] = __builtin_fmaf(s, __builtin_fmaf(-zb, sum[m][0], part[m][j][i]), acc[m][j][i]);
+      }
+  };
+  Chunk<MT, CT, SPG> ca, cb;
+  load(ca, wave);
+  for (int at = wave;; at += 2 * KS) {
+    load(cb, at + KS);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(ca);
+    if (at + KS >= chunks) break;
+    load(ca, at + 2 * KS);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(cb);
+    if (at + 2 * KS >= chunks) break;
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[m][(4 * u + e) % CT][(4 * u + e) / CT];
+      red[wave][m * CT + u][lane] = v;
+    }
+  __syncthreads();
+  // a thread four channels: the waves' sums in their order
+  for (int f = tid; f < MT * CT * 64; f += 64 * KS) {
+    const int l = f & 63, u = (f >> 6) % CT, m = f / (64 * CT);
+    f32x4 v = red[0][f >> 6][l];
+#pragma unroll
+    for (int w = 1; w < KS; ++w) v += red[w][f >> 6][l];
+    const int t = t0 + 16 * m + (l & 15), n = c0 + 4 * CT * (l >> 4) + 4 * u;
+    if (t >= a.T || n >= a.N) continue;
+    T out[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (a.bias) v[e] += Elem<DT>::get(static_cast<const T*>(a.bias)[n + e]);
+      out[e] = Elem<DT>::put(v[e]);
+    }
+    __builtin_memcpy(static_cast<T*>(a.out) + (int64_t)t * a.N + n, out, sizeof(out));
+  }
+}
+
+// x / d is the upper half of x * magic(d) where x * d < 2^32; d == 1 would need 2^32 itself.
+uint32_t magic(uint32_t d) { return (uint32_t)(((uint64_t(1) << 32) + d - 1) / d); }
+
+template <int DT, int MT, int CT, int SPG, int KS>
+hipError_t launch_stream(const Int4Args& a, hipStream_t s) {
+  const int row_tiles = (a.T + 16 * MT - 1) / (16 * MT), tiles = (a.N + 16 * CT - 1) / (16 * CT);
+  const int64_t blocks = (int64_t)((tiles + 7) / 8 * 8) * row_tiles;
+  hipLaunchKernelGGL((int4_stream_kernel<DT, MT, CT, SPG, KS>), dim3((unsigned)blocks),
+                     dim3(64 * KS), 0, s, a, (uint32_t)row_tiles, magic((uint32_t)row_tiles),
+                     magic((uint32_t)(a.G / (32 * SPG))));
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- many rows
+// Two launches. The first turns the words into the integers q - z as fp8 (e4m3 holds 4 significant bits:
+// exact), a wave 64 channels x 64 k, stored as the tiles below take them: [K / 64][N][64], a row's 16-byte
+// chunk c holding k 8 c .. + 7 and 32 + 8 c .. + 7, zeros past K; and for each 64 k (32 where groups may end
+// there) the ratio of the scale before to the one from there on. The second is a product of x with them, turned into x's type (exact) on the way from LDS.
+//
+// The product keeps its sums in units of the present group's scale: where a group ends they are multiplied
+// by s[g - 1] / s[g], which takes an operation a sum and no second set of sums. A scale of zero counts as
+// one, with integers of zero.
+constexpr int kBK = 64;
+
+MOE_DEV float scale_unit(uint32_t s) {
+  const float f = f16_to_f32(s & 0xFFFFu);
+  return f == 0.0f ? 1.0f : f;
+}
+
+// Four nibbles of a word, from bit `at` on, less the zero point.
+MOE_DEV uint32_t integers(uint32_t w, int at, float z) {
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (float)((w >> (at + 4 * i)) & 15u) - z;
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], v, true);
+}
+
+__global__ __launch_bounds__(256) void int4_unpack_kernel(Int4Args a, uint8_t* __restrict__ w,
+                                                          float* __restrict__ ratio, int halves) {
+  const int lane = threadIdx.x & 63, c = lane & 3;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks_n = (a.N + 255) / 256;
+  const int n = (blockIdx.x % blocks_n * 4 + wave) * 64 + (lane >> 2) * 4, stage = blockIdx.x / blocks_n;
+  if (n >= a.N) return;
+  uint32_t row[4][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = stage * kBK + 32 * h + 8 * c;
+    const bool in = k < a.K;
+    const int g = in ? k / a.G : 0;
+    const u32x4 q = ld128(a.qweight + (int64_t)(in ? k / 8 : 0) * a.N + n);
+    const uint32_t z = a.qzeros[(int64_t)g * (a.N / 8) + n / 8] >> (4 * (n & 7));
+    const u32x2 s = *reinterpret_cast<const u32x2*>(a.scales + (int64_t)g * a.N + n);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t keep = in && (s[j >> 1] >> (16 * (j & 1)) & 0x7FFFu) != 0 ? ~0u : 0u;
+      const float zf = (float)((z >> (4 * j)) & 15u);
+      row[j][2 * h] = integers(q[j], 0, zf) & keep;
+      row[j][2 * h + 1] = integers(q[j], 16, zf) & keep;
+    }
+    if (c == 0 && (h == 0 || halves)) {
+      const int before = in ? max(k - 1, 0) / a.G : 0;
+      const u32x2 p = *reinterpret_cast<const u32x2*>(a.scales + (int64_t)before * a.N + n);
+      f32x4 r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        r[j] = scale_unit(p[j >> 1] >> (16 * (j & 1))) / scale_unit(s[j >> 1] >> (16 * (j & 1)));
+      *reinterpret_cast<f32x4*>(ratio + (int64_t)(halves ? 2 * stage + h : stage) * a.N + n) = r;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<u32x4*>(w + ((int64_t)stage * a.N + n + j) * kBK + 16 * c) =
+        u32x4{row[j][0], row[j][1], row[j][2], row[j][3]};
+}
+
+// Workgroup: BM tokens x BN channels on WM x WN waves, K steps of 64 in a ring of RING stages in LDS, filled
+// by loads that bypass the registers. One wait and barrier in the middle of a step orders the arrival of the
+// next stage and the reuse of this one, whose second half is in registers by then: loads have RING - 1 steps
+// to arrive. LDS rows of x are 128 bytes, the 16-byte chunk c of row r at position c ^ (r & 7); rows of
+// integers 64 bytes, chunk c at c ^ (r / 2 & 3): the 8 rows that a phase of a 16-byte read spans lie in
+// different banks. EVERY: groups end at multiples of so many half steps (1, 2 or 4).
+constexpr int kGroupM = 4;
+// The kernel's body in pieces: called many times over, they would become functions.
+#define MOE_INLINE __attribute__((always_inline))
+// s_waitcnt immediate waiting for lgkmcnt <= 0 only.
+constexpr int kWaitLgkm0 = 15 | (3 << 14) | (0x7 << 4);
+
+// 8 integers in fp8 as an MFMA operand.
+template <int DT>
+MOE_DEV u32x4 operand(uint32_t lo, uint32_t hi) {
+  if constexpr (DT == kBf16)
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
+}
+
+template <int BM, int BN, int WM, int WN, int RING, int DT, int EVERY>
+__global__ __launch_bounds__(64 * WM * WN) void int4_tile_kernel(Int4Args a,
+                                                                 const uint8_t* __restrict__ w,
+                                                                 const float* __restrict__ ratio) {
+  using T = typename Elem<DT>::T;
+  using O = Op<DT>;
+  constexpr int NT = 64 * WM * WN, BK = kBK;
+  constexpr int MT = BM / WM / 16, NG = BN / WN / 16, LA = BM * 8 / NT, LB = BN * 4 / NT, LR = EVERY == 1 ? 2 : 1;
+  constexpr int kRowsAt = BM * 128, kRatioAt = kRowsAt + BN * 64, kStage = kRatioAt + LR * 1024;  // bytes
+  static_assert(LA * NT == BM * 8 && LB * NT == BN * 4 && BN <= 256, "whole loads");
+  static_assert(RING >= 2 && RING <= 4, "a stage an array");
+  // separate arrays: the compiler then knows which stage a load to LDS writes
+  __shared__ __attribute__((aligned(16))) uint8_t lds0[kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t lds1[kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t lds2[RING > 2 ? kStage : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t lds3[RING > 3 ? kStage : 16];
+  const int m_tiles = (a.T + BM - 1) / BM, blocks_n = (a.N + BN - 1) / BN;
+  // each XCD takes a run of tiles, down kGroupM row blocks before the next channels
+  const int idx = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+  const int total = m_tiles * blocks_n, per = (total + 7) / 8, id = xcd * per + idx;
+  if (idx >= per || id >= total) return;
+  const int group = id / (kGroupM * blocks_n), in = id - group * kGroupM * blocks_n;
+  const int grows = min(kGroupM, m_tiles - group * kGroupM);
+  const int t0 = (group * kGroupM + in % grows) * BM, n0 = in / grows * BN;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN, lr = lane & 15, lq = lane >> 4;
+  const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.K * 2u);
+  const uint32_t kc = (uint32_t)((tid & 7) ^ ((tid >> 3) & 7)) * 16;  // the chunk's byte of x's row
+  // One offset a lane and a scalar one for each load. Rows behind the last token or channel may hold
+  // anything (a lane's results are of its own token and channels, which are then not stored), but are read
+  // inside the buffers: a load whose first row lies behind reads another one's rows.
+  const uint32_t xoff = (uint32_t)(tid / 8) * (uint32_t)a.K * 2u + kc;
+  const uint32_t woff = (uint32_t)(tid / 4) * kBK + 16u * ((tid & 3) ^ ((tid >> 3) & 3));
+  uint32_t xrow[LA], wrow[LB];
+#pragma unroll
+  for (int j = 0; j < LA; ++j) {
+    const int t = t0 + j * (NT / 8);
+    xrow[j] = t < a.T ? (uint32_t)t * (uint32_t)a.K * 2u : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < LB; ++j) {
+    const int n = n0 + j * (NT / 4);
+    wrow[j] = n < a.N ? (uint32_t)n * kBK : 0u;
+  }
+  const uint32_t roff = 4 * lane < BN && n0 + 4 * lane < a.N ? (uint32_t)(n0 + 4 * lane) * 4u : kOutOfRange;
+  // A stage past K reads zeros without a memory access, so that as many loads are in flight in every step.
+  // The scalar offsets stay inside the buffers: the bounds check takes them off the buffers' sizes.
+  auto stage = [&](uint8_t* lds, int k0) MOE_INLINE {
+    const uint32_t out = 2 * k0 + (int)kc < 2 * a.K ? 0u : kOutOfRange;
+    const uint32_t at = k0 < a.K ? (uint32_t)k0 : 0u, none = k0 < a.K ? 0u : kOutOfRange;
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(w + (int64_t)at * a.N, (uint32_t)a.N * (uint32_t)BK);
+#pragma unroll
+    for (int j = 0; j < LA; ++j)
+      buf_ld128_lds(rx, lds + (j * NT + wave * 64) * 16, xoff | out, xrow[j] + at * 2u);
+#pragma unroll
+    for (int j = 0; j < LB; ++j)
+      buf_ld128_lds(rw, lds + kRowsAt + (j * NT + wave * 64) * 16, woff | none, wrow[j]);
+    // the ratios; every wave stores the same
+    const __amdgpu_buffer_rsrc_t rr = buf_rsrc(ratio + (int64_t)(at / kBK) * LR * a.N, LR * (uint32_t)a.N * 4u);
+#pragma unroll
+    for (int h = 0; h < LR; ++h)
+      buf_ld128_lds(rr, lds + kRatioAt + h * 1024, roff | none, (uint32_t)h * (uint32_t)a.N * 4u);
+  };
+  // The barrier without __syncthreads' release fence, which would wait for every load to LDS: this wave's
+  // LDS accesses ahead of it are waited for, and the compiler keeps accesses on their sides.
+  auto barrier = []() MOE_INLINE {
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  f32x4 acc[NG][MT];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[g][m] = f32x4{0, 0, 0, 0};
+  const int sw0 = (lq ^ (lr & 7)) * 16, sw1 = ((4 + lq) ^ (lr & 7)) * 16, sww = (lq ^ ((lr >> 1) & 3)) * 16;
+  const int fa_at = (wm * 16 + lr) * 128, fb_at = kRowsAt + (wn * NG * 16 + lr) * 64 + sww;
+  // A step is four phases of half the wave's rows and half of the step's K, pipelined through two register
+  // sets: while one phase's rows are multiplied the next one's are read from LDS. A phase in which a group
+  // starts multiplies its sums by the ratios first, in the MFMA's shadow.
+  constexpr int PM = MT / 2;
+  static_assert(MT % 2 == 0, "phases of half the rows");
+  u32x4 fa[2][PM], raw[NG], fb[2][NG];
+  f32x4 unit[NG];
+  auto fetch_x = [&](const uint8_t* lds, int half, int part) MOE_INLINE {
+    const int sw = half ? sw1 : sw0;
+#pragma unroll
+    for (int m = 0; m < PM; ++m) fa[part][m] = ld128(lds + fa_at + (part * PM + m) * WM * 16 * 128 + sw);
+  };
+  auto fetch_w = [&](const uint8_t* lds) MOE_INLINE {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) raw[g] = ld128(lds + fb_at + g * 16 * 64);
+  };
+  auto fetch_unit = [&](const uint8_t* lds, int half) MOE_INLINE {
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      unit[g] = *reinterpret_cast<const f32x4*>(lds + kRatioAt + half * 1024 + ((wn * NG + g) * 16 + 4 * lq) * 4);
+  };
+  auto operands = [&](int half) MOE_INLINE {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) fb[half][g] = operand<DT>(raw[g][2 * half], raw[g][2 * half + 1]);
+  };
+  // reads, loads: the LDS reads and the loads to LDS of the phase, spread over its multiplications
+  auto multiply = [&](int half, int part, bool starts, auto reads_c, auto loads_c) MOE_INLINE {
+    constexpr int kReads = decltype(reads_c)::value, kLoads = decltype(loads_c)::value, kOps = PM * NG;
+#pragma unroll
+    for (int m = 0; m < PM; ++m)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        f32x4& c = acc[g][part * PM + m];
+        if (starts) c *= unit[g];
+        c = O::mfma(fb[half][g], fa[part][m], c);
+      }
+    constexpr int kEach = kOps / (kReads + 1) > 0 ? kOps / (kReads + 1) : 1;
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (i < kLoads) __builtin_amdgcn_sched_group_barrier(0x010, (kLoads + kReads - 1) / kReads, 0);
+      if (starts) __builtin_amdgcn_sched_group_barrier(0x002, 4 * kEach, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using std::integral_constant;
+  auto step = [&](uint8_t* here, uint8_t* next, int k0, bool starts) MOE_INLINE {
+    if (EVERY == 1) fetch_unit(here, 0);
+    operands(1);
+    fetch_x(here, 0, 1);
+    multiply(0, 0, starts, integral_constant<int, PM>{}, integral_constant<int, 0>{});
+    fetch_x(here, 1, 0);
+    multiply(0, 1, starts, integral_constant<int, PM>{}, integral_constant<int, 0>{});
+    if (EVERY == 1) fetch_unit(here, 1);
+    fetch_x(here, 1, 1);
+    multiply(1, 0, EVERY == 1, integral_constant<int, PM>{}, integral_constant<int, 0>{});
+    // This wave's loads of the next stage have landed (those of the stages after it stay in flight); behind
+    // the barrier everybody's have, and this stage, all of it in registers, is free.
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm((RING - 2) * (LA + LB + LR)));
+    barrier();
+    stage(here, k0 + RING * BK);
+    fetch_w(next);  // behind the last step: zeros that nothing multiplies
+    fetch_x(next, 0, 0);
+    // past K both operands are zeros
+    multiply(1, 1, EVERY == 1, integral_constant<int, PM + NG>{}, integral_constant<int, LA + LB + LR>{});
+    if (EVERY != 1) fetch_unit(next, 0);
+    operands(0);
+  };
+  stage(lds0, 0);
+  stage(lds1, BK);
+  if constexpr (RING > 2) stage(lds2, 2 * BK);
+  if constexpr (RING > 3) stage(lds3, 3 * BK);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm((RING - 1) * (LA + LB + LR)));
+  barrier();
+  fetch_w(lds0);
+  fetch_x(lds0, 0, 0);
+  fetch_unit(lds0, 0);
+  operands(0);
+  // Which stage a step works on and whether a group may start there is known in a run of kSteps. Whole runs
+  // first, without branches between their steps: at a join the compiler would wait for all loads to LDS.
+  constexpr int kSteps = EVERY == 4 && RING % 2 ? 2 * RING : RING;
+  auto nth = [&](auto i_c, int k0) MOE_INLINE {
+    constexpr int i = decltype(i_c)::value, at = i % RING, to = (i + 1) % RING;
+    uint8_t* const here = at == 0 ? lds0 : at == 1 ? lds1 : at == 2 ? lds2 : lds3;
+    uint8_t* const next = to == 0 ? lds0 : to == 1 ? lds1 : to == 2 ? lds2 : lds3;
+    step(here, next, k0 + i * BK, EVERY < 4 || i % 2 == 0);
+  };
+  int k0 = 0;
+#pragma unroll 1
+  for (; k0 + (kSteps - 1) * BK < a.K; k0 += kSteps * BK) {
+    nth(integral_constant<int, 0>{}, k0);
+    nth(integral_constant<int, 1>{}, k0);
+    if constexpr (kSteps > 2) nth(integral_constant<int, 2>{}, k0);
+    if constexpr (kSteps > 3) nth(integral_constant<int, 3>{}, k0);
+    if constexpr (kSteps > 4) nth(integral_constant<int, 4>{}, k0);
+    if constexpr (kSteps > 5) nth(integral_constant<int, 5>{}, k0);
+  }
+  if (k0 < a.K) nth(integral_constant<int, 0>{}, k0);
+  if constexpr (kSteps > 2)
+    if (k0 + BK < a.K) nth(integral_constant<int, 1>{}, k0);
+  if constexpr (kSteps > 3)
+    if (k0 + 2 * BK < a.K) nth(integral_constant<int, 2>{}, k0);
+  if constexpr (kSteps > 4)
+    if (k0 + 3 * BK < a.K) nth(integral_constant<int, 3>{}, k0);
+  if constexpr (kSteps > 5)
+    if (k0 + 4 * BK < a.K) nth(integral_constant<int, 4>{}, k0);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no load to LDS may meet the rows below
+  // Epilogue: 16 rows at a time through the wave's share of LDS, whole lines stored.
+  constexpr int CH = NG * 16, PITCH = CH + 8;
+  static_assert(NT / 64 * 16 * PITCH * 2 <= kStage, "the rows fit a stage");
+  const int n_wave = n0 + wn * CH, lk4 = 4 * lq;
+  u32x2 last[NG], bits[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const int c = min(n_wave + g * 16 + lk4, a.N - 4);
+    last[g] = *reinterpret_cast<const u32x2*>(a.scales + (int64_t)(a.groups - 1) * a.N + c);
+    bits[g] = u32x2{0, 0};
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      __builtin_memcpy(&bits[g], static_cast<const T*>(a.bias) + min(n_wave + g * 16 + lk4, a.N - 4), 8);
+  }
+  __syncthreads();  // the stages have been read
+  T* mine = reinterpret_cast<T*>(lds0) + wave * 16 * PITCH;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r0 = t0 + (m * WM + wm) * 16;
+    if (r0 >= a.T) continue;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      T v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = Elem<DT>::put(__builtin_fmaf(acc[g][m][i], scale_unit(last[g][i >> 1] >> (16 * (i & 1))),
+                                            Elem<DT>::get((T)(bits[g][i >> 1] >> (16 * (i & 1))))));
+      __builtin_memcpy(__builtin_assume_aligned(mine + lr * PITCH + g * 16 + lk4, 8), v, sizeof(v));
+    }
+    // the lanes of this wave have written what its lanes read (one wave's LDS accesses are in order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int kPerRow = CH / 8;  // lanes a row
+#pragma unroll
+    for (int q = 0; q < (16 * kPerRow + 63) / 64; ++q) {
+      const int row = (q * 64 + lane) / kPerRow, c = (lane % kPerRow) * 8;
+      if (row < 16 && r0 + row < a.T && n_wave + c < a.N)
+        *reinterpret_cast<u32x4*>(static_cast<T*>(a.out) + (int64_t)(r0 + row) * a.N + n_wave + c) =
+            *reinterpret_cast<const u32x4*>(mine + row * PITCH + c);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int RING, int DT>
+hipError_t launch_tile(const Int4Args& a, hipStream_t s) {
+  const int64_t tiles = (int64_t)((a.T + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  const int stages = (a.K + kBK - 1) / kBK;
+  uint8_t* w = static_cast<uint8_t*>(a.workspace);
+  float* ratio = reinterpret_cast<float*>(w + (int64_t)stages * a.N * kBK);
+  const int halves = a.G % kBK != 0;
+  hipLaunchKernelGGL(int4_unpack_kernel, dim3((unsigned)stages * (unsigned)((a.N + 255) / 256)),
+                     dim3(256), 0, s, a, w, ratio, halves);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(64 * WM * WN);
+  if (halves)
+    hipLaunchKernelGGL((int4_tile_kernel<BM, BN, WM, WN, RING, DT, 1>), grid, block, 0, s, a, w, ratio);
+  else if (a.G % (2 * kBK))
+    hipLaunchKernelGGL((int4_tile_kernel<BM, BN, WM, WN, RING, DT, 2>), grid, block, 0, s, a, w, ratio);
+  else
+    hipLaunchKernelGGL((int4_tile_kernel<BM, BN, WM, WN, RING, DT, 4>), grid, block, 0, s, a, w, ratio);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- any alignment
+// A thread an output channel, kRows tokens, value by value: for tensors that start between two 16-byte
+// boundaries.
 constexpr int kRows = 8;
 
-// A thread an output channel, kRows tokens.
 template <int DT>
-__global__ __launch_bounds__(256) void int4_linear_kernel(Int4Args a) {
+__global__ __launch_bounds__(256) void int4_values_kernel(Int4Args a) {
   using T = typename Elem<DT>::T;
   const int blocks_n = (a.N + 255) / 256;
   const int n = blockIdx.x % blocks_n * 256 + threadIdx.x, t0 = blockIdx.x / blocks_n * kRows;
@@ -65,11 +651,57 @@ __global__ __launch_bounds__(256) void int4_linear_kernel(Int4Args a) {
     if (r < rows) static_cast<T*>(a.out)[(int64_t)(t0 + r) * a.N + n] = Elem<DT>::put(acc[r] + b);
 }
 
+// Workgroups of the few-rows kernel.
+int64_t stream_groups(int T, int N, int rows, int channels) {
+  return (int64_t)((T + rows - 1) / rows) * ((N + channels - 1) / channels);
+}
+
+// The larger a tile the fewer bytes of x and weights a workgroup reads for a result, the smaller the more
+// workgroups there are: the largest of these that still gives about one a CU. us with 16 x 16, 16 x 32,
+// 16 x 64, 32 x 64, 64 x 64: 1 row of 2048 x 4096 4.3 / 4.7 / 5.7, of 4096 x 8192 9.3 / 7.1 / 8.4, of 8192 x
+// 16384 32 / 19 / 16; 64 rows of 2048 x 4096 13 / 8.9 / 7.4 / 9.5, of 4096 x 8192 40 / 24 / 18 / 15 / 24; 203
+// of 1056 x 2008 13 / 9.2 / 8.1 / 7.0 / 10; 256 of 4096 x 8192 146 / 88 / 66 / 54 / 47.
+constexpr int kEnough = 224;
+template <int DT, int SPG>
+hipError_t launch_few_rows(const Int4Args& a, hipStream_t s) {
+  if (stream_groups(a.T, a.N, 64, 64) >= kEnough) return launch_stream<DT, 4, 4, SPG, 4>(a, s);
+  if (stream_groups(a.T, a.N, 32, 64) >= kEnough) return launch_stream<DT, 2, 4, SPG, 8>(a, s);
+  if (stream_groups(a.T, a.N, 16, 64) >= kEnough) return launch_stream<DT, 1, 4, SPG, 8>(a, s);
+  if (stream_groups(a.T, a.N, 16, 32) >= kEnough) return launch_stream<DT, 1, 2, SPG, 8>(a, s);
+  return launch_stream<DT, 1, 1, SPG, 8>(a, s);
+}
+
+// Unpacking takes the weights' bytes three times over and a launch, which the tiles have to win back: us
+// with the few-rows kernel / tiles: 256 rows of 4096 x 8192 44 / 39, 512 of 2048 x 4096 28 / 25, 1000 of 1088
+// x 2008 18 / 16, 128 of 2048 x 4096 9.3 / 22, 203 of 1056 x 2008 6.9 / 16. The sides meet at about the same
+// T sqrt(N K). (The tiles' 32-bit offsets hold 2^24 channels.)
+bool many_rows(int T, int K, int N) {
+  return T >= 64 && N <= (1 << 24) && (double)T * T * N * K >= 1.5e12;
+}
+
+// By the number of 128 x 128 tiles, us with 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256: 128 tiles (256 rows
+// of 4096 x 8192) 39 / 51 / 66 / 104, 256 (512 rows) 55 / 52 / 67 / 104, 512 (1024 rows) 89 / 85 / 73 / 105,
+// 2048 (4096 rows) 305 / 291 / 242 / 214.
 template <int DT>
-hipError_t launch_int4(const Int4Args& a, hipStream_t s) {
-  hipLaunchKernelGGL(int4_linear_kernel<DT>, dim3((a.N + 255) / 256 * ((a.T + kRows - 1) / kRows)),
-                     dim3(256), 0, s, a);
-  return hipGetLastError();
+hipError_t launch_many_rows(const Int4Args& a, hipStream_t s) {
+  const int64_t tiles = (int64_t)((a.T + 127) / 128) * ((a.N + 127) / 128);
+  if (tiles <= 160) return launch_tile<64, 128, 2, 2, 4, DT>(a, s);
+  if (tiles <= 320) return launch_tile<128, 128, 2, 2, 4, DT>(a, s);
+  if (tiles <= 1024) return launch_tile<128, 256, 2, 4, 3, DT>(a, s);
+  return launch_tile<256, 256, 2, 4, 2, DT>(a, s);
+}
+
+template <int DT>
+hipError_t launch_int4(const Int4Args& a, bool aligned, hipStream_t s) {
+  if (!aligned) {
+    const int64_t blocks = (int64_t)((a.N + 255) / 256) * ((a.T + kRows - 1) / kRows);
+    hipLaunchKernelGGL(int4_values_kernel<DT>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  if (many_rows(a.T, a.K, a.N)) return launch_many_rows<DT>(a, s);
+  if (a.G % 128 == 0) return launch_few_rows<DT, 4>(a, s);
+  if (a.G % 64 == 0) return launch_few_rows<DT, 2>(a, s);
+  return launch_few_rows<DT, 1>(a, s);
 }
 
 int check_int4(int32_t T, int32_t K, int32_t N, int32_t G, int32_t dtype) {
@@ -96,7 +728,8 @@ extern "C" {
 
 int64_t moe_int4_linear_workspace_bytes_v1(int32_t T, int32_t K, int32_t N, int32_t group_size) {
   if (check_int4(T, K, N, group_size, kBf16)) return -1;
-  return 0;
+  // the integers, and two ratios for each 64 of them
+  return many_rows(T, K, N) ? (int64_t)((K + 63) / 64) * N * (64 + 8) : 0;
 }
 
 int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,
@@ -111,7 +744,14 @@ int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,
     return op_fail(MOE_ERR_NULL, "int4 linear: NULL pointer");
   if (!aligned4(weight->qweight) || !aligned4(weight->qzeros))
     return op_fail(MOE_ERR_SHAPE, "int4 linear: qweight and qzeros must start on 4-byte boundaries");
-  const int64_t need = 0;
+  const int64_t need = moe_int4_linear_workspace_bytes_v1(T, K, N, group_size);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return op_fail(MOE_ERR_WORKSPACE, "int4 linear: workspace of %lld bytes, needs %lld",
+                     (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (!workspace_aligned(workspace))
+      return op_fail(MOE_ERR_WORKSPACE, "int4 linear: workspace must be 256-byte aligned");
+  }
   const int64_t nx = (int64_t)T * K * 2, no = (int64_t)T * N * 2, ng = K / group_size;
   const struct {
     const void* p;
@@ -123,12 +763,14 @@ int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,
       return op_fail(MOE_ERR_SHAPE, "int4 linear: out and the workspace must not overlap the inputs");
   if (overlaps(out, no, workspace, need))
     return op_fail(MOE_ERR_SHAPE, "int4 linear: out must not overlap the workspace");
-  (void)workspace_bytes;
   const Int4Args a{x, reinterpret_cast<const uint32_t*>(weight->qweight),
                    reinterpret_cast<const uint32_t*>(weight->qzeros), weight->scales, bias, out, T,
-                   K, N, group_size};
+                   K, N, group_size, K / group_size, workspace};
+  const bool aligned = aligned16(x) && aligned16(weight->qweight) && aligned16(weight->scales) &&
+                       aligned16(out);
   const auto s = (hipStream_t)stream;
-  MOE_OP_HIP(dtype == kBf16 ? launch_int4<kBf16>(a, s) : launch_int4<kFp16>(a, s), "int4 linear");
+  MOE_OP_HIP(dtype == kBf16 ? launch_int4<kBf16>(a, aligned, s) : launch_int4<kFp16>(a, aligned, s),
+             "int4 linear");
   return MOE_OK;
 }
 

@@ -67,8 +67,33 @@ def test_exact_sums(T, K, N, G, dtype):
     assert torch.equal(got.cpu(), want), int((got.cpu() != want).sum())
 
 
+TILES = [  # T, K, N, G: many rows: every tile, groups that end after one, two and more half steps, K that ends in
+    # the middle of a step, 1 to 13 steps, ragged last tiles
+    (3000, 512, 520, 128), (3001, 416, 776, 32), (2500, 832, 392, 64), (4000, 96, 1032, 96), (9000, 64, 640, 64),
+    (5000, 160, 776, 32), (4990, 256, 904, 128), (5003, 192, 776, 192), (6000, 640, 520, 640),
+    (9000, 96, 1032, 96), (9000, 128, 1032, 64), (8200, 384, 1288, 128), (7000, 448, 1544, 64),
+    (16400, 128, 1160, 128), (16390, 32, 1288, 32), (16500, 64, 1160, 64), (13000, 320, 1544, 64),
+    (12900, 384, 1672, 128), (12850, 224, 1800, 32)]
+
+
+@pytest.mark.parametrize("T,K,N,G", TILES)
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_exact_sums_of_many_rows(T, K, N, G, dtype):
+    """Scales are powers of two again, some of them zero: their groups count nothing."""
+    q, z, qw, qz, g = make(K, N, G)
+    x = torch.randint(-2, 3, (T, K), generator=g).to(dtype)
+    s = torch.tensor([0.25, 0.5, 1.0, 0.0, -0.5])[torch.randint(0, 5, (K // G, N), generator=g)].half()
+    s[-1, ::3] = 0.0
+    bias = torch.randint(-8, 9, (N,), generator=g).to(dtype) if T % 2 else None
+    want = exact(x.cuda(), q.cuda(), z.cuda(), s.cuda(), G, None if bias is None else bias.cuda()).float().to(dtype)
+    got = ops.int4_linear(x.cuda(), qw.cuda(), qz.cuda(), s.cuda(), group_size=G,
+                          bias=None if bias is None else bias.cuda())
+    assert torch.equal(got, want), int((got != want).sum())
+
+
 @pytest.mark.parametrize("T,K,N,G", [(1, 2048, 512, 128), (13, 1056, 200, 32), (40, 512, 264, 64),
-                                     (150, 2048, 328, 128), (700, 1024, 520, 64), (1200, 384, 1032, 384)])
+                                     (150, 2048, 328, 128), (700, 1024, 520, 64), (1200, 384, 1032, 384), (1500, 2048, 1032, 128), (2600, 1056, 520, 32),
+                                     (4400, 512, 4104, 64), (4096, 1024, 2056, 128)])
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_random_values(T, K, N, G, dtype):
     q, z, qw, qz, g = make(K, N, G, 1)
@@ -76,7 +101,8 @@ def test_random_values(T, K, N, G, dtype):
     x = (x * torch.where(torch.rand(K, generator=g) < 0.02, 20.0, 1.0)).to(dtype)
     s = (0.01 * (0.5 + torch.rand(K // G, N, generator=g))).half()
     bias = torch.randn(N, generator=g).to(dtype)
-    want = exact(x, q, z, s, G, bias)
+    on = lambda t: t.cuda()  # noqa: E731
+    want = exact(on(x), on(q), on(z), on(s), G, on(bias)).cpu()
     size = x.double().abs().view(T, -1, G).sum(2) @ s.double()
     got = ops.int4_linear(x.cuda(), qw.cuda(), qz.cuda(), s.cuda(), group_size=G, bias=bias.cuda())
     half = torch.finfo(dtype).eps / 2
@@ -113,7 +139,7 @@ def test_awq_projection():
     assert torch.equal(got.cpu(), want)
 
 
-@pytest.mark.parametrize("T", [1, 20, 100, 600])
+@pytest.mark.parametrize("T", [1, 20, 100, 600, 3500])
 def test_rows_do_not_touch_each_other(T):
     """An infinity or NaN in one token leaves the others' results; zeros of scale and padding of the
     output are left as they are."""
@@ -132,7 +158,7 @@ def test_rows_do_not_touch_each_other(T):
     assert not bool(got[T // 2].isfinite().any())
 
 
-@pytest.mark.parametrize("T", [1, 16, 50, 260, 700])
+@pytest.mark.parametrize("T", [1, 16, 50, 260, 700, 7000])
 def test_unaligned_tensors(T):
     """x, bias and scales 2 bytes off a boundary, int32 tensors 4 bytes off."""
     K, N, G = 256, 136, 64
@@ -157,7 +183,8 @@ def test_no_tokens():
 
 
 @pytest.mark.parametrize("sizes", [((1, 2048, 512, 128), (1, 4096, 264, 128)), ((90, 1024, 520, 64),) * 2,
-                                   ((600, 512, 520, 128), (9, 512, 264, 128))])
+                                   ((3200, 512, 520, 128), (9, 512, 264, 128)),
+                                   ((3000, 640, 520, 64),) * 2])
 def test_captured_calls_on_streams_of_their_own(sizes):
     """Two captured layers replayed on two streams at once, on changing inputs."""
     made = []
