@@ -283,6 +283,36 @@ __global__ __launch_bounds__(block_threads<NT>()) void block_norm_backward_kerne
   if (d.pre) f.store(d.part + 2 * all + me * H, tid, H, apre);
 }
 
+// The weights' gradients from the workgroups' sums: 32 columns a workgroup, 32 threads a column over
+// strided partials, then those 32 in order.
+constexpr int kSumCols = 32;
+struct SumOut {
+  void* out[3];
+};
+template <int DT>
+__global__ __launch_bounds__(1024) void block_norm_sum_kernel(const float* part, int partials,
+                                                              int H, SumOut o) {
+  __shared__ float s_sum[32][kSumCols + 1];
+  const int which = blockIdx.y;
+  if (!o.out[which]) return;
+  const int lane = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + lane;
+  const float* p = part + (int64_t)which * partials * H;
+  float s = 0.0f;
+  if (c < H) {
+#pragma unroll 8
+    for (int i = slot; i < partials; i += 32) s += p[(int64_t)i * H + c];
+  }
+  s_sum[slot][lane] = s;
+  __syncthreads();
+  if (slot == 0 && c < H) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v += s_sum[i][lane];
+    static_cast<typename Elem<DT>::T*>(o.out[which])[c] = Elem<DT>::put(v);
+  }
+}
+
 // Workgroups of the backward pass: each keeps the weights' gradients of its rows in registers and
 // writes them once.
 int backward_groups(int T, int H) {
@@ -315,7 +345,7 @@ hipError_t launch_backward(const NormArgs& a, const NormGrads& d, void* dpost, v
 #undef MOE_NORM_BWD
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(dpost || dgate_channel || dpre)) return e;
-  hipLaunchKernelGGL(column_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 3),
+  hipLaunchKernelGGL(block_norm_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 3),
                      dim3(1024), 0, s, d.part, d.partials, a.H, SumOut{{dpost, dgate_channel, dpre}});
   return hipGetLastError();
 }

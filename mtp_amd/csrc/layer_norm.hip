@@ -5,14 +5,13 @@
 //
 //   g = dy w;  dx = r (g - mean(g) - h mean(g h));  dw = sum_t dy h;  db = sum_t dy
 //
-// HBM-bound in both directions: rows are read and written once, 8 columns a thread held in registers
-// across the reduction. A row takes a wave up to 512 columns, a workgroup of 256 threads up to 2048, of
-// 512 up to 4096, of 1024 up to 8192.
+// HBM-bound in both directions: rows are read and written once, their columns held in registers 8 at a time
+// across the reductions. Sums are taken in a fixed order.
 //
-// One reduction gives both moments: with c the row's first value, d = x - c and both sums in 64 bits,
-// the variance is mean(d^2) - mean(d)^2. (m - c)^2 is at most hidden times the variance, since c is one of
-// the row's own values, so the difference loses at most log2(8192) of the 53 bits. Sums of raw x in 32 bits would lose all of a row whose mean is 2^12 times its
-// spread. x - m is taken as (x - m_hi) - m_lo for the same reason.
+// The mean is a sum in 64 bits of the differences to the row's first value: in 32 bits a row whose mean is 2^12
+// times its spread would lose half of its digits. It is kept in two parts, and x - m taken as (x - m_hi) - m_lo, off by two half steps. The squares of that are
+// summed 8 at a time in fp32 (a tree: 4 roundings) and from there on in 64 bits, so r is off by 3 half steps
+// whatever the row's width and mean.
 #include <algorithm>
 
 #include "common.h"
@@ -30,51 +29,75 @@ struct LayerNormArgs {
   double eps;
 };
 
-// What the backward pass needs of a row: the mean in two parts and r.
-struct RowStats {
-  float hi, lo, r;
-};
-
-template <int DT, int NT, bool VEC>
-__global__ __launch_bounds__(block_threads<NT>()) void layer_norm_kernel(LayerNormArgs a, void* y,
-                                                                         f32x4* stats) {
+// NT threads a row, NC chunks of 8 NT columns: a wave a row while it holds the row (2048 columns), with no
+// barrier and 12 exchanges for up to 32 columns a lane; with 256 threads a row of 2048 these and the barriers
+// were half of the kernel's instructions (16384 x 2048 bf16 31 us). A workgroup takes every so many rows and
+// has the next one's loads in flight while it works on this one.
+template <int DT, int NT, int NC, bool VEC>
+__global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* y, f32x4* stats) {
   using T = typename Elem<DT>::T;
   using C = Cols<DT, NT, VEC>;
-  __shared__ double s_part[NT / 64][2];
+  using Raw = RawCols<DT, NT, VEC>;
+  __shared__ double s_part[NT / 64][1];
   const double inv_h = 1.0 / (double)a.H;
-  const int tid = threadIdx.x % NT;
-  const int rows = block_threads<NT>() / NT;
+  const int tid = threadIdx.x % NT, H = a.H;
+  constexpr int rows = 256 / NT;
   const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
-  for (int64_t t = (int64_t)blockIdx.x * rows + sub; t < a.T; t += (int64_t)gridDim.x * rows) {
-    const T* row = static_cast<const T*>(a.x) + t * a.H;
-    float x[8], w[8], b[8];
-    C::load(row, tid, a.H, x);
-    const double c = (double)Elem<DT>::get(row[0]);
+  const int64_t stride = (int64_t)gridDim.x * rows, first = (int64_t)blockIdx.x * rows + sub;
+  Raw next[NC], w[NC] = {}, b[NC] = {};
+  auto load = [&](Raw (&v)[NC], const void* p, int64_t t) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = 1.0f;
-      b[e] = 0.0f;
-    }
-    if (a.w) C::load(static_cast<const T*>(a.w), tid, a.H, w);
-    if (a.b) C::load(static_cast<const T*>(a.b), tid, a.H, b);
-    double part[2] = {0.0, 0.0}, sum[2];
+    for (int c = 0; c < NC; ++c)
+      v[c].load(static_cast<const T*>(p) + t * H + c * 8 * NT, tid, H - c * 8 * NT);
+  };
+  float next_base = 0.0f;
+  auto load_x = [&](int64_t t) {  // past the last row: read again, not used
+    const int64_t u = min(t, (int64_t)a.T - 1);
+    load(next, a.x, u);
+    next_base = Elem<DT>::get(static_cast<const T*>(a.x)[u * H]);
+  };
+  if (first < a.T) load_x(first);
+  if (a.w) load(w, a.w, 0);
+  if (a.b) load(b, a.b, 0);
+  for (int64_t t = first; t < a.T; t += stride) {
+    float d[NC][8];
+    double part[1] = {0.0}, sum[1];
+    const double base = (double)next_base;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double d = C::col(tid, e) < a.H ? (double)x[e] - c : 0.0;
-      part[0] += d;
-      part[1] = __builtin_fma(d, d, part[1]);
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int left = H - c * 8 * NT;
+        d[c][e] = next[c].get(e, tid, left);
+        part[0] += C::col(tid, e) < left ? (double)d[c][e] - base : 0.0;
+      }
+    load_x(t + stride);
+    row_sums<NT>(part, sum, s_part);
+    const double mean = base + sum[0] * inv_h;
+    const float hi = (float)mean, lo = (float)(mean - (double)hi);
+    part[0] = 0.0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        d[c][e] = C::col(tid, e) < H - c * 8 * NT ? (d[c][e] - hi) - lo : 0.0f;
+      float q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = __builtin_fmaf(d[c][i], d[c][i], d[c][4 + i] * d[c][4 + i]);
+      part[0] += (double)((q[0] + q[1]) + (q[2] + q[3]));
     }
     row_sums<NT>(part, sum, s_part);
-    const double md = sum[0] * inv_h, mean = c + md;
-    // a rounding could leave the variance of a nearly constant row below zero
-    const double var = __builtin_fma(-md, md, sum[1] * inv_h);
-    const RowStats st{(float)mean, (float)(mean - (double)(float)mean),
-                      inv_sqrt((var < 0.0 ? 0.0 : var) + a.eps)};
-    if (stats && tid == 0) stats[t] = f32x4{st.hi, st.lo, st.r, 0.0f};
+    const float r = inv_sqrt(sum[0] * inv_h + a.eps);
+    if (stats && tid == 0) stats[t] = f32x4{hi, lo, r, 0.0f};
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x[e] = __builtin_fmaf(((x[e] - st.hi) - st.lo) * st.r, w[e], b[e]);
-    C::store(static_cast<T*>(y) + t * a.H, tid, a.H, x);
+    for (int c = 0; c < NC; ++c) {
+      const int left = H - c * 8 * NT;
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        o[e] = __builtin_fmaf(d[c][e] * r, a.w ? w[c].get(e, tid, left) : 1.0f, a.b ? b[c].get(e, tid, left) : 0.0f);
+      C::store(static_cast<T*>(y) + t * H + c * 8 * NT, tid, left, o);
+    }
   }
 }
 
@@ -82,8 +105,7 @@ struct LayerNormGrads {
   const void* dy;
   const f32x4* stats;
   void* dx;     // nullable
-  float* part;  // [2][partials][H]: dw, db
-  int partials;
+  float* part;  // [2][workgroups][H]: dw, db
   bool dw, db;  // which of them are wanted
 };
 
@@ -143,28 +165,86 @@ __global__ __launch_bounds__(block_threads<NT>()) void layer_norm_backward_kerne
       C::store(static_cast<T*>(d.dx) + t * H, tid, H, g);
     }
   }
-  const int64_t all = (int64_t)d.partials * H;
+  if constexpr (NT == 64) {  // the rows' waves first
+    __shared__ f32x4 s_all[4][4][64];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float* v = (q < 2 ? dw : db) + 4 * (q & 1);
+      s_all[sub][q][tid] = f32x4{v[0], v[1], v[2], v[3]};
+    }
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 v = s_all[0][q][tid];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += s_all[w][q][tid];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) (q < 2 ? dw : db)[4 * (q & 1) + j] = v[j];
+    }
+  }
+  const int64_t me = blockIdx.x, all = (int64_t)gridDim.x * H;
   Cols<kFp32, NT, VEC> f;
-  if (d.dw) f.store(d.part + first * H, tid, H, dw);
-  if (d.db) f.store(d.part + all + first * H, tid, H, db);
+  if (d.dw) f.store(d.part + me * H, tid, H, dw);
+  if (d.db) f.store(d.part + all + me * H, tid, H, db);
 }
+
+// The weights' gradients from the workgroups' sums: 16 columns a workgroup, 64 threads a column over
+// strided parts (12 loads each for the most workgroups, all in flight), a wave's four by a butterfly, then
+// the 16 waves' in order.
+constexpr int kSumCols = 16;
+template <int DT>
+__global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* part, int parts, int H,
+                                                              void* dw, void* db) {
+  __shared__ float s_sum[16][kSumCols];
+  void* const out = blockIdx.y ? db : dw;
+  if (!out) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = threadIdx.x % kSumCols;
+  const int c = blockIdx.x * kSumCols + col;
+  const float* p = part + (int64_t)blockIdx.y * parts * H + min(c, H - 1);
+  float s = 0.0f;
+#pragma unroll 12
+  for (int i = threadIdx.x / kSumCols; i < parts; i += 64) s += p[(int64_t)i * H];
+  s += xor_partner<32>(s);
+  s += xor_partner<16>(s);
+  if (lane < kSumCols) s_sum[wave][lane] = s;
+  __syncthreads();
+  if (threadIdx.x < kSumCols && c < H) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += s_sum[i][threadIdx.x];
+    static_cast<typename Elem<DT>::T*>(out)[c] = Elem<DT>::put(s);
+  }
+}
+
+// Workgroups of the forward pass: 6 a CU (16384 x 2048 bf16 with 2, 4, 6, 8 and 16 of them 23.5, 23.1, 24.0, 24.0
+// and 26.1 us, 16384 x 512 10.7, 9.8, 9.3, 9.5 and 9.8, 8192 x 4096 fp16 28.6, 24.6, 24.1, 23.8 and 24.8).
+constexpr int kForwardGroups = 1536;
 
 // Workgroups of the backward pass: each keeps the weights' gradients of its rows in registers and
 // writes them once.
 int backward_groups(int T, int H) {
   const int nt = threads_of(H), rows = rows_of(nt);
-  const int most = nt > 256 ? 512 : 768;
+  const int most = nt > 256 ? 256 : 768;
   return std::max(1, std::min((T - 1) / rows + 1, most));  // T + rows may pass 32 bits
 }
 
 template <int DT>
 hipError_t launch_forward(const LayerNormArgs& a, void* y, f32x4* stats, bool vec, hipStream_t s) {
-  const int nt = threads_of(a.H), rows = rows_of(nt);
-  const dim3 grid((unsigned)std::min<int64_t>((a.T + (int64_t)rows - 1) / rows, 1 << 20));
-#define MOE_LN_FWD(NT, V)                                                                      \
-  hipLaunchKernelGGL((layer_norm_kernel<DT, NT, V>), grid, dim3(block_threads<NT>()), 0, s, a, \
-                     y, stats)
-  MOE_ROW_NT(MOE_LN_FWD)
+#define MOE_LN_FWD(NT, NC)                                                                             \
+  do {                                                                                                 \
+    const int64_t groups = (a.T + int64_t(256 / NT) - 1) / (256 / NT);                                 \
+    const dim3 grid((unsigned)std::min<int64_t>(groups, kForwardGroups));  \
+    if (vec)                                                                                           \
+      hipLaunchKernelGGL((layer_norm_kernel<DT, NT, NC, true>), grid, dim3(256), 0, s, a, y, stats);   \
+    else                                                                                               \
+      hipLaunchKernelGGL((layer_norm_kernel<DT, NT, NC, false>), grid, dim3(256), 0, s, a, y, stats);  \
+  } while (0)
+  if (a.H <= 512) MOE_LN_FWD(64, 1);
+  else if (a.H <= 1024) MOE_LN_FWD(64, 2);
+  else if (a.H <= 2048) MOE_LN_FWD(64, 4);
+  else if (a.H <= 4096) MOE_LN_FWD(256, 2);
+  else MOE_LN_FWD(256, 4);
 #undef MOE_LN_FWD
   return hipGetLastError();
 }
@@ -181,8 +261,8 @@ hipError_t launch_backward(const LayerNormArgs& a, const LayerNormGrads& d, void
 #undef MOE_LN_BWD
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(dw || db)) return e;
-  hipLaunchKernelGGL(column_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 2), dim3(1024),
-                     0, s, d.part, d.partials, a.H, SumOut{{dw, db, nullptr}});
+  hipLaunchKernelGGL(layer_norm_sum_kernel<DT>, dim3((a.H + kSumCols - 1) / kSumCols, 2), dim3(1024),
+                     0, s, d.part, (int)grid.x, a.H, dw, db);
   return hipGetLastError();
 }
 
@@ -227,7 +307,7 @@ int moe_layer_norm_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype, c
 
 int64_t moe_layer_norm_workspace_bytes_v1(int32_t T, int32_t hidden) {
   if (T < 0 || hidden < 1 || hidden > kMaxHidden) return -1;
-  return (int64_t)2 * backward_groups(T, hidden) * rows_of(threads_of(hidden)) * hidden * 4;
+  return (int64_t)2 * backward_groups(T, hidden) * hidden * 4;
 }
 
 int moe_layer_norm_backward_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype,
@@ -266,9 +346,7 @@ int moe_layer_norm_backward_v1(const void* x, int32_t T, int32_t hidden, int32_t
   }
   const LayerNormArgs a{x, weight, nullptr, T, hidden, 0.0};
   const LayerNormGrads d{dy, reinterpret_cast<const f32x4*>(stats), dx,
-                         static_cast<float*>(workspace),
-                         backward_groups(T, hidden) * rows_of(threads_of(hidden)),
-                         dweight != nullptr, dbias != nullptr};
+                         static_cast<float*>(workspace), dweight != nullptr, dbias != nullptr};
   const bool vec = vec_ok(hidden, {x, weight, dy, dx, workspace});
   const auto s = (hipStream_t)stream;
   MOE_OP_HIP(dtype == kBf16   ? launch_backward<kBf16>(a, d, dweight, dbias, vec, s)

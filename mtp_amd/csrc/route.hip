@@ -25,8 +25,86 @@
 
 namespace {
 
-constexpr int kWaves = 16, kMaxExperts = 512, kMaxGroups = 256;
-constexpr uint32_t kLowest = 0x007FFFFFu;  // topk_ord(-inf)
+constexpr int kWaves = 16, kMaxExperts = 512, kMaxGroups = 512;
+
+// The order of a token's logits in 32-bit keys, 0 for "not a candidate", and the selection of the largest
+// top_k of a wave's keys (expert lane + 64 c in key[c]): lane r < top_k gets the r-th one's id and value,
+// `mine` false where no logit above -inf was left.
+//
+// Logits of 16 bits leave room for the id: a key is (order, complement of the id), unique, its maximum names
+// the expert, and a round is the maximum and one comparison a register (19 VALU operations at 256 experts).
+template <int DT, int NC>
+struct Select {
+  static constexpr uint32_t kInf = DT == kBf16 ? 0x7F80u : 0x7C00u;
+  static constexpr uint32_t kLowest = (~(kInf | 0x8000u) & 0xFFFFu) << 16 | 0xFFFFu;  // above any -inf
+  MOE_DEV static uint32_t key(uint16_t v, int id) {
+    uint32_t u = v;
+    u = (u & 0x7FFFu) == 0 ? 0u : u;  // -0 -> +0
+    uint32_t o = u & 0x8000u ? ~u & 0xFFFFu : u | 0x8000u;
+    o = (u & 0x7FFFu) > kInf ? 0u : o;  // NaN below every number
+    return o << 16 | (0xFFFFu - (uint32_t)id);
+  }
+  MOE_DEV static float value(uint32_t key) {
+    const uint32_t o = key >> 16;
+    return Elem<DT>::get((uint16_t)(o & 0x8000u ? o & 0x7FFFu : ~o));
+  }
+  MOE_DEV static void select(uint32_t (&key)[NC], int top_k, int lane, int& id, float& v, bool& mine) {
+    uint32_t my = 0;
+    for (int r = 0; r < top_k; ++r) {
+      uint32_t m = key[0];
+#pragma unroll
+      for (int c = 1; c < NC; ++c) m = max(m, key[c]);
+      m = wave_max_u32(m);
+      if (m <= kLowest) break;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) key[c] = key[c] == m ? 0u : key[c];
+      my = lane == r ? m : my;
+    }
+    id = (int)(0xFFFFu - (my & 0xFFFFu));
+    v = value(my);
+    mine = my != 0;
+  }
+};
+// Logits of 32 bits: the lanes that hold the maximum name their lowest id; where several do, the lowest of
+// theirs is looked for register by register.
+template <int NC>
+struct Select<kFp32, NC> {
+  static constexpr uint32_t kLowest = 0x007FFFFFu;  // topk_ord(-inf)
+  MOE_DEV static uint32_t key(float v, int) { return topk_ord(v); }
+  MOE_DEV static float value(uint32_t key) { return topk_ord_value(key); }
+  MOE_DEV static void select(uint32_t (&key)[NC], int top_k, int lane, int& id, float& v, bool& mine) {
+    uint32_t my = 0;
+    id = 0;
+    for (int r = 0; r < top_k; ++r) {
+      uint32_t m = key[0];
+#pragma unroll
+      for (int c = 1; c < NC; ++c) m = max(m, key[c]);
+      m = wave_max_u32(m);
+      if (m <= kLowest) break;
+      int held = -1;
+#pragma unroll
+      for (int c = NC - 1; c >= 0; --c) held = key[c] == m ? lane + 64 * c : held;
+      const uint64_t holds = __ballot(held >= 0);
+      int sel = __builtin_amdgcn_readlane(held, __builtin_ctzll(holds));
+      if (holds & (holds - 1)) {
+        sel = -1;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const uint64_t b = __ballot(key[c] == m);
+          if (sel < 0 && b != 0) sel = 64 * c + __builtin_ctzll(b);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) key[c] = lane + 64 * c == sel ? 0u : key[c];
+      if (lane == r) {
+        id = sel;
+        my = m;
+      }
+    }
+    v = value(my);
+    mine = my != 0;
+  }
+};
 
 // Behind one another in the workspace: the workgroups' sums, and the sums kernel's own.
 struct RouteWs {
@@ -53,7 +131,7 @@ struct RouteArgs {
 
 MOE_DEV float wave_sum(float v) { return bfly_sum(v); }
 
-constexpr int kCols = 32;  // experts a workgroup of the sums
+constexpr int kCols = 16;  // experts a workgroup of the sums: at most 32 workgroups
 
 // The losses from their sums.
 MOE_DEV void finish(const RouteArgs& a, double dot, double zsum, int n) {
@@ -82,25 +160,36 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
   int n = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) psum[c] = 0.0f;
-  for (int64_t t = (int64_t)blockIdx.x * waves + wave; t < a.T; t += (int64_t)gridDim.x * waves) {
-    const T* row = static_cast<const T*>(a.logits) + t * a.E;
+  using S = Select<DT, NC>;
+  const int64_t stride = (int64_t)gridDim.x * waves;
+  T next[NC];
+  bool next_kept = false;
+  auto load = [&](int64_t t) {  // past the last token: read again, not used
+    const int64_t u = min(t, (int64_t)a.T - 1);
+    const T* row = static_cast<const T*>(a.logits) + u * a.E;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) next[c] = row[min(lane + 64 * c, a.E - 1)];
+    next_kept = !a.mask || a.mask[u] != 0;
+  };
+  const int64_t first = (int64_t)blockIdx.x * waves + wave;
+  if (first < a.T) load(first);
+  for (int64_t t = first; t < a.T; t += stride) {
     float l[NC];
     uint32_t key[NC], peak = 0;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) l[c] = Elem<DT>::get(row[min(lane + 64 * c, a.E - 1)]);
-    const bool kept = !a.mask || a.mask[t] != 0;
     bool nan = false;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const bool in = lane + 64 * c < a.E;
-      key[c] = in ? topk_ord(l[c]) : 0u;
-      l[c] = in ? l[c] : -__builtin_inff();
+      key[c] = in ? S::key(next[c], lane + 64 * c) : 0u;
+      l[c] = in ? Elem<DT>::get(next[c]) : -__builtin_inff();
       nan |= l[c] != l[c];
       peak = max(peak, key[c]);
     }
+    const bool kept = next_kept;
+    load(t + stride);
     peak = wave_max_u32(peak);
-    const bool live = kept && (peak > kLowest || __ballot(nan) != 0);
-    const float top = peak > kLowest ? topk_ord_value(peak) : 0.0f;
+    const bool live = kept && (peak > S::kLowest || __ballot(nan) != 0);
+    const float top = peak > S::kLowest ? S::value(peak) : 0.0f;
     float ex[NC], total = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -109,10 +198,10 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
     }
     total = wave_sum(total);
     int my_i;
-    uint32_t my_key;
-    topk_select_keys<NC>(key, a.k, lane, my_i, my_key);
-    const bool chosen = live && lane < a.k && my_key > kLowest;
-    const float mine = chosen ? expf(topk_ord_value(my_key) - top) : 0.0f;
+    float my_v;
+    bool chosen;
+    S::select(key, live ? a.k : 0, lane, my_i, my_v, chosen);
+    const float mine = chosen ? expf(my_v - top) : 0.0f;
     float over = total;
     if (a.renorm) {
       // a NaN or +inf among the logits makes the weights NaN, also where it is not chosen
@@ -179,64 +268,74 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
   }
 }
 
-// The workgroups' sums: kCols experts a workgroup, 32 threads an expert. The last workgroup to arrive
-// adds the workgroups' shares of the balance, in their order.
+// The workgroups' sums: kCols experts a workgroup, 64 threads an expert. The last workgroup to arrive adds
+// the workgroups' shares of the balance, in their order; z and the count each has summed ahead of that.
 __global__ __launch_bounds__(1024) void route_sum_kernel(RouteArgs a) {
-  __shared__ double s_p[32][kCols];
-  __shared__ int s_c[32][kCols];
-  __shared__ bool s_last;
-  const int tid = threadIdx.x, col = tid % kCols, slot = tid / kCols;
-  const int e = blockIdx.x * kCols + col;
+  __shared__ double s_p[16][kCols];
+  __shared__ int s_c[16][kCols];
+  __shared__ double s_z[16];
+  __shared__ int s_n[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = tid % kCols, slot = tid / kCols;
+  const int e = blockIdx.x * kCols + col, at = min(e, a.E - 1);
   double p = 0.0;
   int c = 0;
-  if (e < a.E) {
 #pragma unroll 8
-    for (int g = slot; g < a.groups; g += 32) {
-      p += (double)a.ws.p[(int64_t)g * a.E + e];
-      c += a.ws.c[(int64_t)g * a.E + e];
-    }
+  for (int g = slot; g < a.groups; g += 1024 / kCols) {
+    p += (double)a.ws.p[(int64_t)g * a.E + at];
+    c += a.ws.c[(int64_t)g * a.E + at];
   }
-  s_p[slot][col] = p;
-  s_c[slot][col] = c;
-  __syncthreads();
-  if (tid < 64) {
-    double dot = 0.0;
-    if (tid < kCols && e < a.E) {
-      p = 0.0;
-      c = 0;
-      for (int i = 0; i < 32; ++i) {
-        p += s_p[i][col];
-        c += s_c[i][col];
-      }
-      a.counts[e] = c;
-      dot = (double)c * p;
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) dot += __shfl_xor(dot, m);
-    if (tid == 0) {
-      __hip_atomic_store(a.ws.parts + blockIdx.x, dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      s_last = __hip_atomic_fetch_add(a.ws.arrived, 1u, __ATOMIC_ACQ_REL,
-                                      __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-    }
+  double z = tid < a.groups ? (double)a.ws.z[tid] : 0.0;  // at most 512 workgroups
+  int n = tid < a.groups ? a.ws.n[tid] : 0;
+  // a wave's slots of an expert: lanes col, col + 16, ...
+  for (int m = 32; m >= kCols; m >>= 1) {
+    p += __shfl_xor(p, m);
+    c += __shfl_xor(c, m);
   }
-  __syncthreads();
-  if (!s_last || tid >= 64) return;
-  double z = 0.0, dot = 0.0;
-  int n = 0;
-  for (int g = tid; g < a.groups; g += 64) {
-    z += (double)a.ws.z[g];
-    n += a.ws.n[g];
-  }
-#pragma unroll
   for (int m = 32; m >= 1; m >>= 1) {
     z += __shfl_xor(z, m);
     n += __shfl_xor(n, m);
   }
-  if (tid == 0) {
-    for (unsigned b = 0; b < gridDim.x; ++b)
-      dot += __hip_atomic_load(a.ws.parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    finish(a, dot, z, n);
+  if (lane < kCols) {
+    s_p[wave][lane] = p;
+    s_c[wave][lane] = c;
   }
+  if (lane == 0) {
+    s_z[wave] = z;
+    s_n[wave] = n;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  double dot = 0.0;
+  if (lane < kCols && e < a.E) {
+    p = 0.0;
+    c = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p += s_p[i][lane];
+      c += s_c[i][lane];
+    }
+    a.counts[e] = c;
+    dot = (double)c * p;
+  }
+  z = lane < 16 ? s_z[lane] : 0.0;
+  n = lane < 16 ? s_n[lane] : 0;
+  for (int m = 8; m >= 1; m >>= 1) {  // lanes 0 to 15 hold all of the three
+    dot += __shfl_xor(dot, m);
+    z += __shfl_xor(z, m);
+    n += __shfl_xor(n, m);
+  }
+  uint32_t before = 0;
+  if (lane == 0) {
+    __hip_atomic_store(a.ws.parts + blockIdx.x, dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    before = __hip_atomic_fetch_add(a.ws.arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if ((uint32_t)__builtin_amdgcn_readfirstlane((int)before) != gridDim.x - 1) return;
+  dot = lane < (int)gridDim.x ? __hip_atomic_load(a.ws.parts + lane, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT)
+                              : 0.0;
+  for (int m = 32; m >= 1; m >>= 1) dot += __shfl_xor(dot, m);
+  if (lane == 0) finish(a, dot, z, n);
 }
 
 struct RouteGradArgs {

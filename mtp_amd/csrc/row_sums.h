@@ -77,39 +77,6 @@ constexpr int block_threads() { return NT < 256 ? 256 : NT; }
     if (vec) LAUNCH(1024, true); else LAUNCH(1024, false); \
   }
 
-// Column sums of the workgroups' parts [outputs][partials][H]: 32 columns a workgroup, 32 threads a
-// column over strided partials, then those 32 in order.
-// (Unnamed: each source has its own kernel.)
-namespace {
-constexpr int kSumCols = 32;
-struct SumOut {
-  void* out[3];
-};
-template <int DT>
-__global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, int partials, int H,
-                                                          SumOut o) {
-  __shared__ float s_sum[32][kSumCols + 1];
-  const int which = blockIdx.y;
-  if (!o.out[which]) return;
-  const int lane = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols;
-  const int c = blockIdx.x * kSumCols + lane;
-  const float* p = part + (int64_t)which * partials * H;
-  float s = 0.0f;
-  if (c < H) {
-#pragma unroll 8
-    for (int i = slot; i < partials; i += 32) s += p[(int64_t)i * H + c];
-  }
-  s_sum[slot][lane] = s;
-  __syncthreads();
-  if (slot == 0 && c < H) {
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v += s_sum[i][lane];
-    static_cast<typename Elem<DT>::T*>(o.out[which])[c] = Elem<DT>::put(v);
-  }
-}
-}  // namespace
-
 // A tensor's memory.
 struct Span {
   const void* p;

@@ -1,9 +1,10 @@
 """Layer norm and its gradients against the formulas in 64 bits.
 
-u = 2^-24 is fp32's half step. The moments are taken in 64 bits and 1 / sqrt(var + eps) is rounded once,
-so h = ((x - m_hi) - m_lo) r is off by at most 4 u |h|, and y = fma(h, w, b) by 5 u |h w| + u |y|. The
-means of g and g h are fp32 sums over 8 columns a thread, 6 butterfly steps and up to 16 waves: 30
-roundings and their division, 33 u of the mean of the magnitudes, and 5 u more where h stands in them.
+u = 2^-24 is fp32's half step. The mean is a sum in 64 bits. x - m = (x - m_hi) - m_lo is off by 2 u of
+itself; a square of it by 4 u and its product's rounding, 8 of them in a tree of fp32 by 3 more, the rest in
+64 bits: the variance by 8 u, r by 4 u and its rounding, so h by 2 + 5 + 1 = 8 u |h|, and y = fma(h, w, b) by
+8 u |h w| + u |y|. The means of g and g h are fp32 sums over 8 columns a thread, 6 butterfly steps and up to 16 waves: 30
+roundings and their division, 33 u of the mean of the magnitudes, and 9 u more where h stands in them.
 Sums over tokens add a rounding a token. Each result is rounded once to its type.
 """
 
@@ -51,10 +52,10 @@ def formulas(s):
     g = dy * w
     mean = lambda v: v.mean(1, keepdim=True)  # noqa: E731
     dx = r * (g - mean(g) - h * mean(g * h))
-    slack = r * U * (4 * g.abs() + 36 * mean(g.abs()) + h.abs() * 46 * mean((g * h).abs()))
-    return y, U * (5 * (h * w).abs() + y.abs()), {
+    slack = r * U * (8 * g.abs() + 40 * mean(g.abs()) + h.abs() * 56 * mean((g * h).abs()))
+    return y, U * (8 * (h * w).abs() + y.abs()), {
         "x": (dx, slack),
-        "weight": ((dy * h).sum(0), (T + 40) * U * (dy * h).abs().sum(0)),
+        "weight": ((dy * h).sum(0), (T + 44) * U * (dy * h).abs().sum(0)),
         "bias": (dy.sum(0), (T + 40) * U * dy.abs().sum(0))}
 
 
@@ -104,7 +105,7 @@ def test_rows_far_from_zero(mean, spread, H):
     x[1, 0] = mean + 1000 * spread  # the value that the sums are taken from is an outlier
     d = x.double() - x.double().mean(1, keepdim=True)
     want = d * (d.square().mean(1, keepdim=True) + EPS).rsqrt()
-    near(ops.layer_norm(x.cuda(), eps=EPS), want, 6 * U * want.abs(), torch.float32)
+    near(ops.layer_norm(x.cuda(), eps=EPS), want, 9 * U * want.abs(), torch.float32)
 
 
 def test_constant_rows():
