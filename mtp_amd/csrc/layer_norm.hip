@@ -8,8 +8,8 @@
 // HBM-bound in both directions: rows are read and written once, their columns held in registers 8 at a time
 // across the reductions. Sums are taken in a fixed order.
 //
-// The mean is a sum in 64 bits of the differences to the row's first value: in 32 bits a row whose mean is 2^12
-// times its spread would lose half of its digits. It is kept in two parts, and x - m taken as (x - m_hi) - m_lo, off by two half steps. The squares of that are
+// The mean is a sum in 64 bits and a division (a constant row's sum is exact, and so is then its mean): in 32 bits
+// a row whose mean is 2^12 times its spread would lose half of its digits. It is kept in two parts, and x - m taken as (x - m_hi) - m_lo, off by two half steps. The squares of that are
 // summed 8 at a time in fp32 (a tree: 4 roundings) and from there on in 64 bits, so r is off by 3 half steps
 // whatever the row's width and mean.
 #include <algorithm>
@@ -50,30 +50,23 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
     for (int c = 0; c < NC; ++c)
       v[c].load(static_cast<const T*>(p) + t * H + c * 8 * NT, tid, H - c * 8 * NT);
   };
-  float next_base = 0.0f;
-  auto load_x = [&](int64_t t) {  // past the last row: read again, not used
-    const int64_t u = min(t, (int64_t)a.T - 1);
-    load(next, a.x, u);
-    next_base = Elem<DT>::get(static_cast<const T*>(a.x)[u * H]);
-  };
-  if (first < a.T) load_x(first);
+  if (first < a.T) load(next, a.x, first);
   if (a.w) load(w, a.w, 0);
   if (a.b) load(b, a.b, 0);
   for (int64_t t = first; t < a.T; t += stride) {
     float d[NC][8];
     double part[1] = {0.0}, sum[1];
-    const double base = (double)next_base;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int left = H - c * 8 * NT;
         d[c][e] = next[c].get(e, tid, left);
-        part[0] += C::col(tid, e) < left ? (double)d[c][e] - base : 0.0;
+        part[0] += (double)d[c][e];
       }
-    load_x(t + stride);
+    load(next, a.x, min(t + stride, (int64_t)a.T - 1));  // past the last row: read again, not used
     row_sums<NT>(part, sum, s_part);
-    const double mean = base + sum[0] * inv_h;
+    const double mean = sum[0] / (double)H;
     const float hi = (float)mean, lo = (float)(mean - (double)hi);
     part[0] = 0.0;
 #pragma unroll

@@ -11,17 +11,19 @@
 // A token counts if the mask keeps it and one of its logits is above -inf or a NaN; other tokens have ids
 // -1, weights 0 and no gradient. Only logits above -inf are chosen; places without one have id -1.
 //
-// A wave takes a token, 64 experts a register; the selection's rounds (a wave maximum and a ballot each)
-// bound it, not the bytes: they are a few VALU operations a byte read. A wave keeps its sums of p in
-// registers and its workgroup the counts in LDS (integer atomics: the order does not matter), so that a
-// workgroup leaves one row of partial sums. Sums are taken in a fixed order: fp32 over a wave's tokens
-// and a workgroup's waves, 64 bits over the workgroups.
+// Not the bytes but the instructions of the selection bound it: a wave a token, or for many tokens of 16-bit
+// logits four tokens a wave.
+//
+// A wave keeps its sums of p in registers and its workgroup the counts in LDS (integer atomics: the order does
+// not matter), so that a workgroup leaves one row of partial sums. Sums are taken in a fixed order: fp32 over a
+// wave's tokens and a workgroup's waves, 64 bits over the workgroups.
 #include <algorithm>
 
 #include "common.h"
 #include "elem.h"
 #include "launch.h"
 #include "routing.h"
+#include "row_sums.h"
 
 namespace {
 
@@ -130,6 +132,14 @@ struct RouteArgs {
 };
 
 MOE_DEV float wave_sum(float v) { return bfly_sum(v); }
+MOE_DEV double wave_sum(double v) {
+  v += partner<32>(v);
+  v += partner<16>(v);
+  v += partner<8>(v);
+  v += partner<4>(v);
+  v += partner<2>(v);
+  return v + partner<1>(v);
+}
 
 constexpr int kCols = 16;  // experts a workgroup of the sums: at most 32 workgroups
 
@@ -141,21 +151,237 @@ MOE_DEV void finish(const RouteArgs& a, double dot, double zsum, int n) {
   if (a.lse) a.lse[a.T] = (float)n;
 }
 
+// A workgroup's sums: p of each wave and expert, slots of each expert.
+template <int W, int NE>
+struct BlockSums {
+  float p[W][NE];
+  int c[NE];
+  float z[W];
+  int n[W];
+  double dot[W];
+  MOE_DEV void clear(const RouteArgs& a) {
+    for (int e = threadIdx.x; e < NE; e += blockDim.x) c[e] = 0;
+    if (a.groups > 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.ws.arrived = 0;
+    __syncthreads();
+  }
+};
+
+// Behind every wave's p: the workgroup's row of partial sums, or the results where it is the only one. z and n
+// are the wave's.
+template <int W, int NE>
+MOE_DEV void block_sums(const RouteArgs& a, BlockSums<W, NE>& s, float zsum, int n) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  if (lane == 0) {
+    s.z[wave] = zsum;
+    s.n[wave] = n;
+  }
+  __syncthreads();
+  float z = 0.0f;
+  int live = 0;
+  for (int w = 0; w < waves; ++w) {
+    z += s.z[w];
+    live += s.n[w];
+  }
+  if (a.groups > 1) {
+    for (int e = tid; e < a.E; e += blockDim.x) {
+      float p = 0.0f;
+      for (int w = 0; w < waves; ++w) p += s.p[w][e];
+      a.ws.p[(int64_t)blockIdx.x * a.E + e] = p;
+      a.ws.c[(int64_t)blockIdx.x * a.E + e] = s.c[e];
+    }
+    if (tid == 0) {
+      a.ws.z[blockIdx.x] = z;
+      a.ws.n[blockIdx.x] = live;
+    }
+    return;
+  }
+  double dot = 0.0;
+  for (int e = tid; e < a.E; e += blockDim.x) {
+    float p = 0.0f;
+    for (int w = 0; w < waves; ++w) p += s.p[w][e];
+    a.counts[e] = s.c[e];
+    dot += (double)s.c[e] * (double)p;
+  }
+  dot = wave_sum(dot);
+  if (lane == 0) s.dot[wave] = dot;
+  __syncthreads();
+  if (tid == 0) {
+    dot = 0.0;
+    for (int w = 0; w < waves; ++w) dot += s.dot[w];
+    finish(a, dot, (double)z, live);
+  }
+}
+
+// exp(x) for x <= 0, and a NaN for a NaN: 2^(x log2 e) with the product in two parts, off by about 2 half
+// steps; a third of the library's operations. Below e^-104 there is no fp32 number.
+MOE_DEV float exp_neg(float x) {
+  constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
+  x = x < -110.0f ? -110.0f : x;
+  const float hi = x * kLog2e;
+  const float lo = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -hi));
+  const float r = __builtin_amdgcn_exp2f(hi);
+  return __builtin_fmaf(r * lo, kLn2, r);
+}
+
+// ---------------------------------------------------------------- 16 lanes a token
+template <int M>
+MOE_DEV uint32_t row_partner(uint32_t v) { return __float_as_uint(xor_partner<M>(__uint_as_float(v))); }
+MOE_DEV uint32_t row_max(uint32_t v) {
+  v = max(v, row_partner<8>(v));
+  v = max(v, row_partner<4>(v));
+  v = max(v, row_partner<2>(v));
+  return max(v, row_partner<1>(v));
+}
+MOE_DEV float row_max(float v) {  // of a NaN and a number the number
+  v = __builtin_fmaxf(v, xor_partner<8>(v));
+  v = __builtin_fmaxf(v, xor_partner<4>(v));
+  v = __builtin_fmaxf(v, xor_partner<2>(v));
+  return __builtin_fmaxf(v, xor_partner<1>(v));
+}
+MOE_DEV float row_sum(float v) {
+  v += xor_partner<8>(v);
+  v += xor_partner<4>(v);
+  v += xor_partner<2>(v);
+  return v + xor_partner<1>(v);
+}
+
+// A key for the selection: (order, complement of the id), unique, 25 bits.
+template <int DT>
+struct GroupKey {
+  static constexpr uint32_t kInf = DT == kBf16 ? 0x7F80u : 0x7C00u;
+  static constexpr uint32_t kLowest = (~(kInf | 0x8000u) & 0xFFFFu) << 9 | 511u;  // -inf, of any id
+  MOE_DEV static uint32_t key(uint16_t v, int id) {
+    uint32_t u = v;
+    u = (u & 0x7FFFu) == 0 ? 0u : u;  // -0 -> +0
+    uint32_t o = u & 0x8000u ? ~u & 0xFFFFu : u | 0x8000u;
+    o = (u & 0x7FFFu) > kInf ? 0u : o;  // NaN below every number
+    return o << 9 | (511u - (uint32_t)id);
+  }
+};
+
+// Four tokens a wave: a round of the selection is a subtraction and half a maximum for each of a lane's logits
+// and four exchanges, for all four. us of the routing with a wave a token / with this (bf16): 8192 x 256, top-8
+// 17.4 / 13.7, 32768 x 64 25.7 / 14.3, 1501 x 60 (fp16, top-5) 9.4 / 9.0; of few tokens a wave's own are done
+// sooner (256 x 256 fp32 11.2 / 15.4). fp32 logits leave no room for the id: a selection by their upper bits
+// with a check against the values took 26.3 for 16384 x 256 where a wave a token takes 24.3.
+constexpr int kGroupWaves = 8, kGroupTokens = 4 * kGroupWaves, kGroupMaxTopK = 16, kGroupMinT = 1024;
+bool route_grouped(int T, int k, int dtype) {
+  return dtype != kFp32 && k <= kGroupMaxTopK && T >= kGroupMinT;
+}
+
+// PL logits a lane: expert 16 j + (lane & 15).
+template <int DT, int PL>
+__global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs a) {
+  using T = typename Elem<DT>::T;
+  using K = GroupKey<DT>;
+  __shared__ BlockSums<kGroupWaves, 16 * PL> s;
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = blockDim.x >> 6;
+  s.clear(a);
+  float psum[PL], zsum = 0.0f;
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < PL; ++j) psum[j] = 0.0f;
+  const int64_t stride = (int64_t)gridDim.x * waves * 4;
+  T next[PL];
+  bool next_kept = false;
+  auto load = [&](int64_t t) {  // past the last token: read again, not used
+    const int64_t u = min(t, (int64_t)a.T - 1);
+    const T* row = static_cast<const T*>(a.logits) + u * a.E;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) next[j] = row[min(16 * j + l16, a.E - 1)];
+    next_kept = !a.mask || a.mask[u] != 0;
+  };
+  int64_t t = ((int64_t)blockIdx.x * waves + wave) * 4 + (lane >> 4);
+  if (t - (lane >> 4) < a.T) load(t);
+  for (; t - (lane >> 4) < a.T; t += stride) {
+    float x[PL];
+    uint32_t key[PL], m = 0;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      const bool in = 16 * j + l16 < a.E;
+      x[j] = in ? Elem<DT>::get(next[j]) : -__builtin_inff();
+      key[j] = in ? K::key(next[j], 16 * j + l16) : 0u;
+      top = __builtin_fmaxf(top, x[j]);
+      m = max(m, key[j]);
+    }
+    const bool kept = next_kept && t < a.T;
+    load(t + stride);
+    top = row_max(top);
+    const bool some = top > -__builtin_inff();
+    if (!some) top = 0.0f;
+    m = row_max(m);
+    // lane r of the 16: the r-th largest key; below a maximum m the next one is the largest of key - m, in
+    // which those not below it are the small ones
+    uint32_t my = 0;
+    for (int r = 0; r < a.k; ++r) {
+      if (l16 == r) my = m;
+      uint32_t d = 0;
+#pragma unroll
+      for (int j = 0; j < PL; ++j) d = max(d, key[j] - m);
+      d = row_max(d);
+      m = d >> 31 ? m + d : 0u;  // none left: 0 is below every key
+    }
+    bool chosen = l16 < a.k && my > K::kLowest;
+    const int id = (int)(511u - (my & 511u));
+    const uint32_t o = my >> 9;
+    const float v = Elem<DT>::get((uint16_t)(o & 0x8000u ? o & 0x7FFFu : ~o));
+    float total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      x[j] = exp_neg(x[j] - top);
+      total += x[j];
+    }
+    total = row_sum(total);
+    const bool live = kept && (some || total != total);
+    chosen = chosen && live;
+    const float mine = chosen ? exp_neg(v - top) : 0.0f;
+    float over = total;
+    if (a.renorm) {
+      // a NaN or +inf among the logits makes the weights NaN, also where it is not chosen
+      over = row_sum(mine);
+      if (!(total < __builtin_inff())) over = total;
+    }
+    if (t < a.T && l16 < a.k) {
+      a.ids[t * a.k + l16] = chosen ? id : -1;
+      a.weights[t * a.k + l16] = chosen ? mine / over : 0.0f;
+    }
+    if (chosen) atomicAdd(&s.c[id], 1);
+    const float lse = top + logf(total);
+    if (a.lse && l16 == 0 && t < a.T) a.lse[t] = live ? lse : __builtin_inff();
+    if (live) {
+      const float inv = 1.0f / total;
+#pragma unroll
+      for (int j = 0; j < PL; ++j) psum[j] = __builtin_fmaf(x[j], inv, psum[j]);
+      if (l16 == 0) {
+        zsum = __builtin_fmaf(lse, lse, zsum);
+        ++n;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PL; ++j) {
+    psum[j] += xor_partner<16>(psum[j]);
+    psum[j] += xor_partner<32>(psum[j]);
+    if (lane < 16) s.p[wave][16 * j + l16] = psum[j];
+  }
+  zsum = wave_sum(zsum);
+  n = (int)wave_sum((float)n);  // at most 2^22
+  block_sums(a, s, zsum, n);
+}
+
+// ---------------------------------------------------------------- a wave a token
 // NC registers of 64 experts each.
 template <int DT, int NC>
 __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
   using T = typename Elem<DT>::T;
-  __shared__ float s_p[kWaves][64 * NC];
-  __shared__ int s_c[64 * NC];
-  __shared__ float s_z[kWaves];
-  __shared__ int s_n[kWaves];
-  __shared__ double s_dot[kWaves];
+  __shared__ BlockSums<kWaves, 64 * NC> s;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = blockDim.x >> 6;
-  for (int e = tid; e < 64 * NC; e += blockDim.x) s_c[e] = 0;
-  if (a.groups > 1 && blockIdx.x == 0 && tid == 0) *a.ws.arrived = 0;
-  __syncthreads();
+  s.clear(a);
   float psum[NC], zsum = 0.0f;
   int n = 0;
 #pragma unroll
@@ -193,7 +419,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
     float ex[NC], total = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      ex[c] = expf(l[c] - top);
+      ex[c] = exp_neg(l[c] - top);
       total += ex[c];
     }
     total = wave_sum(total);
@@ -201,7 +427,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
     float my_v;
     bool chosen;
     S::select(key, live ? a.k : 0, lane, my_i, my_v, chosen);
-    const float mine = chosen ? expf(my_v - top) : 0.0f;
+    const float mine = chosen ? exp_neg(my_v - top) : 0.0f;
     float over = total;
     if (a.renorm) {
       // a NaN or +inf among the logits makes the weights NaN, also where it is not chosen
@@ -212,7 +438,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
       a.ids[t * a.k + lane] = chosen ? my_i : -1;
       a.weights[t * a.k + lane] = chosen ? mine / over : 0.0f;
     }
-    if (chosen) atomicAdd(&s_c[my_i], 1);
+    if (chosen) atomicAdd(&s.c[my_i], 1);
     const float lse = live ? top + logf(total) : 0.0f;
     if (a.lse && lane == 0) a.lse[t] = live ? lse : __builtin_inff();
     if (live) {
@@ -224,48 +450,8 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
     }
   }
 #pragma unroll
-  for (int c = 0; c < NC; ++c) s_p[wave][lane + 64 * c] = psum[c];
-  if (lane == 0) {
-    s_z[wave] = zsum;
-    s_n[wave] = n;
-  }
-  __syncthreads();
-  float z = 0.0f;
-  int live = 0;
-  for (int w = 0; w < waves; ++w) {
-    z += s_z[w];
-    live += s_n[w];
-  }
-  if (a.groups > 1) {
-    for (int e = tid; e < a.E; e += blockDim.x) {
-      float p = 0.0f;
-      for (int w = 0; w < waves; ++w) p += s_p[w][e];
-      a.ws.p[(int64_t)blockIdx.x * a.E + e] = p;
-      a.ws.c[(int64_t)blockIdx.x * a.E + e] = s_c[e];
-    }
-    if (tid == 0) {
-      a.ws.z[blockIdx.x] = z;
-      a.ws.n[blockIdx.x] = live;
-    }
-    return;
-  }
-  // one workgroup: the sums are all here
-  double dot = 0.0;
-  for (int e = tid; e < a.E; e += blockDim.x) {
-    float p = 0.0f;
-    for (int w = 0; w < waves; ++w) p += s_p[w][e];
-    a.counts[e] = s_c[e];
-    dot += (double)s_c[e] * (double)p;
-  }
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) dot += __shfl_xor(dot, m);
-  if (lane == 0) s_dot[wave] = dot;
-  __syncthreads();
-  if (tid == 0) {
-    dot = 0.0;
-    for (int w = 0; w < waves; ++w) dot += s_dot[w];
-    finish(a, dot, (double)z, live);
-  }
+  for (int c = 0; c < NC; ++c) s.p[wave][lane + 64 * c] = psum[c];
+  block_sums(a, s, zsum, n);
 }
 
 // The workgroups' sums: kCols experts a workgroup, 64 threads an expert. The last workgroup to arrive adds
@@ -287,15 +473,13 @@ __global__ __launch_bounds__(1024) void route_sum_kernel(RouteArgs a) {
   }
   double z = tid < a.groups ? (double)a.ws.z[tid] : 0.0;  // at most 512 workgroups
   int n = tid < a.groups ? a.ws.n[tid] : 0;
-  // a wave's slots of an expert: lanes col, col + 16, ...
-  for (int m = 32; m >= kCols; m >>= 1) {
-    p += __shfl_xor(p, m);
-    c += __shfl_xor(c, m);
-  }
-  for (int m = 32; m >= 1; m >>= 1) {
-    z += __shfl_xor(z, m);
-    n += __shfl_xor(n, m);
-  }
+  // a wave's four slots of an expert: lanes col, col + 16, ...
+  p += partner<32>(p);
+  p += partner<16>(p);
+  c += (int)row_partner<32>((uint32_t)c);
+  c += (int)row_partner<16>((uint32_t)c);
+  z = wave_sum(z);
+  n = (int)wave_sum((double)n);
   if (lane < kCols) {
     s_p[wave][lane] = p;
     s_c[wave][lane] = c;
@@ -320,11 +504,9 @@ __global__ __launch_bounds__(1024) void route_sum_kernel(RouteArgs a) {
   }
   z = lane < 16 ? s_z[lane] : 0.0;
   n = lane < 16 ? s_n[lane] : 0;
-  for (int m = 8; m >= 1; m >>= 1) {  // lanes 0 to 15 hold all of the three
-    dot += __shfl_xor(dot, m);
-    z += __shfl_xor(z, m);
-    n += __shfl_xor(n, m);
-  }
+  dot = wave_sum(dot);
+  z = wave_sum(z);
+  n = (int)wave_sum((double)n);
   uint32_t before = 0;
   if (lane == 0) {
     __hip_atomic_store(a.ws.parts + blockIdx.x, dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -334,7 +516,7 @@ __global__ __launch_bounds__(1024) void route_sum_kernel(RouteArgs a) {
   dot = lane < (int)gridDim.x ? __hip_atomic_load(a.ws.parts + lane, __ATOMIC_RELAXED,
                                                   __HIP_MEMORY_SCOPE_AGENT)
                               : 0.0;
-  for (int m = 32; m >= 1; m >>= 1) dot += __shfl_xor(dot, m);
+  dot = wave_sum(dot);
   if (lane == 0) finish(a, dot, z, n);
 }
 
@@ -411,11 +593,12 @@ __global__ __launch_bounds__(64 * kGradWaves) void route_backward_kernel(RouteGr
 
 int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
 
-int route_groups(int T) { return std::max(1, std::min((T - 1) / kWaves + 1, kMaxGroups)); }
+// Workgroups; the workspace is sized for a wave a token, which has the more of them.
+int route_groups(int T, int tokens) { return std::max(1, std::min((T - 1) / tokens + 1, kMaxGroups)); }
 
 // The workspace's parts from `base`; its size in *bytes.
 RouteWs route_ws(void* base, int T, int E, int64_t* bytes) {
-  const int64_t g = route_groups(T);
+  const int64_t g = route_groups(T, kWaves);
   int64_t o = 0;
   auto take = [&o](int64_t n) {
     const int64_t at = o;
@@ -433,8 +616,14 @@ RouteWs route_ws(void* base, int T, int E, int64_t* bytes) {
 
 template <int DT, int NC>
 hipError_t launch_route(const RouteArgs& a, hipStream_t s) {
-  const int waves = std::max(1, std::min(a.T, kWaves));
-  hipLaunchKernelGGL((route_kernel<DT, NC>), dim3(a.groups), dim3(64 * waves), 0, s, a);
+  if constexpr (DT != kFp32) {
+    if (route_grouped(a.T, a.k, DT))
+      hipLaunchKernelGGL((route_group_kernel<DT, 4 * NC>), dim3(a.groups), dim3(64 * kGroupWaves), 0, s, a);
+  }
+  if (!route_grouped(a.T, a.k, DT)) {
+    const int waves = std::max(1, std::min(a.T, kWaves));
+    hipLaunchKernelGGL((route_kernel<DT, NC>), dim3(a.groups), dim3(64 * waves), 0, s, a);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.groups == 1) return e;
   hipLaunchKernelGGL(route_sum_kernel, dim3((a.E + kCols - 1) / kCols), dim3(1024), 0, s, a);
@@ -527,7 +716,8 @@ int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dty
   if (any_overlap(outs, ins))
     return op_fail(MOE_ERR_SHAPE,
                    "route: outputs and workspace must not overlap the inputs or each other");
-  const RouteArgs a{logits, mask, T, num_experts, top_k, renormalize != 0, route_groups(T), topk_ids,
+  const RouteArgs a{logits, mask, T, num_experts, top_k, renormalize != 0, 
+                    route_groups(T, route_grouped(T, top_k, dtype) ? kGroupTokens : kWaves), topk_ids,
                     topk_weights, counts, balance, z, lse, ws};
   const auto s = (hipStream_t)stream;
   MOE_OP_HIP(dtype == kBf16   ? launch_route_any<kBf16>(a, s)

@@ -1,10 +1,11 @@
 """Routing with its losses (route_tokens) and the logits' gradient against the formulas in 64 bits.
 
-u = 2^-24 is fp32's half step. exp(l - top) is off by 2 u of itself for the function and |l - top| u for
-the difference it is taken of; a token's sum of them adds at most 14 roundings (8 registers, 6 butterfly
-steps). With logits within 32 of each other a weight is off by at most 100 u of itself, and lse by 50 u
-absolutely plus u |lse|. Sums over tokens: a rounding for each of a wave's tokens and of the workgroup's
-16 waves, the rest in 64 bits. Ids and counts are exact.
+u = 2^-24 is fp32's half step. exp(l - top) is off by 3 u of itself for the function and |l - top| u for
+the difference it is taken of, at most 16 u for logits within 16 of the largest; a token's sum of them adds
+at most 36 roundings (32 registers, 4 exchanges). A weight is the quotient of such a term and such a sum: at
+most 19 + 19 + 36 + 1 u of itself, 100 u taken; lse is off by 55 u absolutely plus u |lse|. Sums over
+tokens: a rounding for each of a wave's tokens and of the workgroup's 16 waves, the rest in 64 bits. Ids and
+counts are exact.
 """
 
 from __future__ import annotations
@@ -101,7 +102,12 @@ CASES = [  # T, E, k, dtype, masked, blocked, renormalised
     (33, 512, 10, torch.bfloat16, False, 0.0, True), (70, 65, 3, torch.float32, True, 0.9, True),
     (300, 128, 8, torch.float32, True, 0.2, False), (65, 511, 64, torch.float32, False, 0.0, True),
     (900, 16, 2, torch.bfloat16, True, 0.97, True), (5000, 8, 2, torch.float32, True, 0.1, True),
-    (129, 129, 1, torch.float16, False, 0.0, True)]
+    (129, 129, 1, torch.float16, False, 0.0, True),
+    (40, 300, 17, torch.bfloat16, True, 0.3, False), (40, 300, 16, torch.bfloat16, True, 0.3, False),
+    (2100, 64, 8, torch.float16, False, 0.0, True), (31, 512, 16, torch.float32, True, 0.95, True),
+    (1100, 300, 16, torch.bfloat16, True, 0.3, False), (1030, 512, 10, torch.float16, True, 0.97, True),
+    (1027, 7, 7, torch.bfloat16, False, 0.5, True), (1501, 60, 5, torch.float16, True, 0.25, False),
+    (1024, 130, 1, torch.bfloat16, True, 0.0, True)]
 
 
 @pytest.mark.parametrize("T,E,k,dtype,masked,blocked,renorm", CASES)
@@ -171,15 +177,30 @@ def test_ties_take_the_lower_id():
     assert int(r.counts.sum()) == 100
 
 
+@pytest.mark.parametrize("E,k", [(12, 3), (60, 8), (256, 16), (500, 10), (500, 20)])
+def test_logits_closer_than_the_keys(E, k):
+    """fp32 logits that agree in their upper bits, equal ones among them, next to ordinary tokens: the
+    order is that of the values."""
+    g = torch.Generator().manual_seed(E)
+    l = torch.randn(64, E, generator=g)
+    l[::2] = 3.0 + torch.randint(0, 40, (32, E), generator=g) * 2.0 ** -20
+    l[1::8] = (2.0 * torch.randn(8, E, generator=g)).bfloat16().float()  # many equal values
+    l[4::16, ::3] = -INF
+    l[6::16] = -1e-30 * torch.randint(0, 9, (4, E), generator=g)
+    l[8::16, E // 2:] = -INF
+    check(ops.route_tokens(l.cuda(), k), formulas(l, k), 64)
+
+
 def test_tokens_without_an_expert():
     """Rows of -inf, of the type's lowest value, and padding that holds NaN and infinities."""
-    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+    for dtype, more in ((torch.float32, 0), (torch.bfloat16, 0), (torch.float16, 0), (torch.bfloat16, 1100),
+                        (torch.float16, 2048)):
         low = torch.finfo(dtype).min
-        l = make(6, 32, dtype)
+        l = make(6 + more, 32, dtype)
         l[0], l[1] = -INF, low
         l[2, :30] = -INF
         l[3], l[4, 5], l[4, 6] = float("nan"), INF, -INF
-        mask = torch.tensor([True, True, True, False, False, True])
+        mask = torch.tensor([True, True, True, False, False, True] + [False] * more)
         x = l.cuda().requires_grad_()
         r = ops.route_tokens(x, 4, mask=mask.cuda())
         ids, w = r.topk_ids.cpu(), r.topk_weights.detach().cpu()
@@ -187,16 +208,17 @@ def test_tokens_without_an_expert():
         assert ids[1].tolist() == [0, 1, 2, 3] and w[1].tolist() == [0.25] * 4  # all equal: even
         assert ids[2].tolist()[2:] == [-1, -1] and sorted(ids[2].tolist()[:2]) == [30, 31]
         assert abs(float(w[2].sum()) - 1) < 8 * U and int(r.counts.sum()) == 4 + 2 + 4
-        dw = torch.full((6, 4), float("nan"))
+        dw = torch.full((6 + more, 4), float("nan"))
         dw[[1, 5]], dw[2, :2] = 1.0, 1.0  # what stands at places without an expert is not looked at
         d, = torch.autograd.grad((r.topk_weights, r.balance_loss), x,
                                  (dw.cuda(), torch.tensor(1.0, device="cuda")))
         assert bool(d.isfinite().all()) and not d[[0, 3, 4]].any()
 
 
-def test_a_counted_nan_shows():
+@pytest.mark.parametrize("T,dtype", [(40, torch.float32), (40, torch.bfloat16), (1040, torch.float16)])
+def test_a_counted_nan_shows(T, dtype):
     for bad in (float("nan"), INF):
-        l = make(40, 24, torch.float32)
+        l = make(T, 24, dtype)
         l[7, 3] = bad
         x = l.cuda().requires_grad_()
         r = ops.route_tokens(x, 2)
@@ -205,7 +227,7 @@ def test_a_counted_nan_shows():
         assert bool(r.balance_loss.isnan()) and bool(r.z_loss.isnan())
         d, = torch.autograd.grad(r.topk_weights, x, torch.ones_like(w))
         assert bool(d[7].isnan().all()) and bool(d[[6, 8]].isfinite().all())
-    l = torch.full((3, 24), float("nan"))
+    l = torch.full((T, 24), float("nan"), dtype=dtype)
     r = ops.route_tokens(l.cuda(), 2)
     assert bool((r.topk_ids == -1).all()) and math.isnan(float(r.z_loss))
 
