@@ -4,7 +4,15 @@
 //   y[t, n] = round(sum_g s[g, n] * (sum_{k in g} x[t, k] (q[k, n] - z[g, n])) (+ bias[n]))
 //
 // The weights are not rounded: a group's products are summed in fp32 on the integers q - z and scaled
-// after that.
+// after that. Three forms:
+//   few rows   operands from memory to registers, the words made into MFMA operands there. Reading the
+//              weights bounds it, and the launch where they are few: 1 row of 2048 x 4096 4.7 us on the
+//              GPU, of 8192 x 16384 16 us (4.4 TB/s), 16 rows of 4096 x 8192 7.2 us (3.6 TB/s).
+//   many rows  integers unpacked once, then a tiled product from LDS: 4096 rows of 4096 x 8192 214 us, 12
+//              of them the unpacking (1360 TFLOP/s in the product). Loads into LDS bound it up to about
+//              1000 rows (of the 51 us of 512 rows 46 are left without a product or a read of LDS, 41
+//              without the loads), the matrix and vector pipes beyond.
+//   unaligned  value by value, for tensors that start between two 16-byte boundaries.
 #include <algorithm>
 #include <type_traits>
 
@@ -107,7 +115,9 @@ struct Chunk {
 };
 
 template <int DT, int MT, int CT, int SPG, int KS>
-__global__ __launch_bounds__(64 * KS) void int4_stream_kernel(Int4Args a, uint32_t row_tiles, uint32_t row_magic, uint32_t group_magic) {
+__global__ __launch_bounds__(64 * KS) void int4_stream_kernel(Int4Args a, uint32_t row_tiles,
+                                                             uint32_t row_magic,
+                                                             uint32_t group_magic) {
   using T = typename Elem<DT>::T;
   using O = Op<DT>;
   __shared__ f32x4 red[KS][MT * CT][64];
@@ -138,7 +148,9 @@ __global__ __launch_bounds__(64 * KS) void int4_stream_kernel(Int4Args a, uint32
   auto load = [&](Chunk<MT, CT, SPG>& c, int at) {
     const bool in = at < chunks;
     const uint32_t out = in ? 0u : kOutOfRange;
-    const uint32_t k = in ? (uint32_t)at * 32u * SPG : 0u, g = in ? (group_magic ? __umulhi((uint32_t)at, group_magic) : (uint32_t)at) : 0u;
+    const uint32_t k = in ? (uint32_t)at * 32u * SPG : 0u;
+    const uint32_t g =
+        !in ? 0u : group_magic ? __umulhi((uint32_t)at, group_magic) : (uint32_t)at;
 #pragma unroll
     for (int s = 0; s < SPG; ++s) {
       const uint32_t row = (k / 8 + 4 * s) * (uint32_t)a.N * 4u;
@@ -269,7 +281,8 @@ hipError_t launch_stream(const Int4Args& a, hipStream_t s) {
 // Two launches. The first turns the words into the integers q - z as fp8 (e4m3 holds 4 significant bits:
 // exact), a wave 64 channels x 64 k, stored as the tiles below take them: [K / 64][N][64], a row's 16-byte
 // chunk c holding k 8 c .. + 7 and 32 + 8 c .. + 7, zeros past K; and for each 64 k (32 where groups may end
-// there) the ratio of the scale before to the one from there on. The second is a product of x with them, turned into x's type (exact) on the way from LDS.
+// there) the ratio of the scale before to the one from there on. The second is a product of x with them,
+// turned into x's type (exact) on the way from LDS.
 //
 // The product keeps its sums in units of the present group's scale: where a group ends they are multiplied
 // by s[g - 1] / s[g], which takes an operation a sum and no second set of sums. A scale of zero counts as
@@ -332,9 +345,10 @@ __global__ __launch_bounds__(256) void int4_unpack_kernel(Int4Args a, uint8_t* _
 // Workgroup: BM tokens x BN channels on WM x WN waves, K steps of 64 in a ring of RING stages in LDS, filled
 // by loads that bypass the registers. One wait and barrier in the middle of a step orders the arrival of the
 // next stage and the reuse of this one, whose second half is in registers by then: loads have RING - 1 steps
-// to arrive. LDS rows of x are 128 bytes, the 16-byte chunk c of row r at position c ^ (r & 7); rows of
-// integers 64 bytes, chunk c at c ^ (r / 2 & 3): the 8 rows that a phase of a 16-byte read spans lie in
-// different banks. EVERY: groups end at multiples of so many half steps (1, 2 or 4).
+// to arrive (whole steps held in registers, or rings of 5 to 8 stages, gained nothing). LDS rows of x are 128
+// bytes, the 16-byte chunk c of row r at position c ^ (r & 7); rows of integers 64 bytes, chunk c at
+// c ^ (r / 2 & 3): the 8 rows that a phase of a 16-byte read spans lie in different banks. EVERY: groups end
+// at multiples of so many half steps (1, 2 or 4).
 constexpr int kGroupM = 4;
 // The kernel's body in pieces: called many times over, they would become functions.
 #define MOE_INLINE __attribute__((always_inline))
@@ -680,14 +694,16 @@ bool many_rows(int T, int K, int N) {
 }
 
 // By the number of 128 x 128 tiles, us with 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256: 128 tiles (256 rows
-// of 4096 x 8192) 39 / 51 / 66 / 104, 256 (512 rows) 55 / 52 / 67 / 104, 512 (1024 rows) 89 / 85 / 73 / 105,
-// 2048 (4096 rows) 305 / 291 / 242 / 214.
+// of 4096 x 8192) 40 / 48 / 66 / 107, 192 (384 rows) 51 / 49 / 67 / 105, 256 (512 rows) 56 / 51 / 67 / 107, 384
+// (768 rows) 76 / 79 / 69 / 108, 512 (1024 rows) 91 / 84 / 76 / 108, 768 (3000 of 2048 x 4096) 71 / 67 / 69 /
+// 61, 2048 (4096 of 4096 x 8192) 302 / 290 / 250 / 217. Between 64 x 128 tiles of 4 waves and of 8 there is
+// nothing to choose; 128 x 128 on 4 waves takes 55 us for the 512 rows.
 template <int DT>
 hipError_t launch_many_rows(const Int4Args& a, hipStream_t s) {
   const int64_t tiles = (int64_t)((a.T + 127) / 128) * ((a.N + 127) / 128);
   if (tiles <= 160) return launch_tile<64, 128, 2, 2, 4, DT>(a, s);
-  if (tiles <= 320) return launch_tile<128, 128, 2, 2, 4, DT>(a, s);
-  if (tiles <= 1024) return launch_tile<128, 256, 2, 4, 3, DT>(a, s);
+  if (tiles <= 320) return launch_tile<128, 128, 2, 4, 4, DT>(a, s);
+  if (tiles <= 640) return launch_tile<128, 256, 2, 4, 3, DT>(a, s);
   return launch_tile<256, 256, 2, 4, 2, DT>(a, s);
 }
 
