@@ -103,6 +103,11 @@ MOE_DEV void buf_ld128_lds(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off, ui
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 16, off, soff, 0, 0);
 }
 
+// The same with 4 bytes per lane: lane i writes lds[4 i, 4 i + 4).
+MOE_DEV void buf_ld32_lds(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off, uint32_t soff = 0) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)lds, 4, off, soff, 0, 0);
+}
+
 MOE_DEV u32x4 ld128(const void* p) { return *reinterpret_cast<const u32x4*>(p); }
 MOE_DEV u32x4 ld128_nt(const void* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));

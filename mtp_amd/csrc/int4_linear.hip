@@ -4,10 +4,12 @@
 //   y[t, n] = round(sum_g s[g, n] * (sum_{k in g} x[t, k] (q[k, n] - z[g, n])) (+ bias[n]))
 //
 // The weights are not rounded: a group's products are summed in fp32 on the integers q - z and scaled
-// after that. Three forms:
+// after that. Four forms:
 //   few rows   operands from memory to registers, the words made into MFMA operands there. Reading the
 //              weights bounds it, and the launch where they are few: 1 row of 2048 x 4096 4.7 us on the
 //              GPU, of 8192 x 16384 16 us (4.4 TB/s), 16 rows of 4096 x 8192 7.2 us (3.6 TB/s).
+//   more rows  the same words, x shared through LDS: 128 rows of 4096 x 8192 18 us, 256 27 us (640 TFLOP/s).
+//              Vector operations and multiplications bound it.
 //   many rows  integers unpacked once, then a tiled product from LDS: 4096 rows of 4096 x 8192 214 us, 12
 //              of them the unpacking (1360 TFLOP/s in the product). Loads into LDS bound it up to about
 //              1000 rows (of the 51 us of 512 rows 46 are left without a product or a read of LDS, 41
@@ -277,6 +279,260 @@ hipError_t launch_stream(const Int4Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// ---------------------------------------------------------------- more rows
+// Workgroup: 64 tokens x 32 WN channels on WN x KS waves: K in KS shares, a share on WN waves in steps
+// of 64, and the shares' sums added at the end. x reaches a share's waves through LDS, the words stay packed:
+// every wave loads those of its own 32 channels, their scales and zero points. All of it goes through a ring
+// of RING stages filled by loads that bypass the registers. The rest is as with few rows. EVERY: groups end at
+// multiples of so many steps (1 or 2), where the sums of the group are scaled and added up.
+//
+// The vector operations (40 to make operands of a step's words, 80 to scale a group's sums) and the
+// multiplications (24 of 16 cycles, 8 of them for the sums of x) bound it: with two waves a SIMD a step takes
+// about the sum of both, with the operations in the multiplications' shadow as well as with the compiler's
+// order. What is shared is x (few rows: 256 rows of 4096 x 8192 44 us, here 27), what is saved the
+// unpacking and its launch (many rows: 39).
+//
+// LDS rows of x are 128 bytes, the 16-byte chunk c of row r at position c ^ (r & 7): the 8 rows that a phase
+// of a 16-byte read spans lie in different banks.
+constexpr int kGroupM = 4;
+constexpr int kBK = 64;
+// The kernels' bodies in pieces: called many times over, they would become functions.
+#define MOE_INLINE __attribute__((always_inline))
+// s_waitcnt immediate waiting for lgkmcnt <= 0 only.
+constexpr int kWaitLgkm0 = 15 | (3 << 14) | (0x7 << 4);
+
+template <int DT, int WN, int KS, int RING, int EVERY>
+__global__ __launch_bounds__(64 * WN * KS) void int4_words_kernel(Int4Args a, uint32_t group_magic) {
+  using T = typename Elem<DT>::T;
+  using O = Op<DT>;
+  constexpr int MT = 4, CT = 2, NT = 64 * WN, BK = kBK, BM = 16 * MT, CH = 16 * CT, BN = CH * WN;
+  constexpr int LA = BM * 8 / NT, kLoads = LA + 3;
+  // bytes: a wave's words, scales and zero points, a share's and all of a stage
+  constexpr int kMine = 1024 + 256 + 256, kPart = BM * 128 + WN * kMine;
+  constexpr int kSums = KS > 1 ? WN * MT * CT * 1024 : 0;
+  constexpr int kStage = KS * kPart > kSums ? KS * kPart : kSums;
+  static_assert(LA * NT == BM * 8, "whole loads");
+  static_assert(RING >= 2 && RING <= 4 && KS <= RING + 1, "a stage an array, a share's sums a stage");
+  // separate arrays: the compiler then knows which stage a load to LDS writes
+  __shared__ __attribute__((aligned(16))) uint8_t lds0[kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t lds1[kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t lds2[RING > 2 ? kStage : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t lds3[RING > 3 ? kStage : 16];
+  const int m_tiles = (a.T + BM - 1) / BM, blocks_n = (a.N + BN - 1) / BN;
+  // each XCD takes a run of tiles, down kGroupM row blocks before the next channels
+  const int idx = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+  const int total = m_tiles * blocks_n, per = (total + 7) / 8, id = xcd * per + idx;
+  if (idx >= per || id >= total) return;
+  const int group = id / (kGroupM * blocks_n), in = id - group * kGroupM * blocks_n;
+  const int grows = min(kGroupM, m_tiles - group * kGroupM);
+  const int t0 = (group * kGroupM + in % grows) * BM, n0 = in / grows * BN;
+  const int ks = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);  // the share of K
+  const int tid = threadIdx.x % NT, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int steps = ((a.K + BK - 1) / BK + 2 * KS - 1) / (2 * KS) * 2;  // of a share
+  const int k_first = ks * steps * BK, k_end = min(a.K, k_first + steps * BK);
+  const int lr = lane & 15, lq = lane >> 4;
+  const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.K * 2u);
+  const __amdgpu_buffer_rsrc_t rw = buf_rsrc(a.qweight, (uint32_t)(a.K / 8) * (uint32_t)a.N * 4u);
+  const __amdgpu_buffer_rsrc_t rs = buf_rsrc(a.scales, (uint32_t)a.groups * (uint32_t)a.N * 2u);
+  const __amdgpu_buffer_rsrc_t rz = buf_rsrc(a.qzeros, (uint32_t)a.groups * (uint32_t)(a.N / 8) * 4u);
+  // One offset a lane and a scalar one for each load. Rows behind the last token may hold anything (a
+  // lane's results are of its own token), but are read inside the buffer: a load whose first row lies
+  // behind reads another one's rows.
+  const uint32_t xoff =
+      (uint32_t)(tid / 8) * (uint32_t)a.K * 2u + (uint32_t)((tid & 7) ^ ((tid >> 3) & 7)) * 16u;
+  uint32_t xrow[LA];
+#pragma unroll
+  for (int j = 0; j < LA; ++j) {
+    const int t = t0 + j * (NT / 8);
+    xrow[j] = t < a.T ? (uint32_t)t * (uint32_t)a.K * 2u : 0u;
+  }
+  const int nw = n0 + wave * CH;  // the wave's first channel
+  const int nl = nw + lane % 8 * 4;  // of the words: 8 lanes a row of 32
+  const uint32_t woff =
+      nl < a.N ? ((uint32_t)(lane / 8) * (uint32_t)a.N + (uint32_t)nl) * 4u : kOutOfRange;
+  const uint32_t soff = lane < CH / 2 && nw + 2 * lane < a.N ? (uint32_t)(nw + 2 * lane) * 2u : kOutOfRange;
+  const uint32_t zoff = lane < CH / 8 && nw + 8 * lane < a.N ? (uint32_t)(nw / 8 + lane) * 4u : kOutOfRange;
+  // A stage past the share reads zeros without a memory access, so that as many loads are in flight in
+  // every step.
+  // The scalar offsets stay inside the buffers: the bounds check takes them off the buffers' sizes.
+  auto stage = [&](uint8_t* lds, int k0) MOE_INLINE {
+    lds += ks * kPart;
+    k0 += k_first;
+    const uint32_t at = k0 < k_end ? (uint32_t)k0 : 0u, out = k0 < k_end ? 0u : kOutOfRange;
+#pragma unroll
+    for (int j = 0; j < LA; ++j)
+      buf_ld128_lds(rx, lds + (j * NT + wave * 64) * 16, xoff | out, xrow[j] + at * 2u);
+    uint8_t* const mine = lds + BM * 128 + wave * kMine;
+    buf_ld128_lds(rw, mine, woff | out, at / 8 * (uint32_t)a.N * 4u);
+    const uint32_t g = at / kBK * group_magic >> 21;
+    buf_ld32_lds(rs, mine + 1024, soff | out, g * (uint32_t)a.N * 2u);
+    buf_ld32_lds(rz, mine + 1024 + 256, zoff | out, g * (uint32_t)(a.N / 8) * 4u);
+  };
+  // The barrier without __syncthreads' release fence, which would wait for every load to LDS: this wave's
+  // LDS accesses ahead of it are waited for, and the compiler keeps accesses on their sides.
+  auto barrier = []() MOE_INLINE {
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  f32x4 acc[MT][CT], part[MT][CT], sum[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < CT; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
+  const u32x4 ones{O::kOnes, O::kOnes, O::kOnes, O::kOnes};
+  const int sw0 = (lq ^ (lr & 7)) * 16, sw1 = ((4 + lq) ^ (lr & 7)) * 16;
+  const int fa_at = ks * kPart + lr * 128;
+  const int mine_at = ks * kPart + BM * 128 + wave * kMine;
+  u32x4 fa[2][MT];
+  uint32_t raw[2][CT];
+  auto fetch = [&](const uint8_t* lds, int half) MOE_INLINE {
+    const int sw = half ? sw1 : sw0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) fa[half][m] = ld128(lds + fa_at + m * 16 * 128 + sw);
+    const uint8_t* p = lds + mine_at + ((4 * half + lq) * CH + CT * lr) * 4;
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    raw[half][0] = v[0];
+    raw[half][1] = v[1];
+  };
+  // fresh: a group starts (or a part of one)
+  auto multiply = [&](int half, bool fresh) MOE_INLINE {
+    const f32x4 zero{0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sum[m] = O::mfma(ones, fa[half][m], fresh ? zero : sum[m]);
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const u32x4 w = O::weights(raw[half][j]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) part[m][j] = O::mfma(w, fa[half][m], fresh ? zero : part[m][j]);
+    }
+  };
+  u32x4 sc;
+  uint32_t zp;
+  auto fetch_unit = [&](const uint8_t* lds) MOE_INLINE {
+    const uint8_t* p = lds + mine_at + 1024;
+    sc = ld128(p + 8 * CT * lq);
+    zp = *reinterpret_cast<const uint32_t*>(p + 256 + 2 * CT * lq);
+  };
+  auto finish = [&]() MOE_INLINE {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const int v = CT * i + j;  // the lane's channel
+        const float s = f16_to_f32(v & 1 ? sc[v / 2] >> 16 : sc[v / 2] & 0xFFFFu);
+        const float zb = O::zero_point(zp, 4 * v);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          acc[m][j][i] = __builtin_fmaf(s, __builtin_fmaf(-zb, sum[m][0], part[m][j][i]), acc[m][j][i]);
+      }
+  };
+  auto step = [&](uint8_t* here, uint8_t* next, int k0, bool starts, bool ends) MOE_INLINE {
+    fetch(here, 1);
+    if (ends) fetch_unit(here);
+    multiply(0, starts);
+    // This wave's loads of the next stage have landed (those of the stages after it stay in flight); behind
+    // the barrier everybody's have, and this stage, all of it in registers, is free.
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm((RING - 2) * kLoads));
+    barrier();
+    stage(here, k0 + RING * BK);
+    fetch(next, 0);  // behind the last step: zeros that nothing multiplies
+    multiply(1, false);
+    if (ends) finish();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  stage(lds0, 0);
+  stage(lds1, BK);
+  if constexpr (RING > 2) stage(lds2, 2 * BK);
+  if constexpr (RING > 3) stage(lds3, 3 * BK);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm((RING - 1) * kLoads));
+  barrier();
+  fetch(lds0, 0);
+  using std::integral_constant;
+  // Which stage a step works on and whether a group may start or end there is known in a run of kSteps. Whole
+  // runs first, without branches between their steps: at a join the compiler would wait for all loads to LDS.
+  constexpr int kSteps = EVERY == 2 && RING % 2 ? 2 * RING : RING;
+  auto nth = [&](auto i_c, int k0) MOE_INLINE {
+    constexpr int i = decltype(i_c)::value, at = i % RING, to = (i + 1) % RING;
+    uint8_t* const here = at == 0 ? lds0 : at == 1 ? lds1 : at == 2 ? lds2 : lds3;
+    uint8_t* const next = to == 0 ? lds0 : to == 1 ? lds1 : to == 2 ? lds2 : lds3;
+    step(here, next, k0 + i * BK, i % EVERY == 0, i % EVERY == EVERY - 1);
+  };
+  int k0 = 0;
+#pragma unroll 1
+  for (; k0 + (kSteps - 1) * BK < steps * BK; k0 += kSteps * BK) {
+    nth(integral_constant<int, 0>{}, k0);
+    nth(integral_constant<int, 1>{}, k0);
+    if constexpr (kSteps > 2) nth(integral_constant<int, 2>{}, k0);
+    if constexpr (kSteps > 3) nth(integral_constant<int, 3>{}, k0);
+    if constexpr (kSteps > 4) nth(integral_constant<int, 4>{}, k0);
+    if constexpr (kSteps > 5) nth(integral_constant<int, 5>{}, k0);
+  }
+  if (k0 < steps * BK) nth(integral_constant<int, 0>{}, k0);
+  if constexpr (kSteps > 2)
+    if (k0 + BK < steps * BK) nth(integral_constant<int, 1>{}, k0);
+  if constexpr (kSteps > 3)
+    if (k0 + 2 * BK < steps * BK) nth(integral_constant<int, 2>{}, k0);
+  if constexpr (kSteps > 4)
+    if (k0 + 3 * BK < steps * BK) nth(integral_constant<int, 3>{}, k0);
+  if constexpr (kSteps > 5)
+    if (k0 + 4 * BK < steps * BK) nth(integral_constant<int, 4>{}, k0);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no load to LDS may meet the sums below
+  if constexpr (KS > 1) {  // the shares' sums, in their order
+    __syncthreads();  // the stages have been read
+    if (ks > 0) {
+      f32x4* const p = reinterpret_cast<f32x4*>(ks == 1 ? lds0 : ks == 2 ? lds1 : lds2);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) p[((wave * MT + m) * CT + j) * 64 + lane] = acc[m][j];
+    }
+    __syncthreads();
+    if (ks > 0) return;
+#pragma unroll
+    for (int q = 1; q < KS; ++q) {
+      const f32x4* const p = reinterpret_cast<const f32x4*>(q == 1 ? lds0 : q == 2 ? lds1 : lds2);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) acc[m][j] += p[((wave * MT + m) * CT + j) * 64 + lane];
+    }
+  }
+  // A lane holds 4 CT neighbouring channels of a token for each m.
+  const int n = nw + 4 * CT * lq;
+  if (n >= a.N) return;
+  u32x4 bits{0, 0, 0, 0};
+  if (a.bias) __builtin_memcpy(&bits, static_cast<const T*>(a.bias) + n, 16);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int t = t0 + m * 16 + lr;
+    if (t >= a.T) continue;
+    T v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = Elem<DT>::put(acc[m][e % CT][e / CT] + Elem<DT>::get((T)(bits[e >> 1] >> (16 * (e & 1)))));
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<T*>(a.out) + (int64_t)t * a.N + n, 16), v, 16);
+  }
+}
+
+template <int DT, int WN, int KS, int RING>
+hipError_t launch_words(const Int4Args& a, hipStream_t s) {
+  constexpr int BM = 64, BN = 32 * WN;
+  const int64_t tiles = (int64_t)((a.T + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(64 * WN * KS);
+  // x / d is x * g >> 21 for x and d up to 1024
+  const uint32_t d = (uint32_t)a.G / kBK, g = ((1u << 21) + d - 1) / d;
+  if (a.G % (2 * kBK))
+    hipLaunchKernelGGL((int4_words_kernel<DT, WN, KS, RING, 1>), grid, block, 0, s, a, g);
+  else
+    hipLaunchKernelGGL((int4_words_kernel<DT, WN, KS, RING, 2>), grid, block, 0, s, a, g);
+  return hipGetLastError();
+}
+
 // ---------------------------------------------------------------- many rows
 // Two launches. The first turns the words into the integers q - z as fp8 (e4m3 holds 4 significant bits:
 // exact), a wave 64 channels x 64 k, stored as the tiles below take them: [K / 64][N][64], a row's 16-byte
@@ -287,7 +543,6 @@ hipError_t launch_stream(const Int4Args& a, hipStream_t s) {
 // The product keeps its sums in units of the present group's scale: where a group ends they are multiplied
 // by s[g - 1] / s[g], which takes an operation a sum and no second set of sums. A scale of zero counts as
 // one, with integers of zero.
-constexpr int kBK = 64;
 
 MOE_DEV float scale_unit(uint32_t s) {
   const float f = f16_to_f32(s & 0xFFFFu);
@@ -349,11 +604,6 @@ __global__ __launch_bounds__(256) void int4_unpack_kernel(Int4Args a, uint8_t* _
 // bytes, the 16-byte chunk c of row r at position c ^ (r & 7); rows of integers 64 bytes, chunk c at
 // c ^ (r / 2 & 3): the 8 rows that a phase of a 16-byte read spans lie in different banks. EVERY: groups end
 // at multiples of so many half steps (1, 2 or 4).
-constexpr int kGroupM = 4;
-// The kernel's body in pieces: called many times over, they would become functions.
-#define MOE_INLINE __attribute__((always_inline))
-// s_waitcnt immediate waiting for lgkmcnt <= 0 only.
-constexpr int kWaitLgkm0 = 15 | (3 << 14) | (0x7 << 4);
 
 // 8 integers in fp8 as an MFMA operand.
 template <int DT>
@@ -376,7 +626,8 @@ __global__ __launch_bounds__(64 * WM * WN) void int4_tile_kernel(Int4Args a,
   using T = typename Elem<DT>::T;
   using O = Op<DT>;
   constexpr int NT = 64 * WM * WN, BK = kBK;
-  constexpr int MT = BM / WM / 16, NG = BN / WN / 16, LA = BM * 8 / NT, LB = BN * 4 / NT, LR = EVERY == 1 ? 2 : 1;
+  constexpr int MT = BM / WM / 16, NG = BN / WN / 16;
+  constexpr int LA = BM * 8 / NT, LB = BN * 4 / NT, LR = EVERY == 1 ? 2 : 1;
   constexpr int kRowsAt = BM * 128, kRatioAt = kRowsAt + BN * 64, kStage = kRatioAt + LR * 1024;  // bytes
   static_assert(LA * NT == BM * 8 && LB * NT == BN * 4 && BN <= 256, "whole loads");
   static_assert(RING >= 2 && RING <= 4, "a stage an array");
@@ -469,7 +720,8 @@ __global__ __launch_bounds__(64 * WM * WN) void int4_tile_kernel(Int4Args a,
   auto fetch_unit = [&](const uint8_t* lds, int half) MOE_INLINE {
 #pragma unroll
     for (int g = 0; g < NG; ++g)
-      unit[g] = *reinterpret_cast<const f32x4*>(lds + kRatioAt + half * 1024 + ((wn * NG + g) * 16 + 4 * lq) * 4);
+      unit[g] = *reinterpret_cast<const f32x4*>(lds + kRatioAt + half * 1024 +
+                                                ((wn * NG + g) * 16 + 4 * lq) * 4);
   };
   auto operands = [&](int half) MOE_INLINE {
 #pragma unroll
@@ -605,17 +857,17 @@ __global__ __launch_bounds__(64 * WM * WN) void int4_tile_kernel(Int4Args a,
   }
 }
 
-template <int BM, int BN, int WM, int WN, int RING, int DT>
+// HALVES: groups may end in the middle of a step.
+template <int BM, int BN, int WM, int WN, int RING, int DT, bool HALVES>
 hipError_t launch_tile(const Int4Args& a, hipStream_t s) {
   const int64_t tiles = (int64_t)((a.T + BM - 1) / BM) * ((a.N + BN - 1) / BN);
   const int stages = (a.K + kBK - 1) / kBK;
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   float* ratio = reinterpret_cast<float*>(w + (int64_t)stages * a.N * kBK);
-  const int halves = a.G % kBK != 0;
   hipLaunchKernelGGL(int4_unpack_kernel, dim3((unsigned)stages * (unsigned)((a.N + 255) / 256)),
-                     dim3(256), 0, s, a, w, ratio, halves);
+                     dim3(256), 0, s, a, w, ratio, (int)HALVES);
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(64 * WM * WN);
-  if (halves)
+  if constexpr (HALVES)
     hipLaunchKernelGGL((int4_tile_kernel<BM, BN, WM, WN, RING, DT, 1>), grid, block, 0, s, a, w, ratio);
   else if (a.G % (2 * kBK))
     hipLaunchKernelGGL((int4_tile_kernel<BM, BN, WM, WN, RING, DT, 2>), grid, block, 0, s, a, w, ratio);
@@ -685,26 +937,56 @@ hipError_t launch_few_rows(const Int4Args& a, hipStream_t s) {
   return launch_stream<DT, 1, 1, SPG, 8>(a, s);
 }
 
-// Unpacking takes the weights' bytes three times over and a launch, which the tiles have to win back: us
-// with the few-rows kernel / tiles: 256 rows of 4096 x 8192 44 / 39, 512 of 2048 x 4096 28 / 25, 1000 of 1088
-// x 2008 18 / 16, 128 of 2048 x 4096 9.3 / 22, 203 of 1056 x 2008 6.9 / 16. The sides meet at about the same
-// T sqrt(N K). (The tiles' 32-bit offsets hold 2^24 channels.)
-bool many_rows(int T, int K, int N) {
-  return T >= 64 && N <= (1 << 24) && (double)T * T * N * K >= 1.5e12;
+// Tiles of 64 tokens x 64 channels.
+int64_t words_tiles(int T, int N) { return (int64_t)((T + 63) / 64) * ((N + 63) / 64); }
+
+// Which form takes aligned tensors. us with few / more / many rows' kernels, groups of 128:
+//   64 rows of 4096 x 8192 (128 tiles of 64 x 64) 15 / 18 / 39, 96 of 2048 x 4096 (128) 11 / 11 / 21, 192 of
+//   2048 x 4096 (192) 16 / 11 / 22, 48 of 4096 x 16384 (256) 25 / 19 / 48, 128 of 4096 x 8192 (256) 23 / 18 /
+//   39, 256 (512) 44 / 27 / 39, 512 (1024) 86 / 48 / 50, 640 (1280) 106 / 71 / 68, 1024 (2048) - / 93 / 75.
+// A row tile of 64 is half empty for 32 rows, which few rows' kernels take in tiles of 32. Unpacking costs as
+// much however few rows read the integers (12 us for 4096 x 8192) and a tile's products save about 28 of 92
+// us for 1024 rows: they pay from some 400 rows on.
+// Groups that are no multiple of 64 end inside a step, which doubles more rows' vector operations (256 rows of
+// 4096 x 8192 with 32 a group 61 us). There few / many rows: 256 rows of 4096 x 8192 44 / 54, 512 80 / 64,
+// 1000 of 1056 x 2048 15 / 19: the sides meet at about the same T sqrt(N K).
+// (The tiles' 32-bit offsets hold 2^24 channels.)
+bool many_rows(int T, int K, int N, int G) {
+  if (T < 64 || N > (1 << 24)) return false;
+  return G % kBK ? (double)T * T * N * K >= 4e12 : T >= 400 && words_tiles(T, N) > 1024;
+}
+bool more_rows(int T, int K, int N, int G) {
+  return G % kBK == 0 && T > 32 && words_tiles(T, N) > 160 && !many_rows(T, K, N, G);
+}
+
+// 64 x 64 in four shares of K while that is a workgroup a CU, 64 x 128 in two then, and in one at two
+// workgroups a CU: us 128 rows of 4096 x 8192 (256 tiles of 64 x 64) 18 / 27 / 33, 256 rows (512) 34 / 27 /
+// 34, 384 rows (768) 49 / 51 / 46.
+template <int DT>
+hipError_t launch_more_rows(const Int4Args& a, hipStream_t s) {
+  const int64_t tiles = words_tiles(a.T, a.N);
+  if (tiles <= 256) return launch_words<DT, 2, 4, 3>(a, s);
+  if (tiles <= 512) return launch_words<DT, 4, 2, 3>(a, s);
+  return launch_words<DT, 4, 1, 4>(a, s);
 }
 
 // By the number of 128 x 128 tiles, us with 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256: 128 tiles (256 rows
 // of 4096 x 8192) 40 / 48 / 66 / 107, 192 (384 rows) 51 / 49 / 67 / 105, 256 (512 rows) 56 / 51 / 67 / 107, 384
 // (768 rows) 76 / 79 / 69 / 108, 512 (1024 rows) 91 / 84 / 76 / 108, 768 (3000 of 2048 x 4096) 71 / 67 / 69 /
 // 61, 2048 (4096 of 4096 x 8192) 302 / 290 / 250 / 217. Between 64 x 128 tiles of 4 waves and of 8 there is
-// nothing to choose; 128 x 128 on 4 waves takes 55 us for the 512 rows.
+// nothing to choose; 128 x 128 on 4 waves takes 55 us for the 512 rows. The small tiles are for groups that
+// are no multiple of 64: the others get here with more than 256 tiles only.
 template <int DT>
 hipError_t launch_many_rows(const Int4Args& a, hipStream_t s) {
   const int64_t tiles = (int64_t)((a.T + 127) / 128) * ((a.N + 127) / 128);
-  if (tiles <= 160) return launch_tile<64, 128, 2, 2, 4, DT>(a, s);
-  if (tiles <= 320) return launch_tile<128, 128, 2, 4, 4, DT>(a, s);
-  if (tiles <= 640) return launch_tile<128, 256, 2, 4, 3, DT>(a, s);
-  return launch_tile<256, 256, 2, 4, 2, DT>(a, s);
+  if (a.G % kBK) {
+    if (tiles <= 160) return launch_tile<64, 128, 2, 2, 4, DT, true>(a, s);
+    if (tiles <= 320) return launch_tile<128, 128, 2, 4, 4, DT, true>(a, s);
+    if (tiles <= 640) return launch_tile<128, 256, 2, 4, 3, DT, true>(a, s);
+    return launch_tile<256, 256, 2, 4, 2, DT, true>(a, s);
+  }
+  if (tiles <= 640) return launch_tile<128, 256, 2, 4, 3, DT, false>(a, s);
+  return launch_tile<256, 256, 2, 4, 2, DT, false>(a, s);
 }
 
 template <int DT>
@@ -714,7 +996,8 @@ hipError_t launch_int4(const Int4Args& a, bool aligned, hipStream_t s) {
     hipLaunchKernelGGL(int4_values_kernel<DT>, dim3((unsigned)blocks), dim3(256), 0, s, a);
     return hipGetLastError();
   }
-  if (many_rows(a.T, a.K, a.N)) return launch_many_rows<DT>(a, s);
+  if (many_rows(a.T, a.K, a.N, a.G)) return launch_many_rows<DT>(a, s);
+  if (more_rows(a.T, a.K, a.N, a.G)) return launch_more_rows<DT>(a, s);
   if (a.G % 128 == 0) return launch_few_rows<DT, 4>(a, s);
   if (a.G % 64 == 0) return launch_few_rows<DT, 2>(a, s);
   return launch_few_rows<DT, 1>(a, s);
@@ -745,7 +1028,7 @@ extern "C" {
 int64_t moe_int4_linear_workspace_bytes_v1(int32_t T, int32_t K, int32_t N, int32_t group_size) {
   if (check_int4(T, K, N, group_size, kBf16)) return -1;
   // the integers, and two ratios for each 64 of them
-  return many_rows(T, K, N) ? (int64_t)((K + 63) / 64) * N * (64 + 8) : 0;
+  return many_rows(T, K, N, group_size) ? (int64_t)((K + 63) / 64) * N * (64 + 8) : 0;
 }
 
 int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,

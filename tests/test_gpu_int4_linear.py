@@ -74,6 +74,14 @@ TILES = [  # T, K, N, G: many rows: every tile, groups that end after one, two a
     (9000, 96, 1032, 96), (9000, 128, 1032, 64), (8200, 384, 1288, 128), (7000, 448, 1544, 64),
     (16400, 128, 1160, 128), (16390, 32, 1288, 32), (16500, 64, 1160, 64), (13000, 320, 1544, 64),
     (12900, 384, 1672, 128), (12850, 224, 1800, 32)]
+TILES += [  # rows between few and many, by tiles of 64 x 64: up to 256, up to 512, up to 1024 of them; groups of one,
+    # two, three and more steps of 64, K of one step (shares of K without any), odd numbers of steps, ragged tiles
+    (33, 64, 10376, 64), (64, 192, 10248, 64), (65, 128, 5256, 128), (70, 1088, 5320, 64), (130, 576, 3496, 192),
+    (500, 2048, 1288, 128), (961, 640, 648, 320), (2000, 512, 392, 512), (4033, 384, 184, 128), (10300, 320, 8, 64),
+    (129, 64, 5640, 64), (40, 448, 16648, 64), (100, 1024, 10504, 256), (300, 896, 3592, 128), (1000, 1088, 2008, 64),
+    (2049, 2048, 648, 2048), (190, 960, 6600, 192), (16500, 128, 72, 128),
+    (255, 64, 8264, 64), (257, 704, 8200, 64), (600, 1280, 4104, 640), (1025, 1536, 2056, 128), (4000, 384, 776, 128),
+    (511, 128, 16392, 128), (65, 192, 33288, 64), (40000, 64, 72, 64)]
 
 
 @pytest.mark.parametrize("T,K,N,G", TILES)
@@ -93,7 +101,8 @@ def test_exact_sums_of_many_rows(T, K, N, G, dtype):
 
 @pytest.mark.parametrize("T,K,N,G", [(1, 2048, 512, 128), (13, 1056, 200, 32), (40, 512, 264, 64),
                                      (150, 2048, 328, 128), (700, 1024, 520, 64), (1200, 384, 1032, 384), (1500, 2048, 1032, 128), (2600, 1056, 520, 32),
-                                     (4400, 512, 4104, 64), (4096, 1024, 2056, 128)])
+                                     (4400, 512, 4104, 64), (4096, 1024, 2056, 128),
+                                     (100, 2048, 5448, 128), (200, 1088, 8200, 64), (700, 1024, 4104, 128)])
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_random_values(T, K, N, G, dtype):
     q, z, qw, qz, g = make(K, N, G, 1)
