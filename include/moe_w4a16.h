@@ -351,21 +351,21 @@ int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,
  *   counts[e]  int32, slots of expert e
  *   balance    num_experts * sum_e (counts[e] / (n * top_k)) * mean_t p[t, e]
  *   z          mean_t (log sum exp logits[t])^2                          (both 0 for n = 0)
- *   lse        NULL, or fp32 [T + 1] for the backward pass: log sum exp of each token (+inf: does not
- *              count), then n
+ *   stats      NULL, or fp32 [2 T + 1] for the backward pass: each token's largest logit and log sum exp
+ *              less it (+inf: does not count), then n
  * Sums in a fixed order. The workspace query gives 0 for few tokens. */
 int64_t moe_route_workspace_bytes_v1(int32_t T, int32_t num_experts);
 int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dtype, int32_t top_k,
                  const uint8_t* mask, int32_t renormalize, void* workspace,
                  int64_t workspace_bytes, int32_t* topk_ids, float* topk_weights, int32_t* counts,
-                 float* balance, float* z, float* lse, void* stream);
+                 float* balance, float* z, float* stats, void* stream);
 
 /* dlogits [T, num_experts] from the gradients of topk_weights (fp32 [T, top_k]), balance and z (fp32
  * [1]; each NULL: zeros) and moe_route_v1's results; counts are constants. Tokens that do not count get
  * zeros; what dweights holds at places without an expert is not looked at. */
 int moe_route_backward_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dtype,
                           int32_t top_k, int32_t renormalize, const int32_t* topk_ids,
-                          const float* topk_weights, const int32_t* counts, const float* lse,
+                          const float* topk_weights, const int32_t* counts, const float* stats,
                           const float* dweights, const float* dbalance, const float* dz,
                           void* dlogits, void* stream);
 

@@ -8,11 +8,15 @@
 //   dl[j] = p[j] ((db E / n) (f[j] - <p, f>) + (2 dz / n) lse - q) + s[j],   f = c / (n top_k)
 //     renormalised: q = 0, s[ids[i]] = w[i] (dw[i] - <w, dw>);  otherwise q = <w, dw>, s[ids[i]] = w[i] dw[i]
 //
+// p is taken as exp((l - max) - log sum exp(l - max)): of lse itself, rounded to fp32, it would be off by as
+// much as lse's half step, |lse| 2^-24.
+//
 // A token counts if the mask keeps it and one of its logits is above -inf or a NaN; other tokens have ids
 // -1, weights 0 and no gradient. Only logits above -inf are chosen; places without one have id -1.
 //
 // Not the bytes but the instructions of the selection bound it: a wave a token, or for many tokens of 16-bit
-// logits four tokens a wave.
+// logits four tokens a wave. us on the GPU: 8 x 256 fp32 4.8, 8192 x 256 bf16 8.3 (0.5 TB/s) and 4.8 for the
+// workgroups' sums, 16384 x 256 fp32 21 (0.8 TB/s) and 5.8; the gradient 12 there (2.8 TB/s).
 //
 // A wave keeps its sums of p in registers and its workgroup the counts in LDS (integer atomics: the order does
 // not matter), so that a workgroup leaves one row of partial sums. Sums are taken in a fixed order: fp32 over a
@@ -127,7 +131,8 @@ struct RouteArgs {
   int32_t* counts;
   float* balance;
   float* z;
-  float* lse;  // nullable: [T + 1], lse of each token (+inf: does not count), then n
+  float* stats;  // nullable: [2 T + 1], each token's largest logit and log sum exp less it (+inf: does not
+                 // count), then n
   RouteWs ws;
 };
 
@@ -148,7 +153,7 @@ MOE_DEV void finish(const RouteArgs& a, double dot, double zsum, int n) {
   const double inv = n > 0 ? 1.0 / (double)n : 0.0;
   *a.balance = (float)((double)a.E * dot * inv * inv / (double)a.k);
   *a.z = (float)(zsum * inv);
-  if (a.lse) a.lse[a.T] = (float)n;
+  if (a.stats) a.stats[2 * (int64_t)a.T] = (float)n;
 }
 
 // A workgroup's sums: p of each wave and expert, slots of each expert.
@@ -349,8 +354,11 @@ __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs
       a.weights[t * a.k + l16] = chosen ? mine / over : 0.0f;
     }
     if (chosen) atomicAdd(&s.c[id], 1);
-    const float lse = top + logf(total);
-    if (a.lse && l16 == 0 && t < a.T) a.lse[t] = live ? lse : __builtin_inff();
+    const float rest = logf(total), lse = top + rest;
+    if (a.stats && l16 == 0 && t < a.T) {
+      a.stats[2 * t] = top;
+      a.stats[2 * t + 1] = live ? rest : __builtin_inff();
+    }
     if (live) {
       const float inv = 1.0f / total;
 #pragma unroll
@@ -439,8 +447,11 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
       a.weights[t * a.k + lane] = chosen ? mine / over : 0.0f;
     }
     if (chosen) atomicAdd(&s.c[my_i], 1);
-    const float lse = live ? top + logf(total) : 0.0f;
-    if (a.lse && lane == 0) a.lse[t] = live ? lse : __builtin_inff();
+    const float rest = logf(total), lse = top + rest;
+    if (a.stats && lane == 0) {
+      a.stats[2 * t] = top;
+      a.stats[2 * t + 1] = live ? rest : __builtin_inff();
+    }
     if (live) {
       const float inv = 1.0f / total;
 #pragma unroll
@@ -526,7 +537,7 @@ struct RouteGradArgs {
   const int32_t* ids;
   const float* weights;
   const int32_t* counts;
-  const float* lse;       // [T + 1]
+  const float* stats;     // [2 T + 1]
   const float* dweights;  // the three are nullable
   const float* dbalance;
   const float* dz;
@@ -541,7 +552,7 @@ __global__ __launch_bounds__(64 * kGradWaves) void route_backward_kernel(RouteGr
   __shared__ float s_d[kGradWaves][64 * NC];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const float n = a.lse[a.T], inv_n = n > 0.0f ? 1.0f / n : 0.0f;
+  const float n = a.stats[2 * (int64_t)a.T], inv_n = n > 0.0f ? 1.0f / n : 0.0f;
   const float cb = a.dbalance ? *a.dbalance * ((float)a.E * inv_n) : 0.0f;
   const float cz = a.dz ? 2.0f * *a.dz * inv_n : 0.0f;
   const float unit = inv_n / (float)a.k;
@@ -557,8 +568,8 @@ __global__ __launch_bounds__(64 * kGradWaves) void route_backward_kernel(RouteGr
     float p[NC], pf = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) p[c] = Elem<DT>::get(row[min(lane + 64 * c, a.E - 1)]);
-    const float lse = a.lse[t];
-    const bool live = lse != __builtin_inff();
+    const float top = a.stats[2 * t], rest = a.stats[2 * t + 1], lse = top + rest;
+    const bool live = rest != __builtin_inff();
     int id = lane < a.k ? a.ids[t * a.k + lane] : -1;
     id = id < a.E ? id : -1;
     float w = 0.0f, dw = 0.0f;
@@ -568,7 +579,7 @@ __global__ __launch_bounds__(64 * kGradWaves) void route_backward_kernel(RouteGr
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      p[c] = live && lane + 64 * c < a.E ? expf(p[c] - lse) : 0.0f;
+      p[c] = live && lane + 64 * c < a.E ? expf((p[c] - top) - rest) : 0.0f;
       pf = __builtin_fmaf(p[c], f[c], pf);
     }
     pf = wave_sum(pf);
@@ -694,7 +705,7 @@ int64_t moe_route_workspace_bytes_v1(int32_t T, int32_t num_experts) {
 int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dtype, int32_t top_k,
                  const uint8_t* mask, int32_t renormalize, void* workspace,
                  int64_t workspace_bytes, int32_t* topk_ids, float* topk_weights, int32_t* counts,
-                 float* balance, float* z, float* lse, void* stream) {
+                 float* balance, float* z, float* stats, void* stream) {
   const int rc = check_route("route", T, num_experts, dtype, top_k);
   if (rc) return rc;
   if ((T > 0 && (!logits || !topk_ids || !topk_weights)) || !counts || !balance || !z)
@@ -711,14 +722,14 @@ int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dty
   const int64_t S = (int64_t)T * top_k;
   const Mem outs[] = {{workspace, need}, {topk_ids, S * 4}, {topk_weights, S * 4},
                       {counts, (int64_t)num_experts * 4}, {balance, 4}, {z, 4},
-                      {lse, ((int64_t)T + 1) * 4}};
+                      {stats, ((int64_t)2 * T + 1) * 4}};
   const Mem ins[] = {{logits, (int64_t)T * num_experts * dtype_bytes(dtype)}, {mask, T}};
   if (any_overlap(outs, ins))
     return op_fail(MOE_ERR_SHAPE,
                    "route: outputs and workspace must not overlap the inputs or each other");
-  const RouteArgs a{logits, mask, T, num_experts, top_k, renormalize != 0, 
+  const RouteArgs a{logits, mask, T, num_experts, top_k, renormalize != 0,
                     route_groups(T, route_grouped(T, top_k, dtype) ? kGroupTokens : kWaves), topk_ids,
-                    topk_weights, counts, balance, z, lse, ws};
+                    topk_weights, counts, balance, z, stats, ws};
   const auto s = (hipStream_t)stream;
   MOE_OP_HIP(dtype == kBf16   ? launch_route_any<kBf16>(a, s)
              : dtype == kFp16 ? launch_route_any<kFp16>(a, s)
@@ -729,23 +740,23 @@ int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dty
 
 int moe_route_backward_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dtype,
                           int32_t top_k, int32_t renormalize, const int32_t* topk_ids,
-                          const float* topk_weights, const int32_t* counts, const float* lse,
+                          const float* topk_weights, const int32_t* counts, const float* stats,
                           const float* dweights, const float* dbalance, const float* dz,
                           void* dlogits, void* stream) {
   const int rc = check_route("route backward", T, num_experts, dtype, top_k);
   if (rc) return rc;
   if (T == 0) return MOE_OK;
-  if (!logits || !topk_ids || !topk_weights || !counts || !lse || !dlogits)
+  if (!logits || !topk_ids || !topk_weights || !counts || !stats || !dlogits)
     return op_fail(MOE_ERR_NULL, "route backward: NULL pointer");
   const int64_t S = (int64_t)T * top_k, nl = (int64_t)T * num_experts * dtype_bytes(dtype);
   const Mem outs[] = {{dlogits, nl}};
   const Mem ins[] = {{logits, nl}, {topk_ids, S * 4}, {topk_weights, S * 4},
-                     {counts, (int64_t)num_experts * 4}, {lse, ((int64_t)T + 1) * 4},
+                     {counts, (int64_t)num_experts * 4}, {stats, ((int64_t)2 * T + 1) * 4},
                      {dweights, S * 4}, {dbalance, 4}, {dz, 4}};
   if (any_overlap(outs, ins))
     return op_fail(MOE_ERR_SHAPE, "route backward: dlogits must not overlap the inputs");
   const RouteGradArgs a{logits, T, num_experts, top_k, renormalize != 0, topk_ids, topk_weights,
-                        counts, lse, dweights, dbalance, dz, dlogits};
+                        counts, stats, dweights, dbalance, dz, dlogits};
   const auto s = (hipStream_t)stream;
   MOE_OP_HIP(dtype == kBf16   ? launch_backward_any<kBf16>(a, s)
              : dtype == kFp16 ? launch_backward_any<kFp16>(a, s)

@@ -853,7 +853,7 @@ class Routing(NamedTuple):
     z_loss: torch.Tensor        # fp32 scalar
 
 
-def _route(logits, top_k, mask, renormalize, want_lse):
+def _route(logits, top_k, mask, renormalize, want_stats):
     T, E = logits.shape
     dev = logits.device
     ids = torch.empty(T, top_k, dtype=torch.int32, device=dev)
@@ -861,22 +861,22 @@ def _route(logits, top_k, mask, renormalize, want_lse):
     counts = torch.empty(E, dtype=torch.int32, device=dev)
     balance = torch.empty((), dtype=torch.float32, device=dev)
     z = torch.empty((), dtype=torch.float32, device=dev)
-    lse = torch.empty(T + 1, dtype=torch.float32, device=dev) if want_lse else None
+    stats = torch.empty(2 * T + 1, dtype=torch.float32, device=dev) if want_stats else None
     need = _lib.load().moe_route_workspace_bytes_v1(T, E)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _call("moe_route_v1", dev, logits.data_ptr(), T, E, OUT_DTYPES[logits.dtype], top_k, _ptr(mask),
           renormalize, _ptr(ws), need, ids.data_ptr(), weights.data_ptr(), counts.data_ptr(),
-          balance.data_ptr(), z.data_ptr(), _ptr(lse))
-    return ids, weights, counts, balance, z, lse
+          balance.data_ptr(), z.data_ptr(), _ptr(stats))
+    return ids, weights, counts, balance, z, stats
 
 
 class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, mask, renormalize):
-        ids, weights, counts, balance, z, lse = _route(logits, top_k, mask, renormalize, True)
+        ids, weights, counts, balance, z, stats = _route(logits, top_k, mask, renormalize, True)
         ctx.mark_non_differentiable(ids, counts)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, ids, weights, counts, lse)
+        ctx.save_for_backward(logits, ids, weights, counts, stats)
         ctx.renormalize = renormalize
         return ids, weights, counts, balance, z
 
@@ -886,14 +886,14 @@ class _RouteFn(torch.autograd.Function):
         if dweights is None and dbalance is None and dz is None:
             return None, None, None, None
         _refuse_dual(dweights, dbalance, dz)
-        logits, ids, weights, counts, lse = ctx.saved_tensors
+        logits, ids, weights, counts, stats = ctx.saved_tensors
         if dweights is not None:
             dweights = dweights.contiguous()
         T, E = logits.shape
         dlogits = torch.empty_like(logits)
         _call("moe_route_backward_v1", logits.device, logits.data_ptr(), T, E,
               OUT_DTYPES[logits.dtype], ids.shape[1], ctx.renormalize, ids.data_ptr(),
-              weights.data_ptr(), counts.data_ptr(), lse.data_ptr(), _ptr(dweights), _ptr(dbalance),
+              weights.data_ptr(), counts.data_ptr(), stats.data_ptr(), _ptr(dweights), _ptr(dbalance),
               _ptr(dz), dlogits.data_ptr())
         return dlogits, None, None, None
 
@@ -911,8 +911,8 @@ def route_tokens(logits: torch.Tensor, top_k: int = 8, *, mask: torch.Tensor | N
     tokens get ids -1, which ``dispatch_tokens`` drops, weights 0 and no gradient; so does a place for
     which no logit above -inf is left. Both losses are 0 for n = 0. A NaN or +inf among the logits of a
     counted token makes its weights and both losses NaN. logits [T, E] bf16, fp16 or fp32; E <= 512,
-    top_k <= 64. Differentiable in logits through topk_weights and both losses (counts are constants);
-    the gradient is rounded once to logits' type."""
+    top_k <= 64, T * top_k <= 2^22. Differentiable in logits through topk_weights and both losses (counts
+    are constants); the gradient is rounded once to logits' type."""
     _rows_2d(logits, "logits")
     T, E = logits.shape
     if not 1 <= E <= 512:

@@ -131,6 +131,22 @@ def test_forward_and_gradient(T, E, k, dtype, masked, blocked, renorm):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("T,E,dtype", [(60, 96, torch.float32), (1100, 40, torch.float16)])
+def test_gradient_of_large_logits(T, E, dtype):
+    """Logits about a common value of 1000 (steps of half a unit, exact in both types): log sum exp has a
+    half step of 512 u there, which neither the probabilities nor the gradient may be off by."""
+    g = torch.Generator().manual_seed(21)
+    l = (1000 + torch.randint(-12, 13, (T, E), generator=g) * 0.5).to(dtype)
+    dw, db = torch.randn(T, 6, generator=g), torch.tensor(3.0)
+    want = formulas(l, 6, None, False, (dw, db, None))
+    x = l.cuda().requires_grad_()
+    r = ops.route_tokens(x, 6, renormalize=False)
+    d, = torch.autograd.grad((r.topk_weights, r.balance_loss), x, (dw.cuda(), db.cuda()))
+    tol = 160 * U * want["size"] + half(dtype) * want["d"].abs() + TINY[dtype]
+    err = (d.cpu().double() - want["d"]).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
 @pytest.mark.parametrize("parts", ["w", "b", "z", "wz"])
 def test_gradient_of_some_results(parts):
     l = make(50, 40, torch.float32)
