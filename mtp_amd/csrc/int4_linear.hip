@@ -923,15 +923,20 @@ int64_t stream_groups(int T, int N, int rows, int channels) {
 }
 
 // The larger a tile the fewer bytes of x and weights a workgroup reads for a result, the smaller the more
-// workgroups there are: the largest of these that still gives about one a CU. us with 16 x 16, 16 x 32,
-// 16 x 64, 32 x 64, 64 x 64: 1 row of 2048 x 4096 4.3 / 4.7 / 5.7, of 4096 x 8192 9.3 / 7.1 / 8.4, of 8192 x
-// 16384 32 / 19 / 16; 64 rows of 2048 x 4096 13 / 8.9 / 7.4 / 9.5, of 4096 x 8192 40 / 24 / 18 / 15 / 24; 203
-// of 1056 x 2008 13 / 9.2 / 8.1 / 7.0 / 10; 256 of 4096 x 8192 146 / 88 / 66 / 54 / 47.
-constexpr int kEnough = 224;
+// workgroups there are: the largest of these that its rows fill half of and that still gives most of the CUs one. us
+// with 16 x 16, 16 x 32, 16 x 64, 32 x 64, 64 x 64: 1 row of 2048 x 4096 4.3 / 4.7 / 5.7, of 4096 x 8192 9.3 /
+// 7.1 / 8.4; 16 rows of 8192 x 16384 41 / 26 / 19 / 23 / 31; 32 of it 74 / 45 / 32 / 25 / 34; 48 rows of 2048 x
+// 4096 9.5 / 8.1 / 6.6 / 8.6 / 13; 64 rows of 2048 x 4096 12 / 8.1 / 6.7 / 8.6 / 14, of 4096 x 8192 38 / 24 / 18 /
+// 15 / 23; 96 of 2048 x 4096 17 / 11 / 11 / 8.6 / 14; 203 of 1056 x 2008 13 / 9.2 / 8.1 / 7.0 / 10; 256 of 4096 x
+// 8192 146 / 88 / 66 / 54 / 47 (there groups of 64 and 128 have the kernel for more rows). 32 x 32 and 64 x 32
+// are never the best.
+constexpr int kEnough = 192;
 template <int DT, int SPG>
 hipError_t launch_few_rows(const Int4Args& a, hipStream_t s) {
-  if (stream_groups(a.T, a.N, 64, 64) >= kEnough) return launch_stream<DT, 4, 4, SPG, 4>(a, s);
-  if (stream_groups(a.T, a.N, 32, 64) >= kEnough) return launch_stream<DT, 2, 4, SPG, 8>(a, s);
+  if constexpr (SPG == 1) {
+    if (a.T > 32 && stream_groups(a.T, a.N, 64, 64) >= kEnough) return launch_stream<DT, 4, 4, SPG, 4>(a, s);
+  }
+  if (a.T > 16 && stream_groups(a.T, a.N, 32, 64) >= kEnough) return launch_stream<DT, 2, 4, SPG, 8>(a, s);
   if (stream_groups(a.T, a.N, 16, 64) >= kEnough) return launch_stream<DT, 1, 4, SPG, 8>(a, s);
   if (stream_groups(a.T, a.N, 16, 32) >= kEnough) return launch_stream<DT, 1, 2, SPG, 8>(a, s);
   return launch_stream<DT, 1, 1, SPG, 8>(a, s);
