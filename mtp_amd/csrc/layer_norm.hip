@@ -9,7 +9,7 @@
 // across the reductions. Sums are taken in a fixed order. us on the GPU (a copy of 1 GiB runs at 5.2 TB/s):
 //   forward   16384 x 2048 bf16 25 (5.4 TB/s), 8192 x 4096 fp16 25 (5.4), 2001 x 1000 fp32 5.2
 //   backward  16384 x 2048 bf16 39 with all gradients (5.2 TB/s; 32 for dx alone), 2001 x 1000 fp32 14
-// Rows of less than 512 columns leave lanes idle: 65536 x 256 fp16 27 and 30.
+// Up to 256 columns 2, 4 or 8 rows share a wave: 524288 x 128 bf16 54 (5.0 TB/s) and 79 (5.1).
 //
 // The mean is a sum in 64 bits and a division (a constant row's sum is exact, and so is then its mean): in 32
 // bits a row whose mean is 2^12 times its spread would lose half of its digits. It is kept in two parts, and
@@ -33,6 +33,22 @@ struct LayerNormArgs {
   double eps;
 };
 
+// The rows of a thread, with NT threads a row in workgroups of BT: those of a wave that holds several run
+// together, so the loop is over the first of them, and the last ones may lie behind the tensor. `mine`: this
+// thread's, of the wave's.
+template <int NT, int BT>
+struct Rows {
+  int mine;
+  int64_t first, stride;
+  MOE_DEV Rows() {
+    constexpr int kWide = NT < 64 ? 64 : NT;
+    mine = NT < 64 ? (int)(threadIdx.x & 63) / NT : 0;
+    first = ((int64_t)blockIdx.x * (BT / kWide) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWide)) *
+            (kWide / NT);
+    stride = (int64_t)gridDim.x * (BT / NT);
+  }
+};
+
 // NT threads a row, NC chunks of 8 NT columns: a wave a row while it holds the row (2048 columns), with no
 // barrier and 12 exchanges for up to 32 columns a lane; with 256 threads a row of 2048 these and the barriers
 // were half of the kernel's instructions (16384 x 2048 bf16 31 us). A workgroup takes every so many rows and
@@ -42,22 +58,22 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
   using T = typename Elem<DT>::T;
   using C = Cols<DT, NT, VEC>;
   using Raw = RawCols<DT, NT, VEC>;
-  __shared__ double s_part[NT / 64][1];
+  __shared__ double s_part[NT > 64 ? NT / 64 : 1][1];
   const double inv_h = 1.0 / (double)a.H;
   const int tid = threadIdx.x % NT, H = a.H;
-  constexpr int rows = 256 / NT;
-  const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
-  const int64_t stride = (int64_t)gridDim.x * rows, first = (int64_t)blockIdx.x * rows + sub;
+  const Rows<NT, 256> rows;
   Raw next[NC], w[NC] = {}, b[NC] = {};
   auto load = [&](Raw (&v)[NC], const void* p, int64_t t) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       v[c].load(static_cast<const T*>(p) + t * H + c * 8 * NT, tid, H - c * 8 * NT);
   };
-  if (first < a.T) load(next, a.x, first);
+  if (rows.first < a.T) load(next, a.x, min(rows.first + rows.mine, (int64_t)a.T - 1));
   if (a.w) load(w, a.w, 0);
   if (a.b) load(b, a.b, 0);
-  for (int64_t t = first; t < a.T; t += stride) {
+  for (int64_t lead = rows.first; lead < a.T; lead += rows.stride) {
+    const int64_t t = lead + rows.mine;
+    const bool in = NT >= 64 || t < a.T;
     float d[NC][8];
     double part[1] = {0.0}, sum[1];
 #pragma unroll
@@ -68,7 +84,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
         d[c][e] = next[c].get(e, tid, left);
         part[0] += (double)d[c][e];
       }
-    load(next, a.x, min(t + stride, (int64_t)a.T - 1));  // past the last row: read again, not used
+    load(next, a.x, min(t + rows.stride, (int64_t)a.T - 1));  // past the last row: read again, not used
     row_sums<NT>(part, sum, s_part);
     const double mean = sum[0] / (double)H;
     const float hi = (float)mean, lo = (float)(mean - (double)hi);
@@ -85,7 +101,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
     }
     row_sums<NT>(part, sum, s_part);
     const float r = inv_sqrt(sum[0] * inv_h + a.eps);
-    if (stats && tid == 0) stats[t] = f32x4{hi, lo, r, 0.0f};
+    if (stats && tid == 0 && in) stats[t] = f32x4{hi, lo, r, 0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int left = H - c * 8 * NT;
@@ -94,7 +110,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
       for (int e = 0; e < 8; ++e)
         o[e] = __builtin_fmaf(d[c][e] * r, a.w ? w[c].get(e, tid, left) : 1.0f,
                               a.b ? b[c].get(e, tid, left) : 0.0f);
-      C::store(static_cast<T*>(y) + t * H + c * 8 * NT, tid, left, o);
+      if (in) C::store(static_cast<T*>(y) + t * H + c * 8 * NT, tid, left, o);
     }
   }
 }
@@ -113,12 +129,10 @@ __global__ __launch_bounds__(block_threads<NT>()) void layer_norm_backward_kerne
   using T = typename Elem<DT>::T;
   using C = Cols<DT, NT, VEC>;
   using Raw = RawCols<DT, NT, VEC>;
-  __shared__ float s_part[NT / 64][2];
+  __shared__ float s_part[NT > 64 ? NT / 64 : 1][2];
   const float inv_h = 1.0f / (float)a.H;
   const int tid = threadIdx.x % NT, H = a.H;
-  const int rows = block_threads<NT>() / NT;
-  const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT);
-  const int64_t stride = (int64_t)gridDim.x * rows, first = (int64_t)blockIdx.x * rows + sub;
+  const Rows<NT, block_threads<NT>()> rows;
   float w[8], dw[8], db[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -137,18 +151,20 @@ __global__ __launch_bounds__(block_threads<NT>()) void layer_norm_backward_kerne
     next.dy.load(static_cast<const T*>(d.dy) + u * H, tid, H);
     next.st = d.stats[u];
   };
-  if (first < a.T) load(first);
-  for (int64_t t = first; t < a.T; t += stride) {
+  if (rows.first < a.T) load(rows.first + rows.mine);
+  for (int64_t lead = rows.first; lead < a.T; lead += rows.stride) {
+    const int64_t t = lead + rows.mine;
+    const bool mine = NT >= 64 || t < a.T;
     const Row row = next;
-    load(t + stride);
+    load(t + rows.stride);
     const float hi = row.st[0], lo = row.st[1], r = row.st[2];
     float part[2] = {0.0f, 0.0f}, tot[2];
     float h[8], g[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool in = C::col(tid, e) < H;
-      const float dy = row.dy.get(e, tid, H);
-      h[e] = in ? ((row.x.get(e, tid, H) - hi) - lo) * r : 0.0f;
+      const float dy = mine ? row.dy.get(e, tid, H) : 0.0f;
+      h[e] = in && mine ? ((row.x.get(e, tid, H) - hi) - lo) * r : 0.0f;
       g[e] = dy * w[e];
       dw[e] = __builtin_fmaf(dy, h[e], dw[e]);
       db[e] += dy;
@@ -160,11 +176,13 @@ __global__ __launch_bounds__(block_threads<NT>()) void layer_norm_backward_kerne
       const float mg = tot[0] * inv_h, mgh = tot[1] * inv_h;
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] = r * ((g[e] - mg) - h[e] * mgh);
-      C::store(static_cast<T*>(d.dx) + t * H, tid, H, g);
+      if (mine) C::store(static_cast<T*>(d.dx) + t * H, tid, H, g);
     }
   }
-  if constexpr (NT == 64) {  // the rows' waves first
-    __shared__ f32x4 s_all[4][4][64];
+  if constexpr (NT <= 64) {  // the workgroup's rows first
+    constexpr int kRows = 256 / NT;
+    const int sub = threadIdx.x / NT;
+    __shared__ f32x4 s_all[kRows][4][NT];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float* v = (q < 2 ? dw : db) + 4 * (q & 1);
@@ -176,7 +194,7 @@ __global__ __launch_bounds__(block_threads<NT>()) void layer_norm_backward_kerne
     for (int q = 0; q < 4; ++q) {
       f32x4 v = s_all[0][q][tid];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) v += s_all[w][q][tid];
+      for (int w = 1; w < kRows; ++w) v += s_all[w][q][tid];
 #pragma unroll
       for (int j = 0; j < 4; ++j) (q < 2 ? dw : db)[4 * (q & 1) + j] = v[j];
     }
@@ -221,8 +239,12 @@ constexpr int kForwardGroups = 1536;
 
 // Workgroups of the backward pass: each keeps the weights' gradients of its rows in registers and
 // writes them once.
+//
+// Rows of up to 256 columns take 32, 16 or 8 threads, forward and backward (us a wave a row / with this): 65536 x
+// 256 fp16 27 and 30 / 16 and 22, 524288 x 128 bf16 186 and 175 / 54 and 79, 300000 x 64 106 and 100 / 16 and 38.
+int narrow_threads_of(int H) { return H <= 64 ? 8 : H <= 128 ? 16 : H <= 256 ? 32 : threads_of(H); }
 int backward_groups(int T, int H) {
-  const int nt = threads_of(H), rows = rows_of(nt);
+  const int nt = narrow_threads_of(H), rows = rows_of(nt);
   const int most = nt > 256 ? 256 : 768;
   return std::max(1, std::min((T - 1) / rows + 1, most));  // T + rows may pass 32 bits
 }
@@ -238,7 +260,10 @@ hipError_t launch_forward(const LayerNormArgs& a, void* y, f32x4* stats, bool ve
     else                                                                                               \
       hipLaunchKernelGGL((layer_norm_kernel<DT, NT, NC, false>), grid, dim3(256), 0, s, a, y, stats);  \
   } while (0)
-  if (a.H <= 512) MOE_LN_FWD(64, 1);
+  if (a.H <= 64) MOE_LN_FWD(8, 1);
+  else if (a.H <= 128) MOE_LN_FWD(16, 1);
+  else if (a.H <= 256) MOE_LN_FWD(32, 1);
+  else if (a.H <= 512) MOE_LN_FWD(64, 1);
   else if (a.H <= 1024) MOE_LN_FWD(64, 2);
   else if (a.H <= 2048) MOE_LN_FWD(64, 4);
   else if (a.H <= 4096) MOE_LN_FWD(256, 2);
@@ -250,12 +275,20 @@ hipError_t launch_forward(const LayerNormArgs& a, void* y, f32x4* stats, bool ve
 template <int DT>
 hipError_t launch_backward(const LayerNormArgs& a, const LayerNormGrads& d, void* dw, void* db,
                            bool vec, hipStream_t s) {
-  const int nt = threads_of(a.H);
+  const int nt = narrow_threads_of(a.H);
   const dim3 grid((unsigned)backward_groups(a.T, a.H));
 #define MOE_LN_BWD(NT, V)                                                                       \
   hipLaunchKernelGGL((layer_norm_backward_kernel<DT, NT, V>), grid, dim3(block_threads<NT>()), \
                      0, s, a, d)
-  MOE_ROW_NT(MOE_LN_BWD)
+  if (nt == 8) {
+    if (vec) MOE_LN_BWD(8, true); else MOE_LN_BWD(8, false);
+  } else if (nt == 16) {
+    if (vec) MOE_LN_BWD(16, true); else MOE_LN_BWD(16, false);
+  } else if (nt == 32) {
+    if (vec) MOE_LN_BWD(32, true); else MOE_LN_BWD(32, false);
+  } else {
+    MOE_ROW_NT(MOE_LN_BWD)
+  }
 #undef MOE_LN_BWD
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(dw || db)) return e;

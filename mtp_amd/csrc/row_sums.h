@@ -22,15 +22,15 @@ template <int M>
 MOE_DEV float partner(float v) { return xor_partner<M>(v); }
 
 // Sums of N values over the NT threads of a row (all threads get them), in a fixed order. A is the type
-// they are taken in, P that of a thread's own part. NT = 64: no barrier.
+// they are taken in, P that of a thread's own part. NT up to 64: no barrier.
 template <int NT, int N, class P, class A>
 MOE_DEV void row_sums(const P (&part)[N], A (&v)[N], A (*s_part)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     v[i] = part[i];
-    v[i] += partner<32>(v[i]);
-    v[i] += partner<16>(v[i]);
-    v[i] += partner<8>(v[i]);
+    if constexpr (NT > 32) v[i] += partner<32>(v[i]);
+    if constexpr (NT > 16) v[i] += partner<16>(v[i]);
+    if constexpr (NT > 8) v[i] += partner<8>(v[i]);
     v[i] += partner<4>(v[i]);
     v[i] += partner<2>(v[i]);
     v[i] += partner<1>(v[i]);

@@ -69,6 +69,11 @@ CASES = [  # T, H, dtype, weight, bias
     (1700, 96, torch.float32, True, True), (2500, 33, torch.bfloat16, True, True),
     (4, 4096, torch.bfloat16, True, False), (1601, 2048, torch.bfloat16, True, True),
     (1100, 4100, torch.float16, True, True)]
+CASES += [  # several rows a wave: 8, 4 and 2 of them, the last ones behind the tensor
+    (1, 8, torch.bfloat16, True, True), (770, 24, torch.bfloat16, True, True), (9, 64, torch.float32, True, True),
+    (50001, 16, torch.bfloat16, True, True), (67, 128, torch.float16, True, False), (50, 65, torch.float32, True, True),
+    (26003, 100, torch.float16, False, True), (13, 256, torch.bfloat16, True, True), (1001, 200, torch.float32, True, True),
+    (12511, 250, torch.bfloat16, True, True), (3, 129, torch.bfloat16, True, True), (2, 257, torch.float32, True, True)]
 
 
 @pytest.mark.parametrize("T,H,dtype,weight,bias", CASES)
@@ -127,6 +132,22 @@ def test_rows_with_infinities_and_nan_are_nan_alone():
     bad[1, 7], bad[3, 0], bad[4, 299] = float("inf"), float("nan"), float("-inf")
     y = ops.layer_norm(bad)
     assert bool(y[[1, 3, 4]].isnan().all()) and torch.equal(y[[0, 2, 5]], clean[[0, 2, 5]])
+
+
+@pytest.mark.parametrize("H", [40, 64, 101, 128, 200, 256])
+def test_rows_of_one_wave_do_not_touch_each_other(H):
+    x = torch.randn(11, H, generator=torch.Generator().manual_seed(4)).cuda()
+    dy = torch.randn(11, H, generator=torch.Generator().manual_seed(5)).cuda()
+    rows = [[], []]
+    for i, x in enumerate((x, x.clone())):
+        if i:
+            x[2, 3], x[10, H - 1] = float("nan"), float("inf")
+        x.requires_grad_()
+        y = ops.layer_norm(x)
+        rows[i] = [y.detach(), *torch.autograd.grad(y, x, dy)]
+    keep = [t for t in range(11) if t not in (2, 10)]
+    for clean, got in zip(*rows):
+        assert torch.equal(clean[keep], got[keep]) and bool(got[[2, 10]].isnan().all())
 
 
 def test_no_tokens():
