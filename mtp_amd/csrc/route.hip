@@ -14,9 +14,10 @@
 // A token counts if the mask keeps it and one of its logits is above -inf or a NaN; other tokens have ids
 // -1, weights 0 and no gradient. Only logits above -inf are chosen; places without one have id -1.
 //
-// Not the bytes but the instructions of the selection bound it: a wave a token, or for many tokens of 16-bit
-// logits four tokens a wave. us on the GPU: 8 x 256 fp32 4.8, 8192 x 256 bf16 8.3 (0.5 TB/s) and 4.8 for the
-// workgroups' sums, 16384 x 256 fp32 21 (0.8 TB/s) and 5.8; the gradient 12 there (2.8 TB/s).
+// Not the bytes but the instructions of the selection bound it: a wave a token, or for many tokens of at most
+// 256 experts (512 with 16 bits) four tokens a wave. us on the GPU: 8 x 256 fp32 4.8, 8192 x 256 bf16 8.3 (0.5
+// TB/s) and 4.8 for the workgroups' sums, 16384 x 256 fp32 19 (0.9 TB/s) and 5.8; the gradient 12 there (2.8
+// TB/s).
 //
 // A wave keeps its sums of p in registers and its workgroup the counts in LDS (integer atomics: the order does
 // not matter), so that a workgroup leaves one row of partial sums. Sums are taken in a fixed order: fp32 over a
@@ -231,11 +232,12 @@ MOE_DEV float exp_neg(float x) {
 // ---------------------------------------------------------------- 16 lanes a token
 template <int M>
 MOE_DEV uint32_t row_partner(uint32_t v) { return __float_as_uint(xor_partner<M>(__uint_as_float(v))); }
+// Neighbour, pair, mirrored half and mirrored row: once they agree within what is mirrored, that is the other.
 MOE_DEV uint32_t row_max(uint32_t v) {
-  v = max(v, row_partner<8>(v));
-  v = max(v, row_partner<4>(v));
-  v = max(v, row_partner<2>(v));
-  return max(v, row_partner<1>(v));
+  v = max(v, MOE_DPP(v, 0xB1, 0xF));
+  v = max(v, MOE_DPP(v, 0x4E, 0xF));
+  v = max(v, MOE_DPP(v, 0x141, 0xF));
+  return max(v, MOE_DPP(v, 0x140, 0xF));
 }
 MOE_DEV float row_max(float v) {  // of a NaN and a number the number
   v = __builtin_fmaxf(v, xor_partner<8>(v));
@@ -250,9 +252,14 @@ MOE_DEV float row_sum(float v) {
   return v + xor_partner<1>(v);
 }
 
-// A key for the selection: (order, complement of the id), unique, 25 bits.
-template <int DT>
-struct GroupKey {
+// The order of a token's logits in PL keys a lane (expert 16 j + lane), 0 for "not a candidate", and the
+// selection: lane r < top_k gets the r-th largest one's id and value, `mine` false where no logit above -inf
+// was left. m: the row's largest key.
+//
+// Logits of 16 bits leave room for the id: (order, complement of the id), unique, 25 bits. Below a maximum m the
+// next one is the largest of key - m, in which those not below it are the small ones.
+template <int DT, int PL>
+struct GroupSelect {
   static constexpr uint32_t kInf = DT == kBf16 ? 0x7F80u : 0x7C00u;
   static constexpr uint32_t kLowest = (~(kInf | 0x8000u) & 0xFFFFu) << 9 | 511u;  // -inf, of any id
   MOE_DEV static uint32_t key(uint16_t v, int id) {
@@ -262,23 +269,69 @@ struct GroupKey {
     o = (u & 0x7FFFu) > kInf ? 0u : o;  // NaN below every number
     return o << 9 | (511u - (uint32_t)id);
   }
+  MOE_DEV static void select(uint32_t (&key)[PL], uint32_t m, int top_k, int l16, int& id, float& v, bool& mine) {
+    uint32_t my = 0;
+    for (int r = 0; r < top_k; ++r) {
+      if (l16 == r) my = m;
+      uint32_t d = 0;
+#pragma unroll
+      for (int j = 0; j < PL; ++j) d = max(d, key[j] - m);
+      d = row_max(d);
+      m = d >> 31 ? m + d : 0u;  // none left: 0 is below every key
+    }
+    mine = l16 < top_k && my > kLowest;
+    id = (int)(511u - (my & 511u));
+    const uint32_t o = my >> 9;
+    v = Elem<DT>::get((uint16_t)(o & 0x8000u ? o & 0x7FFFu : ~o));
+  }
+};
+// Logits of 32 bits: the lowest id among those that hold the maximum, which leave.
+template <int PL>
+struct GroupSelect<kFp32, PL> {
+  static constexpr uint32_t kLowest = 0x007FFFFFu;  // topk_ord(-inf)
+  MOE_DEV static uint32_t key(float v, int) { return topk_ord(v); }
+  MOE_DEV static void select(uint32_t (&key)[PL], uint32_t m, int top_k, int l16, int& id, float& v, bool& mine) {
+    uint32_t my = 0;
+    id = 0;
+    for (int r = 0; r < top_k; ++r) {
+      uint32_t held = 0;  // 512 less the id
+#pragma unroll
+      for (int j = PL - 1; j >= 0; --j) held = key[j] == m ? 512u - 16u * j : held;
+      held = row_max(held != 0 ? held - (uint32_t)l16 : 0u);
+      if (l16 == r) {
+        my = m;
+        id = (int)(512u - held);
+      }
+      const uint32_t at = 512u - held - (uint32_t)l16;
+      m = 0;
+#pragma unroll
+      for (int j = 0; j < PL; ++j) {
+        key[j] = at == 16u * j ? 0u : key[j];
+        m = max(m, key[j]);
+      }
+      m = row_max(m);
+    }
+    mine = l16 < top_k && my > kLowest;
+    v = topk_ord_value(my);
+  }
 };
 
-// Four tokens a wave: a round of the selection is a subtraction and half a maximum for each of a lane's logits
-// and four exchanges, for all four. us of the routing with a wave a token / with this (bf16): 8192 x 256, top-8
-// 17.4 / 13.7, 32768 x 64 25.7 / 14.3, 1501 x 60 (fp16, top-5) 9.4 / 9.0; of few tokens a wave's own are done
-// sooner (256 x 256 fp32 11.2 / 15.4). fp32 logits leave no room for the id: a selection by their upper bits
-// with a check against the values took 26.3 for 16384 x 256 where a wave a token takes 24.3.
+// Four tokens a wave: a round of the selection is a few operations for each of a lane's logits and one or two
+// maxima over 16 lanes, for all four. us of the routing with a wave a token / with this: bf16 8192 x 256, top-8
+// 17.4 / 13.4, 32768 x 64 25.7 / 13.6, 1501 x 60 (fp16, top-5) 9.4 / 8.7; fp32 32768 x 8, top-2 20.2 / 12.0, 32768 x
+// 64 28.9 / 15.9, 32768 x 128 32.8 / 20.4, 16384 x 256 25.4 / 24.1, 32768 x 512, top-10 59.7 / 64.6. Of few tokens
+// a wave's own are done sooner (256 x 256 fp32 11.2 / 15.4).
 constexpr int kGroupWaves = 8, kGroupTokens = 4 * kGroupWaves, kGroupMaxTopK = 16, kGroupMinT = 1024;
-bool route_grouped(int T, int k, int dtype) {
-  return dtype != kFp32 && k <= kGroupMaxTopK && T >= kGroupMinT;
+constexpr int kGroupMaxFp32 = 256;
+bool route_grouped(int T, int E, int k, int dtype) {
+  return (dtype != kFp32 || E <= kGroupMaxFp32) && k <= kGroupMaxTopK && T >= kGroupMinT;
 }
 
 // PL logits a lane: expert 16 j + (lane & 15).
 template <int DT, int PL>
 __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs a) {
   using T = typename Elem<DT>::T;
-  using K = GroupKey<DT>;
+  using S = GroupSelect<DT, PL>;
   __shared__ BlockSums<kGroupWaves, 16 * PL> s;
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -308,7 +361,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs
     for (int j = 0; j < PL; ++j) {
       const bool in = 16 * j + l16 < a.E;
       x[j] = in ? Elem<DT>::get(next[j]) : -__builtin_inff();
-      key[j] = in ? K::key(next[j], 16 * j + l16) : 0u;
+      key[j] = in ? S::key(next[j], 16 * j + l16) : 0u;
       top = __builtin_fmaxf(top, x[j]);
       m = max(m, key[j]);
     }
@@ -318,21 +371,10 @@ __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs
     const bool some = top > -__builtin_inff();
     if (!some) top = 0.0f;
     m = row_max(m);
-    // lane r of the 16: the r-th largest key; below a maximum m the next one is the largest of key - m, in
-    // which those not below it are the small ones
-    uint32_t my = 0;
-    for (int r = 0; r < a.k; ++r) {
-      if (l16 == r) my = m;
-      uint32_t d = 0;
-#pragma unroll
-      for (int j = 0; j < PL; ++j) d = max(d, key[j] - m);
-      d = row_max(d);
-      m = d >> 31 ? m + d : 0u;  // none left: 0 is below every key
-    }
-    bool chosen = l16 < a.k && my > K::kLowest;
-    const int id = (int)(511u - (my & 511u));
-    const uint32_t o = my >> 9;
-    const float v = Elem<DT>::get((uint16_t)(o & 0x8000u ? o & 0x7FFFu : ~o));
+    int id;
+    float v;
+    bool chosen;
+    S::select(key, m, a.k, l16, id, v, chosen);
     float total = 0.0f;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
@@ -627,11 +669,11 @@ RouteWs route_ws(void* base, int T, int E, int64_t* bytes) {
 
 template <int DT, int NC>
 hipError_t launch_route(const RouteArgs& a, hipStream_t s) {
-  if constexpr (DT != kFp32) {
-    if (route_grouped(a.T, a.k, DT))
+  if constexpr (DT != kFp32 || 64 * NC <= kGroupMaxFp32) {
+    if (route_grouped(a.T, a.E, a.k, DT))
       hipLaunchKernelGGL((route_group_kernel<DT, 4 * NC>), dim3(a.groups), dim3(64 * kGroupWaves), 0, s, a);
   }
-  if (!route_grouped(a.T, a.k, DT)) {
+  if (!route_grouped(a.T, a.E, a.k, DT)) {
     const int waves = std::max(1, std::min(a.T, kWaves));
     hipLaunchKernelGGL((route_kernel<DT, NC>), dim3(a.groups), dim3(64 * waves), 0, s, a);
   }
@@ -728,7 +770,7 @@ int moe_route_v1(const void* logits, int32_t T, int32_t num_experts, int32_t dty
     return op_fail(MOE_ERR_SHAPE,
                    "route: outputs and workspace must not overlap the inputs or each other");
   const RouteArgs a{logits, mask, T, num_experts, top_k, renormalize != 0,
-                    route_groups(T, route_grouped(T, top_k, dtype) ? kGroupTokens : kWaves), topk_ids,
+                    route_groups(T, route_grouped(T, num_experts, top_k, dtype) ? kGroupTokens : kWaves), topk_ids,
                     topk_weights, counts, balance, z, stats, ws};
   const auto s = (hipStream_t)stream;
   MOE_OP_HIP(dtype == kBf16   ? launch_route_any<kBf16>(a, s)

@@ -107,7 +107,10 @@ CASES = [  # T, E, k, dtype, masked, blocked, renormalised
     (2100, 64, 8, torch.float16, False, 0.0, True), (31, 512, 16, torch.float32, True, 0.95, True),
     (1100, 300, 16, torch.bfloat16, True, 0.3, False), (1030, 512, 10, torch.float16, True, 0.97, True),
     (1027, 7, 7, torch.bfloat16, False, 0.5, True), (1501, 60, 5, torch.float16, True, 0.25, False),
-    (1024, 130, 1, torch.bfloat16, True, 0.0, True)]
+    (1024, 130, 1, torch.bfloat16, True, 0.0, True),
+    (1025, 8, 2, torch.float32, True, 0.0, True), (1100, 64, 16, torch.float32, True, 0.6, False),
+    (1030, 200, 10, torch.float32, False, 0.0, True), (1026, 256, 8, torch.float32, True, 0.97, True),
+    (1090, 7, 7, torch.float32, False, 0.5, True), (1040, 300, 8, torch.float32, False, 0.0, True)]
 
 
 @pytest.mark.parametrize("T,E,k,dtype,masked,blocked,renorm", CASES)
@@ -193,8 +196,9 @@ def test_ties_take_the_lower_id():
     assert int(r.counts.sum()) == 100
 
 
+@pytest.mark.parametrize("again", [1, 17])
 @pytest.mark.parametrize("E,k", [(12, 3), (60, 8), (256, 16), (500, 10), (500, 20)])
-def test_logits_closer_than_the_keys(E, k):
+def test_logits_closer_than_the_keys(E, k, again):
     """fp32 logits that agree in their upper bits, equal ones among them, next to ordinary tokens: the
     order is that of the values."""
     g = torch.Generator().manual_seed(E)
@@ -204,12 +208,13 @@ def test_logits_closer_than_the_keys(E, k):
     l[4::16, ::3] = -INF
     l[6::16] = -1e-30 * torch.randint(0, 9, (4, E), generator=g)
     l[8::16, E // 2:] = -INF
-    check(ops.route_tokens(l.cuda(), k), formulas(l, k), 64)
+    l = l.repeat(again, 1)
+    check(ops.route_tokens(l.cuda(), k), formulas(l, k), 64 * again)
 
 
 def test_tokens_without_an_expert():
     """Rows of -inf, of the type's lowest value, and padding that holds NaN and infinities."""
-    for dtype, more in ((torch.float32, 0), (torch.bfloat16, 0), (torch.float16, 0), (torch.bfloat16, 1100),
+    for dtype, more in ((torch.float32, 0), (torch.float32, 1100), (torch.bfloat16, 0), (torch.float16, 0), (torch.bfloat16, 1100),
                         (torch.float16, 2048)):
         low = torch.finfo(dtype).min
         l = make(6 + more, 32, dtype)
@@ -231,7 +236,8 @@ def test_tokens_without_an_expert():
         assert bool(d.isfinite().all()) and not d[[0, 3, 4]].any()
 
 
-@pytest.mark.parametrize("T,dtype", [(40, torch.float32), (40, torch.bfloat16), (1040, torch.float16)])
+@pytest.mark.parametrize("T,dtype", [(40, torch.float32), (40, torch.bfloat16), (1040, torch.float16),
+                                     (1040, torch.float32)])
 def test_a_counted_nan_shows(T, dtype):
     for bad in (float("nan"), INF):
         l = make(T, 24, dtype)
