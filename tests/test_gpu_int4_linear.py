@@ -185,6 +185,19 @@ def test_unaligned_tensors(T):
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("T", [4, 150, 500, 1400])
+def test_a_bias_off_a_boundary(T):
+    """Only the bias starts 2 bytes off: the kernels for aligned tensors take it."""
+    K, N, G = 256, 5448, 128
+    q, z, qw, qz, g = make(K, N, G, 6)
+    x = torch.randint(-2, 3, (T, K), generator=g).to(BF)
+    s = torch.tensor([0.25, 0.5, 1.0])[torch.randint(0, 3, (K // G, N), generator=g)].half()
+    bias = torch.randint(-8, 9, (N,), generator=g).to(BF)
+    off = torch.zeros(N + 1, dtype=BF, device="cuda")[1:].copy_(bias)
+    got = ops.int4_linear(x.cuda(), qw.cuda(), qz.cuda(), s.cuda(), group_size=G, bias=off)
+    assert torch.equal(got.cpu(), exact(x, q, z, s, G, bias).float().to(BF))
+
+
 def test_no_tokens():
     _, _, qw, qz, _ = make(128, 64, 128)
     s = torch.ones(1, 64).half().cuda()

@@ -42,6 +42,24 @@ def test_int4_linear(T, K, N):
         assert torch.equal(out[rows.cuda(), c0:c0 + 512].cpu(), want)
 
 
+@pytest.mark.parametrize("T", [3, 64, 130, 450])
+@pytest.mark.parametrize("G", [32, 64, 128, 65536])
+def test_int4_linear_of_the_longest_rows(T, G):
+    """K = 65536 with from one group to 2048, a tenth of x in use: sums below 2^24 / 4."""
+    K, N = 65536, 10_368
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qw = torch.randint(-2 ** 31, 2 ** 31 - 1, (K // 8, N), generator=g, device="cuda", dtype=torch.int32)
+    qz = torch.randint(-2 ** 31, 2 ** 31 - 1, (K // G, N // 8), generator=g, device="cuda", dtype=torch.int32)
+    s = torch.randint(1, 3, (K // G, N), generator=g, device="cuda").half() / 4
+    x = torch.randint(-1, 2, (T, K), generator=g, device="cuda").to(BF)
+    x *= torch.rand(T, K, generator=g, device="cuda") < 0.1
+    out = ops.int4_linear(x, qw, qz, s, group_size=G)
+    for c0 in (0, N - 64):
+        z = nibbles(qz[:, c0 // 8:c0 // 8 + 8].cpu(), False, True).repeat_interleave(G, 0)
+        w = (nibbles(qw[:, c0:c0 + 64].cpu(), True, False) - z) * s[:, c0:c0 + 64].cpu().double().repeat_interleave(G, 0)
+        assert torch.equal(out[:, c0:c0 + 64].cpu(), (x.cpu().double() @ w).float().to(BF))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, BF])
 def test_route_tokens(dtype):
     """2^22 tokens of 512 experts, the most slots; each prefers its number modulo 512."""
