@@ -286,11 +286,11 @@ hipError_t launch_stream(const Int4Args& a, hipStream_t s) {
 // of RING stages filled by loads that bypass the registers. The rest is as with few rows. EVERY: groups end at
 // multiples of so many steps (1 or 2), where the sums of the group are scaled and added up.
 //
-// The vector operations (40 to make operands of a step's words, 80 to scale a group's sums) and the
-// multiplications (24 of 16 cycles, 8 of them for the sums of x) bound it: with two waves a SIMD a step takes
-// about the sum of both, with the operations in the multiplications' shadow as well as with the compiler's
-// order. What is shared is x (few rows: 256 rows of 4096 x 8192 44 us, here 27), what is saved the
-// unpacking and its launch (many rows: 39).
+// What bounds it is issuing vector operations (40 to make operands of a step's words, 80 to scale a group's
+// sums) and multiplications (24, 8 of them for the sums of x; each takes 8 of its 16 cycles of the vector
+// operations' issue): 1220 cycles a step for two waves a SIMD, which takes 1900 with the waits at the barrier.
+// What is shared is x (few rows: 256 rows of 4096 x 8192 44 us, here 27), what is saved the unpacking and its
+// launch (many rows: 39).
 //
 // LDS rows of x are 128 bytes, the 16-byte chunk c of row r at position c ^ (r & 7): the 8 rows that a phase
 // of a 16-byte read spans lie in different banks.
@@ -923,13 +923,13 @@ int64_t stream_groups(int T, int N, int rows, int channels) {
 }
 
 // The larger a tile the fewer bytes of x and weights a workgroup reads for a result, the smaller the more
-// workgroups there are: the largest of these that its rows fill half of and that still gives most of the CUs one. us
-// with 16 x 16, 16 x 32, 16 x 64, 32 x 64, 64 x 64: 1 row of 2048 x 4096 4.3 / 4.7 / 5.7, of 4096 x 8192 9.3 /
-// 7.1 / 8.4; 16 rows of 8192 x 16384 41 / 26 / 19 / 23 / 31; 32 of it 74 / 45 / 32 / 25 / 34; 48 rows of 2048 x
-// 4096 9.5 / 8.1 / 6.6 / 8.6 / 13; 64 rows of 2048 x 4096 12 / 8.1 / 6.7 / 8.6 / 14, of 4096 x 8192 38 / 24 / 18 /
-// 15 / 23; 96 of 2048 x 4096 17 / 11 / 11 / 8.6 / 14; 203 of 1056 x 2008 13 / 9.2 / 8.1 / 7.0 / 10; 256 of 4096 x
-// 8192 146 / 88 / 66 / 54 / 47 (there groups of 64 and 128 have the kernel for more rows). 32 x 32 and 64 x 32
-// are never the best.
+// workgroups there are: the largest of these that its rows fill half of and that still gives most of the CUs
+// one. us with 16 x 16, 16 x 32, 16 x 64, 32 x 64, 64 x 64: 1 row of 2048 x 4096 4.3 / 4.7 / 5.7, of 4096 x 8192
+// 9.3 / 7.1 / 8.4; 16 rows of 8192 x 16384 41 / 26 / 19 / 23 / 31, 32 of it 74 / 45 / 32 / 25 / 34; 48 rows of
+// 2048 x 4096 9.5 / 8.1 / 6.6 / 8.6 / 13; 64 rows of 2048 x 4096 12 / 8.1 / 6.7 / 8.6 / 14, of 4096 x 8192 38 / 24
+// / 18 / 15 / 23; 96 of 2048 x 4096 17 / 11 / 11 / 8.6 / 14; 203 of 1056 x 2008 13 / 9.2 / 8.1 / 7.0 / 10; 256 of
+// 4096 x 8192 146 / 88 / 66 / 54 / 47 (groups of 64 and 128 have the kernel for more rows there). 32 x 32 and 64
+// x 32 are never the best.
 constexpr int kEnough = 192;
 template <int DT, int SPG>
 hipError_t launch_few_rows(const Int4Args& a, hipStream_t s) {

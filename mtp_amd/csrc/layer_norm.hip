@@ -240,8 +240,9 @@ constexpr int kForwardGroups = 1536;
 // Workgroups of the backward pass: each keeps the weights' gradients of its rows in registers and
 // writes them once.
 //
-// Rows of up to 256 columns take 32, 16 or 8 threads, forward and backward (us a wave a row / with this): 65536 x
-// 256 fp16 27 and 30 / 16 and 22, 524288 x 128 bf16 186 and 175 / 54 and 79, 300000 x 64 106 and 100 / 16 and 38.
+// Rows of up to 256 columns take 32, 16 or 8 threads, forward and backward (us a wave a row / with this):
+// 65536 x 256 fp16 27 and 30 / 16 and 22, 524288 x 128 bf16 186 and 175 / 54 and 79, 300000 x 64 106 and 100 / 16
+// and 38.
 int narrow_threads_of(int H) { return H <= 64 ? 8 : H <= 128 ? 16 : H <= 256 ? 32 : threads_of(H); }
 int backward_groups(int T, int H) {
   const int nt = narrow_threads_of(H), rows = rows_of(nt);
