@@ -374,7 +374,8 @@ int moe_route_backward_v1(const void* logits, int32_t T, int32_t num_experts, in
 /* y = round((x - mean) / sqrt(var + eps) * weight + bias) with the biased variance of each row; weight
  * (NULL: ones) and bias (NULL: zeros) [hidden], x and y [T, hidden] of one dtype (0 bf16, 1 fp16,
  * 2 fp32); hidden in [1, 8192]. stats: NULL, or fp32 [T, 4] on a 16-byte boundary for the backward pass
- * (the mean in two parts, 1 / sqrt(var + eps), 0). Outputs overlap nothing. The reference's LayerNorm
+ * (s mean in two parts, 1 / (s sqrt(var + eps)) and s: 1, or the power of two that brings a row back whose
+ * squares leave fp32's range). Outputs overlap nothing. The reference's LayerNorm
  * stands inside its predictor only (src/mtp_expert_prefetch/training/hidden_residual.py:44-106). */
 int moe_layer_norm_v1(const void* x, int32_t T, int32_t hidden, int32_t dtype, const void* weight,
                       const void* bias, float eps, void* y, float* stats, void* stream);

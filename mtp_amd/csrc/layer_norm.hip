@@ -16,7 +16,14 @@
 // x - m taken as (x - m_hi) - m_lo, off by two half steps. The squares of that are summed 8 at a time in fp32
 // (a tree: 4 roundings) and from there on in 64 bits, so r is off by 3 half steps whatever the row's width
 // and mean.
+//
+// A row with var + eps outside [2^-80, 2^126], where squares may leave fp32's range, is taken again from memory
+// with squares of 64 bits, and from there on in units of a power of two (1 / s) that brings it back:
+//   h = (s x - s m) r,  r = 1 / sqrt(s^2 (var + eps)),  dx = s r (...)
+// s x is not rounded but where it is 2^-100 of the row's spread, so such rows are as exact as the others (s = 1).
+// They cost a second read; the test for them is two comparisons a row.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "elem.h"
@@ -48,6 +55,16 @@ struct Rows {
     stride = (int64_t)gridDim.x * (BT / NT);
   }
 };
+
+// var + eps of the rows that fp32's squares hold, and s for the others: 2^100 keeps a row below it in range (its
+// columns are below 2^-7, since two of them are less than 2^-32 apart and differ) and 2^-80 any row above it, and
+// s^2 (var + eps) lies between 2^-98 and 2^120. Without a spread, and with infinities or NaN, s = 1.
+constexpr float kNearLow = 0x1p-80f, kNearHigh = 0x1p126f;
+MOE_DEV bool near(float v) { return v >= kNearLow && v <= kNearHigh; }
+MOE_DEV float row_scale(double var, double v) {
+  if (!(var > 0.0 && v < __builtin_inf())) return 1.0f;
+  return v < kNearLow ? 0x1p100f : v > kNearHigh ? 0x1p-80f : 1.0f;
+}
 
 // NT threads a row, NC chunks of 8 NT columns: a wave a row while it holds the row (2048 columns), with no
 // barrier and 12 exchanges for up to 32 columns a lane; with 256 threads a row of 2048 these and the barriers
@@ -87,7 +104,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
     load(next, a.x, min(t + rows.stride, (int64_t)a.T - 1));  // past the last row: read again, not used
     row_sums<NT>(part, sum, s_part);
     const double mean = sum[0] / (double)H;
-    const float hi = (float)mean, lo = (float)(mean - (double)hi);
+    float hi = (float)mean, lo = (float)(mean - (double)hi);
     part[0] = 0.0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -100,8 +117,38 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(LayerNormArgs a, void* 
       part[0] += (double)((q[0] + q[1]) + (q[2] + q[3]));
     }
     row_sums<NT>(part, sum, s_part);
-    const float r = inv_sqrt(sum[0] * inv_h + a.eps);
-    if (stats && tid == 0 && in) stats[t] = f32x4{hi, lo, r, 0.0f};
+    double v = sum[0] * inv_h + a.eps;
+    float r = inv_sqrt_near(v), scale = 1.0f;
+    // The whole wave, for the exchanges; a near row comes out as it went in. The row is read again, and `at` hides
+    // that it is the same column, so that nothing is kept in registers for this.
+    if (__builtin_expect(__ballot(!near((float)v)) != 0, 0)) {
+      const T* const row = static_cast<const T*>(a.x) + min(t, (int64_t)a.T - 1) * H;
+      int at = tid;
+      asm volatile("" : "+v"(at));
+      part[0] = 0.0;
+#pragma unroll 1
+      for (int c = at; c < H; c += NT) {
+        const double u = (double)Elem<DT>::get(row[c]) - mean;
+        part[0] = __builtin_fma(u, u, part[0]);
+      }
+      row_sums<NT>(part, sum, s_part);
+      if (!near((float)v)) {
+        v = sum[0] * inv_h + a.eps;
+        scale = row_scale(sum[0], v);
+        const double m = mean * (double)scale;
+        hi = (float)m;
+        lo = (float)(m - (double)hi);
+        r = inv_sqrt(v * (double)scale * (double)scale);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = c * 8 * NT + C::col(at, e);
+          d[c][e] = i < H ? __builtin_fmaf(Elem<DT>::get(row[i]), scale, -hi) - lo : 0.0f;
+        }
+    }
+    if (stats && tid == 0 && in) stats[t] = f32x4{hi, lo, r, scale};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int left = H - c * 8 * NT;
@@ -157,26 +204,48 @@ __global__ __launch_bounds__(block_threads<NT>()) void layer_norm_backward_kerne
     const bool mine = NT >= 64 || t < a.T;
     const Row row = next;
     load(t + rows.stride);
-    const float hi = row.st[0], lo = row.st[1], r = row.st[2];
-    float part[2] = {0.0f, 0.0f}, tot[2];
-    float h[8], g[8];
+    const float hi = row.st[0], lo = row.st[1], r = row.st[2], scale = row.st[3];
+    auto take = [&](auto scaled) __attribute__((always_inline)) {
+      float part[2] = {0.0f, 0.0f}, tot[2];
+      float h[8], g[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = C::col(tid, e) < H;
-      const float dy = mine ? row.dy.get(e, tid, H) : 0.0f;
-      h[e] = in && mine ? ((row.x.get(e, tid, H) - hi) - lo) * r : 0.0f;
-      g[e] = dy * w[e];
-      dw[e] = __builtin_fmaf(dy, h[e], dw[e]);
-      db[e] += dy;
-      part[0] += g[e];
-      part[1] = __builtin_fmaf(g[e], h[e], part[1]);
-    }
-    if (d.dx) {
-      row_sums<NT>(part, tot, s_part);
-      const float mg = tot[0] * inv_h, mgh = tot[1] * inv_h;
+      for (int e = 0; e < 8; ++e) h[e] = row.x.get(e, tid, H);
+      if (scaled) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = r * ((g[e] - mg) - h[e] * mgh);
-      if (mine) C::store(static_cast<T*>(d.dx) + t * H, tid, H, g);
+        for (int e = 0; e < 8; ++e) h[e] *= scale;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = C::col(tid, e) < H;
+        const float dy = mine ? row.dy.get(e, tid, H) : 0.0f;
+        h[e] = in && mine ? ((h[e] - hi) - lo) * r : 0.0f;
+        g[e] = dy * w[e];
+        dw[e] = __builtin_fmaf(dy, h[e], dw[e]);
+        db[e] += dy;
+        part[0] += g[e];
+        part[1] = __builtin_fmaf(g[e], h[e], part[1]);
+      }
+      if (d.dx) {
+        row_sums<NT>(part, tot, s_part);
+        const float mg = tot[0] * inv_h, mgh = tot[1] * inv_h;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = r * ((g[e] - mg) - h[e] * mgh);
+        if (scaled) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] *= scale;
+        }
+        if (mine) C::store(static_cast<T*>(d.dx) + t * H, tid, H, g);
+      }
+    };
+    // s is 1 in nearly every wave. us without s / with its products always taken / in branches / in two bodies:
+    // 300000 x 64 bf16 37.8 / 40.3 / 38.0 / 42, 100001 x 99 (element-wise) 24.7 / 25.7 / 28.7 / 24.2, 8192 x 4096
+    // fp16 40.1 / 40.1 / 40.1 / 41.6.
+    const bool scaled = __builtin_expect(__ballot(scale != 1.0f) != 0, 0);
+    if constexpr (VEC || NT >= 64) {
+      take(scaled);
+    } else {
+      if (scaled) take(std::true_type{});
+      else take(std::false_type{});
     }
   }
   if constexpr (NT <= 64) {  // the workgroup's rows first

@@ -53,11 +53,15 @@ MOE_DEV void row_sums(const P (&part)[N], A (&v)[N], A (*s_part)[N]) {
 }
 
 // 1 / sqrt(m), rounded to fp32 at the end: the hardware's approximation and a Newton step in 64 bits.
+// inv_sqrt_near: m within [2^-100, 2^127]. inv_sqrt: outside that of m rounded to fp32 (0 beyond its range).
+MOE_DEV float inv_sqrt_near(double m) {
+  const double r = (double)__builtin_amdgcn_rsqf((float)m);
+  return (float)(r + 0.5 * r * (1.0 - m * r * r));
+}
 MOE_DEV float inv_sqrt(double m) {
   const float v = (float)m;
   if (!(v >= 0x1p-100f && v < __builtin_inff())) return 1.0f / __builtin_sqrtf(v);
-  const double r = (double)__builtin_amdgcn_rsqf(v);
-  return (float)(r + 0.5 * r * (1.0 - m * r * r));
+  return inv_sqrt_near(m);
 }
 
 // Threads a row takes, and the workgroup of (at least 256) threads they lie in.
