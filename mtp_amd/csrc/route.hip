@@ -219,14 +219,19 @@ MOE_DEV void block_sums(const RouteArgs& a, BlockSums<W, NE>& s, float zsum, int
 }
 
 // exp(x) for x <= 0, and a NaN for a NaN: 2^(x log2 e) with the product in two parts, off by about 2 half
-// steps; a third of the library's operations. Below e^-104 there is no fp32 number.
+// steps; a third of the library's operations. The hardware's 2^x gives zero below 2^-126. SMALL: it is taken 2^64
+// higher there, down to fp32's smallest number. The weights take it so. Beside the 1 in a token's sum, and in
+// the balance beside a token's first expert, such a term counts for less than 2^-100.
+template <bool SMALL = false>
 MOE_DEV float exp_neg(float x) {
   constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
   x = x < -110.0f ? -110.0f : x;
   const float hi = x * kLog2e;
   const float lo = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -hi));
-  const float r = __builtin_amdgcn_exp2f(hi);
-  return __builtin_fmaf(r * lo, kLn2, r);
+  const bool small = SMALL && hi < -126.0f;
+  const float r = __builtin_amdgcn_exp2f(small ? hi + 64.0f : hi);
+  const float e = __builtin_fmaf(r * lo, kLn2, r);
+  return small ? e * 0x1p-64f : e;
 }
 
 // ---------------------------------------------------------------- 16 lanes a token
@@ -384,7 +389,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs
     total = row_sum(total);
     const bool live = kept && (some || total != total);
     chosen = chosen && live;
-    const float mine = chosen ? exp_neg(v - top) : 0.0f;
+    const float mine = chosen ? exp_neg<true>(v - top) : 0.0f;
     float over = total;
     if (a.renorm) {
       // a NaN or +inf among the logits makes the weights NaN, also where it is not chosen
@@ -477,7 +482,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
     float my_v;
     bool chosen;
     S::select(key, live ? a.k : 0, lane, my_i, my_v, chosen);
-    const float mine = chosen ? exp_neg(my_v - top) : 0.0f;
+    const float mine = chosen ? exp_neg<true>(my_v - top) : 0.0f;
     float over = total;
     if (a.renorm) {
       // a NaN or +inf among the logits makes the weights NaN, also where it is not chosen
