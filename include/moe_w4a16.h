@@ -329,9 +329,10 @@ int moe_int8_experts_v1(const void* x, int32_t T, int32_t dtype, const int32_t* 
  * group g = k / G), products and sums in fp32 on unrounded weights. The dense counterpart of
  * moe_w2_down_v1; no counterpart in the reference, which multiplies by moe_dequant_v1's weights.
  * x [T, K], bias NULL or [N], out [T, N] of one dtype (0 bf16, 1 fp16). N a multiple of 8; group_size a
- * multiple of 32 that divides K; K <= 65536; x, qweight and scales below 2 GiB each, T * N < 2^33. An
- * infinity in x may come out as a NaN. The workspace query gives 0 where none is needed (then workspace
- * may be NULL). */
+ * multiple of 32 that divides K; K <= 65536; x, qweight and scales below 2 GiB each, T * N < 2^33. x up
+ * to 2^64 in magnitude and finite scales give the sums above; beyond them a token's results (a channel's, of
+ * a scale) may be infinities or NaN where the formula's are finite, and an infinity may come out as a NaN.
+ * The workspace query gives 0 where none is needed (then workspace may be NULL). */
 int64_t moe_int4_linear_workspace_bytes_v1(int32_t T, int32_t K, int32_t N, int32_t group_size);
 int moe_int4_linear_v1(const void* x, int32_t T, int32_t K, int32_t dtype,
                        const moe_gptq_proj_v1* weight, int32_t N, int32_t group_size,

@@ -4,7 +4,9 @@
 //   y[t, n] = round(sum_g s[g, n] * (sum_{k in g} x[t, k] (q[k, n] - z[g, n])) (+ bias[n]))
 //
 // The weights are not rounded: a group's products are summed in fp32 on the integers q - z and scaled
-// after that. Four forms:
+// after that. Of x up to 2^64 all sums stay in fp32's range: sums of x (16 + q) over K <= 2^16 below 2^85, and
+// those of many rows, in units of a scale (2^-24 .. 2^16), below 2^124. Beyond it they may not, and infinities
+// of both signs meet in a NaN. Four forms:
 //   few rows   operands from memory to registers, the words made into MFMA operands there. Reading the
 //              weights bounds it, and the launch where they are few: 1 row of 2048 x 4096 4.7 us on the
 //              GPU, of 8192 x 16384 16 us (4.4 TB/s), 16 rows of 4096 x 8192 7.2 us (3.6 TB/s).

@@ -808,8 +808,10 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor, sc
     g = k // group_size, sums in fp32 on unrounded weights, rounded once to x's type.
 
     x [T, K] bf16 or fp16, qweight int32 [K/8, N], qzeros int32 [K/G, N/8], scales fp16 [K/G, N], bias
-    [N] of x's type. N is a multiple of 8, group_size a multiple of 32. An infinity in x may come out as a
-    NaN. No gradient: a backward pass that reaches the call raises."""
+    [N] of x's type. N is a multiple of 8, group_size a multiple of 32. x is to lie within 2^64 in magnitude
+    and scales are to be finite: beyond that a token's results (a channel's, of a scale) may be infinities or
+    NaN where the formula's are finite, and an infinity may come out as a NaN. No gradient: a backward pass
+    that reaches the call raises."""
     code = _rows_2d(x, "x")
     if code == OUT_DTYPES[torch.float32]:
         raise TypeError("x must be bfloat16 or float16, got torch.float32")
