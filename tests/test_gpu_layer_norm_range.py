@@ -1,4 +1,5 @@
-"""Layer norm of rows whose squares leave fp32's range, against the formulas in 64 bits.
+"""Layer norm of rows whose squares leave fp32's range, against the formulas in 64 bits, and the weights'
+gradients of many rows, exactly.
 
 Such a row is taken in units of a power of two, which rounds nothing, so the bounds are those of any row
 (u = 2^-24): x - m off by 2 u of itself, r by 4 u, h by 8 u |h|, y by 8 u |h w| + u |y|; dx by
@@ -108,3 +109,31 @@ def test_eps_that_outweighs_the_row(H):
     d = x.double() - x.double().mean(1, keepdim=True)
     want = d * (d.square().mean(1, keepdim=True) + eps).rsqrt()
     near(ops.layer_norm(x.cuda(), eps=eps), want, 9 * U * want.abs(), torch.float32, "y")
+
+
+# Rows of +-1, as many of either: mean 0, variance 1, and with eps = 0 h = x exactly. With incoming gradients of
+# small integers the weights' gradients are integers below 2^24, exact in fp32 in any order: equality, to the
+# last row. T lies behind one, two and more passes of all workgroups (768 or 256 of 32, 16, 8, 4 or 1 rows), with ragged
+# ends: a workgroup, a wave, a row more, a row less.
+PASSES = [(8, 32), (64, 32), (66, 16), (100, 16), (128, 16), (130, 8), (256, 8), (258, 4), (512, 4), (514, 1), (2000, 1),
+          (2050, 1), (8192, 1), (8190, 1)]
+
+
+@pytest.mark.parametrize("H,rows", PASSES)
+def test_every_row_counts_once_in_the_weights_gradients(H, rows):
+    groups = 768 if H <= 2048 else 256
+    for T in (rows, rows + 1, groups * rows - 1, groups * rows, groups * rows + 1, 2 * groups * rows - 1,
+              2 * groups * rows + 3, (3 if H < 600 else 2) * groups * rows + rows // 2 + 1):
+        g = torch.Generator(device="cuda").manual_seed(T + H)
+        x = torch.ones(T, H, device="cuda")
+        x[:, ::2] = -1.0
+        x *= 1.0 - 2.0 * torch.randint(0, 2, (T, 1), generator=g, device="cuda")
+        dy = torch.randint(1, 8, (T, H), generator=g, device="cuda").float()
+        w, b = (torch.ones(H, device="cuda", requires_grad=True) for _ in range(2))
+        y = ops.layer_norm(x, w, b, eps=0.0)
+        assert torch.equal(y, x + 1.0)
+        dw, db = torch.autograd.grad(y, (w, b), dy)
+        assert torch.equal(db, dy.double().sum(0).float()), T
+        assert torch.equal(dw, (dy.double() * x).sum(0).float()), T
+        only, = torch.autograd.grad(ops.layer_norm(x, w, b, eps=0.0), (b,), dy)
+        assert torch.equal(only, db)
