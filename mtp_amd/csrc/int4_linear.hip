@@ -73,7 +73,6 @@ template <int DT>
 struct Op;
 template <>
 struct Op<kBf16> {
-  static constexpr float kOff = 16.0f;
   static constexpr uint32_t kOnes = 0x3F803F80u;
   // OFF + the nibble at bit `at`, as a float
   MOE_DEV static float zero_point(uint32_t z, int at) {
@@ -89,7 +88,6 @@ struct Op<kBf16> {
 };
 template <>
 struct Op<kFp16> {
-  static constexpr float kOff = 64.0f;
   static constexpr uint32_t kOnes = 0x3C003C00u;
   MOE_DEV static float zero_point(uint32_t z, int at) {
     return __uint_as_float(((at <= 17 ? z << (17 - at) : z >> (at - 17)) & 0x001E0000u) | 0x42800000u);
