@@ -919,8 +919,8 @@ def route_tokens(logits: torch.Tensor, top_k: int = 8, *, mask: torch.Tensor | N
     T, E = logits.shape
     if not 1 <= E <= 512:
         raise ValueError(f"logits must be [T, E] with E in [1, 512], got {tuple(logits.shape)}")
-    if not 1 <= top_k <= min(E, 64):
-        raise ValueError(f"top_k must lie in [1, {min(E, 64)}], got {top_k}")
+    if not 1 <= top_k <= min(E, 64) or top_k != int(top_k):
+        raise ValueError(f"top_k must be a whole number in [1, {min(E, 64)}], got {top_k}")
     if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (T,)):
         raise ValueError(f"mask must be bool [{T}], got {mask.dtype} {tuple(mask.shape)}")
     _require_gpu(logits, mask)
