@@ -20,8 +20,9 @@
 // TB/s).
 //
 // A wave keeps its sums of p in registers and its workgroup the counts in LDS (integer atomics: the order does
-// not matter), so that a workgroup leaves one row of partial sums. Sums are taken in a fixed order: fp32 over a
-// wave's tokens and a workgroup's waves, 64 bits over the workgroups.
+// not matter), so that a workgroup leaves one row of partial sums. Sums are taken in a fixed order: those of p in
+// fp32 over a wave's tokens and a workgroup's waves, in 64 bits over the workgroups, those of lse^2 in 64 bits
+// (fp32's would overflow for logits of 10^19 whose mean of squares it holds).
 #include <algorithm>
 
 #include "common.h"
@@ -117,7 +118,7 @@ struct Select<kFp32, NC> {
 struct RouteWs {
   uint32_t* arrived;  // [1]
   double* parts;      // [kMaxExperts / kCols] of the balance
-  float* z;           // [groups]
+  double* z;          // [groups]
   int32_t* n;         // [groups]
   float* p;           // [groups][E]
   int32_t* c;         // [groups][E]
@@ -162,7 +163,7 @@ template <int W, int NE>
 struct BlockSums {
   float p[W][NE];
   int c[NE];
-  float z[W];
+  double z[W];
   int n[W];
   double dot[W];
   MOE_DEV void clear(const RouteArgs& a) {
@@ -175,14 +176,14 @@ struct BlockSums {
 // Behind every wave's p: the workgroup's row of partial sums, or the results where it is the only one. z and n
 // are the wave's.
 template <int W, int NE>
-MOE_DEV void block_sums(const RouteArgs& a, BlockSums<W, NE>& s, float zsum, int n) {
+MOE_DEV void block_sums(const RouteArgs& a, BlockSums<W, NE>& s, double zsum, int n) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   if (lane == 0) {
     s.z[wave] = zsum;
     s.n[wave] = n;
   }
   __syncthreads();
-  float z = 0.0f;
+  double z = 0.0;
   int live = 0;
   for (int w = 0; w < waves; ++w) {
     z += s.z[w];
@@ -214,7 +215,7 @@ MOE_DEV void block_sums(const RouteArgs& a, BlockSums<W, NE>& s, float zsum, int
   if (tid == 0) {
     dot = 0.0;
     for (int w = 0; w < waves; ++w) dot += s.dot[w];
-    finish(a, dot, (double)z, live);
+    finish(a, dot, z, live);
   }
 }
 
@@ -342,7 +343,8 @@ __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int waves = blockDim.x >> 6;
   s.clear(a);
-  float psum[PL], zsum = 0.0f;
+  float psum[PL];
+  double zsum = 0.0;
   int n = 0;
 #pragma unroll
   for (int j = 0; j < PL; ++j) psum[j] = 0.0f;
@@ -411,7 +413,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void route_group_kernel(RouteArgs
 #pragma unroll
       for (int j = 0; j < PL; ++j) psum[j] = __builtin_fmaf(x[j], inv, psum[j]);
       if (l16 == 0) {
-        zsum = __builtin_fmaf(lse, lse, zsum);
+        zsum = __builtin_fma((double)lse, (double)lse, zsum);
         ++n;
       }
     }
@@ -437,7 +439,8 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = blockDim.x >> 6;
   s.clear(a);
-  float psum[NC], zsum = 0.0f;
+  float psum[NC];
+  double zsum = 0.0;
   int n = 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) psum[c] = 0.0f;
@@ -503,7 +506,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(RouteArgs a) {
       const float inv = 1.0f / total;
 #pragma unroll
       for (int c = 0; c < NC; ++c) psum[c] = __builtin_fmaf(ex[c], inv, psum[c]);
-      zsum = __builtin_fmaf(lse, lse, zsum);
+      zsum = __builtin_fma((double)lse, (double)lse, zsum);
       ++n;
     }
   }
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(1024) void route_sum_kernel(RouteArgs a) {
     p += (double)a.ws.p[(int64_t)g * a.E + at];
     c += a.ws.c[(int64_t)g * a.E + at];
   }
-  double z = tid < a.groups ? (double)a.ws.z[tid] : 0.0;  // at most 512 workgroups
+  double z = tid < a.groups ? a.ws.z[tid] : 0.0;  // at most 512 workgroups
   int n = tid < a.groups ? a.ws.n[tid] : 0;
   // a wave's four slots of an expert: lanes col, col + 16, ...
   p += partner<32>(p);
@@ -663,12 +666,12 @@ RouteWs route_ws(void* base, int T, int E, int64_t* bytes) {
     o += align256(n);
     return at;
   };
-  const int64_t arrived = take(4), parts = take(kMaxExperts / kCols * 8), z = take(g * 4),
+  const int64_t arrived = take(4), parts = take(kMaxExperts / kCols * 8), z = take(g * 8),
                 n = take(g * 4), p = take(g * E * 4), c = take(g * E * 4);
   *bytes = g > 1 ? o : 0;
   char* b = static_cast<char*>(base);
   return RouteWs{reinterpret_cast<uint32_t*>(b + arrived), reinterpret_cast<double*>(b + parts),
-                 reinterpret_cast<float*>(b + z), reinterpret_cast<int32_t*>(b + n),
+                 reinterpret_cast<double*>(b + z), reinterpret_cast<int32_t*>(b + n),
                  reinterpret_cast<float*>(b + p), reinterpret_cast<int32_t*>(b + c)};
 }
 
