@@ -402,7 +402,9 @@ int moe_layer_norm_backward_v1(const void* x, int32_t T, int32_t hidden, int32_t
  *   x_out = round(res_out * rsqrt(mean(res_out^2) + eps) * (1 + pre_w))  (pre_w NULL: not written)
  * with mtp_rms_norm's (1 + w) scaling (src/mtp_expert_prefetch/mtp/extra_tensors.py:40-48), which
  * moe_rmsnorm_v1 applies to the plain residual sum. All tensors of one dtype (0 bf16, 1 fp16,
- * 2 fp32); hidden in [1, 8192]; res_out may be res; otherwise outputs overlap nothing. */
+ * 2 fp32); hidden in [1, 8192]; res_out may be res; otherwise outputs overlap nothing. Squares are taken in
+ * fp32: y and res_out within 2^60 in magnitude, and mean squares + eps of at least 2^-100 (past them a row's
+ * norm is 0, infinity or NaN). */
 int moe_block_norm_v1(const void* y, const void* res, int32_t T, int32_t hidden, int32_t dtype,
                       const void* post_w, const void* gate, int32_t gate_kind, float res_scale,
                       float branch_scale, const void* pre_w, float eps, void* res_out, void* x_out,

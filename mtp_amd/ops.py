@@ -1058,7 +1058,8 @@ def block_norm(y: torch.Tensor, res: torch.Tensor, *, post_w: torch.Tensor | Non
     with the (1 + w) scaling of ``rmsnorm``. y (the block's output) and res (the residual stream)
     [T, H], post_w and pre_w [H], gate [H] (per channel), [T, 1] (per token) or [T, H], all of one
     type (bf16, fp16 or fp32); H up to 8192. res_out is rounded to the type before x is computed
-    from it. Returns (res_out, x); differentiable in y, res, post_w, gate and pre_w."""
+    from it. Squares are taken in fp32: y and res_out within 2^60 in magnitude, their mean squares + eps
+    at least 2^-100 (past them a row's norm is 0, infinity or NaN). Returns (res_out, x); differentiable in y, res, post_w, gate and pre_w."""
     _rows_2d(y, "y")
     T, H = y.shape
     if res.shape != y.shape or res.dtype != y.dtype:
