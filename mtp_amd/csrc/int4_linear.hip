@@ -8,15 +8,14 @@
 // those of many rows, in units of a scale (2^-24 .. 2^16), below 2^124. Beyond it they may not, and infinities
 // of both signs meet in a NaN. Four forms:
 //   few rows   operands from memory to registers, the words made into MFMA operands there. Reading the
-//              weights bounds it, and the launch where they are few: 1 row of 2048 x 4096 4.7 us on the
-//              GPU, of 8192 x 16384 16 us (4.4 TB/s), 16 rows of 4096 x 8192 7.2 us (3.6 TB/s).
-//   more rows  the same words, x shared through LDS: 128 rows of 4096 x 8192 18 us, 256 27 us (640 TFLOP/s).
+//              weights bounds it, and the launch where they are few: 1 row of 2048 x 4096 4.2 us, of 8192 x
+//              16384 17 (4.1 TB/s), 16 rows of 4096 x 8192 8.8 (2.0 TB/s), of 8192 x 16384 21 (3.3 TB/s).
+//   more rows  the same words, x shared through LDS: 128 rows of 4096 x 8192 18 us, 256 28 (605 TFLOP/s).
 //              Vector operations and multiplications bound it.
-//   many rows  integers unpacked once, then a tiled product from LDS: 4096 rows of 4096 x 8192 214 us, 12
-//              of them the unpacking (1360 TFLOP/s in the product). Loads into LDS bound it up to about
-//              1000 rows (of the 51 us of 512 rows 46 are left without a product or a read of LDS, 41
-//              without the loads), the matrix and vector pipes beyond.
+//   many rows  integers unpacked once, then a tiled product from LDS: 4096 rows of 4096 x 8192 219 us, 12
+//              of them the unpacking (1.33 PFLOP/s in the product). The matrix and vector pipes bound it.
 //   unaligned  value by value, for tensors that start between two 16-byte boundaries.
+// Times are of captured graphs, a call behind the other, each with weights of its own that come from HBM.
 #include <algorithm>
 #include <type_traits>
 

@@ -14,10 +14,13 @@
 // A token counts if the mask keeps it and one of its logits is above -inf or a NaN; other tokens have ids
 // -1, weights 0 and no gradient. Only logits above -inf are chosen; places without one have id -1.
 //
-// Not the bytes but the instructions of the selection bound it: a wave a token, or for many tokens of at most
-// 256 experts (512 with 16 bits) four tokens a wave. us on the GPU: 8 x 256 fp32 4.8, 8192 x 256 bf16 8.3 (0.5
-// TB/s) and 4.8 for the workgroups' sums, 16384 x 256 fp32 19 (0.9 TB/s) and 5.8; the gradient 12 there (2.8
-// TB/s).
+// Not the bytes but vector instructions bound it: a wave a token, or for many tokens of at most 256 experts (512
+// with 16 bits) four tokens a wave. Of the 1341 that four tokens of 256 16-bit logits take with top-8 the
+// selection's rounds are 264 (33 a round: a subtraction and a maximum a key, and the row's maximum), the keys
+// 240, exponentials and the sums of p 270, and what a wave does once, however many tokens it takes, 450
+// (addresses, the butterflies and the workgroup's sums; with 8192 tokens that is once for every four). Of 1701
+// for fp32 the rounds are 704. us on the GPU: 8 x 256 fp32 4.8, 8192 x 256 bf16 8.3 (0.5 TB/s) and 4.9 for the
+// workgroups' sums, 16384 x 256 fp32 20 (0.9 TB/s) and 5.8; the gradient 12 there (2.8 TB/s).
 //
 // A wave keeps its sums of p in registers and its workgroup the counts in LDS (integer atomics: the order does
 // not matter), so that a workgroup leaves one row of partial sums. Sums are taken in a fixed order: those of p in
